@@ -67,6 +67,14 @@ PROTOTYPES = {
     "cudeep_b200_matmul_bf16": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
     "cudeep_b200_matmul_f16_tuned": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                                              ctypes.c_uint32, ctypes.c_uint32, c_void_p]),
+    "cudeep_b200_quantize_fp8": (c_int, [c_void_p, c_int, ctypes.c_longlong, c_int, c_int, c_void_p, c_void_p,
+                                         _stream]),
+    "cudeep_b200_dequantize_fp8": (c_int, [c_void_p, c_void_p, ctypes.c_longlong, c_int, c_int, c_void_p, c_int,
+                                           _stream]),
+    "cudeep_b200_grouped_matmul_nt": (c_int, [_fp, _fp, _fp, c_int, c_void_p, c_int, c_int, c_int, c_int, _stream]),
+    "cudeep_b200_grouped_matmul_nn": (c_int, [_fp, _fp, _fp, c_int, c_void_p, c_int, c_int, c_int, c_int, _stream]),
+    "cudeep_b200_grouped_matmul_tn": (c_int, [_fp, _fp, _fp, c_int, c_int, c_void_p, c_int, c_int, c_int, c_int,
+                                              _stream]),
     "cudeep_b200_pool_alloc": (c_int, [c_size_t, POINTER(c_void_p)]),
     "cudeep_b200_pool_free": (c_int, [c_void_p]),
     "cudeep_b200_pool_alloc_on_stream": (c_int, [c_size_t, c_void_p, POINTER(c_void_p)]),

@@ -4,6 +4,7 @@
 #include "cudeep_b200.h"
 
 #include "cudeep/kernels/conv.cuh"
+#include "cudeep/kernels/lowp.cuh"
 #include "cudeep/kernels/matmul.cuh"
 #include "cudeep/memory.cuh"
 #include "conv_igemm.h"
@@ -39,6 +40,11 @@ cudaStream_t as_stream(cudeep_b200_stream_t s) { return static_cast<cudaStream_t
 cudeep::kernels::GemmEpilogue as_epilogue(int code) {
     CB200_REQUIRE(code >= 0 && code <= 4, "unknown epilogue code");
     return static_cast<cudeep::kernels::GemmEpilogue>(code);
+}
+
+cudeep::kernels::ElementType as_element_type(int code) {
+    CB200_REQUIRE(code >= 0 && code <= 2, "unknown element type");
+    return static_cast<cudeep::kernels::ElementType>(code);
 }
 
 // Device buffer from the pool, returned on scope exit.
@@ -195,6 +201,49 @@ int cudeep_b200_matmul_f16_tuned(const void* A, const void* B, float* C, int M, 
         CB200_REQUIRE(A != nullptr && B != nullptr && C != nullptr, "gemm: null operand pointer");
         cudeep_b200::gemm_f16(static_cast<const __half*>(A), static_cast<const __half*>(B), C, M, N, K, ctas,
                               b_lbo, b_sbo, as_stream(stream));
+    });
+}
+
+int cudeep_b200_quantize_fp8(const void* x, int x_type, long long rows, int cols, int block_rows, void* q,
+                             float* scales, cudeep_b200_stream_t stream) {
+    return guarded([&] {
+        cudeep::kernels::launch_quantize_fp8(x, as_element_type(x_type), rows, cols,
+                                             static_cast<cudeep::kernels::Fp8Block>(block_rows), q, scales,
+                                             as_stream(stream));
+    });
+}
+
+int cudeep_b200_dequantize_fp8(const void* q, const float* scales, long long rows, int cols, int block_rows,
+                               void* y, int y_type, cudeep_b200_stream_t stream) {
+    return guarded([&] {
+        cudeep::kernels::launch_dequantize_fp8(q, scales, rows, cols,
+                                               static_cast<cudeep::kernels::Fp8Block>(block_rows), y,
+                                               as_element_type(y_type), as_stream(stream));
+    });
+}
+
+int cudeep_b200_grouped_matmul_nt(const void* A, const void* B, void* C, int type, const int32_t* offsets,
+                                  int groups, int rows, int N, int K, cudeep_b200_stream_t stream) {
+    return guarded([&] {
+        cudeep::kernels::launch_grouped_matmul_nt(A, B, C, as_element_type(type), offsets, groups, rows, N, K,
+                                                  as_stream(stream));
+    });
+}
+
+int cudeep_b200_grouped_matmul_nn(const void* A, const void* B, void* C, int type, const int32_t* offsets,
+                                  int groups, int rows, int N, int K, cudeep_b200_stream_t stream) {
+    return guarded([&] {
+        cudeep::kernels::launch_grouped_matmul_nn(A, B, C, as_element_type(type), offsets, groups, rows, N, K,
+                                                  as_stream(stream));
+    });
+}
+
+int cudeep_b200_grouped_matmul_tn(const void* A, const void* B, void* C, int type, int c_type,
+                                  const int32_t* offsets, int groups, int rows, int M, int N,
+                                  cudeep_b200_stream_t stream) {
+    return guarded([&] {
+        cudeep::kernels::launch_grouped_matmul_tn(A, B, C, as_element_type(type), as_element_type(c_type), offsets,
+                                                  groups, rows, M, N, as_stream(stream));
     });
 }
 

@@ -1,0 +1,191 @@
+// Launchers of the ragged products of ragged_gemm.cuh.
+#include "grouped_gemm.h"
+
+#include "ragged_gemm.cuh"
+
+namespace cudeep_b200 {
+
+namespace {
+
+struct RaggedPlan {
+    int ctas;
+    int tile_cols;
+    long long units;      // most tiles there can be, whatever the group sizes
+};
+
+RaggedPlan plan_rows(int groups, int rows, int features) {
+    const int sms = device_info().num_sms;
+    RaggedPlan plan{features <= 128 ? 1 : 2, 256, 0};
+    const long long f_tiles = (features + 128 * plan.ctas - 1) / (128 * plan.ctas);
+    const int used = groups < rows ? groups : rows;
+    for (int tile = 256; tile >= 32; tile /= 2) {
+        plan.tile_cols = tile;
+        // Each group that has rows ends in a partial tile: half a tile on average.
+        const long long expected = f_tiles * (rows / tile + (used + 1) / 2);
+        if (expected * plan.ctas >= sms) break;
+    }
+    const int most = (rows + 31) / 32 * 32;
+    if (plan.tile_cols > most) plan.tile_cols = most;
+    plan.units = f_tiles * (rows / plan.tile_cols + used);
+    return plan;
+}
+
+RaggedPlan plan_weight(int groups, int features, int cols) {
+    const int sms = device_info().num_sms;
+    RaggedPlan plan{features <= 128 ? 1 : 2, 256, 0};
+    const long long f_tiles = (features + 128 * plan.ctas - 1) / (128 * plan.ctas);
+    if (cols <= 128 || groups * f_tiles * ((cols + 255) / 256) * plan.ctas < sms) plan.tile_cols = 128;
+    plan.units = groups * f_tiles * ((cols + plan.tile_cols - 1) / plan.tile_cols);
+    return plan;
+}
+
+template <RaggedForm FORM, int CTAS, bool BF16, class OutT>
+void launch(RaggedParams& p, const RaggedPlan& plan, cudaStream_t stream) {
+    const DeviceInfo& dev = device_info();
+    CB200_REQUIRE(dev.cc_major == 10, "grouped products need an sm_100 device");
+    p.tile_cols = plan.tile_cols;
+    p.stage_bytes = RAGGED_A_BYTES + uint32_t(plan.tile_cols / CTAS) * 128u;
+    const int fit = int(RAGGED_SMEM_BUDGET / p.stage_bytes);
+    p.stages = fit < RAGGED_MAX_STAGES ? fit : RAGGED_MAX_STAGES;
+    p.status = dev.status_word;
+    p.wait_limit_ns = 2000000000ull;
+    long long clusters = dev.num_sms / CTAS;
+    if (clusters > plan.units) clusters = plan.units;
+    const uint32_t smem_bytes = uint32_t(p.stages) * p.stage_bytes + 1024;
+    CB200_TRACE("grouped %s %s tcgen05: rows=%d groups=%d features=%d %s=%d tile=%dx%d stages=%d clusters=%lld",
+                FORM == RaggedForm::NT ? "nt" : FORM == RaggedForm::NN ? "nn" : "tn", BF16 ? "bf16" : "f16", p.rows, p.groups,
+                p.features, FORM == RaggedForm::TN ? "cols" : "k", FORM == RaggedForm::TN ? p.cols : p.k, 128 * CTAS,
+                plan.tile_cols, p.stages, clusters);
+    auto kernel = ragged_gemm_kernel<FORM, CTAS, BF16, OutT>;
+    ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), RAGGED_SMEM_BUDGET + 1024);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(clusters * CTAS), 1, 1);
+    cfg.blockDim = dim3(UMMA_THREADS, 1, 1);
+    cfg.dynamicSmemBytes = smem_bytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    int count = 0;
+    if (CTAS > 1) {
+        attr[count].id = cudaLaunchAttributeClusterDimension;
+        attr[count].val.clusterDim.x = CTAS;
+        attr[count].val.clusterDim.y = 1;
+        attr[count].val.clusterDim.z = 1;
+        ++count;
+    }
+    if (programmatic_launch_enabled()) {
+        attr[count].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[count].val.programmaticStreamSerializationAllowed = 1;
+        ++count;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = unsigned(count);
+    CB200_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
+}
+
+template <RaggedForm FORM>
+void launch_rows(RaggedParams& p, const RaggedPlan& plan, int type, cudaStream_t stream) {
+    if (type == TYPE_BF16) {
+        if (plan.ctas == 2) launch<FORM, 2, true, __nv_bfloat16>(p, plan, stream);
+        else launch<FORM, 1, true, __nv_bfloat16>(p, plan, stream);
+    } else {
+        if (plan.ctas == 2) launch<FORM, 2, false, __half>(p, plan, stream);
+        else launch<FORM, 1, false, __half>(p, plan, stream);
+    }
+}
+
+void rows_by_weight(bool nn, const void* a, const void* w, void* c, int type, const int32_t* offsets, int groups, int rows,
+                    int n, int k, cudaStream_t stream) {
+    const AlignedRows x = aligned_rows(a, rows, k, 2, stream);
+    const int w_cols = nn ? n : k, w_rows = nn ? k : n;
+    const AlignedRows wt = aligned_rows(w, (long long)groups * w_rows, w_cols, 2, stream);
+    RaggedParams p{};
+    {
+        const uint64_t dims[3] = {uint64_t(w_cols), uint64_t(w_rows), uint64_t(groups)};
+        const uint64_t strides[2] = {uint64_t(wt.ld) * 2, uint64_t(wt.ld) * 2 * uint64_t(w_rows)};
+        const uint32_t box[3] = {64, nn ? 64u : 128u, 1};
+        encode_tensor_map_f16(&p.map_a, wt.ptr, 3, dims, strides, box, TmaSwizzle::B128);
+    }
+    {
+        const uint64_t dims[2] = {uint64_t(k), uint64_t(rows)};
+        const uint64_t strides[1] = {uint64_t(x.ld) * 2};
+        const uint32_t box[2] = {64, 128}, box16[2] = {64, 16};
+        encode_tensor_map_f16(&p.map_b, x.ptr, 2, dims, strides, box, TmaSwizzle::B128);
+        encode_tensor_map_f16(&p.map_b16, x.ptr, 2, dims, strides, box16, TmaSwizzle::B128);
+    }
+    p.c = c;
+    p.offsets = offsets;
+    p.groups = groups;
+    p.rows = rows;
+    p.features = n;
+    p.k = k;
+    p.chunk_rows = RAGGED_BK;
+    const RaggedPlan plan = plan_rows(groups, rows, n);
+    if (nn) launch_rows<RaggedForm::NN>(p, plan, type, stream);
+    else launch_rows<RaggedForm::NT>(p, plan, type, stream);
+}
+
+template <int CTAS, bool BF16>
+void launch_weight(RaggedParams& p, const RaggedPlan& plan, int c_type, cudaStream_t stream) {
+    if (c_type == TYPE_F32) launch<RaggedForm::TN, CTAS, BF16, float>(p, plan, stream);
+    else if constexpr (BF16) launch<RaggedForm::TN, CTAS, BF16, __nv_bfloat16>(p, plan, stream);
+    else launch<RaggedForm::TN, CTAS, BF16, __half>(p, plan, stream);
+}
+
+}  // namespace
+
+void grouped_nt(const void* a, const void* w, void* c, int type, const int32_t* offsets, int groups, int rows, int n, int k,
+                cudaStream_t stream) {
+    rows_by_weight(false, a, w, c, type, offsets, groups, rows, n, k, stream);
+}
+
+void grouped_nn(const void* a, const void* w, void* c, int type, const int32_t* offsets, int groups, int rows, int n, int k,
+                cudaStream_t stream) {
+    rows_by_weight(true, a, w, c, type, offsets, groups, rows, n, k, stream);
+}
+
+void grouped_tn(const void* a, long long lda, const void* b, long long ldb, void* c, int type, int c_type,
+                const int32_t* offsets, int groups, int rows, int m, int n, const float* col_scale, cudaStream_t stream) {
+    AlignedRows y, x;
+    if (lda != 0) { y.ptr = a; y.ld = lda; } else y = aligned_rows(a, rows, m, 2, stream);
+    if (ldb != 0) { x.ptr = b; x.ld = ldb; } else x = aligned_rows(b, rows, n, 2, stream);
+    RaggedParams p{};
+    {
+        const uint64_t dims[2] = {uint64_t(m), uint64_t(rows)};
+        const uint64_t strides[1] = {uint64_t(y.ld) * 2};
+        const uint32_t box[2] = {64, 64}, box16[2] = {64, 16};
+        encode_tensor_map_f16(&p.map_a, y.ptr, 2, dims, strides, box, TmaSwizzle::B128);
+        encode_tensor_map_f16(&p.map_a16, y.ptr, 2, dims, strides, box16, TmaSwizzle::B128);
+    }
+    {
+        const uint64_t dims[2] = {uint64_t(n), uint64_t(rows)};
+        const uint64_t strides[1] = {uint64_t(x.ld) * 2};
+        const uint32_t box[2] = {64, 64}, box16[2] = {64, 16};
+        encode_tensor_map_f16(&p.map_b, x.ptr, 2, dims, strides, box, TmaSwizzle::B128);
+        encode_tensor_map_f16(&p.map_b16, x.ptr, 2, dims, strides, box16, TmaSwizzle::B128);
+    }
+    p.a = y.ptr;
+    p.b = x.ptr;
+    p.lda = y.ld;
+    p.ldb = x.ld;
+    p.c = c;
+    p.offsets = offsets;
+    p.groups = groups;
+    p.rows = rows;
+    p.features = m;
+    p.cols = n;
+    p.col_scale = col_scale;
+    // The tensor core's accumulation loses about 2.4e-9 relative per row summed (it truncates), so a gradient in
+    // single precision is summed over 2048 rows at a time, added up with rounding in the epilogue; a 16-bit one
+    // (2e-3 from its own rounding) in one go.
+    p.chunk_rows = c_type == TYPE_F32 ? 2048 : (rows + RAGGED_BK - 1) / RAGGED_BK * RAGGED_BK;
+    const RaggedPlan plan = plan_weight(groups, m, n);
+    if (type == TYPE_BF16) {
+        if (plan.ctas == 2) launch_weight<2, true>(p, plan, c_type, stream);
+        else launch_weight<1, true>(p, plan, c_type, stream);
+    } else {
+        if (plan.ctas == 2) launch_weight<2, false>(p, plan, c_type, stream);
+        else launch_weight<1, false>(p, plan, c_type, stream);
+    }
+}
+
+}  // namespace cudeep_b200

@@ -1,0 +1,30 @@
+// One-pass kernels around the 8-bit and the grouped products (see lowp_rows.cu).
+#pragma once
+
+#include "runtime.h"
+
+namespace cudeep_b200 {
+
+// Element types of the low-precision entry points; values equal CUDEEP_B200_TYPE_*.
+enum ElemType : int { TYPE_F32 = 0, TYPE_F16 = 1, TYPE_BF16 = 2 };
+inline int elem_bytes(int type) { return type == TYPE_F32 ? 4 : 2; }
+
+constexpr int FP8_BLOCK = 128;      // elements along a row that share a scale
+
+// A row-major matrix whose rows the TMA unit can read: 16-byte aligned, rows of 16-byte multiples.
+struct AlignedRows {
+    const void* ptr = nullptr;
+    long long ld = 0;      // elements between rows
+    Scratch copy;          // holds ptr where the caller's matrix had to be copied
+};
+// The caller's matrix itself where it qualifies, else a copy with zero-padded rows.
+AlignedRows aligned_rows(const void* src, long long rows, int cols, int elem_size, cudaStream_t stream);
+
+// q = e4m3(x / s), s a power of two for each block of 128 columns and block_rows (1 or 128) rows.
+void quantize_fp8(const void* x, int x_type, long long rows, int cols, int block_rows, uint8_t* q, float* scales,
+                  cudaStream_t stream);
+// y = q * s.
+void dequantize_fp8(const uint8_t* q, const float* scales, long long rows, int cols, int block_rows, void* y, int y_type,
+                    cudaStream_t stream);
+
+}  // namespace cudeep_b200

@@ -1,0 +1,495 @@
+// Products of ragged row groups with a weight per group, 16-bit operands, FP32 accumulation (tcgen05 kind::f16).
+//
+// Rows [offsets[g], offsets[g+1]) of a [rows, ...] matrix form group g.  Three products, with W[g] as Linear stores it:
+//   NT  C[r, f] = sum_k X[r, k] W[g][f, k]        forward
+//   NN  C[r, f] = sum_k X[r, k] W[g][k, f]        gradient of the rows
+//   TN  C[g][f, c] = sum_{r in g} Y[r, f] X[r, c]  gradient of the weight
+//
+// The group sizes are known on the device only, so every CTA (or CTA pair) reads the offsets, makes the running
+// count of tiles and walks its share of them; the grid never depends on the sizes and nothing is read back.
+//
+// NT and NN put the FEATURES on the accumulator's 128 (256 for a pair) lanes and the ROWS of the group on its
+// columns.  The number of columns of one MMA is free (any multiple of 16 per CTA), so a group's ragged end costs at most
+// 31 columns and a group of a few rows costs a narrow MMA, where lanes come in 128s only.  Rows behind a group's
+// end that fall into its last columns are computed and not stored: they cannot reach another row's result.
+//
+// TN sums over the rows, so a row behind the group's end must not be multiplied at all (a zero on one side does not
+// do: 0 * Inf = NaN).  MMAs run for whole steps of 16 rows; the last step of a group, if it is partial, is brought
+// by the producer warp itself with ordinary loads that replace rows behind the end by zeros in both operands.
+#pragma once
+
+#include "runtime.h"
+#include "sm100_ptx.cuh"
+#include "umma_gemm.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace cudeep_b200 {
+
+enum class RaggedForm { NT, NN, TN };
+
+constexpr int RAGGED_MAX_GROUPS = 1024;
+constexpr int RAGGED_BK = 64;                        // 16-bit elements per K block = one 128-byte swizzle row
+constexpr uint32_t RAGGED_A_BYTES = 128 * 128;       // one CTA's features of a K block
+constexpr int RAGGED_MAX_STAGES = 12;
+constexpr uint32_t RAGGED_SMEM_BUDGET = 232448 - 1024 - 13 * 1024;   // minus alignment slack, group tables and barriers
+constexpr uint32_t UMMA_BAD_OFFSETS = 6;             // status word: the offsets decrease or leave [0, rows]
+
+struct RaggedParams {
+    CUtensorMap map_a;       // NT {K, F, G} box {64, 128, 1}; NN {F, K, G} box {64, 64, 1}; TN {F, rows} box {64, 64}
+    CUtensorMap map_a16;     // TN: {F, rows} box {64, 16}
+    CUtensorMap map_b;       // NT, NN {K, rows} box {64, 128}; TN {C, rows} box {64, 64}
+    CUtensorMap map_b16;     // NT, NN {K, rows} box {64, 16};  TN {C, rows} box {64, 16}
+    const void* a;           // TN: the operands' addresses and row lengths, for the partial last step
+    const void* b;
+    long long lda, ldb;
+    void* c;
+    const int32_t* offsets;  // [groups + 1], or nullptr: one group of all rows
+    int groups;
+    int rows;                // rows of X (and of Y)
+    int features;            // F
+    int cols;                // TN: C
+    int k;                   // NT, NN: length of the sums
+    int tile_cols;           // columns of a tile at most: rows of a group (NT, NN) or C (TN); <= 256
+    int stages;
+    uint32_t stage_bytes;
+    int chunk_rows;          // TN: rows summed in the tensor core's accumulator before they are added into C
+    const float* col_scale;  // TN: nullptr, or a factor for each 128 columns of C
+    uint32_t* status;
+    unsigned long long wait_limit_ns;
+};
+
+// One tile: which group, its first feature and column, how many columns, and what it sums over.
+struct RaggedTile {
+    int group;
+    int feature0;      // of the whole CTA group
+    int col0;          // NT, NN: first row of X; TN: first column of C
+    int col_count;     // real columns
+    int umma_n;        // columns of the MMA
+    int row0, row1;    // TN: rows of the group
+};
+
+template <RaggedForm FORM, int CTAS>
+struct RaggedWalk {
+    const int* off;
+    const int* start;
+    int groups, f_tiles, c_tiles_tn, tile_cols, features, cols;
+    int g = 0;
+
+    __device__ __forceinline__ int total() const { return start[groups]; }
+    __device__ __forceinline__ RaggedTile at(int u) {
+        while (u >= start[g + 1]) ++g;
+        RaggedTile t;
+        t.group = g;
+        t.row0 = off[2 * g];
+        t.row1 = off[2 * g + 1];
+        const int in_group = u - start[g];
+        int ct, ft;
+        if (FORM == RaggedForm::TN) {
+            raster_coords(in_group, f_tiles, c_tiles_tn, 8, ft, ct);
+            t.col0 = ct * tile_cols;
+            t.col_count = min(tile_cols, cols - t.col0);
+            t.umma_n = tile_cols;
+        } else {
+            // Equal shares of the group's rows, so that no tile of it is much shorter than the others.
+            const int size = t.row1 - t.row0;
+            const int c_tiles = (size + tile_cols - 1) / tile_cols;
+            constexpr int unit = 16 * CTAS;
+            const int share = ((size + c_tiles - 1) / c_tiles + unit - 1) / unit * unit;
+            raster_coords(in_group, c_tiles, f_tiles, 8, ct, ft);
+            t.col0 = t.row0 + ct * share;
+            t.col_count = min(share, t.row1 - t.col0);
+            t.umma_n = max(unit, (t.col_count + unit - 1) / unit * unit);
+        }
+        t.feature0 = ft * 128 * CTAS;
+        return t;
+    }
+};
+
+template <class T>
+__device__ __forceinline__ T round_to(float v);
+template <>
+__device__ __forceinline__ float round_to<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half round_to<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 round_to<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+template <RaggedForm FORM, int CTAS, bool BF16, class OutT>
+__global__ void __launch_bounds__(UMMA_THREADS, 1) ragged_gemm_kernel(const __grid_constant__ RaggedParams p) {
+#if defined(__CUDA_ARCH_FEAT_SM100_ALL) || defined(__CUDA_ARCH_FEAT_SM101_ALL) || \
+    defined(__CUDA_ARCH_FEAT_SM103_ALL)
+    constexpr bool A_MN = FORM != RaggedForm::NT;
+    constexpr bool B_MN = FORM == RaggedForm::TN;
+    // TN over a pair: the partner may have written operand rows with ordinary stores before it arrived.
+    constexpr bool FULL_CLUSTER = FORM == RaggedForm::TN && CTAS == 2;
+
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t bar_full[RAGGED_MAX_STAGES];
+    __shared__ __align__(8) uint64_t bar_empty[RAGGED_MAX_STAGES];
+    __shared__ __align__(8) uint64_t bar_acc_full[2];
+    __shared__ __align__(8) uint64_t bar_acc_empty[2];
+    __shared__ uint32_t tmem_base_holder;
+    __shared__ uint32_t abort_flag;
+    __shared__ int group_rows[2 * RAGGED_MAX_GROUPS];      // first and last row of each group
+    __shared__ int group_start[RAGGED_MAX_GROUPS + 1];     // tiles before each group
+
+    const uint32_t warp = threadIdx.x >> 5;
+    const uint32_t lane = threadIdx.x & 31;
+    const uint32_t cta_rank = CTAS == 2 ? ptx::cluster_ctarank() : 0u;
+    const bool is_leader = cta_rank == 0;
+    const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
+    ptx::WaitCtx wctx{&abort_flag, p.status, p.wait_limit_ns};
+
+    if (threadIdx.x == 0) {
+        abort_flag = 0;
+        ptx::prefetch_tensormap(&p.map_a);
+        ptx::prefetch_tensormap(&p.map_b);
+        ptx::prefetch_tensormap(&p.map_b16);
+        for (int s = 0; s < RAGGED_MAX_STAGES; ++s) {
+            ptx::mbar_init(ptx::smem_u32(&bar_full[s]), CTAS);      // each CTA's producer arrives with its bytes
+            ptx::mbar_init(ptx::smem_u32(&bar_empty[s]), 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            ptx::mbar_init(ptx::smem_u32(&bar_acc_full[a]), 1);
+            ptx::mbar_init(ptx::smem_u32(&bar_acc_empty[a]), 4 * CTAS);
+        }
+        ptx::fence_mbar_init();
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc<CTAS>(ptx::smem_u32(&tmem_base_holder), 512);
+        ptx::tmem_relinquish<CTAS>();
+    }
+    ptx::grid_dependency_wait();      // the offsets may come from the kernel before
+    const int f_tiles = (p.features + 128 * CTAS - 1) / (128 * CTAS);
+    const int c_tiles_tn = FORM == RaggedForm::TN ? (p.cols + p.tile_cols - 1) / p.tile_cols : 0;
+    if (warp == 0) {
+        int carry = 0;
+        bool bad = false;
+        for (int base = 0; base < p.groups; base += 32) {
+            const int g = base + int(lane);
+            int lo = 0, hi = 0;
+            if (g < p.groups) {
+                hi = p.rows;
+                if (p.offsets != nullptr) {
+                    lo = __ldg(p.offsets + g);
+                    hi = __ldg(p.offsets + g + 1);
+                }
+                const int lo_in = min(max(lo, 0), p.rows), hi_in = min(max(hi, lo_in), p.rows);
+                bad = bad || lo_in != lo || hi_in != hi;      // nothing is read or written outside the matrices
+                lo = lo_in;
+                hi = hi_in;
+                group_rows[2 * g] = lo;
+                group_rows[2 * g + 1] = hi;
+            }
+            int tiles = 0;
+            if (g < p.groups)
+                tiles = FORM == RaggedForm::TN ? f_tiles * c_tiles_tn
+                                               : f_tiles * ((hi - lo + p.tile_cols - 1) / p.tile_cols);
+            int sum = tiles;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int other = __shfl_up_sync(0xffffffffu, sum, d);
+                if (int(lane) >= d) sum += other;
+            }
+            if (g < p.groups) group_start[g + 1] = carry + sum;
+            carry += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        if (lane == 0) group_start[0] = 0;
+        if (__any_sync(0xffffffffu, bad) && lane == 0) atomicCAS(p.status, 0u, UMMA_BAD_OFFSETS);
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    if (CTAS == 2) {
+        ptx::cluster_arrive();
+        ptx::cluster_wait();
+    }
+    ptx::tc_fence_after();
+    const uint32_t tmem_base = tmem_base_holder;
+    ptx::grid_launch_dependents();
+
+    const int unit_stride = gridDim.x / CTAS;
+    const int first_unit = blockIdx.x / CTAS;
+    RaggedWalk<FORM, CTAS> walk{group_rows, group_start, p.groups, f_tiles, c_tiles_tn, p.tile_cols, p.features, p.cols};
+    const int num_units = walk.total();
+    const int k_blocks_row = FORM == RaggedForm::TN ? 0 : (p.k + RAGGED_BK - 1) / RAGGED_BK;
+    // TN: blocks of a chunk of the group's rows that starts at `row`.
+    auto chunk_blocks = [&](const RaggedTile& t, int row) {
+        return (min(p.chunk_rows, t.row1 - row) + RAGGED_BK - 1) / RAGGED_BK;
+    };
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ producer
+        uint32_t stage = 0, phase = 0;
+        for (int u = first_unit; u < num_units; u += unit_stride) {
+            const RaggedTile t = walk.at(u);
+            const int per = t.umma_n / CTAS;                               // columns this CTA stages
+            const int feature = t.feature0 + int(cta_rank) * 128;
+            const int col = t.col0 + int(cta_rank) * per;
+            const int blocks = FORM == RaggedForm::TN ? (t.row1 - t.row0 + RAGGED_BK - 1) / RAGGED_BK : k_blocks_row;
+            for (int kb = 0; kb < blocks; ++kb) {
+                const bool ok = ptx::mbar_wait(ptx::smem_u32(&bar_empty[stage]), phase ^ 1u, wctx, UMMA_TIMEOUT_PRODUCER);
+                if (!__all_sync(0xffffffffu, ok)) goto producer_done;
+                const uint32_t a_smem = smem_base + stage * p.stage_bytes;
+                const uint32_t b_smem = a_smem + RAGGED_A_BYTES;
+                const uint32_t full_local = ptx::smem_u32(&bar_full[stage]);
+                const uint32_t full = CTAS == 2 ? ptx::mapa(full_local, 0) : full_local;
+                uint32_t bytes;
+                if constexpr (FORM != RaggedForm::TN) {
+                    bytes = RAGGED_A_BYTES + uint32_t(per) * 128u;
+                    if (lane == 0) {
+                        const int k0 = kb * RAGGED_BK;
+                        if constexpr (FORM == RaggedForm::NT) {
+                            if constexpr (CTAS == 2) ptx::tma_load_3d_pair(a_smem, &p.map_a, full, k0, feature, t.group);
+                            else ptx::tma_load_3d(a_smem, &p.map_a, full, k0, feature, t.group);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+                                if constexpr (CTAS == 2)
+                                    ptx::tma_load_3d_pair(a_smem + j * 8192, &p.map_a, full, feature + j * 64, k0, t.group);
+                                else
+                                    ptx::tma_load_3d(a_smem + j * 8192, &p.map_a, full, feature + j * 64, k0, t.group);
+                            }
+                        }
+                        for (int r = 0; r < per;) {
+                            const bool big = per - r >= 128;
+                            const CUtensorMap* map = big ? &p.map_b : &p.map_b16;
+                            if constexpr (CTAS == 2) ptx::tma_load_2d_pair(b_smem + r * 128, map, full, k0, col + r);
+                            else ptx::tma_load_2d(b_smem + r * 128, map, full, k0, col + r);
+                            r += big ? 128 : 16;
+                        }
+                    }
+                } else {
+                    const int row = t.row0 + kb * RAGGED_BK;
+                    const int have = t.row1 - row;                         // rows of the group from here on
+                    const bool whole = have >= RAGGED_BK;
+                    const int steps = whole ? 4 : have / 16;               // whole steps of 16 rows
+                    const int chunks = per / 64;
+                    bytes = uint32_t(steps) * 2048u * uint32_t(2 + chunks);
+                    if (lane == 0) {
+                        const CUtensorMap* ma = whole ? &p.map_a : &p.map_a16;
+                        const CUtensorMap* mb = whole ? &p.map_b : &p.map_b16;
+                        const int boxes = whole ? 1 : steps;
+                        for (int s = 0; s < boxes; ++s) {
+                            for (int j = 0; j < 2; ++j) {
+                                const uint32_t dst = a_smem + j * 8192 + s * 2048;
+                                if constexpr (CTAS == 2) ptx::tma_load_2d_pair(dst, ma, full, feature + j * 64, row + s * 16);
+                                else ptx::tma_load_2d(dst, ma, full, feature + j * 64, row + s * 16);
+                            }
+                            for (int j = 0; j < chunks; ++j) {
+                                const uint32_t dst = b_smem + j * 8192 + s * 2048;
+                                if constexpr (CTAS == 2) ptx::tma_load_2d_pair(dst, mb, full, col + j * 64, row + s * 16);
+                                else ptx::tma_load_2d(dst, mb, full, col + j * 64, row + s * 16);
+                            }
+                        }
+                    }
+                    if (!whole && have % 16 != 0) {
+                        // The partial step: 16 rows x (128 + per) columns in 16-byte units, a unit per lane and turn.
+                        const int row_s = row + steps * 16;
+                        const int units_row = 16 + per / 8;
+                        for (int i = int(lane); i < 16 * units_row; i += 32) {
+                            const int r = i / units_row, q = i - r * units_row;
+                            const bool of_a = q < 16;
+                            const int e = (of_a ? q : q - 16) * 8;          // first element within the CTA's columns
+                            const int x = (of_a ? feature : col) + e;
+                            uint4 v = make_uint4(0, 0, 0, 0);
+                            if (row_s + r < t.row1 && x < (of_a ? p.features : p.cols)) {
+                                const uint16_t* src = static_cast<const uint16_t*>(of_a ? p.a : p.b);
+                                v = __ldg(reinterpret_cast<const uint4*>(src + (long long)(row_s + r) * (of_a ? p.lda : p.ldb) + x));
+                            }
+                            const int k_row = steps * 16 + r;              // 128-byte swizzle: unit c of row r at c ^ (r & 7)
+                            const uint32_t dst = (of_a ? a_smem : b_smem) + uint32_t(e / 64) * 8192u + uint32_t(k_row) * 128u +
+                                                 ((uint32_t(e / 8) & 7u) ^ (uint32_t(k_row) & 7u)) * 16u;
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z),
+                                         "r"(v.w) : "memory");
+                        }
+                        ptx::fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                }
+                if (lane == 0) {
+                    if (CTAS == 2) ptx::mbar_arrive_expect_tx_cluster(full, bytes);
+                    else ptx::mbar_arrive_expect_tx(full_local, bytes);
+                }
+                __syncwarp();
+                if (++stage == uint32_t(p.stages)) { stage = 0; phase ^= 1u; }
+            }
+        }
+    producer_done:
+        __syncwarp();
+        if (CTAS == 2) ptx::cluster_arrive();
+    } else if (warp == 1) {
+        // ------------------------------------------------------------ MMA issuer
+        if (is_leader) {
+            constexpr uint32_t KSTEP_MN = 2048u, KSTEP_K = 32u;
+            const uint64_t a_desc0 = ptx::smem_desc_at(
+                A_MN ? ptx::smem_desc(8192, 1024, ptx::SMEM_LAYOUT_SW128) : ptx::smem_desc(16, 1024, ptx::SMEM_LAYOUT_SW128),
+                smem_base);
+            const uint64_t b_desc0 = ptx::smem_desc_at(
+                B_MN ? ptx::smem_desc(8192, 1024, ptx::SMEM_LAYOUT_SW128) : ptx::smem_desc(16, 1024, ptx::SMEM_LAYOUT_SW128),
+                smem_base + RAGGED_A_BYTES);
+            uint32_t stage = 0, phase = 0;
+            int it = 0;      // accumulators handed over
+            for (int u = first_unit; u < num_units; u += unit_stride) {
+                const RaggedTile t = walk.at(u);
+                const uint32_t idesc = ptx::idesc_f16(128 * CTAS, t.umma_n, A_MN ? 1 : 0, B_MN ? 1 : 0, BF16 ? 1 : 0);
+                int row = t.row0;
+                do {
+                    const int blocks = FORM == RaggedForm::TN ? chunk_blocks(t, row) : k_blocks_row;
+                    if (blocks <= 0) break;
+                    const uint32_t acc = it & 1;
+                    const uint32_t acc_phase = (it >> 1) & 1;
+                    if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&bar_acc_empty[acc]), acc_phase ^ 1u, wctx,
+                                                                UMMA_TIMEOUT_MMA_ACC)))
+                        goto mma_done;
+                    ptx::tc_fence_after();
+                    const uint32_t d_tmem = tmem_base + acc * 256u;
+                    bool ready = __all_sync(0xffffffffu, ptx::mbar_test<FULL_CLUSTER>(ptx::smem_u32(&bar_full[stage]), phase));
+                    for (int kb = 0; kb < blocks; ++kb) {
+                        if (!ready &&
+                            !__all_sync(0xffffffffu, ptx::mbar_wait<FULL_CLUSTER>(ptx::smem_u32(&bar_full[stage]), phase, wctx,
+                                                                                  UMMA_TIMEOUT_MMA_FULL)))
+                            goto mma_done;
+                        ptx::tc_fence_after();
+                        uint32_t next_stage = stage + 1, next_phase = phase;
+                        if (next_stage == uint32_t(p.stages)) { next_stage = 0; next_phase ^= 1u; }
+                        ready = __all_sync(0xffffffffu, ptx::mbar_test<FULL_CLUSTER>(ptx::smem_u32(&bar_full[next_stage]), next_phase));
+                        int steps = 4;
+                        if (FORM == RaggedForm::TN) steps = min(4, (t.row1 - row - kb * RAGGED_BK + 15) / 16);
+                        if (ptx::elect_one()) {
+                            const uint64_t a_stage = a_desc0 + ((stage * p.stage_bytes) >> 4);
+                            const uint64_t b_stage = b_desc0 + ((stage * p.stage_bytes) >> 4);
+#pragma unroll
+                            for (int kk = 0; kk < 4; ++kk)
+                                if (kk < steps)
+                                    ptx::umma_f16<CTAS>(d_tmem, a_stage + ((kk * (A_MN ? KSTEP_MN : KSTEP_K)) >> 4),
+                                                        b_stage + ((kk * (B_MN ? KSTEP_MN : KSTEP_K)) >> 4), idesc,
+                                                        (kb | kk) != 0);
+                            const uint32_t empty_local = ptx::smem_u32(&bar_empty[stage]);
+                            ptx::umma_commit<CTAS>(empty_local);
+                            if constexpr (CTAS == 2) ptx::umma_commit<CTAS>(ptx::mapa(empty_local, 1));
+                            if (kb + 1 == blocks) {
+                                const uint32_t accf_local = ptx::smem_u32(&bar_acc_full[acc]);
+                                ptx::umma_commit<CTAS>(accf_local);
+                                if constexpr (CTAS == 2) ptx::umma_commit<CTAS>(ptx::mapa(accf_local, 1));
+                            }
+                        }
+                        __syncwarp();
+                        stage = next_stage;
+                        phase = next_phase;
+                    }
+                    ++it;
+                    row += p.chunk_rows;
+                } while (FORM == RaggedForm::TN && row < t.row1);
+            }
+        }
+    mma_done:
+        __syncwarp();
+        if (CTAS == 2) ptx::cluster_arrive();
+    } else {
+        // ------------------------------------------------------------ epilogue
+        const uint32_t quarter = warp & 3u;
+        int it = 0;
+        for (int u = first_unit; u < num_units; u += unit_stride) {
+            const RaggedTile t = walk.at(u);
+            const int feature = t.feature0 + int(cta_rank) * 128 + int(quarter) * 32 + int(lane);
+            if constexpr (FORM == RaggedForm::TN) {
+                OutT* dst_row = static_cast<OutT*>(p.c) + ((long long)t.group * p.features + feature) * p.cols + t.col0;
+                int row = t.row0;
+                do {
+                    const bool any = chunk_blocks(t, row) > 0;       // an empty group's gradient is zero
+                    const uint32_t acc = it & 1;
+                    if (any) {
+                        const bool ok = ptx::mbar_wait(ptx::smem_u32(&bar_acc_full[acc]), (it >> 1) & 1, wctx, UMMA_TIMEOUT_EPILOGUE);
+                        if (!__all_sync(0xffffffffu, ok)) goto epilogue_done;
+                        ptx::tc_fence_after();
+                    }
+                    const uint32_t t_row = tmem_base + acc * 256u + ((quarter * 32u) << 16);
+                    for (int c = 0; c < t.col_count; c += 32) {
+                        uint32_t r[32];
+                        if (any) {
+                            ptx::tmem_ld_32x32(t_row + c, r);
+                            ptx::tmem_ld_wait();
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) r[j] = 0u;
+                        }
+                        if (feature < p.features) {
+                            const float scale = p.col_scale != nullptr ? __ldg(p.col_scale + (t.col0 + c) / 128) : 1.0f;
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) {
+                                if (c + j < t.col_count) {
+                                    float v = __uint_as_float(r[j]) * scale;
+                                    if constexpr (sizeof(OutT) == 4)
+                                        if (row != t.row0) v += float(dst_row[c + j]);
+                                    dst_row[c + j] = round_to<OutT>(v);
+                                }
+                            }
+                        }
+                    }
+                    if (any) {
+                        ptx::tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) {
+                            const uint32_t e = ptx::smem_u32(&bar_acc_empty[acc]);
+                            if constexpr (CTAS == 2) ptx::mbar_arrive_cluster(ptx::mapa(e, 0));
+                            else ptx::mbar_arrive(e);
+                        }
+                        ++it;
+                    }
+                    row += p.chunk_rows;
+                } while (row < t.row1);
+            } else {
+                const uint32_t acc = it & 1;
+                const bool ok = ptx::mbar_wait(ptx::smem_u32(&bar_acc_full[acc]), (it >> 1) & 1, wctx, UMMA_TIMEOUT_EPILOGUE);
+                if (!__all_sync(0xffffffffu, ok)) goto epilogue_done;
+                ptx::tc_fence_after();
+                const uint32_t t_row = tmem_base + acc * 256u + ((quarter * 32u) << 16);
+                OutT* dst = static_cast<OutT*>(p.c) + (long long)t.col0 * p.features + feature;
+                for (int c = 0; c < t.col_count; c += 32) {
+                    uint32_t r[32];
+                    ptx::tmem_ld_32x32(t_row + c, r);
+                    ptx::tmem_ld_wait();
+                    if (feature < p.features) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (c + j < t.col_count)
+                                dst[(long long)(c + j) * p.features] = round_to<OutT>(__uint_as_float(r[j]));
+                    }
+                }
+                ptx::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    const uint32_t e = ptx::smem_u32(&bar_acc_empty[acc]);
+                    if constexpr (CTAS == 2) ptx::mbar_arrive_cluster(ptx::mapa(e, 0));
+                    else ptx::mbar_arrive(e);
+                }
+                ++it;
+            }
+        }
+    epilogue_done:
+        __syncwarp();
+        if (CTAS == 2) ptx::cluster_arrive();
+    }
+
+    // ---------------------------------------------------------------- teardown
+    ptx::tc_fence_before();
+    __syncthreads();
+    if (abort_flag) {
+        // A wait ran out: copies still in flight get a bounded time to land before the shared memory goes.
+        const uint64_t t0 = ptx::globaltimer_ns();
+        while (ptx::globaltimer_ns() - t0 < 2000000ull) { }
+        __syncthreads();
+    }
+    if (CTAS == 2) ptx::cluster_wait();
+    if (warp == 1) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc<CTAS>(tmem_base, 512);
+    }
+#else
+    if (threadIdx.x == 0 && blockIdx.x == 0) atomicCAS(p.status, 0u, 0xdeadu);
+#endif
+}
+
+}  // namespace cudeep_b200

@@ -220,4 +220,9 @@ void encode_tensor_map_f16(CUtensorMap* map, const void* base, int rank, const u
     encode_map(map, base, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, rank, dims, strides_bytes, box, swizzle, nullptr);
 }
 
+void encode_tensor_map_u8(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
+                          const uint64_t* strides_bytes, const uint32_t* box, TmaSwizzle swizzle) {
+    encode_map(map, base, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, rank, dims, strides_bytes, box, swizzle, nullptr);
+}
+
 }  // namespace cudeep_b200

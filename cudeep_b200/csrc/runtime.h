@@ -62,6 +62,27 @@ void* scratch_alloc(size_t bytes, cudaStream_t stream);
 void scratch_free(void* ptr, cudaStream_t stream) noexcept;
 void scratch_trim(size_t keep_bytes);
 
+// One temporary of a launcher, given back (in stream order) when it goes out of scope.
+struct Scratch {
+    void* ptr = nullptr;
+    cudaStream_t stream = nullptr;
+    Scratch() = default;
+    Scratch(size_t bytes, cudaStream_t s) : ptr(scratch_alloc(bytes, s)), stream(s) {}
+    Scratch(Scratch&& o) noexcept : ptr(o.ptr), stream(o.stream) { o.ptr = nullptr; }
+    Scratch& operator=(Scratch&& o) noexcept {
+        if (this != &o) {
+            scratch_free(ptr, stream);
+            ptr = o.ptr;
+            stream = o.stream;
+            o.ptr = nullptr;
+        }
+        return *this;
+    }
+    Scratch(const Scratch&) = delete;
+    Scratch& operator=(const Scratch&) = delete;
+    ~Scratch() { scratch_free(ptr, stream); }
+};
+
 // Read-and-clear the current device's kernel status word (synchronises the device).
 uint32_t read_device_status(bool clear);
 
@@ -79,6 +100,9 @@ enum class TmaSwizzle {
 // The same for 2-byte (FP16) elements: dims, boxes and coordinates count elements.
 void encode_tensor_map_f16(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
                            const uint64_t* strides_bytes, const uint32_t* box, TmaSwizzle swizzle);
+// And for 1-byte elements.
+void encode_tensor_map_u8(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
+                          const uint64_t* strides_bytes, const uint32_t* box, TmaSwizzle swizzle);
 // element_strides (optional, one per dimension): traverse dimension i in steps of that many
 // elements; box[i] then is the extent traversed (a multiple of the step) and box[i] / step
 // elements are loaded.

@@ -1,0 +1,33 @@
+// Launchers of the low-precision and grouped products (additions: the reference has no counterpart).
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "cudeep/kernels/matmul.cuh"
+
+namespace cudeep {
+namespace kernels {
+
+// Element types of the operands that are passed as void pointers.
+enum class ElementType : int { F32 = 0, F16 = 1, BF16 = 2 };
+
+// Blocks of an 8-bit matrix that share a scale: 128 columns of one row (activations), or 128 rows x 128 columns
+// (weights).  Scales lie [column block][row] and [row block][column block].
+enum class Fp8Block : int { Row = 1, Tile = 128 };
+
+void launch_quantize_fp8(const void* x, ElementType type, long long rows, int cols, Fp8Block block, void* q, float* scales,
+                         cudaStream_t stream = nullptr);
+void launch_dequantize_fp8(const void* q, const float* scales, long long rows, int cols, Fp8Block block, void* y,
+                           ElementType type, cudaStream_t stream = nullptr);
+
+// Products of ragged row groups; `offsets` (device) holds groups + 1 ascending row numbers in [0, rows].
+void launch_grouped_matmul_nt(const void* A, const void* B, void* C, ElementType type, const int32_t* offsets, int groups,
+                              int rows, int N, int K, cudaStream_t stream = nullptr);
+void launch_grouped_matmul_nn(const void* A, const void* B, void* C, ElementType type, const int32_t* offsets, int groups,
+                              int rows, int N, int K, cudaStream_t stream = nullptr);
+void launch_grouped_matmul_tn(const void* A, const void* B, void* C, ElementType type, ElementType c_type,
+                              const int32_t* offsets, int groups, int rows, int M, int N, cudaStream_t stream = nullptr);
+
+}  // namespace kernels
+}  // namespace cudeep

@@ -144,6 +144,50 @@ int cudeep_b200_gemm_tf32_tuned(const float* A, const float* B, int b_is_nk, flo
                                 int bn, int raster_group, int max_ctas, uint32_t b_lbo,
                                 uint32_t b_sbo, cudeep_b200_stream_t stream);
 
+/* ---- 8-bit and grouped products (device pointers) ---------------------------------------- */
+
+/* No counterpart in the reference: the products of low-precision Linear layers and of layers whose
+ * rows are split among experts.  All matrices are row-major and contiguous; any base address that
+ * suits its element type and any row length is taken (rows that are not 16-byte multiples are first
+ * copied to a padded temporary).  Zero rows are a valid size. */
+
+/* Element types of the operands passed as void pointers. */
+#define CUDEEP_B200_TYPE_F32 0
+#define CUDEEP_B200_TYPE_F16 1
+#define CUDEEP_B200_TYPE_BF16 2
+
+/* q[rows, cols] = x / scale in 8-bit floating point (e4m3: 4 exponent bits, 3 of mantissa, largest
+ * 448, no infinities), rounded to nearest even, with one scale for each block of 128 columns and
+ * block_rows = 1 (activations) or 128 (weights) rows:
+ *   block_rows 1:   scales[ceil(cols / 128)][rows]      (column block by column block)
+ *   block_rows 128: scales[ceil(rows / 128)][ceil(cols / 128)]
+ * A scale is the least power of two, 2^-126 at least, under which the block's largest finite
+ * magnitude is at most 448 (1 for a block of zeros), so q * scale has no error but q's own rounding.
+ * Infinities and NaN become NaN and do not enter the scale. */
+int cudeep_b200_quantize_fp8(const void* x, int x_type, long long rows, int cols, int block_rows, void* q,
+                             float* scales, cudeep_b200_stream_t stream);
+/* y = q * scale. */
+int cudeep_b200_dequantize_fp8(const void* q, const float* scales, long long rows, int cols,
+                               int block_rows, void* y, int y_type, cudeep_b200_stream_t stream);
+
+/* Products of row groups of any sizes, each group with a matrix of its own.  Group g is the rows
+ * [offsets[g], offsets[g + 1]); `offsets` is a DEVICE array of groups + 1 ascending row numbers in
+ * [0, rows], read by the kernel, so sizes may come from the kernel before and are never copied to
+ * the host.  A group may be empty.  1 to 1024 groups.  type: F16 or BF16; sums are FP32.
+ *   nt: C[r, N] = A[r, K] * B[g][N, K]^T     (forward of Linear layers)
+ *   nn: C[r, N] = A[r, K] * B[g][K, N]       (gradient of the rows)
+ *   tn: C[g][M, N] = A_g[., M]^T * B_g[., N] (gradient of the matrices; zeros for an empty group)
+ * nt and nn leave rows of C outside all groups as they are.  C has the operands' type; tn's C may be
+ * F32 as well.  Offsets that decrease or leave [0, rows] give unspecified rows of C (nothing outside
+ * the matrices is touched) and set cudeep_b200_device_status() to 6. */
+int cudeep_b200_grouped_matmul_nt(const void* A, const void* B, void* C, int type, const int32_t* offsets,
+                                  int groups, int rows, int N, int K, cudeep_b200_stream_t stream);
+int cudeep_b200_grouped_matmul_nn(const void* A, const void* B, void* C, int type, const int32_t* offsets,
+                                  int groups, int rows, int N, int K, cudeep_b200_stream_t stream);
+int cudeep_b200_grouped_matmul_tn(const void* A, const void* B, void* C, int type, int c_type,
+                                  const int32_t* offsets, int groups, int rows, int M, int N,
+                                  cudeep_b200_stream_t stream);
+
 /* ---- conv2d forward (device pointers) -------------------------------------------------- */
 
 /* output[N,OC,OH,OW] = conv(input[N,C,H,W], weight[OC,C,KH,KW]) + bias[OC]
