@@ -71,6 +71,10 @@ PROTOTYPES = {
                                          _stream]),
     "cudeep_b200_dequantize_fp8": (c_int, [c_void_p, c_void_p, ctypes.c_longlong, c_int, c_int, c_void_p, c_int,
                                            _stream]),
+    "cudeep_b200_linear_forward_fp8": (c_int, [_fp] * 6 + [c_int] * 5 + [_stream]),
+    "cudeep_b200_linear_backward_data_fp8": (c_int, [_fp] * 5 + [c_int] * 4 + [_stream]),
+    "cudeep_b200_linear_backward_saved_fp8": (c_int, [_fp, c_int, _fp, _fp, _fp, _fp, c_int, _fp, _fp, _fp, c_int, _fp,
+                                                      c_int, c_int, c_int, _stream]),
     "cudeep_b200_grouped_matmul_nt": (c_int, [_fp, _fp, _fp, c_int, c_void_p, c_int, c_int, c_int, c_int, _stream]),
     "cudeep_b200_grouped_matmul_nn": (c_int, [_fp, _fp, _fp, c_int, c_void_p, c_int, c_int, c_int, c_int, _stream]),
     "cudeep_b200_grouped_matmul_tn": (c_int, [_fp, _fp, _fp, c_int, c_int, c_void_p, c_int, c_int, c_int, c_int,

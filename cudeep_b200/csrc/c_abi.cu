@@ -222,6 +222,34 @@ int cudeep_b200_dequantize_fp8(const void* q, const float* scales, long long row
     });
 }
 
+int cudeep_b200_linear_forward_fp8(const void* x, const float* x_scales, const void* W, const float* w_scales,
+                                   const float* bias, void* y, int y_type, int M, int N, int K, int epilogue,
+                                   cudeep_b200_stream_t stream) {
+    return guarded([&] {
+        cudeep::kernels::launch_linear_forward_fp8(x, x_scales, W, w_scales, bias, y, as_element_type(y_type), M, N, K,
+                                                   as_epilogue(epilogue), as_stream(stream));
+    });
+}
+
+int cudeep_b200_linear_backward_data_fp8(const void* dy, const float* dy_scales, const void* W, const float* w_scales,
+                                         void* dx, int dx_type, int M, int N, int K, cudeep_b200_stream_t stream) {
+    return guarded([&] {
+        cudeep::kernels::launch_linear_backward_data_fp8(dy, dy_scales, W, w_scales, dx, as_element_type(dx_type), M, N,
+                                                         K, as_stream(stream));
+    });
+}
+
+int cudeep_b200_linear_backward_saved_fp8(const void* dy, int type, const void* x8, const float* x_scales,
+                                          const void* z8, const float* z_scales, int epilogue, const void* W, void* dx,
+                                          void* dw, int dw_type, float* db, int M, int N, int K,
+                                          cudeep_b200_stream_t stream) {
+    return guarded([&] {
+        cudeep::kernels::launch_linear_backward_saved_fp8(dy, as_element_type(type), x8, x_scales, z8, z_scales,
+                                                          as_epilogue(epilogue), W, dx, dw, as_element_type(dw_type), db,
+                                                          M, N, K, as_stream(stream));
+    });
+}
+
 int cudeep_b200_grouped_matmul_nt(const void* A, const void* B, void* C, int type, const int32_t* offsets,
                                   int groups, int rows, int N, int K, cudeep_b200_stream_t stream) {
     return guarded([&] {

@@ -2,33 +2,11 @@
 #include "grouped_gemm.h"
 
 #include "ragged_gemm.cuh"
+#include "ragged_plan.h"
 
 namespace cudeep_b200 {
 
 namespace {
-
-struct RaggedPlan {
-    int ctas;
-    int tile_cols;
-    long long units;      // most tiles there can be, whatever the group sizes
-};
-
-RaggedPlan plan_rows(int groups, int rows, int features) {
-    const int sms = device_info().num_sms;
-    RaggedPlan plan{features <= 128 ? 1 : 2, 256, 0};
-    const long long f_tiles = (features + 128 * plan.ctas - 1) / (128 * plan.ctas);
-    const int used = groups < rows ? groups : rows;
-    for (int tile = 256; tile >= 32; tile /= 2) {
-        plan.tile_cols = tile;
-        // Each group that has rows ends in a partial tile: half a tile on average.
-        const long long expected = f_tiles * (rows / tile + (used + 1) / 2);
-        if (expected * plan.ctas >= sms) break;
-    }
-    const int most = (rows + 31) / 32 * 32;
-    if (plan.tile_cols > most) plan.tile_cols = most;
-    plan.units = f_tiles * (rows / plan.tile_cols + used);
-    return plan;
-}
 
 RaggedPlan plan_weight(int groups, int features, int cols) {
     const int sms = device_info().num_sms;
@@ -56,30 +34,8 @@ void launch(RaggedParams& p, const RaggedPlan& plan, cudaStream_t stream) {
                 FORM == RaggedForm::NT ? "nt" : FORM == RaggedForm::NN ? "nn" : "tn", BF16 ? "bf16" : "f16", p.rows, p.groups,
                 p.features, FORM == RaggedForm::TN ? "cols" : "k", FORM == RaggedForm::TN ? p.cols : p.k, 128 * CTAS,
                 plan.tile_cols, p.stages, clusters);
-    auto kernel = ragged_gemm_kernel<FORM, CTAS, BF16, OutT>;
-    ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), RAGGED_SMEM_BUDGET + 1024);
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(unsigned(clusters * CTAS), 1, 1);
-    cfg.blockDim = dim3(UMMA_THREADS, 1, 1);
-    cfg.dynamicSmemBytes = smem_bytes;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    int count = 0;
-    if (CTAS > 1) {
-        attr[count].id = cudaLaunchAttributeClusterDimension;
-        attr[count].val.clusterDim.x = CTAS;
-        attr[count].val.clusterDim.y = 1;
-        attr[count].val.clusterDim.z = 1;
-        ++count;
-    }
-    if (programmatic_launch_enabled()) {
-        attr[count].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[count].val.programmaticStreamSerializationAllowed = 1;
-        ++count;
-    }
-    cfg.attrs = attr;
-    cfg.numAttrs = unsigned(count);
-    CB200_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
+    launch_clusters(ragged_gemm_kernel<FORM, CTAS, BF16, OutT>, p, clusters, CTAS, UMMA_THREADS, smem_bytes,
+                    RAGGED_SMEM_BUDGET + 1024, stream);
 }
 
 template <RaggedForm FORM>
@@ -93,9 +49,17 @@ void launch_rows(RaggedParams& p, const RaggedPlan& plan, int type, cudaStream_t
     }
 }
 
-void rows_by_weight(bool nn, const void* a, const void* w, void* c, int type, const int32_t* offsets, int groups, int rows,
+AlignedRows rows_of(const void* src, long long ld, int rows, int cols, cudaStream_t stream) {
+    if (ld == 0) return aligned_rows(src, rows, cols, 2, stream);
+    AlignedRows out;
+    out.ptr = src;
+    out.ld = ld;
+    return out;
+}
+
+void rows_by_weight(bool nn, const void* a, long long lda, const void* w, void* c, int type, const int32_t* offsets, int groups, int rows,
                     int n, int k, cudaStream_t stream) {
-    const AlignedRows x = aligned_rows(a, rows, k, 2, stream);
+    const AlignedRows x = rows_of(a, lda, rows, k, stream);
     const int w_cols = nn ? n : k, w_rows = nn ? k : n;
     const AlignedRows wt = aligned_rows(w, (long long)groups * w_rows, w_cols, 2, stream);
     RaggedParams p{};
@@ -135,19 +99,18 @@ void launch_weight(RaggedParams& p, const RaggedPlan& plan, int c_type, cudaStre
 
 void grouped_nt(const void* a, const void* w, void* c, int type, const int32_t* offsets, int groups, int rows, int n, int k,
                 cudaStream_t stream) {
-    rows_by_weight(false, a, w, c, type, offsets, groups, rows, n, k, stream);
+    rows_by_weight(false, a, 0, w, c, type, offsets, groups, rows, n, k, stream);
 }
 
-void grouped_nn(const void* a, const void* w, void* c, int type, const int32_t* offsets, int groups, int rows, int n, int k,
-                cudaStream_t stream) {
-    rows_by_weight(true, a, w, c, type, offsets, groups, rows, n, k, stream);
+void grouped_nn(const void* a, long long lda, const void* w, void* c, int type, const int32_t* offsets, int groups, int rows,
+                int n, int k, cudaStream_t stream) {
+    rows_by_weight(true, a, lda, w, c, type, offsets, groups, rows, n, k, stream);
 }
 
 void grouped_tn(const void* a, long long lda, const void* b, long long ldb, void* c, int type, int c_type,
                 const int32_t* offsets, int groups, int rows, int m, int n, const float* col_scale, cudaStream_t stream) {
-    AlignedRows y, x;
-    if (lda != 0) { y.ptr = a; y.ld = lda; } else y = aligned_rows(a, rows, m, 2, stream);
-    if (ldb != 0) { x.ptr = b; x.ld = ldb; } else x = aligned_rows(b, rows, n, 2, stream);
+    const AlignedRows y = rows_of(a, lda, rows, m, stream);
+    const AlignedRows x = rows_of(b, ldb, rows, n, stream);
     RaggedParams p{};
     {
         const uint64_t dims[2] = {uint64_t(m), uint64_t(rows)};

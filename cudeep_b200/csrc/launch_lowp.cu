@@ -1,6 +1,8 @@
 // cudeep::kernels launchers of the low-precision and grouped products: argument checks.
 #include "cudeep/kernels/lowp.cuh"
 
+#include "epilogue_math.cuh"
+#include "fp8_gemm.h"
 #include "grouped_gemm.h"
 #include "lowp_rows.h"
 
@@ -38,6 +40,12 @@ void check_grouped(const void* a, const void* b, const void* c, const int32_t* o
     check_element_address(a, 2, "A");
     check_element_address(b, 2, "B");
     check_element_address(offsets, 4, "offsets");
+}
+
+int checked_epilogue(GemmEpilogue epilogue) {
+    const int act = static_cast<int>(epilogue);
+    CB200_REQUIRE(act >= 0 && act <= 4, "unknown epilogue code");
+    return act;
 }
 
 }  // namespace
@@ -79,7 +87,7 @@ void launch_grouped_matmul_nn(const void* A, const void* B, void* C, ElementType
     check_grouped(A, B, C, offsets, groups, rows, N, K);
     check_element_address(C, 2, "C");
     if (rows == 0) return;
-    cudeep_b200::grouped_nn(A, B, C, t, offsets, groups, rows, N, K, stream);
+    cudeep_b200::grouped_nn(A, 0, B, C, t, offsets, groups, rows, N, K, stream);
 }
 
 void launch_grouped_matmul_tn(const void* A, const void* B, void* C, ElementType type, ElementType c_type,
@@ -93,6 +101,95 @@ void launch_grouped_matmul_tn(const void* A, const void* B, void* C, ElementType
         return;
     }
     cudeep_b200::grouped_tn(A, 0, B, 0, C, t, ct, offsets, groups, rows, M, N, nullptr, stream);
+}
+
+void launch_linear_forward_fp8(const void* x, const float* x_scales, const void* W, const float* w_scales, const float* bias,
+                               void* y, ElementType y_type, int M, int N, int K, GemmEpilogue epilogue, cudaStream_t stream) {
+    const int t = checked_type(y_type), act = checked_epilogue(epilogue);
+    CB200_REQUIRE(x != nullptr && x_scales != nullptr && W != nullptr && w_scales != nullptr && y != nullptr,
+                  "linear_fp8: null pointer");
+    CB200_REQUIRE(M >= 0 && N > 0 && K > 0, "linear_fp8: M must not be negative, N and K positive");
+    check_element_address(y, cudeep_b200::elem_bytes(t), "y");
+    check_element_address(x_scales, 4, "x_scales");
+    check_element_address(w_scales, 4, "w_scales");
+    check_element_address(bias, 4, "bias");
+    if (M == 0) return;
+    cudeep_b200::fp8_nt(static_cast<const uint8_t*>(x), x_scales, static_cast<const uint8_t*>(W), w_scales, bias, y, t, M, N, K,
+                        act, stream);
+}
+
+void launch_linear_backward_data_fp8(const void* dy, const float* dy_scales, const void* W, const float* w_scales, void* dx,
+                                     ElementType dx_type, int M, int N, int K, cudaStream_t stream) {
+    const int t = checked_type(dx_type);
+    CB200_REQUIRE(dy != nullptr && dy_scales != nullptr && W != nullptr && w_scales != nullptr && dx != nullptr,
+                  "linear_fp8: null pointer");
+    CB200_REQUIRE(M >= 0 && N > 0 && K > 0, "linear_fp8: M must not be negative, N and K positive");
+    check_element_address(dx, cudeep_b200::elem_bytes(t), "dx");
+    check_element_address(dy_scales, 4, "dy_scales");
+    check_element_address(w_scales, 4, "w_scales");
+    if (M == 0) return;
+    cudeep_b200::fp8_nn(static_cast<const uint8_t*>(dy), dy_scales, static_cast<const uint8_t*>(W), w_scales, dx, t, M, N, K,
+                        stream);
+}
+
+void launch_linear_backward_saved_fp8(const void* dy, ElementType type, const void* x8, const float* x_scales, const void* z8,
+                                      const float* z_scales, GemmEpilogue epilogue, const void* W, void* dx, void* dw,
+                                      ElementType dw_type, float* db, int M, int N, int K, cudaStream_t stream) {
+    using namespace cudeep_b200;
+    const int t = checked_half_type(type), act = checked_epilogue(epilogue);
+    CB200_REQUIRE(dy != nullptr, "linear_backward_saved: null dy");
+    CB200_REQUIRE(dx != nullptr || dw != nullptr || db != nullptr, "linear_backward_saved: no gradient asked for");
+    CB200_REQUIRE(dx == nullptr || W != nullptr, "linear_backward_saved: dx needs W");
+    CB200_REQUIRE(dw == nullptr || (x8 != nullptr && x_scales != nullptr), "linear_backward_saved: dw needs x8 and its scales");
+    CB200_REQUIRE(act == EPI_NONE || (z8 != nullptr && z_scales != nullptr),
+                  "linear_backward_saved: an activation needs z8 and its scales");
+    CB200_REQUIRE(M >= 0 && N > 0 && K > 0, "linear_backward_saved: M must not be negative, N and K positive");
+    const int wt = dw != nullptr ? checked_type(dw_type) : t;
+    CB200_REQUIRE(wt == t || wt == TYPE_F32, "linear_backward_saved: dw is F32 or of dy's type");
+    check_element_address(dy, 2, "dy");
+    check_element_address(W, 2, "W");
+    check_element_address(dx, 2, "dx");
+    check_element_address(dw, elem_bytes(wt), "dw");
+    check_element_address(db, 4, "db");
+    check_element_address(x_scales, 4, "x_scales");
+    check_element_address(z_scales, 4, "z_scales");
+    if (M == 0) {
+        if (dw != nullptr) CB200_CUDA(cudaMemsetAsync(dw, 0, size_t(N) * K * elem_bytes(wt), stream));
+        if (db != nullptr) CB200_CUDA(cudaMemsetAsync(db, 0, size_t(N) * sizeof(float), stream));
+        return;
+    }
+    // dz goes to the tensor cores in dy's type: both products take it as an operand next to 16-bit W and x.  db is summed
+    // from its FP32 values.
+    const void* dz = dy;
+    long long ld_dz = 0;      // contiguous, of any row length
+    Scratch dz_buf;
+    if (act != EPI_NONE) {
+        if (dx != nullptr || dw != nullptr) {
+            ld_dz = (N + 7) / 8 * 8;
+            dz_buf = Scratch(size_t(M) * ld_dz * 2, stream);
+            dz = dz_buf.ptr;
+        }
+        activation_backward_fp8(dy, t, static_cast<const uint8_t*>(z8), z_scales, act, dz_buf.ptr, ld_dz, db, M, N, stream);
+    } else if (db != nullptr) {
+        activation_backward_fp8(dy, t, nullptr, nullptr, act, nullptr, 0, db, M, N, stream);
+    }
+    if (dx != nullptr) grouped_nn(dz, ld_dz, W, dx, t, nullptr, 1, M, K, N, stream);
+    if (dw != nullptr) {
+        // x as a 16-bit operand.  q * s is exact in BF16 for the power-of-two scales of quantize_fp8; FP16 has too few
+        // exponents for that, so there each column block is taken relative to its largest scale (products below
+        // 2^-24 of that are lost) and the result is multiplied by it.
+        const long long ld_x = (K + 7) / 8 * 8;
+        Scratch x_buf(size_t(M) * ld_x * 2, stream);
+        Scratch top_buf;
+        float* top = nullptr;
+        if (t == TYPE_F16) {
+            top_buf = Scratch(size_t((K + FP8_BLOCK - 1) / FP8_BLOCK) * sizeof(float), stream);
+            top = static_cast<float*>(top_buf.ptr);
+            block_tops(x_scales, M, K, top, stream);
+        }
+        dequantize_rows(static_cast<const uint8_t*>(x8), x_scales, top, M, K, x_buf.ptr, ld_x, t, stream);
+        grouped_tn(dz, ld_dz, x_buf.ptr, ld_x, dw, t, wt, nullptr, 1, M, N, K, top, stream);
+    }
 }
 
 }  // namespace kernels

@@ -2,6 +2,8 @@
 // in blocks and back.  All are bound by HBM: each input is read once and each output written once.
 #include "lowp_rows.h"
 
+#include "epilogue_math.cuh"
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -219,6 +221,162 @@ __global__ void dequantize_kernel(const uint8_t* __restrict__ q, const float* __
     }
 }
 
+// Slope of the epilogue activations (tanh-form GELU) from CUDA's own expf and tanhf: the pass is bound by HBM, so the
+// accurate functions cost nothing.
+__device__ __forceinline__ float act_slope(float z, int act) {
+    if (act == EPI_RELU) return z > 0.0f ? 1.0f : 0.0f;
+    if (act == EPI_GELU) {
+        // Beyond +-30 the slope is 0 or 1 to the last bit, and z * z * z must not overflow.
+        z = fminf(fmaxf(z, -30.0f), 30.0f);
+        const float c = 0.7978845608028654f;
+        const float th = tanhf(c * (z + 0.044715f * z * z * z));
+        return 0.5f * (1.0f + th) + 0.5f * z * (1.0f - th * th) * c * (1.0f + 3.0f * 0.044715f * z * z);
+    }
+    if (act == EPI_NONE) return 1.0f;
+    const float s = 1.0f / (1.0f + expf(-z));
+    if (act == EPI_SIGMOID) return s * (1.0f - s);
+    return s > 0.0f ? s * (1.0f + z * (1.0f - s)) : 0.0f;
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
+    alignas(16) T t[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[j] = from_float<T>(v[j]);
+    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(t);
+}
+
+// A CTA takes 256 columns and `rows_per` rows: 32 threads with eight columns each lie along a row, eight rows are worked on at
+// once.  Column sums stay in registers over the rows, are added across the eight threads of a column in a fixed order and go
+// to partial[row band][cols], which one more kernel adds up, again in order: the result does not depend on timing.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kThreads) act_backward_kernel(const T* __restrict__ dy, const uint8_t* __restrict__ z8,
+                                                                const float* __restrict__ zs, int act, T* __restrict__ dz,
+                                                                long long ld_dz, float* __restrict__ partial, int rows, int cols,
+                                                                int rows_per) {
+    __shared__ float s_sum[8][264];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int c0 = blockIdx.x * 256 + tx * 8;
+    const int r_end = min(rows, int(blockIdx.y + 1) * rows_per);
+    float sum[8] = {};
+    if (c0 < cols) {
+        const float* s_col = zs + (long long)(c0 / FP8_BLOCK) * rows;
+        for (int r = blockIdx.y * rows_per + ty; r < r_end; r += 8) {
+            const long long at = (long long)r * cols + c0;
+            float g[8];
+            if (VEC) {
+                load8(dy + at, g);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) g[j] = c0 + j < cols ? to_float(dy[at + j]) : 0.0f;
+            }
+            if (act != EPI_NONE) {
+                uint8_t q[8];
+                if (VEC) {
+                    *reinterpret_cast<uint2*>(q) = __ldg(reinterpret_cast<const uint2*>(z8 + at));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) q[j] = c0 + j < cols ? z8[at + j] : uint8_t(0);
+                }
+                const float s = __ldg(s_col + r);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) g[j] *= act_slope(e4m3_value(q[j]) * s, act);
+            }
+            if (!VEC) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (c0 + j >= cols) g[j] = 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum[j] += g[j];
+            if (dz != nullptr) store8(dz + r * ld_dz + c0, g);
+        }
+    }
+    if (partial == nullptr) return;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s_sum[ty][tx * 8 + j] = sum[j];
+    __syncthreads();
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c < cols) {
+        float total = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) total += s_sum[i][threadIdx.x];
+        partial[(long long)blockIdx.y * cols + c] = total;
+    }
+}
+
+__global__ void __launch_bounds__(kThreads) add_bands_kernel(const float* __restrict__ partial, int bands, int cols,
+                                                             float* __restrict__ out) {
+    const int c = blockIdx.x * kThreads + threadIdx.x;
+    if (c >= cols) return;
+    float total = 0.0f;
+    for (int b = 0; b < bands; ++b) total += partial[(long long)b * cols + c];
+    out[c] = total;
+}
+
+__global__ void __launch_bounds__(kThreads) block_tops_kernel(const float* __restrict__ scales, int rows, float* __restrict__ top) {
+    __shared__ float s_max[kThreads / 32];
+    float m = 0.0f;
+    for (int r = threadIdx.x; r < rows; r += kThreads) m = fmaxf(m, finite_abs(__ldg(scales + (long long)blockIdx.x * rows + r)));
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) m = fmaxf(m, s_max[w]);
+    if (threadIdx.x == 0) top[blockIdx.x] = m > 0.0f ? m : 1.0f;
+}
+
+// Eight elements per thread; the padding behind cols is written as zeros.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kThreads) dequantize_rows_kernel(const uint8_t* __restrict__ q, const float* __restrict__ scales,
+                                                                   const float* __restrict__ top, int rows, int cols,
+                                                                   T* __restrict__ y, long long ld_y) {
+    const int units = int(ld_y / 8);
+    const long long total = (long long)rows * units;
+    for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
+        const long long r = i / units;
+        const int c0 = int(i - r * units) * 8;
+        const int b = c0 / FP8_BLOCK;
+        float s = __ldg(scales + (long long)b * rows + r);
+        if (top != nullptr) s /= __ldg(top + b);
+        uint8_t v[8];
+        if (VEC) {
+            *reinterpret_cast<uint2*>(v) = __ldg(reinterpret_cast<const uint2*>(q + r * cols + c0));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = c0 + j < cols ? q[r * cols + c0 + j] : uint8_t(0);
+        }
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = e4m3_value(v[j]) * s;
+        store8(y + i * 8, f);
+    }
+}
+
+template <typename T>
+void act_backward_typed(const T* dy, const uint8_t* z8, const float* z_scales, int act, T* dz, long long ld_dz, float* db,
+                        int rows, int cols, cudaStream_t stream) {
+    const bool vec = cols % 8 == 0 && reinterpret_cast<uintptr_t>(dy) % 16 == 0 && reinterpret_cast<uintptr_t>(z8) % 8 == 0;
+    const int rows_per = rows > 2048 ? 128 : 32;
+    const int bands = (rows + rows_per - 1) / rows_per;
+    CB200_REQUIRE(bands <= 65535, "too many rows");
+    Scratch partial;
+    float* to = db;
+    if (db != nullptr && bands > 1) {
+        partial = Scratch(size_t(bands) * cols * sizeof(float), stream);
+        to = static_cast<float*>(partial.ptr);
+    }
+    const dim3 grid((cols + 255) / 256, bands);
+    if (vec) act_backward_kernel<T, true><<<grid, kThreads, 0, stream>>>(dy, z8, z_scales, act, dz, ld_dz, to, rows, cols, rows_per);
+    else act_backward_kernel<T, false><<<grid, kThreads, 0, stream>>>(dy, z8, z_scales, act, dz, ld_dz, to, rows, cols, rows_per);
+    CB200_CHECK_LAUNCH();
+    if (to != db) {
+        add_bands_kernel<<<(cols + kThreads - 1) / kThreads, kThreads, 0, stream>>>(to, bands, cols, db);
+        CB200_CHECK_LAUNCH();
+    }
+}
+
 unsigned pass_grid(long long items) {
     const long long most = 16ll * device_info().num_sms;
     const long long want = (items + kThreads - 1) / kThreads;
@@ -286,6 +444,37 @@ void dequantize_fp8(const uint8_t* q, const float* scales, long long rows, int c
         dequantize_kernel<<<grid, kThreads, 0, stream>>>(q, scales, rows, cols, block_rows, static_cast<__half*>(y));
     else
         dequantize_kernel<<<grid, kThreads, 0, stream>>>(q, scales, rows, cols, block_rows, static_cast<__nv_bfloat16*>(y));
+    CB200_CHECK_LAUNCH();
+}
+
+void activation_backward_fp8(const void* dy, int type, const uint8_t* z8, const float* z_scales, int act, void* dz,
+                             long long ld_dz, float* db, int rows, int cols, cudaStream_t stream) {
+    if (type == TYPE_F16)
+        act_backward_typed(static_cast<const __half*>(dy), z8, z_scales, act, static_cast<__half*>(dz), ld_dz, db, rows, cols,
+                           stream);
+    else
+        act_backward_typed(static_cast<const __nv_bfloat16*>(dy), z8, z_scales, act, static_cast<__nv_bfloat16*>(dz), ld_dz, db,
+                           rows, cols, stream);
+}
+
+void block_tops(const float* scales, int rows, int cols, float* top, cudaStream_t stream) {
+    block_tops_kernel<<<(cols + FP8_BLOCK - 1) / FP8_BLOCK, kThreads, 0, stream>>>(scales, rows, top);
+    CB200_CHECK_LAUNCH();
+}
+
+void dequantize_rows(const uint8_t* q, const float* scales, const float* top, int rows, int cols, void* y, long long ld_y,
+                     int y_type, cudaStream_t stream) {
+    const bool vec = cols % 8 == 0 && reinterpret_cast<uintptr_t>(q) % 8 == 0;
+    const unsigned grid = pass_grid(rows * (ld_y / 8));
+    if (y_type == TYPE_F16) {
+        __half* out = static_cast<__half*>(y);
+        if (vec) dequantize_rows_kernel<__half, true><<<grid, kThreads, 0, stream>>>(q, scales, top, rows, cols, out, ld_y);
+        else dequantize_rows_kernel<__half, false><<<grid, kThreads, 0, stream>>>(q, scales, top, rows, cols, out, ld_y);
+    } else {
+        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(y);
+        if (vec) dequantize_rows_kernel<__nv_bfloat16, true><<<grid, kThreads, 0, stream>>>(q, scales, top, rows, cols, out, ld_y);
+        else dequantize_rows_kernel<__nv_bfloat16, false><<<grid, kThreads, 0, stream>>>(q, scales, top, rows, cols, out, ld_y);
+    }
     CB200_CHECK_LAUNCH();
 }
 

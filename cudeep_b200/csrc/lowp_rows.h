@@ -27,4 +27,15 @@ void quantize_fp8(const void* x, int x_type, long long rows, int cols, int block
 void dequantize_fp8(const uint8_t* q, const float* scales, long long rows, int cols, int block_rows, void* y, int y_type,
                     cudaStream_t stream);
 
+
+// dz = dy * act'(z8 * z_scales), rounded to dy's type, rows ld_dz elements apart (zeros behind cols); dz may be nullptr.
+// db[cols] = column sums of dz before its rounding; db may be nullptr.  type: TYPE_F16 or TYPE_BF16.
+void activation_backward_fp8(const void* dy, int type, const uint8_t* z8, const float* z_scales, int act, void* dz,
+                             long long ld_dz, float* db, int rows, int cols, cudaStream_t stream);
+// y = q * (s / top[b]) in a 16-bit type, rows ld_y elements apart, for blocks of 1 x 128; top[b] = the largest finite
+// scale of column block b.  With top == nullptr: y = q * s.
+void block_tops(const float* scales, int rows, int cols, float* top, cudaStream_t stream);
+void dequantize_rows(const uint8_t* q, const float* scales, const float* top, int rows, int cols, void* y, long long ld_y,
+                     int y_type, cudaStream_t stream);
+
 }  // namespace cudeep_b200

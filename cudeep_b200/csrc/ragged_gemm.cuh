@@ -107,6 +107,41 @@ struct RaggedWalk {
     }
 };
 
+// One warp: the row range of each group, brought into [0, rows], and the number of tiles before it.  col_tiles >= 0:
+// column tiles of every group (TN); otherwise -col_tiles is the number of a group's rows that a tile takes.
+__device__ __forceinline__ void group_tables(const int32_t* offsets, int groups, int rows, int f_tiles, int col_tiles,
+                                             int* group_rows, int* group_start, uint32_t* status) {
+    const int lane = int(threadIdx.x & 31);
+    int carry = 0;
+    bool bad = false;
+    for (int base = 0; base < groups; base += 32) {
+        const int g = base + lane;
+        int tiles = 0;
+        if (g < groups) {
+            int lo = 0, hi = rows;
+            if (offsets != nullptr) {
+                lo = __ldg(offsets + g);
+                hi = __ldg(offsets + g + 1);
+            }
+            const int lo_in = min(max(lo, 0), rows), hi_in = min(max(hi, lo_in), rows);
+            bad = bad || lo_in != lo || hi_in != hi;      // nothing is read or written outside the matrices
+            group_rows[2 * g] = lo_in;
+            group_rows[2 * g + 1] = hi_in;
+            tiles = f_tiles * (col_tiles >= 0 ? col_tiles : (hi_in - lo_in - col_tiles - 1) / -col_tiles);
+        }
+        int sum = tiles;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int other = __shfl_up_sync(0xffffffffu, sum, d);
+            if (lane >= d) sum += other;
+        }
+        if (g < groups) group_start[g + 1] = carry + sum;
+        carry += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (lane == 0) group_start[0] = 0;
+    if (__any_sync(0xffffffffu, bad) && lane == 0) atomicCAS(status, 0u, UMMA_BAD_OFFSETS);
+}
+
 template <class T>
 __device__ __forceinline__ T round_to(float v);
 template <>
@@ -164,41 +199,9 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) ragged_gemm_kernel(const __gr
     ptx::grid_dependency_wait();      // the offsets may come from the kernel before
     const int f_tiles = (p.features + 128 * CTAS - 1) / (128 * CTAS);
     const int c_tiles_tn = FORM == RaggedForm::TN ? (p.cols + p.tile_cols - 1) / p.tile_cols : 0;
-    if (warp == 0) {
-        int carry = 0;
-        bool bad = false;
-        for (int base = 0; base < p.groups; base += 32) {
-            const int g = base + int(lane);
-            int lo = 0, hi = 0;
-            if (g < p.groups) {
-                hi = p.rows;
-                if (p.offsets != nullptr) {
-                    lo = __ldg(p.offsets + g);
-                    hi = __ldg(p.offsets + g + 1);
-                }
-                const int lo_in = min(max(lo, 0), p.rows), hi_in = min(max(hi, lo_in), p.rows);
-                bad = bad || lo_in != lo || hi_in != hi;      // nothing is read or written outside the matrices
-                lo = lo_in;
-                hi = hi_in;
-                group_rows[2 * g] = lo;
-                group_rows[2 * g + 1] = hi;
-            }
-            int tiles = 0;
-            if (g < p.groups)
-                tiles = FORM == RaggedForm::TN ? f_tiles * c_tiles_tn
-                                               : f_tiles * ((hi - lo + p.tile_cols - 1) / p.tile_cols);
-            int sum = tiles;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const int other = __shfl_up_sync(0xffffffffu, sum, d);
-                if (int(lane) >= d) sum += other;
-            }
-            if (g < p.groups) group_start[g + 1] = carry + sum;
-            carry += __shfl_sync(0xffffffffu, sum, 31);
-        }
-        if (lane == 0) group_start[0] = 0;
-        if (__any_sync(0xffffffffu, bad) && lane == 0) atomicCAS(p.status, 0u, UMMA_BAD_OFFSETS);
-    }
+    if (warp == 0)
+        group_tables(p.offsets, p.groups, p.rows, f_tiles, FORM == RaggedForm::TN ? c_tiles_tn : -p.tile_cols, group_rows,
+                     group_start, p.status);
     ptx::tc_fence_before();
     __syncthreads();
     if (CTAS == 2) {

@@ -170,6 +170,29 @@ int cudeep_b200_quantize_fp8(const void* x, int x_type, long long rows, int cols
 int cudeep_b200_dequantize_fp8(const void* q, const float* scales, long long rows, int cols,
                                int block_rows, void* y, int y_type, cudeep_b200_stream_t stream);
 
+/* y[M,N] = act(x[M,K] * W[N,K]^T + bias[N]) with x and W in 8 bits, x with blocks of 1 x 128 and W
+ * with blocks of 128 x 128 as cudeep_b200_quantize_fp8 lays them out (any finite scales are taken,
+ * not only powers of two).  Each block of 128 products is summed by the tensor cores, the scaled
+ * blocks are added in FP32.  bias (FP32) may be NULL; y_type: any of the three. */
+int cudeep_b200_linear_forward_fp8(const void* x, const float* x_scales, const void* W,
+                                   const float* w_scales, const float* bias, void* y, int y_type, int M,
+                                   int N, int K, int epilogue, cudeep_b200_stream_t stream);
+/* dx[M,K] = dy[M,N] * W[N,K]: dy with blocks of 1 x 128 along N, the same W and scales as forward. */
+int cudeep_b200_linear_backward_data_fp8(const void* dy, const float* dy_scales, const void* W,
+                                         const float* w_scales, void* dx, int dx_type, int M, int N, int K,
+                                         cudeep_b200_stream_t stream);
+
+/* Backward pass of y = act(z), z = x * W^T + bias, from x and z that were kept in 8 bits (blocks of
+ * 1 x 128) instead of 16: with dz = dy * act'(z),
+ *   dx[M,K] = dz * W,   dw[N,K] = dz^T * x,   db[N] = column sums of dz (FP32).
+ * type is that of dy, W and dx, F16 or BF16; dw has it or is F32.  dx, dw and db may each be NULL, and
+ * then so may what only they need; z8 is not read without an activation.  dz is rounded to `type`
+ * before the products, db is not. */
+int cudeep_b200_linear_backward_saved_fp8(const void* dy, int type, const void* x8, const float* x_scales,
+                                          const void* z8, const float* z_scales, int epilogue,
+                                          const void* W, void* dx, void* dw, int dw_type, float* db, int M,
+                                          int N, int K, cudeep_b200_stream_t stream);
+
 /* Products of row groups of any sizes, each group with a matrix of its own.  Group g is the rows
  * [offsets[g], offsets[g + 1]); `offsets` is a DEVICE array of groups + 1 ascending row numbers in
  * [0, rows], read by the kernel, so sizes may come from the kernel before and are never copied to
