@@ -138,8 +138,8 @@ __global__ void __launch_bounds__(FP8_THREADS, 1) fp8_gemm_kernel(const __grid_c
                     const uint32_t b_smem = a_smem + RAGGED_A_BYTES;
                     const uint32_t full_local = ptx::smem_u32(&bar_full[stage]);
                     const uint32_t full = CTAS == 2 ? ptx::mapa(full_local, 0) : full_local;
-                    if (CTAS == 2) ptx::mbar_arrive_expect_tx_cluster(full, bytes);
-                    else ptx::mbar_arrive_expect_tx(full_local, bytes);
+                    if (is_leader) ptx::mbar_arrive_expect_tx(full_local, bytes);
+                    else ptx::mbar_arrive_expect_tx_cluster_relaxed(full, bytes);
                     const int k0 = kb * FP8_BK;
                     const int ax = A_MN ? feature : k0, ay = A_MN ? k0 : feature;
                     if constexpr (CTAS == 2) ptx::tma_load_3d_pair(a_smem, &p.map_a, full, ax, ay, t.group);
@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(FP8_THREADS, 1) fp8_gemm_kernel(const __grid_c
                 __syncwarp();
                 if (lane == 0) {
                     const uint32_t e = ptx::smem_u32(&bar_acc_empty[buf]);
-                    if constexpr (CTAS == 2) ptx::mbar_arrive_cluster(ptx::mapa(e, 0));
+                    if (CTAS == 2 && !is_leader) ptx::mbar_arrive_cluster_relaxed(ptx::mapa(e, 0));
                     else ptx::mbar_arrive(e);
                 }
             }

@@ -239,6 +239,7 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) ragged_gemm_kernel(const __gr
                 const uint32_t full_local = ptx::smem_u32(&bar_full[stage]);
                 const uint32_t full = CTAS == 2 ? ptx::mapa(full_local, 0) : full_local;
                 uint32_t bytes;
+                bool stored = false;      // this stage holds rows written with ordinary stores
                 if constexpr (FORM != RaggedForm::TN) {
                     bytes = RAGGED_A_BYTES + uint32_t(per) * 128u;
                     if (lane == 0) {
@@ -309,11 +310,13 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) ragged_gemm_kernel(const __gr
                         }
                         ptx::fence_proxy_async_smem();
                         __syncwarp();
+                        stored = true;
                     }
                 }
                 if (lane == 0) {
-                    if (CTAS == 2) ptx::mbar_arrive_expect_tx_cluster(full, bytes);
-                    else ptx::mbar_arrive_expect_tx(full_local, bytes);
+                    if (is_leader) ptx::mbar_arrive_expect_tx(full_local, bytes);
+                    else if (stored) ptx::mbar_arrive_expect_tx_cluster(full, bytes);
+                    else ptx::mbar_arrive_expect_tx_cluster_relaxed(full, bytes);
                 }
                 __syncwarp();
                 if (++stage == uint32_t(p.stages)) { stage = 0; phase ^= 1u; }
@@ -436,7 +439,7 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) ragged_gemm_kernel(const __gr
                         __syncwarp();
                         if (lane == 0) {
                             const uint32_t e = ptx::smem_u32(&bar_acc_empty[acc]);
-                            if constexpr (CTAS == 2) ptx::mbar_arrive_cluster(ptx::mapa(e, 0));
+                            if (CTAS == 2 && !is_leader) ptx::mbar_arrive_cluster_relaxed(ptx::mapa(e, 0));
                             else ptx::mbar_arrive(e);
                         }
                         ++it;
@@ -465,7 +468,7 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) ragged_gemm_kernel(const __gr
                 __syncwarp();
                 if (lane == 0) {
                     const uint32_t e = ptx::smem_u32(&bar_acc_empty[acc]);
-                    if constexpr (CTAS == 2) ptx::mbar_arrive_cluster(ptx::mapa(e, 0));
+                    if (CTAS == 2 && !is_leader) ptx::mbar_arrive_cluster_relaxed(ptx::mapa(e, 0));
                     else ptx::mbar_arrive(e);
                 }
                 ++it;

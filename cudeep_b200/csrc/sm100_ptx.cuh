@@ -114,9 +114,20 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar)
                  : "memory");
 }
-// The same with the transaction bytes this CTA will deliver there.
+// The same without ordering this thread's memory operations before it.  A release at cluster scope waits for a round trip of
+// what the thread has in flight, about 1900 cycles on a busy SM: too much for something that happens with every
+// K block, where no ordinary store has to be seen by the other CTA (TMA loads count their own bytes, and
+// accumulators that were read lie in registers).
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_bar) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+// Arrivals with the transaction bytes this CTA will deliver to the barrier.
 __device__ __forceinline__ void mbar_arrive_expect_tx_cluster(uint32_t cluster_bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(cluster_bar), "r"(bytes)
+                 : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_expect_tx_cluster_relaxed(uint32_t cluster_bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(cluster_bar), "r"(bytes)
                  : "memory");
 }
 // One non-blocking look at a barrier phase.  CLUSTER_ACQUIRE as for mbar_wait.
