@@ -2,6 +2,7 @@
 #include "fp8_gemm.h"
 
 #include "fp8_gemm.cuh"
+#include "fp8_rows.cuh"
 #include "ragged_plan.h"
 
 namespace cudeep_b200 {
@@ -13,7 +14,7 @@ void launch(Fp8Params& p, const RaggedPlan& plan, cudaStream_t stream) {
     const DeviceInfo& dev = device_info();
     CB200_REQUIRE(dev.cc_major == 10, "8-bit products need an sm_100 device");
     p.tile_cols = plan.tile_cols;
-    p.stage_bytes = RAGGED_A_BYTES + uint32_t(plan.tile_cols / CTAS) * 128u;
+    p.stage_bytes = RAGGED_A_BYTES + uint32_t(RowMaps::loaded(plan.tile_cols / CTAS)) * 128u;
     const int fit = int(FP8_SMEM_BUDGET / p.stage_bytes);
     p.stages = fit < RAGGED_MAX_STAGES ? fit : RAGGED_MAX_STAGES;
     p.status = dev.status_word;
@@ -32,6 +33,34 @@ void launch_out(Fp8Params& p, const RaggedPlan& plan, cudaStream_t stream) {
     else launch<FORM, 1, OutT>(p, plan, stream);
 }
 
+template <RaggedForm FORM, class OutT>
+void launch_by_rows(Fp8RowsParams& p, cudaStream_t stream) {
+    const DeviceInfo& dev = device_info();
+    CB200_REQUIRE(dev.cc_major == 10, "8-bit products need an sm_100 device");
+    p.tma_store = (size_t(p.features) * sizeof(OutT)) % 16 == 0 && reinterpret_cast<uintptr_t>(p.c) % 16 == 0;
+    if (p.tma_store) {
+        const uint64_t dims[2] = {uint64_t(p.features), uint64_t(p.rows)};
+        const uint64_t strides[1] = {uint64_t(p.features) * sizeof(OutT)};
+        const uint32_t box[2] = {uint32_t(128 / sizeof(OutT)), 32};
+        if (sizeof(OutT) == 4) encode_tensor_map(&p.map_c, static_cast<const float*>(p.c), 2, dims, strides, box, TmaSwizzle::B128);
+        else encode_tensor_map_f16(&p.map_c, p.c, 2, dims, strides, box, TmaSwizzle::B128);
+    }
+    p.status = dev.status_word;
+    p.wait_limit_ns = 2000000000ull;
+    p.tiles_m = (p.rows + 255) / 256;
+    p.tiles_n = (p.features + 255) / 256;
+    const long long tiles = (long long)p.tiles_m * p.tiles_n;
+    const long long clusters = tiles < dev.num_sms / 2 ? tiles : dev.num_sms / 2;
+    CB200_TRACE("fp8 %s tcgen05, rows on lanes: rows=%d features=%d k=%d tile=256x256 stages=%d clusters=%lld store=%s",
+                FORM == RaggedForm::NT ? "nt" : "nn", p.rows, p.features, p.k, FP8R_STAGES, clusters,
+                p.tma_store ? "bulk-tensor" : "rows");
+    launch_clusters(fp8_rows_kernel<FORM, OutT>, p, clusters, 2, FP8R_THREADS, FP8R_SMEM_BYTES, FP8R_SMEM_BYTES, stream);
+}
+
+// Rows go on the accumulator's lanes, 256 to a tile, when there are many of them: fewer would leave lanes idle, and on the
+// columns a tile is as wide as it has rows.
+bool rows_on_lanes(int m) { return m > 256; }
+
 // x[m, k] by w, stored [n, k] (NT: features n) or [k, n] (NN: features n).
 template <RaggedForm FORM>
 void product(const uint8_t* x, const float* x_scales, const uint8_t* w, const float* w_scales, const float* bias, void* y,
@@ -40,6 +69,29 @@ void product(const uint8_t* x, const float* x_scales, const uint8_t* w, const fl
     const int w_cols = nn ? n : k, w_rows = nn ? k : n;
     const AlignedRows xr = aligned_rows(x, m, k, 1, stream);
     const AlignedRows wr = aligned_rows(w, w_rows, w_cols, 1, stream);
+    if (rows_on_lanes(m)) {
+        Fp8RowsParams p{};
+        const uint32_t box[2] = {128, 128};
+        const uint64_t x_dims[2] = {uint64_t(k), uint64_t(m)}, x_strides[1] = {uint64_t(xr.ld)};
+        encode_tensor_map_u8(&p.map_x, xr.ptr, 2, x_dims, x_strides, box, TmaSwizzle::B128);
+        const uint64_t w_dims[2] = {uint64_t(w_cols), uint64_t(w_rows)}, w_strides[1] = {uint64_t(wr.ld)};
+        encode_tensor_map_u8(&p.map_w, wr.ptr, 2, w_dims, w_strides, box, TmaSwizzle::B128);
+        p.x_scales = x_scales;
+        p.w_scales = w_scales;
+        const long long scale_cols = (w_cols + FP8_BLOCK - 1) / FP8_BLOCK;
+        p.ws_feature = nn ? 1 : scale_cols;
+        p.ws_k = nn ? scale_cols : 1;
+        p.bias = bias;
+        p.act = act;
+        p.c = y;
+        p.rows = m;
+        p.features = n;
+        p.k = k;
+        if (y_type == TYPE_F32) launch_by_rows<FORM, float>(p, stream);
+        else if (y_type == TYPE_F16) launch_by_rows<FORM, __half>(p, stream);
+        else launch_by_rows<FORM, __nv_bfloat16>(p, stream);
+        return;
+    }
     Fp8Params p{};
     {
         const uint64_t dims[3] = {uint64_t(w_cols), uint64_t(w_rows), 1};
@@ -50,9 +102,10 @@ void product(const uint8_t* x, const float* x_scales, const uint8_t* w, const fl
     {
         const uint64_t dims[2] = {uint64_t(k), uint64_t(m)};
         const uint64_t strides[1] = {uint64_t(xr.ld)};
-        const uint32_t box[2] = {128, 128}, box16[2] = {128, 16};
-        encode_tensor_map_u8(&p.map_b, xr.ptr, 2, dims, strides, box, TmaSwizzle::B128);
-        encode_tensor_map_u8(&p.map_b16, xr.ptr, 2, dims, strides, box16, TmaSwizzle::B128);
+        for (uint32_t i = 0; i < 5; ++i) {
+            const uint32_t box[2] = {128, i < 4 ? 32 * (i + 1) : 16};
+            encode_tensor_map_u8(i < 4 ? &p.x.box[i] : &p.x.box16, xr.ptr, 2, dims, strides, box, TmaSwizzle::B128);
+        }
     }
     p.x_scales = x_scales;
     p.w_scales = w_scales;

@@ -25,8 +25,7 @@ constexpr uint32_t FP8_SMEM_BUDGET = 232448 - 1024 - 22 * 1024;   // minus align
 
 struct Fp8Params {
     CUtensorMap map_a;       // NT {K, F, G} box {128, 128, 1}; NN {F, K, G} box {128, 128, 1}
-    CUtensorMap map_b;       // {K, rows} box {128, 128}
-    CUtensorMap map_b16;     // {K, rows} box {128, 16}
+    RowMaps x;               // {K, rows}
     const float* x_scales;   // [K blocks][rows]
     const float* w_scales;   // + group * ws_group + feature block * ws_feature + K block * ws_k
     long long ws_group, ws_feature, ws_k;
@@ -86,8 +85,7 @@ __global__ void __launch_bounds__(FP8_THREADS, 1) fp8_gemm_kernel(const __grid_c
     if (threadIdx.x == 0) {
         abort_flag = 0;
         ptx::prefetch_tensormap(&p.map_a);
-        ptx::prefetch_tensormap(&p.map_b);
-        ptx::prefetch_tensormap(&p.map_b16);
+        p.x.prefetch();
         for (int s = 0; s < RAGGED_MAX_STAGES; ++s) {
             ptx::mbar_init(ptx::smem_u32(&bar_full[s]), CTAS);
             ptx::mbar_init(ptx::smem_u32(&bar_empty[s]), 1);
@@ -130,7 +128,7 @@ __global__ void __launch_bounds__(FP8_THREADS, 1) fp8_gemm_kernel(const __grid_c
                 const int per = t.umma_n / CTAS;
                 const int feature = t.feature0 + int(cta_rank) * 128;
                 const int col = t.col0 + int(cta_rank) * per;
-                const uint32_t bytes = RAGGED_A_BYTES + uint32_t(per) * 128u;
+                const uint32_t bytes = RAGGED_A_BYTES + uint32_t(RowMaps::loaded(per)) * 128u;
                 for (int kb = 0; kb < k_blocks; ++kb) {
                     if (!ptx::mbar_wait(ptx::smem_u32(&bar_empty[stage]), phase ^ 1u, wctx, UMMA_TIMEOUT_PRODUCER))
                         goto producer_done;
@@ -144,13 +142,7 @@ __global__ void __launch_bounds__(FP8_THREADS, 1) fp8_gemm_kernel(const __grid_c
                     const int ax = A_MN ? feature : k0, ay = A_MN ? k0 : feature;
                     if constexpr (CTAS == 2) ptx::tma_load_3d_pair(a_smem, &p.map_a, full, ax, ay, t.group);
                     else ptx::tma_load_3d(a_smem, &p.map_a, full, ax, ay, t.group);
-                    for (int r = 0; r < per;) {
-                        const bool big = per - r >= 128;
-                        const CUtensorMap* map = big ? &p.map_b : &p.map_b16;
-                        if constexpr (CTAS == 2) ptx::tma_load_2d_pair(b_smem + r * 128, map, full, k0, col + r);
-                        else ptx::tma_load_2d(b_smem + r * 128, map, full, k0, col + r);
-                        r += big ? 128 : 16;
-                    }
+                    p.x.template load<CTAS>(b_smem, full, k0, col, per);
                     if (++stage == uint32_t(p.stages)) { stage = 0; phase ^= 1u; }
                 }
             }

@@ -1,0 +1,332 @@
+// The 8-bit products of fp8_gemm.cuh with the ROWS on the accumulator's lanes, for matrices of many rows.
+//
+//   NT  C[r, f] = sum_b xs[b][r] ws[f / 128][b] ( sum_{k in block b} X[r, k] W[f, k] )
+//   NN  C[r, f] = sum_b xs[b][r] ws[b][f / 128] ( sum_{k in block b} X[r, k] W[k, f] )
+//
+// A thread then owns one row and 128 consecutive features, which share one scale of W: a K block's sum is added with a
+// single factor per thread, xs * ws, that waits in a register, where the other orientation reads a factor per column from
+// shared memory.  What bounds the kernel is taking the accumulators out of TMEM: each block of 128 (512 cycles of MMAs on
+// a 256 x 256 tile of a CTA pair) hands 128 x 256 sums to eight warps, 64 packed multiply-adds a thread.  To hold
+// 128 sums, 64 values on their way out of TMEM and the rest, those warps take the registers that the first four warps
+// (producer, MMA issuer, two that only wait) give up.
+#pragma once
+
+#include "fp8_gemm.cuh"
+
+namespace cudeep_b200 {
+
+constexpr int FP8R_THREADS = 384;               // three groups of four warps
+// Registers per thread: 384 * 168 at launch; 128 * 56 + 256 * 216 = 62464 <= 64512 afterwards.
+constexpr int FP8R_REGS_FEW = 56;
+constexpr int FP8R_REGS_MANY = 216;
+constexpr uint32_t FP8R_STAGE_BYTES = 2 * 128 * 128;
+constexpr uint32_t FP8R_STAGING_BYTES = 8 * 4096;      // 32 rows x 128 bytes per epilogue warp
+constexpr int FP8R_STAGES = 6;
+constexpr uint32_t FP8R_SMEM_BYTES = FP8R_STAGES * FP8R_STAGE_BYTES + FP8R_STAGING_BYTES + 1024;
+
+struct Fp8RowsParams {
+    CUtensorMap map_x;       // {K, rows} box {128, 128}
+    CUtensorMap map_w;       // NT {K, F}, NN {F, K}: box {128, 128}
+    CUtensorMap map_c;       // {F, rows} box {128 bytes, 32}; used when `tma_store`
+    const float* x_scales;   // [K blocks][rows]
+    const float* w_scales;   // + feature block * ws_feature + K block * ws_k
+    long long ws_feature, ws_k;
+    const float* bias;
+    int act;
+    void* c;
+    int tma_store;
+    int rows;
+    int features;
+    int k;
+    int tiles_m, tiles_n;
+    uint32_t* status;
+    unsigned long long wait_limit_ns;
+};
+
+template <int REGS>
+__device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS)); }
+template <int REGS>
+__device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS)); }
+
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+__device__ __forceinline__ void st_shared_u4(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
+template <RaggedForm FORM, class OutT>
+__global__ void __launch_bounds__(FP8R_THREADS, 1) fp8_rows_kernel(const __grid_constant__ Fp8RowsParams p) {
+#if defined(__CUDA_ARCH_FEAT_SM100_ALL) || defined(__CUDA_ARCH_FEAT_SM101_ALL) || \
+    defined(__CUDA_ARCH_FEAT_SM103_ALL)
+    constexpr bool B_MN = FORM == RaggedForm::NN;
+
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t bar_full[FP8R_STAGES];
+    __shared__ __align__(8) uint64_t bar_empty[FP8R_STAGES];
+    __shared__ __align__(8) uint64_t bar_acc_full[2];
+    __shared__ __align__(8) uint64_t bar_acc_empty[2];
+    __shared__ uint32_t tmem_base_holder;
+    __shared__ uint32_t abort_flag;
+
+    const uint32_t warp = threadIdx.x >> 5;
+    const uint32_t lane = threadIdx.x & 31;
+    const uint32_t cta_rank = ptx::cluster_ctarank();
+    const bool is_leader = cta_rank == 0;
+    const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
+    ptx::WaitCtx wctx{&abort_flag, p.status, p.wait_limit_ns};
+
+    if (threadIdx.x == 0) {
+        abort_flag = 0;
+        ptx::prefetch_tensormap(&p.map_x);
+        ptx::prefetch_tensormap(&p.map_w);
+        ptx::prefetch_tensormap(&p.map_c);
+        for (int s = 0; s < FP8R_STAGES; ++s) {
+            ptx::mbar_init(ptx::smem_u32(&bar_full[s]), 1);
+            ptx::mbar_init(ptx::smem_u32(&bar_empty[s]), 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            ptx::mbar_init(ptx::smem_u32(&bar_acc_full[a]), 1);
+            ptx::mbar_init(ptx::smem_u32(&bar_acc_empty[a]), 8 * 2);
+        }
+        ptx::fence_mbar_init();
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc<2>(ptx::smem_u32(&tmem_base_holder), 512);
+        ptx::tmem_relinquish<2>();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::cluster_arrive();
+    ptx::cluster_wait();
+    ptx::tc_fence_after();
+    const uint32_t tmem_base = tmem_base_holder;
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
+
+    const int unit_stride = gridDim.x / 2;
+    const int first_unit = blockIdx.x / 2;
+    const int num_units = p.tiles_m * p.tiles_n;
+    const int k_blocks = (p.k + FP8_BK - 1) / FP8_BK;
+
+    if (warp < 4) {
+        give_registers<FP8R_REGS_FEW>();
+        if (warp == 0) {
+            // -------------------------------------------------------- producer
+            if (lane == 0) {
+                uint32_t stage = 0, phase = 0;
+                for (int u = first_unit; u < num_units; u += unit_stride) {
+                    int tm, tn;
+                    raster_coords(u, p.tiles_m, p.tiles_n, 8, tm, tn);
+                    const int row = (tm * 2 + int(cta_rank)) * 128;
+                    const int feature = tn * 256 + int(cta_rank) * 128;
+                    for (int kb = 0; kb < k_blocks; ++kb) {
+                        if (!ptx::mbar_wait(ptx::smem_u32(&bar_empty[stage]), phase ^ 1u, wctx, UMMA_TIMEOUT_PRODUCER))
+                            goto producer_done;
+                        const uint32_t a_smem = smem_base + stage * FP8R_STAGE_BYTES;
+                        const uint32_t full_local = ptx::smem_u32(&bar_full[stage]);
+                        if (is_leader) ptx::mbar_arrive_expect_tx(full_local, 2 * FP8R_STAGE_BYTES);
+                        const uint32_t full = ptx::mapa(full_local, 0);
+                        const int k0 = kb * FP8_BK;
+                        ptx::tma_load_2d_pair(a_smem, &p.map_x, full, k0, row);
+                        ptx::tma_load_2d_pair(a_smem + 16384, &p.map_w, full, B_MN ? feature : k0, B_MN ? k0 : feature);
+                        if (++stage == FP8R_STAGES) { stage = 0; phase ^= 1u; }
+                    }
+                }
+            }
+        producer_done:
+            __syncwarp();
+        } else if (warp == 1 && is_leader) {
+            // -------------------------------------------------------- MMA issuer
+            constexpr uint32_t B_KSTEP = B_MN ? 4096u : 32u;
+            constexpr uint32_t idesc = ptx::idesc_e4m3(256, 256, 0, B_MN ? 1 : 0);
+            const uint64_t a_desc0 = ptx::smem_desc_at(ptx::smem_desc(16, 1024, ptx::SMEM_LAYOUT_SW128), smem_base);
+            const uint64_t b_desc0 =
+                ptx::smem_desc_at(ptx::smem_desc(B_MN ? 16384 : 16, 1024, ptx::SMEM_LAYOUT_SW128), smem_base + 16384);
+            uint32_t stage = 0, phase = 0, it = 0;
+            for (int u = first_unit; u < num_units; u += unit_stride) {
+                for (int kb = 0; kb < k_blocks; ++kb, ++it) {
+                    const uint32_t acc = it & 1;
+                    if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&bar_full[stage]), phase, wctx,
+                                                                UMMA_TIMEOUT_MMA_FULL)))
+                        goto mma_done;
+                    if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&bar_acc_empty[acc]), ((it >> 1) & 1) ^ 1u,
+                                                                wctx, UMMA_TIMEOUT_MMA_ACC)))
+                        goto mma_done;
+                    ptx::tc_fence_after();
+                    if (ptx::elect_one()) {
+                        const uint64_t a_stage = a_desc0 + ((stage * FP8R_STAGE_BYTES) >> 4);
+                        const uint64_t b_stage = b_desc0 + ((stage * FP8R_STAGE_BYTES) >> 4);
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk)
+                            ptx::umma_f8<2>(tmem_base + acc * 256u, a_stage + ((kk * 32u) >> 4),
+                                            b_stage + ((kk * B_KSTEP) >> 4), idesc, kk != 0);
+                        const uint32_t accf_local = ptx::smem_u32(&bar_acc_full[acc]);
+                        ptx::umma_commit<2>(accf_local);
+                        ptx::umma_commit<2>(ptx::mapa(accf_local, 1));
+                        const uint32_t empty_local = ptx::smem_u32(&bar_empty[stage]);
+                        ptx::umma_commit<2>(empty_local);
+                        ptx::umma_commit<2>(ptx::mapa(empty_local, 1));
+                    }
+                    __syncwarp();
+                    if (++stage == FP8R_STAGES) { stage = 0; phase ^= 1u; }
+                }
+            }
+        mma_done:
+            __syncwarp();
+        }
+        ptx::cluster_arrive();
+    } else {
+        take_registers<FP8R_REGS_MANY>();
+        // ------------------------------------------------------------ sums and epilogue
+        const uint32_t quarter = warp & 3u;
+        const int half = int(warp - 4) >> 2;
+        const uint32_t staging = smem_base + FP8R_STAGES * FP8R_STAGE_BYTES + (warp - 4) * 4096u;
+        uint32_t it = 0;
+        for (int u = first_unit; u < num_units; u += unit_stride) {
+            int tm, tn;
+            raster_coords(u, p.tiles_m, p.tiles_n, 8, tm, tn);
+            const int row0 = (tm * 2 + int(cta_rank)) * 128 + int(quarter) * 32;
+            const int row = row0 + int(lane);
+            const int feature0 = tn * 256 + half * 128;
+            // Rows and features outside the matrices take some factor that exists; what it makes is not stored.
+            const float* xs = p.x_scales + (row < p.rows ? row : 0);
+            const float* ws = p.w_scales + (feature0 < p.features ? feature0 / 128 : 0) * p.ws_feature;
+            float acc[4][32];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 32; ++j) acc[i][j] = 0.0f;
+            float next_x = __ldg(xs), next_w = __ldg(ws);
+#pragma unroll 1
+            for (int kb = 0; kb < k_blocks; ++kb, ++it) {
+                const float s = next_x * next_w;
+                if (kb + 1 < k_blocks) {
+                    next_x = __ldg(xs + (long long)(kb + 1) * p.rows);
+                    next_w = __ldg(ws + (kb + 1) * p.ws_k);
+                }
+                const uint32_t buf = it & 1;
+                const bool ok = ptx::mbar_wait(ptx::smem_u32(&bar_acc_full[buf]), (it >> 1) & 1, wctx, UMMA_TIMEOUT_EPILOGUE);
+                if (!__all_sync(0xffffffffu, ok)) goto epilogue_done;
+                ptx::tc_fence_after();
+                const uint32_t t_row = tmem_base + buf * 256u + uint32_t(half) * 128u + ((quarter * 32u) << 16);
+                uint32_t r[2][32];
+                ptx::tmem_ld_32x32(t_row, r[0]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    ptx::tmem_ld_wait();
+                    if (i < 3) {
+                        ptx::tmem_ld_32x32(t_row + 32 * (i + 1), r[(i + 1) & 1]);
+                    } else {      // all sums of the buffer are in registers
+                        ptx::tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) {
+                            const uint32_t e = ptx::smem_u32(&bar_acc_empty[buf]);
+                            if (is_leader) ptx::mbar_arrive(e);
+                            else ptx::mbar_arrive_cluster_relaxed(ptx::mapa(e, 0));
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) fma2(acc[i][j], acc[i][j + 1], r[i & 1][j], r[i & 1][j + 1], s, s);
+                }
+            }
+            constexpr int V = 16 / sizeof(OutT);              // values per 16 bytes
+            constexpr int COLS = 128 / sizeof(OutT);          // columns of a staged block: 128 bytes per row
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (p.bias != nullptr) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        const int f = feature0 + 32 * i + j;
+                        acc[i][j] += __ldg(p.bias + min(f, p.features - 1));
+                    }
+                }
+                apply_activation(acc[i], p.act);
+                const int c0 = 32 * i / COLS * COLS;          // first column of the staged block this chunk belongs to
+                if (32 * i == c0) {
+                    if (lane == 0) ptx::bulk_wait_group_read<0>();      // the block's last store has read it
+                    __syncwarp();
+                }
+#pragma unroll
+                for (int j = 0; j < 32; j += V) {
+                    const uint32_t unit = uint32_t(32 * i - c0 + j) / V;
+                    const uint32_t dst = staging + lane * 128u + ((unit ^ (lane & 7u)) << 4);
+                    if constexpr (sizeof(OutT) == 4)
+                        ptx::st_shared_v4(dst, acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3]);
+                    else
+                        st_shared_u4(dst, pack2<OutT>(acc[i][j], acc[i][j + 1]), pack2<OutT>(acc[i][j + 2], acc[i][j + 3]),
+                                     pack2<OutT>(acc[i][j + 4], acc[i][j + 5]), pack2<OutT>(acc[i][j + 6], acc[i][j + 7]));
+                }
+                if (32 * (i + 1) - c0 == COLS) {              // the block is full
+                    const int f0 = feature0 + c0;
+                    if (p.tma_store) {
+                        ptx::fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0 && row0 < p.rows && f0 < p.features) {
+                            ptx::tma_store_2d(&p.map_c, staging, f0, row0);
+                            ptx::bulk_commit_group();
+                        }
+                    } else {
+                        // Rows of C that are no 16-byte multiples: the warp writes them one by one.
+                        __syncwarp();
+                        const int f = f0 + int(lane);
+                        OutT* dst = static_cast<OutT*>(p.c) + (long long)row0 * p.features + f;
+                        for (int r = 0; r < 32 && row0 + r < p.rows; ++r, dst += p.features) {
+#pragma unroll
+                            for (int h = 0; h < COLS / 32; ++h) {
+                                const uint32_t byte = uint32_t(lane + 32 * h) * sizeof(OutT);
+                                const uint32_t at = staging + uint32_t(r) * 128u + (((byte >> 4) ^ (uint32_t(r) & 7u)) << 4) + (byte & 15u);
+                                if (f + 32 * h < p.features) {
+                                    if constexpr (sizeof(OutT) == 4) {
+                                        uint32_t v;
+                                        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+                                        reinterpret_cast<uint32_t*>(dst)[32 * h] = v;
+                                    } else {
+                                        uint16_t v;
+                                        asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
+                                        reinterpret_cast<uint16_t*>(dst)[32 * h] = v;
+                                    }
+                                }
+                            }
+                        }
+                        __syncwarp();
+                    }
+                }
+            }
+        }
+    epilogue_done:
+        __syncwarp();
+        ptx::cluster_arrive();
+        if (lane == 0) ptx::bulk_wait_group_read<0>();
+        __syncwarp();
+    }
+
+    // ---------------------------------------------------------------- teardown
+    ptx::tc_fence_before();
+    __syncthreads();
+    if (abort_flag) {
+        const uint64_t t0 = ptx::globaltimer_ns();
+        while (ptx::globaltimer_ns() - t0 < 2000000ull) { }
+        __syncthreads();
+    }
+    ptx::cluster_wait();
+    if (warp == 1) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc<2>(tmem_base, 512);
+    }
+#else
+    if (threadIdx.x == 0 && blockIdx.x == 0) atomicCAS(p.status, 0u, 0xdeadu);
+#endif
+}
+
+}  // namespace cudeep_b200

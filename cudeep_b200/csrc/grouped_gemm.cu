@@ -22,7 +22,7 @@ void launch(RaggedParams& p, const RaggedPlan& plan, cudaStream_t stream) {
     const DeviceInfo& dev = device_info();
     CB200_REQUIRE(dev.cc_major == 10, "grouped products need an sm_100 device");
     p.tile_cols = plan.tile_cols;
-    p.stage_bytes = RAGGED_A_BYTES + uint32_t(plan.tile_cols / CTAS) * 128u;
+    p.stage_bytes = RAGGED_A_BYTES + uint32_t(RowMaps::loaded(plan.tile_cols / CTAS)) * 128u;
     const int fit = int(RAGGED_SMEM_BUDGET / p.stage_bytes);
     p.stages = fit < RAGGED_MAX_STAGES ? fit : RAGGED_MAX_STAGES;
     p.status = dev.status_word;
@@ -72,9 +72,10 @@ void rows_by_weight(bool nn, const void* a, long long lda, const void* w, void* 
     {
         const uint64_t dims[2] = {uint64_t(k), uint64_t(rows)};
         const uint64_t strides[1] = {uint64_t(x.ld) * 2};
-        const uint32_t box[2] = {64, 128}, box16[2] = {64, 16};
-        encode_tensor_map_f16(&p.map_b, x.ptr, 2, dims, strides, box, TmaSwizzle::B128);
-        encode_tensor_map_f16(&p.map_b16, x.ptr, 2, dims, strides, box16, TmaSwizzle::B128);
+        for (uint32_t i = 0; i < 5; ++i) {
+            const uint32_t box[2] = {64, i < 4 ? 32 * (i + 1) : 16};
+            encode_tensor_map_f16(i < 4 ? &p.x.box[i] : &p.x.box16, x.ptr, 2, dims, strides, box, TmaSwizzle::B128);
+        }
     }
     p.c = c;
     p.offsets = offsets;

@@ -36,11 +36,34 @@ constexpr int RAGGED_MAX_STAGES = 12;
 constexpr uint32_t RAGGED_SMEM_BUDGET = 232448 - 1024 - 13 * 1024;   // minus alignment slack, group tables and barriers
 constexpr uint32_t UMMA_BAD_OFFSETS = 6;             // status word: the offsets decrease or leave [0, rows]
 
+// Rows of a matrix as K blocks of 128 bytes.  One box brings all rows that a CTA stages for a tile, up to 128, rounded up to a
+// size there is a map for: the TMA unit spends about 130 cycles on a box however small (2 KB boxes of 16 rows loaded
+// a 112-row operand at a third of one 16 KB box's rate: 16384 x 4096 x 2048 in 224-row tiles 335 us, in 256-row tiles 183 us).
+struct RowMaps {
+    CUtensorMap box16;
+    CUtensorMap box[4];      // 32, 64, 96, 128 rows
+    __device__ __forceinline__ void prefetch() const {
+        ptx::prefetch_tensormap(&box16);
+        ptx::prefetch_tensormap(&box[3]);
+    }
+    // Rows that loads of `per` rows bring.
+    __host__ __device__ static constexpr int loaded(int per) { return per <= 16 ? 16 : (per + 31) / 32 * 32; }
+    template <int CTAS>
+    __device__ __forceinline__ void load(uint32_t dst, uint32_t bar, int k0, int row, int per) const {
+        for (int left = loaded(per); left > 0; left -= 128, row += 128, dst += 128 * 128) {
+            const CUtensorMap* map = left == 16 ? &box16 : &box[left >= 128 ? 3 : left / 32 - 1];
+            if constexpr (CTAS == 2) ptx::tma_load_2d_pair(dst, map, bar, k0, row);
+            else ptx::tma_load_2d(dst, map, bar, k0, row);
+        }
+    }
+};
+
 struct RaggedParams {
     CUtensorMap map_a;       // NT {K, F, G} box {64, 128, 1}; NN {F, K, G} box {64, 64, 1}; TN {F, rows} box {64, 64}
     CUtensorMap map_a16;     // TN: {F, rows} box {64, 16}
-    CUtensorMap map_b;       // NT, NN {K, rows} box {64, 128}; TN {C, rows} box {64, 64}
-    CUtensorMap map_b16;     // NT, NN {K, rows} box {64, 16};  TN {C, rows} box {64, 16}
+    RowMaps x;               // NT, NN {K, rows}
+    CUtensorMap map_b;       // TN {C, rows} box {64, 64}
+    CUtensorMap map_b16;     // TN {C, rows} box {64, 16}
     const void* a;           // TN: the operands' addresses and row lengths, for the partial last step
     const void* b;
     long long lda, ldb;
@@ -180,8 +203,13 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) ragged_gemm_kernel(const __gr
     if (threadIdx.x == 0) {
         abort_flag = 0;
         ptx::prefetch_tensormap(&p.map_a);
-        ptx::prefetch_tensormap(&p.map_b);
-        ptx::prefetch_tensormap(&p.map_b16);
+        if constexpr (FORM == RaggedForm::TN) {
+            ptx::prefetch_tensormap(&p.map_b);
+            ptx::prefetch_tensormap(&p.map_b16);
+            ptx::prefetch_tensormap(&p.map_a16);
+        } else {
+            p.x.prefetch();
+        }
         for (int s = 0; s < RAGGED_MAX_STAGES; ++s) {
             ptx::mbar_init(ptx::smem_u32(&bar_full[s]), CTAS);      // each CTA's producer arrives with its bytes
             ptx::mbar_init(ptx::smem_u32(&bar_empty[s]), 1);
@@ -241,7 +269,7 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) ragged_gemm_kernel(const __gr
                 uint32_t bytes;
                 bool stored = false;      // this stage holds rows written with ordinary stores
                 if constexpr (FORM != RaggedForm::TN) {
-                    bytes = RAGGED_A_BYTES + uint32_t(per) * 128u;
+                    bytes = RAGGED_A_BYTES + uint32_t(RowMaps::loaded(per)) * 128u;
                     if (lane == 0) {
                         const int k0 = kb * RAGGED_BK;
                         if constexpr (FORM == RaggedForm::NT) {
@@ -256,13 +284,7 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) ragged_gemm_kernel(const __gr
                                     ptx::tma_load_3d(a_smem + j * 8192, &p.map_a, full, feature + j * 64, k0, t.group);
                             }
                         }
-                        for (int r = 0; r < per;) {
-                            const bool big = per - r >= 128;
-                            const CUtensorMap* map = big ? &p.map_b : &p.map_b16;
-                            if constexpr (CTAS == 2) ptx::tma_load_2d_pair(b_smem + r * 128, map, full, k0, col + r);
-                            else ptx::tma_load_2d(b_smem + r * 128, map, full, k0, col + r);
-                            r += big ? 128 : 16;
-                        }
+                        p.x.template load<CTAS>(b_smem, full, k0, col, per);
                     }
                 } else {
                     const int row = t.row0 + kb * RAGGED_BK;
