@@ -57,6 +57,39 @@ __device__ __forceinline__ void fma2(float& d0, float& d1, uint32_t a0, uint32_t
         : "+f"(d0), "+f"(d1) : "r"(a0), "r"(a1), "f"(s0), "f"(s1));
 }
 
+// The epilogue's activations as one formula, y = g * sigmoid(a z + b z^3), g = z (GELU in its tanh form, SiLU) or 1
+// (sigmoid), with log2(e) folded into a and b.  Two values share one reciprocal, 1 / d0 = d1 / (d0 d1): the SFU is what bounds
+// an epilogue that activates 128 values a thread, and this takes three of its operations per pair instead of four.  The
+// exponents are held below 60 so that d0 d1 stays finite (sigmoid = 2^-60 there instead of less).
+struct Fp8Activation {
+    int act;
+    float a, b;
+    __device__ __forceinline__ explicit Fp8Activation(int act_) : act(act_) {
+        const float c = act == EPI_GELU ? 2.0f * 0.7978845608028654f : 1.0f;
+        a = -1.4426950408889634f * c;
+        b = act == EPI_GELU ? a * 0.044715f : 0.0f;
+    }
+};
+
+__device__ __forceinline__ void fp8_activation(float (&v)[32], const Fp8Activation& f) {
+    if (f.act == EPI_NONE) return;
+    if (f.act == EPI_RELU) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = fmaxf(v[j], 0.0f);
+        return;
+    }
+    const bool gate = f.act != EPI_SIGMOID;
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+        const float x0 = v[j], x1 = v[j + 1];
+        const float d0 = 1.0f + sfu_ex2(fminf(x0 * fmaf(f.b, x0 * x0, f.a), 60.0f));
+        const float d1 = 1.0f + sfu_ex2(fminf(x1 * fmaf(f.b, x1 * x1, f.a), 60.0f));
+        const float r = sfu_rcp(d0 * d1);
+        v[j] = (gate ? x0 : 1.0f) * (d1 * r);
+        v[j + 1] = (gate ? x1 : 1.0f) * (d0 * r);
+    }
+}
+
 template <RaggedForm FORM, int CTAS, class OutT>
 __global__ void __launch_bounds__(FP8_THREADS, 1) fp8_gemm_kernel(const __grid_constant__ Fp8Params p) {
 #if defined(__CUDA_ARCH_FEAT_SM100_ALL) || defined(__CUDA_ARCH_FEAT_SM101_ALL) || \
@@ -265,6 +298,7 @@ __global__ void __launch_bounds__(FP8_THREADS, 1) fp8_gemm_kernel(const __grid_c
                     else ptx::mbar_arrive(e);
                 }
             }
+            const Fp8Activation act(p.act);
             if (feature < p.features) {
                 const float bias = p.bias != nullptr ? __ldg(p.bias + feature) : 0.0f;
                 OutT* dst = static_cast<OutT*>(p.c) + (long long)(t.col0 + c_begin) * p.features + feature;
@@ -274,7 +308,7 @@ __global__ void __launch_bounds__(FP8_THREADS, 1) fp8_gemm_kernel(const __grid_c
                     if (32 * i < stored) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j) acc[i][j] += bias;
-                        apply_activation(acc[i], p.act);
+                        fp8_activation(acc[i], act);
 #pragma unroll
                         for (int j = 0; j < 32; ++j)
                             if (32 * i + j < stored) dst[(long long)(32 * i + j) * p.features] = round_to<OutT>(acc[i][j]);

@@ -7,8 +7,9 @@
 // single factor per thread, xs * ws, that waits in a register, where the other orientation reads a factor per column from
 // shared memory.  What bounds the kernel is taking the accumulators out of TMEM: each block of 128 (512 cycles of MMAs on
 // a 256 x 256 tile of a CTA pair) hands 128 x 256 sums to eight warps, 64 packed multiply-adds a thread.  To hold
-// 128 sums, 64 values on their way out of TMEM and the rest, those warps take the registers that the first four warps
-// (producer, MMA issuer, two that only wait) give up.
+// 128 sums, two sets of 16 values on their way out of TMEM and the rest, those warps take the registers that the first four
+// warps (producer, MMA issuer, two that only wait) give up.  (With sets of 32 the compiler spilled in this loop: 8192 x 4096 x
+// 16384 took 778 us, with sets of 16 it takes 491 us; without any sums taken out, 448 us.)
 #pragma once
 
 #include "fp8_gemm.cuh"
@@ -192,6 +193,7 @@ __global__ void __launch_bounds__(FP8R_THREADS, 1) fp8_rows_kernel(const __grid_
         const uint32_t quarter = warp & 3u;
         const int half = int(warp - 4) >> 2;
         const uint32_t staging = smem_base + FP8R_STAGES * FP8R_STAGE_BYTES + (warp - 4) * 4096u;
+        const Fp8Activation act(p.act);
         uint32_t it = 0;
         for (int u = first_unit; u < num_units; u += unit_stride) {
             int tm, tn;
@@ -207,27 +209,37 @@ __global__ void __launch_bounds__(FP8R_THREADS, 1) fp8_rows_kernel(const __grid_
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int j = 0; j < 32; ++j) acc[i][j] = 0.0f;
-            float next_x = __ldg(xs), next_w = __ldg(ws);
+            // The factors come four blocks ahead: a block takes 500 cycles and a load from L2 under this traffic longer.
+            float px[4], pw[4];
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                px[d] = d < k_blocks ? __ldg(xs + (long long)d * p.rows) : 0.0f;
+                pw[d] = d < k_blocks ? __ldg(ws + d * p.ws_k) : 0.0f;
+            }
 #pragma unroll 1
-            for (int kb = 0; kb < k_blocks; ++kb, ++it) {
-                const float s = next_x * next_w;
-                if (kb + 1 < k_blocks) {
-                    next_x = __ldg(xs + (long long)(kb + 1) * p.rows);
-                    next_w = __ldg(ws + (kb + 1) * p.ws_k);
+            for (int kb4 = 0; kb4 < k_blocks; kb4 += 4) {
+#pragma unroll
+              for (int d = 0; d < 4; ++d) {
+                const int kb = kb4 + d;
+                if (kb >= k_blocks) break;
+                const float s = px[d] * pw[d];
+                if (kb + 4 < k_blocks) {
+                    px[d] = __ldg(xs + (long long)(kb + 4) * p.rows);
+                    pw[d] = __ldg(ws + (kb + 4) * p.ws_k);
                 }
                 const uint32_t buf = it & 1;
                 const bool ok = ptx::mbar_wait(ptx::smem_u32(&bar_acc_full[buf]), (it >> 1) & 1, wctx, UMMA_TIMEOUT_EPILOGUE);
                 if (!__all_sync(0xffffffffu, ok)) goto epilogue_done;
                 ptx::tc_fence_after();
                 const uint32_t t_row = tmem_base + buf * 256u + uint32_t(half) * 128u + ((quarter * 32u) << 16);
-                uint32_t r[2][32];
-                ptx::tmem_ld_32x32(t_row, r[0]);
+                uint32_t r[2][16];
+                ptx::tmem_ld_32x16(t_row, r[0]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < 8; ++i) {
                     ptx::tmem_ld_wait();
-                    if (i < 3) {
-                        ptx::tmem_ld_32x32(t_row + 32 * (i + 1), r[(i + 1) & 1]);
-                    } else {      // all sums of the buffer are in registers
+                    if (i < 7) {
+                        ptx::tmem_ld_32x16(t_row + 16 * (i + 1), r[(i + 1) & 1]);
+                    } else {
                         ptx::tc_fence_before();
                         __syncwarp();
                         if (lane == 0) {
@@ -237,8 +249,10 @@ __global__ void __launch_bounds__(FP8R_THREADS, 1) fp8_rows_kernel(const __grid_
                         }
                     }
 #pragma unroll
-                    for (int j = 0; j < 32; j += 2) fma2(acc[i][j], acc[i][j + 1], r[i & 1][j], r[i & 1][j + 1], s, s);
+                    for (int j = 0; j < 16; j += 2) fma2(acc[i >> 1][(i & 1) * 16 + j], acc[i >> 1][(i & 1) * 16 + j + 1], r[i & 1][j], r[i & 1][j + 1], s, s);
                 }
+                ++it;
+              }
             }
             constexpr int V = 16 / sizeof(OutT);              // values per 16 bytes
             constexpr int COLS = 128 / sizeof(OutT);          // columns of a staged block: 128 bytes per row
@@ -251,7 +265,7 @@ __global__ void __launch_bounds__(FP8R_THREADS, 1) fp8_rows_kernel(const __grid_
                         acc[i][j] += __ldg(p.bias + min(f, p.features - 1));
                     }
                 }
-                apply_activation(acc[i], p.act);
+                fp8_activation(acc[i], act);
                 const int c0 = 32 * i / COLS * COLS;          // first column of the staged block this chunk belongs to
                 if (32 * i == c0) {
                     if (lane == 0) ptx::bulk_wait_group_read<0>();      // the block's last store has read it
