@@ -9,28 +9,29 @@ namespace cudeep_b200 {
 
 namespace {
 
-template <RaggedForm FORM, int CTAS, class OutT>
-void launch(Fp8Params& p, const RaggedPlan& plan, cudaStream_t stream) {
-    const DeviceInfo& dev = device_info();
-    CB200_REQUIRE(dev.cc_major == 10, "8-bit products need an sm_100 device");
-    p.tile_cols = plan.tile_cols;
-    p.stage_bytes = RAGGED_A_BYTES + uint32_t(RowMaps::loaded(plan.tile_cols / CTAS)) * 128u;
-    const int fit = int(FP8_SMEM_BUDGET / p.stage_bytes);
-    p.stages = fit < RAGGED_MAX_STAGES ? fit : RAGGED_MAX_STAGES;
-    p.status = dev.status_word;
-    p.wait_limit_ns = 2000000000ull;
-    long long clusters = dev.num_sms / CTAS;
-    if (clusters > plan.units) clusters = plan.units;
-    CB200_TRACE("fp8 %s tcgen05: rows=%d features=%d k=%d tile=%dx%d stages=%d clusters=%lld",
-                FORM == RaggedForm::NT ? "nt" : "nn", p.rows, p.features, p.k, 128 * CTAS, plan.tile_cols, p.stages, clusters);
-    launch_clusters(fp8_gemm_kernel<FORM, CTAS, OutT>, p, clusters, CTAS, FP8_THREADS,
-                    uint32_t(p.stages) * p.stage_bytes + 1024, FP8_SMEM_BUDGET + 1024, stream);
+// CTAs that share a tile of 128 features: as many as the device has SMs for, while each keeps four blocks of K.
+int cluster_split(int features, int k) {
+    const int tiles = (features + 127) / 128, blocks = (k + FP8_BK - 1) / FP8_BK;
+    int split = 1;
+    while (split < 8 && tiles * split * 2 <= device_info().num_sms && blocks >= 8 * split) split *= 2;
+    return split;
 }
 
 template <RaggedForm FORM, class OutT>
-void launch_out(Fp8Params& p, const RaggedPlan& plan, cudaStream_t stream) {
-    if (plan.ctas == 2) launch<FORM, 2, OutT>(p, plan, stream);
-    else launch<FORM, 1, OutT>(p, plan, stream);
+void launch_few(Fp8FewParams& p, cudaStream_t stream) {
+    const DeviceInfo& dev = device_info();
+    CB200_REQUIRE(dev.cc_major == 10, "8-bit products need an sm_100 device");
+    p.split = cluster_split(p.features, p.k);
+    p.stage_bytes = RAGGED_A_BYTES + uint32_t(RowMaps::loaded((p.rows + 15) / 16 * 16)) * 128u;
+    const int fit = int(FP8F_SMEM_BUDGET / p.stage_bytes);
+    p.stages = fit < FP8F_MAX_STAGES ? fit : FP8F_MAX_STAGES;
+    p.status = dev.status_word;
+    p.wait_limit_ns = 2000000000ull;
+    const long long tiles = (p.features + 127) / 128;
+    CB200_TRACE("fp8 %s tcgen05, features on lanes: rows=%d features=%d k=%d stages=%d tiles=%lld split=%d",
+                FORM == RaggedForm::NT ? "nt" : "nn", p.rows, p.features, p.k, p.stages, tiles, p.split);
+    launch_clusters(fp8_few_kernel<FORM, OutT>, p, tiles, p.split, FP8F_THREADS, uint32_t(p.stages) * p.stage_bytes + 1024,
+                    FP8F_SMEM_BUDGET + 1024, stream);
 }
 
 template <RaggedForm FORM, class OutT>
@@ -57,10 +58,6 @@ void launch_by_rows(Fp8RowsParams& p, cudaStream_t stream) {
     launch_clusters(fp8_rows_kernel<FORM, OutT>, p, clusters, 2, FP8R_THREADS, FP8R_SMEM_BYTES, FP8R_SMEM_BYTES, stream);
 }
 
-// Rows go on the accumulator's lanes, 256 to a tile, when there are many of them: fewer would leave lanes idle, and on the
-// columns a tile is as wide as it has rows.
-bool rows_on_lanes(int m) { return m > 256; }
-
 // x[m, k] by w, stored [n, k] (NT: features n) or [k, n] (NN: features n).
 template <RaggedForm FORM>
 void product(const uint8_t* x, const float* x_scales, const uint8_t* w, const float* w_scales, const float* bias, void* y,
@@ -69,16 +66,14 @@ void product(const uint8_t* x, const float* x_scales, const uint8_t* w, const fl
     const int w_cols = nn ? n : k, w_rows = nn ? k : n;
     const AlignedRows xr = aligned_rows(x, m, k, 1, stream);
     const AlignedRows wr = aligned_rows(w, w_rows, w_cols, 1, stream);
-    if (rows_on_lanes(m)) {
-        Fp8RowsParams p{};
-        const uint32_t box[2] = {128, 128};
-        const uint64_t x_dims[2] = {uint64_t(k), uint64_t(m)}, x_strides[1] = {uint64_t(xr.ld)};
-        encode_tensor_map_u8(&p.map_x, xr.ptr, 2, x_dims, x_strides, box, TmaSwizzle::B128);
-        const uint64_t w_dims[2] = {uint64_t(w_cols), uint64_t(w_rows)}, w_strides[1] = {uint64_t(wr.ld)};
+    const uint32_t box[2] = {128, 128};
+    const uint64_t w_dims[2] = {uint64_t(w_cols), uint64_t(w_rows)}, w_strides[1] = {uint64_t(wr.ld)};
+    const uint64_t x_dims[2] = {uint64_t(k), uint64_t(m)}, x_strides[1] = {uint64_t(xr.ld)};
+    const long long scale_cols = (w_cols + FP8_BLOCK - 1) / FP8_BLOCK;
+    auto fill = [&](auto& p) {
         encode_tensor_map_u8(&p.map_w, wr.ptr, 2, w_dims, w_strides, box, TmaSwizzle::B128);
         p.x_scales = x_scales;
         p.w_scales = w_scales;
-        const long long scale_cols = (w_cols + FP8_BLOCK - 1) / FP8_BLOCK;
         p.ws_feature = nn ? 1 : scale_cols;
         p.ws_k = nn ? scale_cols : 1;
         p.bias = bias;
@@ -87,42 +82,25 @@ void product(const uint8_t* x, const float* x_scales, const uint8_t* w, const fl
         p.rows = m;
         p.features = n;
         p.k = k;
+    };
+    if (m > FP8F_MAX_ROWS) {
+        Fp8RowsParams p{};
+        fill(p);
+        encode_tensor_map_u8(&p.map_x, xr.ptr, 2, x_dims, x_strides, box, TmaSwizzle::B128);
         if (y_type == TYPE_F32) launch_by_rows<FORM, float>(p, stream);
         else if (y_type == TYPE_F16) launch_by_rows<FORM, __half>(p, stream);
         else launch_by_rows<FORM, __nv_bfloat16>(p, stream);
-        return;
-    }
-    Fp8Params p{};
-    {
-        const uint64_t dims[3] = {uint64_t(w_cols), uint64_t(w_rows), 1};
-        const uint64_t strides[2] = {uint64_t(wr.ld), uint64_t(wr.ld) * uint64_t(w_rows)};
-        const uint32_t box[3] = {128, 128, 1};
-        encode_tensor_map_u8(&p.map_a, wr.ptr, 3, dims, strides, box, TmaSwizzle::B128);
-    }
-    {
-        const uint64_t dims[2] = {uint64_t(k), uint64_t(m)};
-        const uint64_t strides[1] = {uint64_t(xr.ld)};
+    } else {
+        Fp8FewParams p{};
+        fill(p);
         for (uint32_t i = 0; i < 5; ++i) {
-            const uint32_t box[2] = {128, i < 4 ? 32 * (i + 1) : 16};
-            encode_tensor_map_u8(i < 4 ? &p.x.box[i] : &p.x.box16, xr.ptr, 2, dims, strides, box, TmaSwizzle::B128);
+            const uint32_t rows_box[2] = {128, i < 4 ? 32 * (i + 1) : 16};
+            encode_tensor_map_u8(i < 4 ? &p.x.box[i] : &p.x.box16, xr.ptr, 2, x_dims, x_strides, rows_box, TmaSwizzle::B128);
         }
+        if (y_type == TYPE_F32) launch_few<FORM, float>(p, stream);
+        else if (y_type == TYPE_F16) launch_few<FORM, __half>(p, stream);
+        else launch_few<FORM, __nv_bfloat16>(p, stream);
     }
-    p.x_scales = x_scales;
-    p.w_scales = w_scales;
-    const long long scale_cols = (w_cols + FP8_BLOCK - 1) / FP8_BLOCK;
-    p.ws_feature = nn ? 1 : scale_cols;
-    p.ws_k = nn ? scale_cols : 1;
-    p.bias = bias;
-    p.act = act;
-    p.c = y;
-    p.groups = 1;
-    p.rows = m;
-    p.features = n;
-    p.k = k;
-    const RaggedPlan plan = plan_rows(1, m, n);
-    if (y_type == TYPE_F32) launch_out<FORM, float>(p, plan, stream);
-    else if (y_type == TYPE_F16) launch_out<FORM, __half>(p, plan, stream);
-    else launch_out<FORM, __nv_bfloat16>(p, plan, stream);
 }
 
 }  // namespace
