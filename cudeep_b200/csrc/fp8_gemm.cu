@@ -5,37 +5,91 @@
 #include "fp8_rows.cuh"
 #include "ragged_plan.h"
 
+#include <map>
+#include <mutex>
+#include <utility>
+
 namespace cudeep_b200 {
 
 namespace {
 
-// CTAs that share a tile of 128 features: as many as the device has SMs for, while each keeps four blocks of K.
-int cluster_split(int features, int k) {
-    const int tiles = (features + 127) / 128, blocks = (k + FP8_BK - 1) / FP8_BK;
-    int split = 1;
-    while (split < 8 && tiles * split * 2 <= device_info().num_sms && blocks >= 8 * split) split *= 2;
-    return split;
+struct FewPlan {
+    int step;       // features per tile
+    int split;      // CTAs per tile, each with a range of K
+};
+
+// Clusters of `size` CTAs, an SM each, that the device runs at once: fewer than SMs / size, as a cluster lies within one
+// part of the chip.  (148 CTAs as 37 clusters of four took two turns: 1 row, 4096 -> 4096 13.2 us, 128 CTAs 8.1 us.)
+int resident_clusters(int size) {
+    static std::mutex mu;
+    static std::map<std::pair<int, int>, int> known;
+    const DeviceInfo& dev = device_info();
+    if (size == 1) return dev.num_sms;
+    std::lock_guard<std::mutex> lock(mu);
+    const auto key = std::make_pair(dev.device, size);
+    const auto at = known.find(key);
+    if (at != known.end()) return at->second;
+    auto kernel = fp8_few_kernel<RaggedForm::NT, float>;
+    ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), FP8F_SMEM_BUDGET + 1024);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(size), 1, 1);
+    cfg.blockDim = dim3(FP8F_THREADS, 1, 1);
+    cfg.dynamicSmemBytes = FP8F_SMEM_BUDGET + 1024;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = unsigned(size);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int count = 0;
+    CB200_CUDA(cudaOccupancyMaxActiveClusters(&count, kernel, &cfg));
+    return known[key] = count < 1 ? 1 : count;
+}
+
+// The cheapest of all steps and splits by what an SM's stream of operands costs, in cycles: 20 bytes of weights a cycle (they
+// come from HBM), 40 of rows (from L2, read by every tile), and fixed costs of a wave and of adding up a split tile.
+FewPlan plan_few(int rows, int features, int k) {
+    const int blocks = (k + FP8_BK - 1) / FP8_BK;
+    const int loaded = RowMaps::loaded((rows + 15) / 16 * 16);
+    FewPlan best{128, 1};
+    double best_cost = 1e30;
+    for (int step = 128; step >= 64; step -= 16) {
+        for (int split = 1; split <= 8; split *= 2) {
+            if (split > 1 && blocks < 4 * split) break;      // four blocks of K for each CTA at least
+            const long long tiles = (features + step - 1) / step, resident = resident_clusters(split);
+            const long long waves = (tiles + resident - 1) / resident;
+            const double per_block = step * 128 / 20.0 + loaded * 128 / 40.0;
+            const double cost = waves * ((blocks + split - 1) / split * per_block + 3000.0 + (split > 1 ? 2000.0 + 20.0 * rows : 0.0));
+            if (cost < best_cost * 0.98) {
+                best_cost = cost;
+                best = FewPlan{step, split};
+            }
+        }
+    }
+    return best;
 }
 
 template <RaggedForm FORM, class OutT>
 void launch_few(Fp8FewParams& p, cudaStream_t stream) {
     const DeviceInfo& dev = device_info();
     CB200_REQUIRE(dev.cc_major == 10, "8-bit products need an sm_100 device");
-    p.split = cluster_split(p.features, p.k);
+    p.w_bytes = FORM == RaggedForm::NT ? uint32_t(p.step) * 128u : RAGGED_A_BYTES;
     p.stage_bytes = RAGGED_A_BYTES + uint32_t(RowMaps::loaded((p.rows + 15) / 16 * 16)) * 128u;
     const int fit = int(FP8F_SMEM_BUDGET / p.stage_bytes);
     p.stages = fit < FP8F_MAX_STAGES ? fit : FP8F_MAX_STAGES;
     p.status = dev.status_word;
     p.wait_limit_ns = 2000000000ull;
-    const long long tiles = (p.features + 127) / 128;
-    CB200_TRACE("fp8 %s tcgen05, features on lanes: rows=%d features=%d k=%d stages=%d tiles=%lld split=%d",
-                FORM == RaggedForm::NT ? "nt" : "nn", p.rows, p.features, p.k, p.stages, tiles, p.split);
+    const long long tiles = (p.features + p.step - 1) / p.step;
+    CB200_TRACE("fp8 %s tcgen05, features on lanes: rows=%d features=%d k=%d stages=%d tiles=%lld step=%d split=%d",
+                FORM == RaggedForm::NT ? "nt" : "nn", p.rows, p.features, p.k, p.stages, tiles, p.step,
+                p.split);
     launch_clusters(fp8_few_kernel<FORM, OutT>, p, tiles, p.split, FP8F_THREADS, uint32_t(p.stages) * p.stage_bytes + 1024,
                     FP8F_SMEM_BUDGET + 1024, stream);
 }
 
-template <RaggedForm FORM, class OutT>
-void launch_by_rows(Fp8RowsParams& p, cudaStream_t stream) {
+template <RaggedForm FORM, int BN, class OutT>
+void launch_by_rows_bn(Fp8RowsParams& p, cudaStream_t stream) {
     const DeviceInfo& dev = device_info();
     CB200_REQUIRE(dev.cc_major == 10, "8-bit products need an sm_100 device");
     p.tma_store = (size_t(p.features) * sizeof(OutT)) % 16 == 0 && reinterpret_cast<uintptr_t>(p.c) % 16 == 0;
@@ -49,13 +103,26 @@ void launch_by_rows(Fp8RowsParams& p, cudaStream_t stream) {
     p.status = dev.status_word;
     p.wait_limit_ns = 2000000000ull;
     p.tiles_m = (p.rows + 255) / 256;
-    p.tiles_n = (p.features + 255) / 256;
+    p.tiles_n = (p.features + BN - 1) / BN;
     const long long tiles = (long long)p.tiles_m * p.tiles_n;
     const long long clusters = tiles < dev.num_sms / 2 ? tiles : dev.num_sms / 2;
-    CB200_TRACE("fp8 %s tcgen05, rows on lanes: rows=%d features=%d k=%d tile=256x256 stages=%d clusters=%lld store=%s",
-                FORM == RaggedForm::NT ? "nt" : "nn", p.rows, p.features, p.k, FP8R_STAGES, clusters,
+    CB200_TRACE("fp8 %s tcgen05, rows on lanes: rows=%d features=%d k=%d tile=256x%d stages=%d clusters=%lld store=%s",
+                FORM == RaggedForm::NT ? "nt" : "nn", p.rows, p.features, p.k, BN, FP8R_STAGES, clusters,
                 p.tma_store ? "bulk-tensor" : "rows");
-    launch_clusters(fp8_rows_kernel<FORM, OutT>, p, clusters, 2, FP8R_THREADS, FP8R_SMEM_BYTES, FP8R_SMEM_BYTES, stream);
+    launch_clusters(fp8_rows_kernel<FORM, BN, OutT>, p, clusters, 2, FP8R_THREADS, FP8R_SMEM_BYTES, FP8R_SMEM_BYTES, stream);
+}
+
+// Tiles of 256 rows x 256 features; of 128 features where even those do not outnumber the pairs of SMs.
+bool narrow_tiles(int m, int n) {
+    return (long long)((m + 255) / 256) * ((n + 127) / 128) <= device_info().num_sms / 2;
+}
+
+template <RaggedForm FORM, class OutT>
+void launch_by_rows(Fp8RowsParams& p, bool narrow, cudaStream_t stream) {
+    if constexpr (FORM == RaggedForm::NT) {
+        if (narrow) return launch_by_rows_bn<FORM, 128, OutT>(p, stream);
+    }
+    launch_by_rows_bn<FORM, 256, OutT>(p, stream);
 }
 
 // x[m, k] by w, stored [n, k] (NT: features n) or [k, n] (NN: features n).
@@ -87,12 +154,24 @@ void product(const uint8_t* x, const float* x_scales, const uint8_t* w, const fl
         Fp8RowsParams p{};
         fill(p);
         encode_tensor_map_u8(&p.map_x, xr.ptr, 2, x_dims, x_strides, box, TmaSwizzle::B128);
-        if (y_type == TYPE_F32) launch_by_rows<FORM, float>(p, stream);
-        else if (y_type == TYPE_F16) launch_by_rows<FORM, __half>(p, stream);
-        else launch_by_rows<FORM, __nv_bfloat16>(p, stream);
+        const bool narrow = !nn && narrow_tiles(m, n);
+        if (narrow) {
+            const uint32_t w_box[2] = {128, 64};
+            encode_tensor_map_u8(&p.map_w, wr.ptr, 2, w_dims, w_strides, w_box, TmaSwizzle::B128);
+        }
+        if (y_type == TYPE_F32) launch_by_rows<FORM, float>(p, narrow, stream);
+        else if (y_type == TYPE_F16) launch_by_rows<FORM, __half>(p, narrow, stream);
+        else launch_by_rows<FORM, __nv_bfloat16>(p, narrow, stream);
     } else {
         Fp8FewParams p{};
         fill(p);
+        const FewPlan plan = plan_few(m, n, k);
+        p.step = plan.step;
+        p.split = plan.split;
+        if (!nn) {
+            const uint32_t w_box[2] = {128, uint32_t(plan.step)};
+            encode_tensor_map_u8(&p.map_w, wr.ptr, 2, w_dims, w_strides, w_box, TmaSwizzle::B128);
+        }
         for (uint32_t i = 0; i < 5; ++i) {
             const uint32_t rows_box[2] = {128, i < 4 ? 32 * (i + 1) : 16};
             encode_tensor_map_u8(i < 4 ? &p.x.box[i] : &p.x.box16, xr.ptr, 2, x_dims, x_strides, rows_box, TmaSwizzle::B128);

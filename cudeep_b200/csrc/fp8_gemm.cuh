@@ -71,7 +71,8 @@ __device__ __forceinline__ void fp8_activation(float (&v)[N], const Fp8Activatio
 // For up to 128 rows the FEATURES lie on the 128 lanes and the rows on the columns: the width of the MMA follows the number
 // of rows, and a CTA streams its 128 features' weights once, which is all such a product costs.  One tile per CTA; where the
 // features make fewer tiles than the device has SMs, a cluster of up to eight CTAs shares a tile, each with a range of K,
-// and adds the parts up through distributed shared memory in rank order.
+// and adds the parts up through distributed shared memory in rank order.  A tile may take fewer than 128 features (the last
+// lanes then idle), so that the tiles fill the SMs: 16384 features are 128 tiles of 128, but 147 of 112.
 //
 // The factors xs * ws change along the columns here: each epilogue warp fetches those of its columns four blocks ahead and
 // reads them back from shared memory.  With so few columns TMEM holds up to eight accumulators, so the tensor core runs
@@ -85,7 +86,7 @@ constexpr int FP8F_MAX_BUFFERS = 8;
 constexpr uint32_t FP8F_SMEM_BUDGET = 232448 - 1024 - 6 * 1024;   // minus alignment slack, factors and barriers
 
 struct Fp8FewParams {
-    CUtensorMap map_w;       // NT {K, F}, NN {F, K}: box {128, 128}
+    CUtensorMap map_w;       // NT {K, F} box {128, step}; NN {F, K} box {128, 128}
     RowMaps x;               // {K, rows}
     const float* x_scales;   // [K blocks][rows]
     const float* w_scales;   // + feature block * ws_feature + K block * ws_k
@@ -97,6 +98,8 @@ struct Fp8FewParams {
     int features;
     int k;
     int split;               // CTAs per tile
+    int step;                // features per tile, a multiple of 16 up to 128
+    uint32_t w_bytes;        // of a stage
     int stages;
     uint32_t stage_bytes;
     uint32_t* status;
@@ -125,7 +128,8 @@ __global__ void __launch_bounds__(FP8F_THREADS, 1) fp8_few_kernel(const __grid_c
 
     const int split = p.split;
     const uint32_t rank = split > 1 ? ptx::cluster_ctarank() : 0u;
-    const int feature0 = int(blockIdx.x) / split * 128;
+    const int feature0 = int(blockIdx.x) / split * p.step;
+    const int f_end = min(p.features, feature0 + p.step);
     const int umma_n = (p.rows + 15) / 16 * 16;
     const int buf_cols = (p.rows + 31) / 32 * 32;
     const int buffers = min(FP8F_MAX_BUFFERS, 512 / buf_cols);
@@ -172,7 +176,7 @@ __global__ void __launch_bounds__(FP8F_THREADS, 1) fp8_few_kernel(const __grid_c
         // ------------------------------------------------------------ producer
         if (lane == 0) {
             uint32_t stage = 0, phase = 0;
-            const uint32_t bytes = RAGGED_A_BYTES + uint32_t(RowMaps::loaded(umma_n)) * 128u;
+            const uint32_t bytes = p.w_bytes + uint32_t(RowMaps::loaded(umma_n)) * 128u;
             for (int kb = 0; kb < blocks; ++kb) {
                 if (!ptx::mbar_wait(ptx::smem_u32(&bar_empty[stage]), phase ^ 1u, wctx, UMMA_TIMEOUT_PRODUCER)) break;
                 const uint32_t a_smem = smem_base + stage * p.stage_bytes;
@@ -217,7 +221,8 @@ __global__ void __launch_bounds__(FP8F_THREADS, 1) fp8_few_kernel(const __grid_c
         // ------------------------------------------------------------ sums
         float* mine = &factors[warp - 2][0][0];
         const float* xs = p.x_scales + (long long)kb0 * p.rows + c_begin;
-        const float* ws = p.w_scales + (feature0 / 128) * p.ws_feature + kb0 * p.ws_k;
+        // A tile's features may belong to two blocks of scales; lanes behind the last feature take some that exist.
+        const float* ws = p.w_scales + (min(feature, p.features - 1) / 128) * p.ws_feature + kb0 * p.ws_k;
         float px[4][2], pw[4];
         auto fetch = [&](int kb, float (&x)[2], float& w) {
             w = kb < blocks ? __ldg(ws + kb * p.ws_k) : 0.0f;
@@ -242,8 +247,9 @@ __global__ void __launch_bounds__(FP8F_THREADS, 1) fp8_few_kernel(const __grid_c
                 const int kb = kb4 + d;
                 if (kb >= blocks) break;
                 float* f = mine + (d & 1) * 64;
-                f[lane] = px[d][0] * pw[d];
-                f[lane + 32] = px[d][1] * pw[d];
+                const float w = pw[d];
+                f[lane] = px[d][0];
+                f[lane + 32] = px[d][1];
                 __syncwarp();
                 fetch(kb + 4, px[d], pw[d]);
                 ok = ptx::mbar_wait(ptx::smem_u32(&bar_acc_full[buf]), buf_phase, wctx, UMMA_TIMEOUT_EPILOGUE);
@@ -260,8 +266,8 @@ __global__ void __launch_bounds__(FP8F_THREADS, 1) fp8_few_kernel(const __grid_c
 #pragma unroll
                         for (int j = 0; j < 16; j += 4) {
                             const float4 sc = *reinterpret_cast<const float4*>(f + 16 * i + j);
-                            fma2(acc[i][j], acc[i][j + 1], r[j], r[j + 1], sc.x, sc.y);
-                            fma2(acc[i][j + 2], acc[i][j + 3], r[j + 2], r[j + 3], sc.z, sc.w);
+                            fma2(acc[i][j], acc[i][j + 1], r[j], r[j + 1], sc.x * w, sc.y * w);
+                            fma2(acc[i][j + 2], acc[i][j + 3], r[j + 2], r[j + 3], sc.z * w, sc.w * w);
                         }
                     }
                 }
@@ -274,7 +280,7 @@ __global__ void __launch_bounds__(FP8F_THREADS, 1) fp8_few_kernel(const __grid_c
         const Fp8Activation act(p.act);
         const int stored = min(c_count, p.rows - c_begin);
         if (split == 1) {
-            if (feature < p.features) {
+            if (feature < f_end) {
                 const float bias = p.bias != nullptr ? __ldg(p.bias + feature) : 0.0f;
                 OutT* dst = static_cast<OutT*>(p.c) + (long long)c_begin * p.features + feature;
 #pragma unroll
@@ -305,18 +311,39 @@ __global__ void __launch_bounds__(FP8F_THREADS, 1) fp8_few_kernel(const __grid_c
         ptx::cluster_arrive();
         ptx::cluster_wait();
         if (warp >= 2) {
-            // Rank r finishes columns r, r + split, ...: two at a time, 128 threads each.
+            // Rank r finishes columns r, r + split, ...: a warp takes a column, four features a lane, and reads the parts of
+            // all ranks of two columns at once.
             const Fp8Activation act(p.act);
-            const int f_in = int(threadIdx.x - 64) & 127;
-            const int f = feature0 + f_in;
-            const float bias = p.bias != nullptr && f < p.features ? __ldg(p.bias + f) : 0.0f;
-            for (int c = int(rank) + split * (int(threadIdx.x - 64) >> 7); c < p.rows; c += 2 * split) {
-                float v[2] = {0.0f, 0.0f};
-                for (int s = 0; s < split; ++s)
-                    v[0] += ptx::ld_cluster_f32(ptx::mapa(smem_base + (uint32_t(c) * 128u + uint32_t(f_in)) * 4u, uint32_t(s)));
-                v[0] += bias;
-                fp8_activation(v, act);
-                if (f < p.features) static_cast<OutT*>(p.c)[(long long)c * p.features + f] = round_to<OutT>(v[0]);
+            const int f_in = 4 * int(lane), f = feature0 + f_in;
+            float bias[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) bias[j] = p.bias != nullptr && f + j < f_end ? __ldg(p.bias + f + j) : 0.0f;
+            const int step = split * FP8F_EPI_WARPS;
+            for (int c = int(rank) + split * int(warp - 2); c < p.rows; c += 2 * step) {
+                float v[2][4] = {};
+                for (int s = 0; s < split; ++s) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int cc = c + i * step < p.rows ? c + i * step : c;
+                        const float4 q = ptx::ld_cluster_v4(
+                            ptx::mapa(smem_base + (uint32_t(cc) * 128u + uint32_t(f_in)) * 4u, uint32_t(s)));
+                        v[i][0] += q.x;
+                        v[i][1] += q.y;
+                        v[i][2] += q.z;
+                        v[i][3] += q.w;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    if (c + i * step >= p.rows) break;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[i][j] += bias[j];
+                    fp8_activation(v[i], act);
+                    OutT* dst = static_cast<OutT*>(p.c) + (long long)(c + i * step) * p.features + f;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (f + j < f_end) dst[j] = round_to<OutT>(v[i][j]);
+                }
             }
         }
         __syncwarp();

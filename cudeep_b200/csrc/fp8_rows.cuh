@@ -27,7 +27,7 @@ constexpr uint32_t FP8R_SMEM_BYTES = FP8R_STAGES * FP8R_STAGE_BYTES + FP8R_STAGI
 
 struct Fp8RowsParams {
     CUtensorMap map_x;       // {K, rows} box {128, 128}
-    CUtensorMap map_w;       // NT {K, F}, NN {F, K}: box {128, 128}
+    CUtensorMap map_w;       // NT {K, F} box {128, BN / 2}; NN {F, K} box {128, 128}
     CUtensorMap map_c;       // {F, rows} box {128 bytes, 32}; used when `tma_store`
     const float* x_scales;   // [K blocks][rows]
     const float* w_scales;   // + feature block * ws_feature + K block * ws_k
@@ -66,11 +66,14 @@ __device__ __forceinline__ void st_shared_u4(uint32_t addr, uint32_t x, uint32_t
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
-template <RaggedForm FORM, class OutT>
+template <RaggedForm FORM, int BN, class OutT>
 __global__ void __launch_bounds__(FP8R_THREADS, 1) fp8_rows_kernel(const __grid_constant__ Fp8RowsParams p) {
 #if defined(__CUDA_ARCH_FEAT_SM100_ALL) || defined(__CUDA_ARCH_FEAT_SM101_ALL) || \
     defined(__CUDA_ARCH_FEAT_SM103_ALL)
     constexpr bool B_MN = FORM == RaggedForm::NN;
+    static_assert(BN == 256 || (BN == 128 && !B_MN), "a row of features in a box is one 128-byte swizzle row");
+    constexpr int CHUNKS = BN / 32;      // of 16 columns, per epilogue warp (half of the tile's columns)
+    constexpr uint32_t TX_BYTES = 2 * 16384 + BN * 128;
 
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bar_full[FP8R_STAGES];
@@ -130,13 +133,13 @@ __global__ void __launch_bounds__(FP8R_THREADS, 1) fp8_rows_kernel(const __grid_
                     int tm, tn;
                     raster_coords(u, p.tiles_m, p.tiles_n, 8, tm, tn);
                     const int row = (tm * 2 + int(cta_rank)) * 128;
-                    const int feature = tn * 256 + int(cta_rank) * 128;
+                    const int feature = tn * BN + int(cta_rank) * (BN / 2);
                     for (int kb = 0; kb < k_blocks; ++kb) {
                         if (!ptx::mbar_wait(ptx::smem_u32(&bar_empty[stage]), phase ^ 1u, wctx, UMMA_TIMEOUT_PRODUCER))
                             goto producer_done;
                         const uint32_t a_smem = smem_base + stage * FP8R_STAGE_BYTES;
                         const uint32_t full_local = ptx::smem_u32(&bar_full[stage]);
-                        if (is_leader) ptx::mbar_arrive_expect_tx(full_local, 2 * FP8R_STAGE_BYTES);
+                        if (is_leader) ptx::mbar_arrive_expect_tx(full_local, TX_BYTES);
                         const uint32_t full = ptx::mapa(full_local, 0);
                         const int k0 = kb * FP8_BK;
                         ptx::tma_load_2d_pair(a_smem, &p.map_x, full, k0, row);
@@ -150,7 +153,7 @@ __global__ void __launch_bounds__(FP8R_THREADS, 1) fp8_rows_kernel(const __grid_
         } else if (warp == 1 && is_leader) {
             // -------------------------------------------------------- MMA issuer
             constexpr uint32_t B_KSTEP = B_MN ? 4096u : 32u;
-            constexpr uint32_t idesc = ptx::idesc_e4m3(256, 256, 0, B_MN ? 1 : 0);
+            constexpr uint32_t idesc = ptx::idesc_e4m3(256, BN, 0, B_MN ? 1 : 0);
             const uint64_t a_desc0 = ptx::smem_desc_at(ptx::smem_desc(16, 1024, ptx::SMEM_LAYOUT_SW128), smem_base);
             const uint64_t b_desc0 =
                 ptx::smem_desc_at(ptx::smem_desc(B_MN ? 16384 : 16, 1024, ptx::SMEM_LAYOUT_SW128), smem_base + 16384);
@@ -200,13 +203,13 @@ __global__ void __launch_bounds__(FP8R_THREADS, 1) fp8_rows_kernel(const __grid_
             raster_coords(u, p.tiles_m, p.tiles_n, 8, tm, tn);
             const int row0 = (tm * 2 + int(cta_rank)) * 128 + int(quarter) * 32;
             const int row = row0 + int(lane);
-            const int feature0 = tn * 256 + half * 128;
+            const int feature0 = tn * BN + half * (BN / 2);
             // Rows and features outside the matrices take some factor that exists; what it makes is not stored.
             const float* xs = p.x_scales + (row < p.rows ? row : 0);
             const float* ws = p.w_scales + (feature0 < p.features ? feature0 / 128 : 0) * p.ws_feature;
-            float acc[4][32];
+            float acc[BN / 64][32];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < BN / 64; ++i)
 #pragma unroll
                 for (int j = 0; j < 32; ++j) acc[i][j] = 0.0f;
             // The factors come four blocks ahead: a block takes 500 cycles and a load from L2 under this traffic longer.
@@ -231,13 +234,13 @@ __global__ void __launch_bounds__(FP8R_THREADS, 1) fp8_rows_kernel(const __grid_
                 const bool ok = ptx::mbar_wait(ptx::smem_u32(&bar_acc_full[buf]), (it >> 1) & 1, wctx, UMMA_TIMEOUT_EPILOGUE);
                 if (!__all_sync(0xffffffffu, ok)) goto epilogue_done;
                 ptx::tc_fence_after();
-                const uint32_t t_row = tmem_base + buf * 256u + uint32_t(half) * 128u + ((quarter * 32u) << 16);
+                const uint32_t t_row = tmem_base + buf * 256u + uint32_t(half) * uint32_t(BN / 2) + ((quarter * 32u) << 16);
                 uint32_t r[2][16];
                 ptx::tmem_ld_32x16(t_row, r[0]);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 0; i < CHUNKS; ++i) {
                     ptx::tmem_ld_wait();
-                    if (i < 7) {
+                    if (i + 1 < CHUNKS) {
                         ptx::tmem_ld_32x16(t_row + 16 * (i + 1), r[(i + 1) & 1]);
                     } else {
                         ptx::tc_fence_before();
@@ -249,7 +252,10 @@ __global__ void __launch_bounds__(FP8R_THREADS, 1) fp8_rows_kernel(const __grid_
                         }
                     }
 #pragma unroll
-                    for (int j = 0; j < 16; j += 2) fma2(acc[i >> 1][(i & 1) * 16 + j], acc[i >> 1][(i & 1) * 16 + j + 1], r[i & 1][j], r[i & 1][j + 1], s, s);
+                    for (int j = 0; j < 16; j += 2) {
+                        float* sum = &acc[i >> 1][(i & 1) * 16 + j];
+                        fma2(sum[0], sum[1], r[i & 1][j], r[i & 1][j + 1], s, s);
+                    }
                 }
                 ++it;
               }
@@ -257,7 +263,7 @@ __global__ void __launch_bounds__(FP8R_THREADS, 1) fp8_rows_kernel(const __grid_
             constexpr int V = 16 / sizeof(OutT);              // values per 16 bytes
             constexpr int COLS = 128 / sizeof(OutT);          // columns of a staged block: 128 bytes per row
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < BN / 64; ++i) {
                 if (p.bias != nullptr) {
 #pragma unroll
                     for (int j = 0; j < 32; ++j) {

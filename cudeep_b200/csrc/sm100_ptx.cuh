@@ -83,10 +83,13 @@ __device__ __forceinline__ void st_async_v4(uint32_t cluster_addr, uint32_t x, u
                  ::"r"(cluster_addr), "r"(x), "r"(y), "r"(z), "r"(w), "r"(cluster_bar)
                  : "memory");
 }
-// One word from the shared memory of a CTA of the cluster (address from mapa).
-__device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+// 16 bytes from the shared memory of a CTA of the cluster (address from mapa).
+__device__ __forceinline__ float4 ld_cluster_v4(uint32_t cluster_addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(cluster_addr)
+                 : "memory");
     return v;
 }
 __device__ __forceinline__ float4 ld_shared_v4(uint32_t addr) {
