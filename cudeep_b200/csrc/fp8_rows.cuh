@@ -49,23 +49,6 @@ __device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.
 template <int REGS>
 __device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS)); }
 
-template <class T>
-__device__ __forceinline__ uint32_t pack2(float a, float b);
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
-    const __half2 v = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-
-__device__ __forceinline__ void st_shared_u4(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
-}
-
 template <RaggedForm FORM, int BN, class OutT>
 __global__ void __launch_bounds__(FP8R_THREADS, 1) fp8_rows_kernel(const __grid_constant__ Fp8RowsParams p) {
 #if defined(__CUDA_ARCH_FEAT_SM100_ALL) || defined(__CUDA_ARCH_FEAT_SM101_ALL) || \
@@ -260,7 +243,6 @@ __global__ void __launch_bounds__(FP8R_THREADS, 1) fp8_rows_kernel(const __grid_
                 ++it;
               }
             }
-            constexpr int V = 16 / sizeof(OutT);              // values per 16 bytes
             constexpr int COLS = 128 / sizeof(OutT);          // columns of a staged block: 128 bytes per row
 #pragma unroll
             for (int i = 0; i < BN / 64; ++i) {
@@ -277,16 +259,7 @@ __global__ void __launch_bounds__(FP8R_THREADS, 1) fp8_rows_kernel(const __grid_
                     if (lane == 0) ptx::bulk_wait_group_read<0>();      // the block's last store has read it
                     __syncwarp();
                 }
-#pragma unroll
-                for (int j = 0; j < 32; j += V) {
-                    const uint32_t unit = uint32_t(32 * i - c0 + j) / V;
-                    const uint32_t dst = staging + lane * 128u + ((unit ^ (lane & 7u)) << 4);
-                    if constexpr (sizeof(OutT) == 4)
-                        ptx::st_shared_v4(dst, acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3]);
-                    else
-                        st_shared_u4(dst, pack2<OutT>(acc[i][j], acc[i][j + 1]), pack2<OutT>(acc[i][j + 2], acc[i][j + 3]),
-                                     pack2<OutT>(acc[i][j + 4], acc[i][j + 5]), pack2<OutT>(acc[i][j + 6], acc[i][j + 7]));
-                }
+                stage_block<OutT>(staging, lane, 32 * i - c0, acc[i]);
                 if (32 * (i + 1) - c0 == COLS) {              // the block is full
                     const int f0 = feature0 + c0;
                     if (p.tma_store) {
@@ -299,27 +272,8 @@ __global__ void __launch_bounds__(FP8R_THREADS, 1) fp8_rows_kernel(const __grid_
                     } else {
                         // Rows of C that are no 16-byte multiples: the warp writes them one by one.
                         __syncwarp();
-                        const int f = f0 + int(lane);
-                        OutT* dst = static_cast<OutT*>(p.c) + (long long)row0 * p.features + f;
-                        for (int r = 0; r < 32 && row0 + r < p.rows; ++r, dst += p.features) {
-#pragma unroll
-                            for (int h = 0; h < COLS / 32; ++h) {
-                                const uint32_t byte = uint32_t(lane + 32 * h) * sizeof(OutT);
-                                const uint32_t at = staging + uint32_t(r) * 128u + (((byte >> 4) ^ (uint32_t(r) & 7u)) << 4) + (byte & 15u);
-                                if (f + 32 * h < p.features) {
-                                    if constexpr (sizeof(OutT) == 4) {
-                                        uint32_t v;
-                                        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
-                                        reinterpret_cast<uint32_t*>(dst)[32 * h] = v;
-                                    } else {
-                                        uint16_t v;
-                                        asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
-                                        reinterpret_cast<uint16_t*>(dst)[32 * h] = v;
-                                    }
-                                }
-                            }
-                        }
-                        __syncwarp();
+                        OutT* dst = static_cast<OutT*>(p.c) + (long long)row0 * p.features + f0;
+                        write_block<OutT>(staging, lane, dst, p.features, min(32, p.rows - row0), p.features - f0, false);
                     }
                 }
             }

@@ -23,13 +23,14 @@ void launch(RaggedParams& p, const RaggedPlan& plan, cudaStream_t stream) {
     CB200_REQUIRE(dev.cc_major == 10, "grouped products need an sm_100 device");
     p.tile_cols = plan.tile_cols;
     p.stage_bytes = RAGGED_A_BYTES + uint32_t(RowMaps::loaded(plan.tile_cols / CTAS)) * 128u;
-    const int fit = int(RAGGED_SMEM_BUDGET / p.stage_bytes);
+    const uint32_t staging_bytes = FORM == RaggedForm::TN ? RAGGED_STAGING_BYTES : 0u;
+    const int fit = int((RAGGED_SMEM_BUDGET - staging_bytes) / p.stage_bytes);
     p.stages = fit < RAGGED_MAX_STAGES ? fit : RAGGED_MAX_STAGES;
     p.status = dev.status_word;
     p.wait_limit_ns = 2000000000ull;
     long long clusters = dev.num_sms / CTAS;
     if (clusters > plan.units) clusters = plan.units;
-    const uint32_t smem_bytes = uint32_t(p.stages) * p.stage_bytes + 1024;
+    const uint32_t smem_bytes = uint32_t(p.stages) * p.stage_bytes + staging_bytes + 1024;
     CB200_TRACE("grouped %s %s tcgen05: rows=%d groups=%d features=%d %s=%d tile=%dx%d stages=%d clusters=%lld",
                 FORM == RaggedForm::NT ? "nt" : FORM == RaggedForm::NN ? "nn" : "tn", BF16 ? "bf16" : "f16", p.rows, p.groups,
                 p.features, FORM == RaggedForm::TN ? "cols" : "k", FORM == RaggedForm::TN ? p.cols : p.k, 128 * CTAS,
@@ -126,6 +127,15 @@ void grouped_tn(const void* a, long long lda, const void* b, long long ldb, void
         const uint32_t box[2] = {64, 64}, box16[2] = {64, 16};
         encode_tensor_map_f16(&p.map_b, x.ptr, 2, dims, strides, box, TmaSwizzle::B128);
         encode_tensor_map_f16(&p.map_b16, x.ptr, 2, dims, strides, box16, TmaSwizzle::B128);
+    }
+    const uint32_t c_bytes = uint32_t(elem_bytes(c_type));
+    p.tma_store = (size_t(n) * c_bytes) % 16 == 0 && reinterpret_cast<uintptr_t>(c) % 16 == 0;
+    if (p.tma_store) {
+        const uint64_t dims[3] = {uint64_t(n), uint64_t(m), uint64_t(groups)};
+        const uint64_t strides[2] = {uint64_t(n) * c_bytes, uint64_t(n) * c_bytes * uint64_t(m)};
+        const uint32_t box[3] = {128 / c_bytes, 32, 1};
+        if (c_type == TYPE_F32) encode_tensor_map(&p.map_c, static_cast<const float*>(c), 3, dims, strides, box, TmaSwizzle::B128);
+        else encode_tensor_map_f16(&p.map_c, c, 3, dims, strides, box, TmaSwizzle::B128);
     }
     p.a = y.ptr;
     p.b = x.ptr;

@@ -31,6 +31,7 @@ enum class RaggedForm { NT, NN, TN };
 
 constexpr int RAGGED_MAX_GROUPS = 1024;
 constexpr int RAGGED_BK = 64;                        // 16-bit elements per K block = one 128-byte swizzle row
+constexpr uint32_t RAGGED_STAGING_BYTES = 4 * 4096;   // TN: a block of 32 rows x 128 bytes per epilogue warp
 constexpr uint32_t RAGGED_A_BYTES = 128 * 128;       // one CTA's features of a K block
 constexpr int RAGGED_MAX_STAGES = 12;
 constexpr uint32_t RAGGED_SMEM_BUDGET = 232448 - 1024 - 13 * 1024;   // minus alignment slack, group tables and barriers
@@ -64,6 +65,8 @@ struct RaggedParams {
     RowMaps x;               // NT, NN {K, rows}
     CUtensorMap map_b;       // TN {C, rows} box {64, 64}
     CUtensorMap map_b16;     // TN {C, rows} box {64, 16}
+    CUtensorMap map_c;       // TN: {C, F, G} box {128 bytes, 32, 1}, where rows of C are 16-byte multiples
+    int tma_store;           // ... and whether it is so
     const void* a;           // TN: the operands' addresses and row lengths, for the partial last step
     const void* b;
     long long lda, ldb;
@@ -129,6 +132,57 @@ struct RaggedWalk {
         return t;
     }
 };
+
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// A warp's block of 32 rows x 128 bytes in shared memory, 16-byte unit q of row r at q ^ (r & 7) (the 128-byte swizzle of a
+// tensor map): lane `lane` writes 32 values of its row from column `col` of the block on, rounded to T.
+template <class T>
+__device__ __forceinline__ void stage_block(uint32_t block, uint32_t lane, int col, const float (&v)[32]) {
+    constexpr int V = 16 / sizeof(T);
+#pragma unroll
+    for (int j = 0; j < 32; j += V) {
+        const uint32_t dst = block + lane * 128u + (((uint32_t(col + j) / V) ^ (lane & 7u)) << 4);
+        if constexpr (sizeof(T) == 4)
+            ptx::st_shared_v4(dst, v[j], v[j + 1], v[j + 2], v[j + 3]);
+        else
+            ptx::st_shared_u4(dst, pack2<T>(v[j], v[j + 1]), pack2<T>(v[j + 2], v[j + 3]), pack2<T>(v[j + 4], v[j + 5]),
+                              pack2<T>(v[j + 6], v[j + 7]));
+    }
+}
+
+// Writes (or adds: FP32) the first `rows` rows and `cols` columns of such a block to dst, whole warp, row by row.
+template <class T>
+__device__ __forceinline__ void write_block(uint32_t block, uint32_t lane, T* dst, long long ld, int rows, int cols, bool add) {
+    for (int r = 0; r < rows; ++r, dst += ld) {
+#pragma unroll
+        for (int h = 0; h < int(128 / sizeof(T)) / 32; ++h) {
+            const int c = int(lane) + 32 * h;
+            const uint32_t byte = uint32_t(c) * sizeof(T);
+            const uint32_t at = block + uint32_t(r) * 128u + (((byte >> 4) ^ (uint32_t(r) & 7u)) << 4) + (byte & 15u);
+            if (c < cols) {
+                if constexpr (sizeof(T) == 4) {
+                    const float v = ptx::ld_shared_f32(at);
+                    dst[c] = add ? dst[c] + v : v;
+                } else {
+                    reinterpret_cast<uint16_t*>(dst)[c] = ptx::ld_shared_u16(at);
+                }
+            }
+        }
+    }
+    __syncwarp();
+}
 
 // One warp: the row range of each group, brought into [0, rows], and the number of tiles before it.  col_tiles >= 0:
 // column tiles of every group (TN); otherwise -col_tiles is the number of a group's rows that a tile takes.
@@ -327,8 +381,7 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) ragged_gemm_kernel(const __gr
                             const int k_row = steps * 16 + r;              // 128-byte swizzle: unit c of row r at c ^ (r & 7)
                             const uint32_t dst = (of_a ? a_smem : b_smem) + uint32_t(e / 64) * 8192u + uint32_t(k_row) * 128u +
                                                  ((uint32_t(e / 8) & 7u) ^ (uint32_t(k_row) & 7u)) * 16u;
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z),
-                                         "r"(v.w) : "memory");
+                            ptx::st_shared_u4(dst, v.x, v.y, v.z, v.w);
                         }
                         ptx::fence_proxy_async_smem();
                         __syncwarp();
@@ -421,18 +474,25 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) ragged_gemm_kernel(const __gr
         int it = 0;
         for (int u = first_unit; u < num_units; u += unit_stride) {
             const RaggedTile t = walk.at(u);
-            const int feature = t.feature0 + int(cta_rank) * 128 + int(quarter) * 32 + int(lane);
             if constexpr (FORM == RaggedForm::TN) {
-                OutT* dst_row = static_cast<OutT*>(p.c) + ((long long)t.group * p.features + feature) * p.cols + t.col0;
+                // A chunk's sums leave as blocks of 32 features x 128 bytes, staged in shared memory: by a tensor store (the
+                // later chunks of an FP32 gradient by a tensor reduction, an FP32 addition in L2; each element has this one
+                // writer, in order), or, where rows of C are no 16-byte multiples, row by row.
+                const int feature_w = t.feature0 + int(cta_rank) * 128 + int(quarter) * 32;
+                const uint32_t staging = smem_base + uint32_t(p.stages) * p.stage_bytes + quarter * 4096u;
+                constexpr int COLS = 128 / sizeof(OutT);
                 int row = t.row0;
                 do {
                     const bool any = chunk_blocks(t, row) > 0;       // an empty group's gradient is zero
+                    const bool add = row != t.row0;
                     const uint32_t acc = it & 1;
                     if (any) {
                         const bool ok = ptx::mbar_wait(ptx::smem_u32(&bar_acc_full[acc]), (it >> 1) & 1, wctx, UMMA_TIMEOUT_EPILOGUE);
                         if (!__all_sync(0xffffffffu, ok)) goto epilogue_done;
                         ptx::tc_fence_after();
                     }
+                    if (add && lane == 0) ptx::bulk_wait_group<0>();      // the chunk before has arrived in C
+                    __syncwarp();
                     const uint32_t t_row = tmem_base + acc * 256u + ((quarter * 32u) << 16);
                     for (int c = 0; c < t.col_count; c += 32) {
                         uint32_t r[32];
@@ -443,16 +503,30 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) ragged_gemm_kernel(const __gr
 #pragma unroll
                             for (int j = 0; j < 32; ++j) r[j] = 0u;
                         }
-                        if (feature < p.features) {
-                            const float scale = p.col_scale != nullptr ? __ldg(p.col_scale + (t.col0 + c) / 128) : 1.0f;
+                        const float scale = p.col_scale != nullptr ? __ldg(p.col_scale + (t.col0 + c) / 128) : 1.0f;
+                        const int c0 = c / COLS * COLS;
+                        if (c == c0) {      // the block's last store has read it
+                            if (lane == 0) ptx::bulk_wait_group_read<0>();
+                            __syncwarp();
+                        }
+                        float v[32];
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) {
-                                if (c + j < t.col_count) {
-                                    float v = __uint_as_float(r[j]) * scale;
-                                    if constexpr (sizeof(OutT) == 4)
-                                        if (row != t.row0) v += float(dst_row[c + j]);
-                                    dst_row[c + j] = round_to<OutT>(v);
+                        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) * scale;
+                        stage_block<OutT>(staging, lane, c - c0, v);
+                        if (c + 32 - c0 == COLS || c + 32 >= t.col_count) {
+                            if (p.tma_store) {
+                                ptx::fence_proxy_async_smem();
+                                __syncwarp();
+                                if (lane == 0 && feature_w < p.features) {
+                                    if (add) ptx::tma_reduce_add_3d(&p.map_c, staging, t.col0 + c0, feature_w, t.group);
+                                    else ptx::tma_store_3d(&p.map_c, staging, t.col0 + c0, feature_w, t.group);
+                                    ptx::bulk_commit_group();
                                 }
+                            } else {
+                                __syncwarp();
+                                OutT* dst = static_cast<OutT*>(p.c) +
+                                            ((long long)t.group * p.features + feature_w) * p.cols + t.col0 + c0;
+                                write_block<OutT>(staging, lane, dst, p.cols, min(32, p.features - feature_w), t.col_count - c0, add);
                             }
                         }
                     }
@@ -469,6 +543,7 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) ragged_gemm_kernel(const __gr
                     row += p.chunk_rows;
                 } while (row < t.row1);
             } else {
+                const int feature = t.feature0 + int(cta_rank) * 128 + int(quarter) * 32 + int(lane);
                 const uint32_t acc = it & 1;
                 const bool ok = ptx::mbar_wait(ptx::smem_u32(&bar_acc_full[acc]), (it >> 1) & 1, wctx, UMMA_TIMEOUT_EPILOGUE);
                 if (!__all_sync(0xffffffffu, ok)) goto epilogue_done;
@@ -499,6 +574,8 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) ragged_gemm_kernel(const __gr
     epilogue_done:
         __syncwarp();
         if (CTAS == 2) ptx::cluster_arrive();
+        if (FORM == RaggedForm::TN && lane == 0) ptx::bulk_wait_group_read<0>();      // bulk stores still read shared memory
+        __syncwarp();
     }
 
     // ---------------------------------------------------------------- teardown
