@@ -90,6 +90,21 @@ void rows_by_weight(bool nn, const void* a, long long lda, const void* w, void* 
     else launch_rows<RaggedForm::NT>(p, plan, type, stream);
 }
 
+// The maps of load_columns and of the partial block; returns whether the first is by chunks.
+int encode_columns(CUtensorMap* map, CUtensorMap* map16, const AlignedRows& m, int rows, int cols, int chunks) {
+    const uint64_t dims[2] = {uint64_t(cols), uint64_t(rows)}, strides[1] = {uint64_t(m.ld) * 2};
+    const uint32_t box[2] = {64, 64}, box16[2] = {64, 16};
+    encode_tensor_map_f16(map16, m.ptr, 2, dims, strides, box16, TmaSwizzle::B128);
+    if (m.ld >= (cols + 63) / 64 * 64) {
+        const uint64_t dims3[3] = {64, uint64_t(rows), uint64_t((cols + 63) / 64)}, strides3[2] = {uint64_t(m.ld) * 2, 128};
+        const uint32_t box3[3] = {64, 64, uint32_t(chunks)};
+        encode_tensor_map_f16(map, m.ptr, 3, dims3, strides3, box3, TmaSwizzle::B128);
+        return 1;
+    }
+    encode_tensor_map_f16(map, m.ptr, 2, dims, strides, box, TmaSwizzle::B128);
+    return 0;
+}
+
 template <int CTAS, bool BF16>
 void launch_weight(RaggedParams& p, const RaggedPlan& plan, int c_type, cudaStream_t stream) {
     if (c_type == TYPE_F32) launch<RaggedForm::TN, CTAS, BF16, float>(p, plan, stream);
@@ -114,20 +129,9 @@ void grouped_tn(const void* a, long long lda, const void* b, long long ldb, void
     const AlignedRows y = rows_of(a, lda, rows, m, stream);
     const AlignedRows x = rows_of(b, ldb, rows, n, stream);
     RaggedParams p{};
-    {
-        const uint64_t dims[2] = {uint64_t(m), uint64_t(rows)};
-        const uint64_t strides[1] = {uint64_t(y.ld) * 2};
-        const uint32_t box[2] = {64, 64}, box16[2] = {64, 16};
-        encode_tensor_map_f16(&p.map_a, y.ptr, 2, dims, strides, box, TmaSwizzle::B128);
-        encode_tensor_map_f16(&p.map_a16, y.ptr, 2, dims, strides, box16, TmaSwizzle::B128);
-    }
-    {
-        const uint64_t dims[2] = {uint64_t(n), uint64_t(rows)};
-        const uint64_t strides[1] = {uint64_t(x.ld) * 2};
-        const uint32_t box[2] = {64, 64}, box16[2] = {64, 16};
-        encode_tensor_map_f16(&p.map_b, x.ptr, 2, dims, strides, box, TmaSwizzle::B128);
-        encode_tensor_map_f16(&p.map_b16, x.ptr, 2, dims, strides, box16, TmaSwizzle::B128);
-    }
+    const RaggedPlan plan = plan_weight(groups, m, n);
+    p.a_chunked = encode_columns(&p.map_a, &p.map_a16, y, rows, m, 2);
+    p.b_chunked = encode_columns(&p.map_b, &p.map_b16, x, rows, n, plan.tile_cols / plan.ctas / 64);
     const uint32_t c_bytes = uint32_t(elem_bytes(c_type));
     p.tma_store = (size_t(n) * c_bytes) % 16 == 0 && reinterpret_cast<uintptr_t>(c) % 16 == 0;
     if (p.tma_store) {
@@ -152,7 +156,6 @@ void grouped_tn(const void* a, long long lda, const void* b, long long ldb, void
     // single precision is summed over 2048 rows at a time, added up with rounding in the epilogue; a 16-bit one
     // (2e-3 from its own rounding) in one go.
     p.chunk_rows = c_type == TYPE_F32 ? 2048 : (rows + RAGGED_BK - 1) / RAGGED_BK * RAGGED_BK;
-    const RaggedPlan plan = plan_weight(groups, m, n);
     if (type == TYPE_BF16) {
         if (plan.ctas == 2) launch_weight<2, true>(p, plan, c_type, stream);
         else launch_weight<1, true>(p, plan, c_type, stream);

@@ -165,7 +165,7 @@ void launch_linear_backward_saved_fp8(const void* dy, ElementType type, const vo
     Scratch dz_buf;
     if (act != EPI_NONE) {
         if (dx != nullptr || dw != nullptr) {
-            ld_dz = (N + 7) / 8 * 8;
+            ld_dz = (N + 63) / 64 * 64;      // whole 128-byte rows of a box
             dz_buf = Scratch(size_t(M) * ld_dz * 2, stream);
             dz = dz_buf.ptr;
         }
@@ -178,7 +178,7 @@ void launch_linear_backward_saved_fp8(const void* dy, ElementType type, const vo
         // x as a 16-bit operand.  q * s is exact in BF16 for the power-of-two scales of quantize_fp8; FP16 has too few
         // exponents for that, so there each column block is taken relative to its largest scale (products below
         // 2^-24 of that are lost) and the result is multiplied by it.
-        const long long ld_x = (K + 7) / 8 * 8;
+        const long long ld_x = (K + 63) / 64 * 64;
         Scratch x_buf(size_t(M) * ld_x * 2, stream);
         Scratch top_buf;
         float* top = nullptr;

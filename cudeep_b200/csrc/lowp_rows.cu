@@ -327,12 +327,12 @@ __global__ void __launch_bounds__(kThreads) block_tops_kernel(const float* __res
     if (threadIdx.x == 0) top[blockIdx.x] = m > 0.0f ? m : 1.0f;
 }
 
-// Eight elements per thread; the padding behind cols is written as zeros.
+// Eight elements per thread, zeros behind cols up to the next multiple of eight.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads) dequantize_rows_kernel(const uint8_t* __restrict__ q, const float* __restrict__ scales,
                                                                    const float* __restrict__ top, int rows, int cols,
                                                                    T* __restrict__ y, long long ld_y) {
-    const int units = int(ld_y / 8);
+    const int units = (cols + 7) / 8;
     const long long total = (long long)rows * units;
     for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
         const long long r = i / units;
@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(kThreads) dequantize_rows_kernel(const uint8_t
         float f[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] = e4m3_value(v[j]) * s;
-        store8(y + i * 8, f);
+        store8(y + r * ld_y + c0, f);
     }
 }
 
@@ -465,7 +465,7 @@ void block_tops(const float* scales, int rows, int cols, float* top, cudaStream_
 void dequantize_rows(const uint8_t* q, const float* scales, const float* top, int rows, int cols, void* y, long long ld_y,
                      int y_type, cudaStream_t stream) {
     const bool vec = cols % 8 == 0 && reinterpret_cast<uintptr_t>(q) % 8 == 0;
-    const unsigned grid = pass_grid(rows * (ld_y / 8));
+    const unsigned grid = pass_grid((long long)rows * ((cols + 7) / 8));
     if (y_type == TYPE_F16) {
         __half* out = static_cast<__half*>(y);
         if (vec) dequantize_rows_kernel<__half, true><<<grid, kThreads, 0, stream>>>(q, scales, top, rows, cols, out, ld_y);

@@ -60,10 +60,11 @@ struct RowMaps {
 };
 
 struct RaggedParams {
-    CUtensorMap map_a;       // NT {K, F, G} box {64, 128, 1}; NN {F, K, G} box {64, 64, 1}; TN {F, rows} box {64, 64}
+    CUtensorMap map_a;       // NT {K, F, G} box {64, 128, 1}; NN {F, K, G} box {64, 64, 1}; TN see load_columns
     CUtensorMap map_a16;     // TN: {F, rows} box {64, 16}
     RowMaps x;               // NT, NN {K, rows}
-    CUtensorMap map_b;       // TN {C, rows} box {64, 64}
+    CUtensorMap map_b;       // TN see load_columns
+    int a_chunked, b_chunked;
     CUtensorMap map_b16;     // TN {C, rows} box {64, 16}
     CUtensorMap map_c;       // TN: {C, F, G} box {128 bytes, 32, 1}, where rows of C are 16-byte multiples
     int tma_store;           // ... and whether it is so
@@ -228,14 +229,29 @@ __device__ __forceinline__ __half round_to<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 round_to<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// TN: 64 rows of `chunks` times 64 columns, each chunk 64 rows of 128 bytes.  Where the rows hold whole chunks the map is
+// {64, rows, columns / 64} with all chunks in one box; otherwise {columns, rows} with one chunk per box (a map by chunks would
+// read past the last row's end).
+template <int CTAS>
+__device__ __forceinline__ void load_columns(uint32_t dst, const CUtensorMap* map, int chunked, int chunks, uint32_t bar, int col,
+                                             int row) {
+    if (chunked) {
+        if constexpr (CTAS == 2) ptx::tma_load_3d_pair(dst, map, bar, 0, row, col / 64);
+        else ptx::tma_load_3d(dst, map, bar, 0, row, col / 64);
+        return;
+    }
+    for (int j = 0; j < chunks; ++j) {
+        if constexpr (CTAS == 2) ptx::tma_load_2d_pair(dst + j * 8192, map, bar, col + j * 64, row);
+        else ptx::tma_load_2d(dst + j * 8192, map, bar, col + j * 64, row);
+    }
+}
+
 template <RaggedForm FORM, int CTAS, bool BF16, class OutT>
 __global__ void __launch_bounds__(UMMA_THREADS, 1) ragged_gemm_kernel(const __grid_constant__ RaggedParams p) {
 #if defined(__CUDA_ARCH_FEAT_SM100_ALL) || defined(__CUDA_ARCH_FEAT_SM101_ALL) || \
     defined(__CUDA_ARCH_FEAT_SM103_ALL)
     constexpr bool A_MN = FORM != RaggedForm::NT;
     constexpr bool B_MN = FORM == RaggedForm::TN;
-    // TN over a pair: the partner may have written operand rows with ordinary stores before it arrived.
-    constexpr bool FULL_CLUSTER = FORM == RaggedForm::TN && CTAS == 2;
 
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bar_full[RAGGED_MAX_STAGES];
@@ -348,19 +364,21 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) ragged_gemm_kernel(const __gr
                     const int chunks = per / 64;
                     bytes = uint32_t(steps) * 2048u * uint32_t(2 + chunks);
                     if (lane == 0) {
-                        const CUtensorMap* ma = whole ? &p.map_a : &p.map_a16;
-                        const CUtensorMap* mb = whole ? &p.map_b : &p.map_b16;
-                        const int boxes = whole ? 1 : steps;
-                        for (int s = 0; s < boxes; ++s) {
+                        // The last block goes in steps of 16 rows, chunk by chunk of 64 columns.
+                        if (whole) {
+                            load_columns<CTAS>(a_smem, &p.map_a, p.a_chunked, 2, full, feature, row);
+                            load_columns<CTAS>(b_smem, &p.map_b, p.b_chunked, chunks, full, col, row);
+                        }
+                        for (int s = 0; !whole && s < steps; ++s) {
                             for (int j = 0; j < 2; ++j) {
                                 const uint32_t dst = a_smem + j * 8192 + s * 2048;
-                                if constexpr (CTAS == 2) ptx::tma_load_2d_pair(dst, ma, full, feature + j * 64, row + s * 16);
-                                else ptx::tma_load_2d(dst, ma, full, feature + j * 64, row + s * 16);
+                                if constexpr (CTAS == 2) ptx::tma_load_2d_pair(dst, &p.map_a16, full, feature + j * 64, row + s * 16);
+                                else ptx::tma_load_2d(dst, &p.map_a16, full, feature + j * 64, row + s * 16);
                             }
                             for (int j = 0; j < chunks; ++j) {
                                 const uint32_t dst = b_smem + j * 8192 + s * 2048;
-                                if constexpr (CTAS == 2) ptx::tma_load_2d_pair(dst, mb, full, col + j * 64, row + s * 16);
-                                else ptx::tma_load_2d(dst, mb, full, col + j * 64, row + s * 16);
+                                if constexpr (CTAS == 2) ptx::tma_load_2d_pair(dst, &p.map_b16, full, col + j * 64, row + s * 16);
+                                else ptx::tma_load_2d(dst, &p.map_b16, full, col + j * 64, row + s * 16);
                             }
                         }
                     }
@@ -426,18 +444,28 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) ragged_gemm_kernel(const __gr
                         goto mma_done;
                     ptx::tc_fence_after();
                     const uint32_t d_tmem = tmem_base + acc * 256u;
-                    bool ready = __all_sync(0xffffffffu, ptx::mbar_test<FULL_CLUSTER>(ptx::smem_u32(&bar_full[stage]), phase));
+                    bool ready = __all_sync(0xffffffffu, ptx::mbar_test(ptx::smem_u32(&bar_full[stage]), phase));
                     for (int kb = 0; kb < blocks; ++kb) {
                         if (!ready &&
-                            !__all_sync(0xffffffffu, ptx::mbar_wait<FULL_CLUSTER>(ptx::smem_u32(&bar_full[stage]), phase, wctx,
-                                                                                  UMMA_TIMEOUT_MMA_FULL)))
+                            !__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&bar_full[stage]), phase, wctx,
+                                                                    UMMA_TIMEOUT_MMA_FULL)))
                             goto mma_done;
                         ptx::tc_fence_after();
                         uint32_t next_stage = stage + 1, next_phase = phase;
                         if (next_stage == uint32_t(p.stages)) { next_stage = 0; next_phase ^= 1u; }
-                        ready = __all_sync(0xffffffffu, ptx::mbar_test<FULL_CLUSTER>(ptx::smem_u32(&bar_full[next_stage]), next_phase));
+                        ready = __all_sync(0xffffffffu, ptx::mbar_test(ptx::smem_u32(&bar_full[next_stage]), next_phase));
                         int steps = 4;
-                        if (FORM == RaggedForm::TN) steps = min(4, (t.row1 - row - kb * RAGGED_BK + 15) / 16);
+                        if (FORM == RaggedForm::TN) {
+                            const int have = t.row1 - row - kb * RAGGED_BK;
+                            steps = min(4, (have + 15) / 16);
+                            // The partner wrote rows of this stage with ordinary stores before it arrived: look once more, now
+                            // acquiring what it released (at every stage that look would cost more than the MMAs).
+                            if (CTAS == 2 && have < RAGGED_BK && have % 16 != 0) {
+                                const bool seen = ptx::mbar_wait<true>(ptx::smem_u32(&bar_full[stage]), phase, wctx,
+                                                                       UMMA_TIMEOUT_MMA_FULL);
+                                if (!__all_sync(0xffffffffu, seen)) goto mma_done;
+                            }
+                        }
                         if (ptx::elect_one()) {
                             const uint64_t a_stage = a_desc0 + ((stage * p.stage_bytes) >> 4);
                             const uint64_t b_stage = b_desc0 + ((stage * p.stage_bytes) >> 4);
