@@ -31,7 +31,10 @@ enum class RaggedForm { NT, NN, TN };
 
 constexpr int RAGGED_MAX_GROUPS = 1024;
 constexpr int RAGGED_BK = 64;                        // 16-bit elements per K block = one 128-byte swizzle row
-constexpr uint32_t RAGGED_STAGING_BYTES = 4 * 4096;   // TN: a block of 32 rows x 128 bytes per epilogue warp
+// Epilogue warps: with four, a gradient tile of 512 summed rows took longer to leave than to compute.
+__host__ __device__ constexpr int ragged_epilogue_warps(RaggedForm form) { return form == RaggedForm::TN ? 8 : 4; }
+__host__ __device__ constexpr int ragged_threads(RaggedForm form) { return 64 + 32 * ragged_epilogue_warps(form); }
+constexpr uint32_t RAGGED_STAGING_BYTES = 8 * 2 * 4096;   // TN: two blocks of 32 rows x 128 bytes per epilogue warp
 constexpr uint32_t RAGGED_A_BYTES = 128 * 128;       // one CTA's features of a K block
 constexpr int RAGGED_MAX_STAGES = 12;
 constexpr uint32_t RAGGED_SMEM_BUDGET = 232448 - 1024 - 13 * 1024;   // minus alignment slack, group tables and barriers
@@ -247,7 +250,7 @@ __device__ __forceinline__ void load_columns(uint32_t dst, const CUtensorMap* ma
 }
 
 template <RaggedForm FORM, int CTAS, bool BF16, class OutT>
-__global__ void __launch_bounds__(UMMA_THREADS, 1) ragged_gemm_kernel(const __grid_constant__ RaggedParams p) {
+__global__ void __launch_bounds__(ragged_threads(FORM), 1) ragged_gemm_kernel(const __grid_constant__ RaggedParams p) {
 #if defined(__CUDA_ARCH_FEAT_SM100_ALL) || defined(__CUDA_ARCH_FEAT_SM101_ALL) || \
     defined(__CUDA_ARCH_FEAT_SM103_ALL)
     constexpr bool A_MN = FORM != RaggedForm::NT;
@@ -286,7 +289,7 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) ragged_gemm_kernel(const __gr
         }
         for (int a = 0; a < 2; ++a) {
             ptx::mbar_init(ptx::smem_u32(&bar_acc_full[a]), 1);
-            ptx::mbar_init(ptx::smem_u32(&bar_acc_empty[a]), 4 * CTAS);
+            ptx::mbar_init(ptx::smem_u32(&bar_acc_empty[a]), ragged_epilogue_warps(FORM) * CTAS);
         }
         ptx::fence_mbar_init();
     }
@@ -329,6 +332,27 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) ragged_gemm_kernel(const __gr
             const int feature = t.feature0 + int(cta_rank) * 128;
             const int col = t.col0 + int(cta_rank) * per;
             const int blocks = FORM == RaggedForm::TN ? (t.row1 - t.row0 + RAGGED_BK - 1) / RAGGED_BK : k_blocks_row;
+            // TN: the partial step at the end of the group, 16 rows x (128 + per) columns in 16-byte units dealt out to the
+            // lanes, is fetched now and stored when its stage comes (fetched then, its latency held up every tile).
+            constexpr int UNITS = FORM != RaggedForm::TN ? 1 : CTAS == 2 ? 16 : 24;
+            uint4 tail[UNITS];
+            const int tail_rows = (t.row1 - t.row0) % 16;
+            const int units_row = 16 + per / 8;
+            if (FORM == RaggedForm::TN && tail_rows != 0) {
+#pragma unroll
+                for (int n = 0; n < UNITS; ++n) {
+                    const int i = int(lane) + 32 * n;
+                    const int r = i / units_row, q = i - r * units_row;
+                    const bool of_a = q < 16;
+                    const int x = of_a ? feature + q * 8 : col + (q - 16) * 8;
+                    tail[n] = make_uint4(0, 0, 0, 0);
+                    if (r < tail_rows && x < (of_a ? p.features : p.cols)) {
+                        const uint16_t* src = static_cast<const uint16_t*>(of_a ? p.a : p.b);
+                        tail[n] = __ldg(reinterpret_cast<const uint4*>(
+                            src + (long long)(t.row1 - tail_rows + r) * (of_a ? p.lda : p.ldb) + x));
+                    }
+                }
+            }
             for (int kb = 0; kb < blocks; ++kb) {
                 const bool ok = ptx::mbar_wait(ptx::smem_u32(&bar_empty[stage]), phase ^ 1u, wctx, UMMA_TIMEOUT_PRODUCER);
                 if (!__all_sync(0xffffffffu, ok)) goto producer_done;
@@ -383,23 +407,17 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) ragged_gemm_kernel(const __gr
                         }
                     }
                     if (!whole && have % 16 != 0) {
-                        // The partial step: 16 rows x (128 + per) columns in 16-byte units, a unit per lane and turn.
-                        const int row_s = row + steps * 16;
-                        const int units_row = 16 + per / 8;
-                        for (int i = int(lane); i < 16 * units_row; i += 32) {
+#pragma unroll
+                        for (int n = 0; n < UNITS; ++n) {
+                            const int i = int(lane) + 32 * n;
                             const int r = i / units_row, q = i - r * units_row;
+                            if (r >= 16) break;
                             const bool of_a = q < 16;
-                            const int e = (of_a ? q : q - 16) * 8;          // first element within the CTA's columns
-                            const int x = (of_a ? feature : col) + e;
-                            uint4 v = make_uint4(0, 0, 0, 0);
-                            if (row_s + r < t.row1 && x < (of_a ? p.features : p.cols)) {
-                                const uint16_t* src = static_cast<const uint16_t*>(of_a ? p.a : p.b);
-                                v = __ldg(reinterpret_cast<const uint4*>(src + (long long)(row_s + r) * (of_a ? p.lda : p.ldb) + x));
-                            }
-                            const int k_row = steps * 16 + r;              // 128-byte swizzle: unit c of row r at c ^ (r & 7)
+                            const int e = (of_a ? q : q - 16) * 8;      // first element within the CTA's columns
+                            const int k_row = steps * 16 + r;          // 128-byte swizzle: unit c of row r at c ^ (r & 7)
                             const uint32_t dst = (of_a ? a_smem : b_smem) + uint32_t(e / 64) * 8192u + uint32_t(k_row) * 128u +
                                                  ((uint32_t(e / 8) & 7u) ^ (uint32_t(k_row) & 7u)) * 16u;
-                            ptx::st_shared_u4(dst, v.x, v.y, v.z, v.w);
+                            ptx::st_shared_u4(dst, tail[n].x, tail[n].y, tail[n].z, tail[n].w);
                         }
                         ptx::fence_proxy_async_smem();
                         __syncwarp();
@@ -499,6 +517,7 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) ragged_gemm_kernel(const __gr
     } else {
         // ------------------------------------------------------------ epilogue
         const uint32_t quarter = warp & 3u;
+        uint32_t block_turn = 0;      // TN
         int it = 0;
         for (int u = first_unit; u < num_units; u += unit_stride) {
             const RaggedTile t = walk.at(u);
@@ -507,8 +526,10 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) ragged_gemm_kernel(const __gr
                 // later chunks of an FP32 gradient by a tensor reduction, an FP32 addition in L2; each element has this one
                 // writer, in order), or, where rows of C are no 16-byte multiples, row by row.
                 const int feature_w = t.feature0 + int(cta_rank) * 128 + int(quarter) * 32;
-                const uint32_t staging = smem_base + uint32_t(p.stages) * p.stage_bytes + quarter * 4096u;
+                const uint32_t staging = smem_base + uint32_t(p.stages) * p.stage_bytes + (warp - 2) * 8192u;
                 constexpr int COLS = 128 / sizeof(OutT);
+                const int c_begin = (int(warp - 2) >> 2) * (t.umma_n / 2);      // warps 6..9 take the second half of the columns
+                const int c_end = min(t.col_count, c_begin + t.umma_n / 2);
                 int row = t.row0;
                 do {
                     const bool any = chunk_blocks(t, row) > 0;       // an empty group's gradient is zero
@@ -522,7 +543,8 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) ragged_gemm_kernel(const __gr
                     if (add && lane == 0) ptx::bulk_wait_group<0>();      // the chunk before has arrived in C
                     __syncwarp();
                     const uint32_t t_row = tmem_base + acc * 256u + ((quarter * 32u) << 16);
-                    for (int c = 0; c < t.col_count; c += 32) {
+                    uint32_t block = staging;
+                    for (int c = c_begin; c < c_end; c += 32) {
                         uint32_t r[32];
                         if (any) {
                             ptx::tmem_ld_32x32(t_row + c, r);
@@ -533,28 +555,30 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) ragged_gemm_kernel(const __gr
                         }
                         const float scale = p.col_scale != nullptr ? __ldg(p.col_scale + (t.col0 + c) / 128) : 1.0f;
                         const int c0 = c / COLS * COLS;
-                        if (c == c0) {      // the block's last store has read it
-                            if (lane == 0) ptx::bulk_wait_group_read<0>();
+                        if (c == c0) {      // the two blocks take turns: the store before the last has read this one
+                            block = staging + (block_turn++ & 1u) * 4096u;
+                            if (lane == 0) ptx::bulk_wait_group_read<1>();
                             __syncwarp();
                         }
                         float v[32];
 #pragma unroll
                         for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) * scale;
-                        stage_block<OutT>(staging, lane, c - c0, v);
-                        if (c + 32 - c0 == COLS || c + 32 >= t.col_count) {
+                        stage_block<OutT>(block, lane, c - c0, v);
+                        if (c + 32 - c0 == COLS || c + 32 >= c_end) {
                             if (p.tma_store) {
                                 ptx::fence_proxy_async_smem();
                                 __syncwarp();
-                                if (lane == 0 && feature_w < p.features) {
-                                    if (add) ptx::tma_reduce_add_3d(&p.map_c, staging, t.col0 + c0, feature_w, t.group);
-                                    else ptx::tma_store_3d(&p.map_c, staging, t.col0 + c0, feature_w, t.group);
+                                if (lane == 0) {
+                                    if (feature_w >= p.features) {      // nothing to write, but a group of stores all the same
+                                    } else if (add) ptx::tma_reduce_add_3d(&p.map_c, block, t.col0 + c0, feature_w, t.group);
+                                    else ptx::tma_store_3d(&p.map_c, block, t.col0 + c0, feature_w, t.group);
                                     ptx::bulk_commit_group();
                                 }
                             } else {
                                 __syncwarp();
                                 OutT* dst = static_cast<OutT*>(p.c) +
                                             ((long long)t.group * p.features + feature_w) * p.cols + t.col0 + c0;
-                                write_block<OutT>(staging, lane, dst, p.cols, min(32, p.features - feature_w), t.col_count - c0, add);
+                                write_block<OutT>(block, lane, dst, p.cols, min(32, p.features - feature_w), c_end - c0, add);
                             }
                         }
                     }
