@@ -8,6 +8,30 @@ namespace cudeep_b200 {
 
 namespace {
 
+// Copies of two maps for each group (one warp each), cut off at the group's last row (their dimension 1).
+__global__ void __launch_bounds__(32) group_maps_kernel(const __grid_constant__ CUtensorMap map_a,
+                                                        const __grid_constant__ CUtensorMap map_b,
+                                                        const int32_t* __restrict__ offsets, int rows, CUtensorMap* out) {
+#if defined(__CUDA_ARCH_FEAT_SM100_ALL) || defined(__CUDA_ARCH_FEAT_SM101_ALL) || \
+    defined(__CUDA_ARCH_FEAT_SM103_ALL)
+    __shared__ __align__(128) uint32_t copy[2][32];
+    const uint32_t lane = threadIdx.x;
+    copy[0][lane] = reinterpret_cast<const uint32_t*>(&map_a)[lane];
+    copy[1][lane] = reinterpret_cast<const uint32_t*>(&map_b)[lane];
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
+    __syncwarp();
+    // An empty group loads nothing; its map only has to be a map.
+    const uint32_t end = uint32_t(min(max(__ldg(offsets + blockIdx.x + 1), 1), rows));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if (lane == 0) ptx::tensormap_replace_dim1(ptx::smem_u32(copy[i]), end);
+        __syncwarp();
+        ptx::tensormap_publish(out + 2 * blockIdx.x + i, ptx::smem_u32(copy[i]));
+    }
+#endif
+}
+
 RaggedPlan plan_weight(int groups, int features, int cols) {
     const int sms = device_info().num_sms;
     RaggedPlan plan{features <= 128 ? 1 : 2, 256, 0};
@@ -65,10 +89,19 @@ void rows_by_weight(bool nn, const void* a, long long lda, const void* w, void* 
     const AlignedRows wt = aligned_rows(w, (long long)groups * w_rows, w_cols, 2, stream);
     RaggedParams p{};
     {
-        const uint64_t dims[3] = {uint64_t(w_cols), uint64_t(w_rows), uint64_t(groups)};
-        const uint64_t strides[2] = {uint64_t(wt.ld) * 2, uint64_t(wt.ld) * 2 * uint64_t(w_rows)};
-        const uint32_t box[3] = {64, nn ? 64u : 128u, 1};
-        encode_tensor_map_f16(&p.map_a, wt.ptr, 3, dims, strides, box, TmaSwizzle::B128);
+        const uint64_t row_bytes = uint64_t(wt.ld) * 2, group_bytes = row_bytes * uint64_t(w_rows);
+        p.a_chunked = nn && wt.ld >= (w_cols + 63) / 64 * 64;
+        if (p.a_chunked) {
+            const uint64_t dims[4] = {64, uint64_t(w_rows), uint64_t((w_cols + 63) / 64), uint64_t(groups)};
+            const uint64_t strides[3] = {row_bytes, 128, group_bytes};
+            const uint32_t box[4] = {64, 64, 2, 1};
+            encode_tensor_map_f16(&p.map_a, wt.ptr, 4, dims, strides, box, TmaSwizzle::B128);
+        } else {
+            const uint64_t dims[3] = {uint64_t(w_cols), uint64_t(w_rows), uint64_t(groups)};
+            const uint64_t strides[2] = {row_bytes, group_bytes};
+            const uint32_t box[3] = {64, nn ? 64u : 128u, 1};
+            encode_tensor_map_f16(&p.map_a, wt.ptr, 3, dims, strides, box, TmaSwizzle::B128);
+        }
     }
     {
         const uint64_t dims[2] = {uint64_t(k), uint64_t(rows)};
@@ -90,19 +123,15 @@ void rows_by_weight(bool nn, const void* a, long long lda, const void* w, void* 
     else launch_rows<RaggedForm::NT>(p, plan, type, stream);
 }
 
-// The maps of load_columns and of the partial block; returns whether the first is by chunks.
-int encode_columns(CUtensorMap* map, CUtensorMap* map16, const AlignedRows& m, int rows, int cols, int chunks) {
+// The map of load_columns; returns whether it is by chunks.
+int encode_columns(CUtensorMap* map, const AlignedRows& m, int rows, int cols, int chunks) {
+    const bool chunked = m.ld >= (cols + 63) / 64 * 64;
     const uint64_t dims[2] = {uint64_t(cols), uint64_t(rows)}, strides[1] = {uint64_t(m.ld) * 2};
-    const uint32_t box[2] = {64, 64}, box16[2] = {64, 16};
-    encode_tensor_map_f16(map16, m.ptr, 2, dims, strides, box16, TmaSwizzle::B128);
-    if (m.ld >= (cols + 63) / 64 * 64) {
-        const uint64_t dims3[3] = {64, uint64_t(rows), uint64_t((cols + 63) / 64)}, strides3[2] = {uint64_t(m.ld) * 2, 128};
-        const uint32_t box3[3] = {64, 64, uint32_t(chunks)};
-        encode_tensor_map_f16(map, m.ptr, 3, dims3, strides3, box3, TmaSwizzle::B128);
-        return 1;
-    }
-    encode_tensor_map_f16(map, m.ptr, 2, dims, strides, box, TmaSwizzle::B128);
-    return 0;
+    const uint64_t dims3[3] = {64, uint64_t(rows), uint64_t((cols + 63) / 64)}, strides3[2] = {uint64_t(m.ld) * 2, 128};
+    const uint32_t box[3] = {64, 64, uint32_t(chunks)};
+    if (chunked) encode_tensor_map_f16(map, m.ptr, 3, dims3, strides3, box, TmaSwizzle::B128);
+    else encode_tensor_map_f16(map, m.ptr, 2, dims, strides, box, TmaSwizzle::B128);
+    return chunked ? 1 : 0;
 }
 
 template <int CTAS, bool BF16>
@@ -130,8 +159,8 @@ void grouped_tn(const void* a, long long lda, const void* b, long long ldb, void
     const AlignedRows x = rows_of(b, ldb, rows, n, stream);
     RaggedParams p{};
     const RaggedPlan plan = plan_weight(groups, m, n);
-    p.a_chunked = encode_columns(&p.map_a, &p.map_a16, y, rows, m, 2);
-    p.b_chunked = encode_columns(&p.map_b, &p.map_b16, x, rows, n, plan.tile_cols / plan.ctas / 64);
+    p.a_chunked = encode_columns(&p.map_a, y, rows, m, 2);
+    p.b_chunked = encode_columns(&p.map_b, x, rows, n, plan.tile_cols / plan.ctas / 64);
     const uint32_t c_bytes = uint32_t(elem_bytes(c_type));
     p.tma_store = (size_t(n) * c_bytes) % 16 == 0 && reinterpret_cast<uintptr_t>(c) % 16 == 0;
     if (p.tma_store) {
@@ -141,10 +170,13 @@ void grouped_tn(const void* a, long long lda, const void* b, long long ldb, void
         if (c_type == TYPE_F32) encode_tensor_map(&p.map_c, static_cast<const float*>(c), 3, dims, strides, box, TmaSwizzle::B128);
         else encode_tensor_map_f16(&p.map_c, c, 3, dims, strides, box, TmaSwizzle::B128);
     }
-    p.a = y.ptr;
-    p.b = x.ptr;
-    p.lda = y.ld;
-    p.ldb = x.ld;
+    Scratch maps;
+    if (offsets != nullptr) {
+        maps = Scratch(size_t(groups) * 2 * sizeof(CUtensorMap), stream);
+        p.group_maps = static_cast<const CUtensorMap*>(maps.ptr);
+        launch_dependent(group_maps_kernel, dim3(unsigned(groups)), 32, stream, p.map_a, p.map_b, offsets, rows,
+                         static_cast<CUtensorMap*>(maps.ptr));
+    }
     p.c = c;
     p.offsets = offsets;
     p.groups = groups;

@@ -14,8 +14,10 @@
 // end that fall into its last columns are computed and not stored: they cannot reach another row's result.
 //
 // TN sums over the rows, so a row behind the group's end must not be multiplied at all (a zero on one side does not
-// do: 0 * Inf = NaN).  MMAs run for whole steps of 16 rows; the last step of a group, if it is partial, is brought
-// by the producer warp itself with ordinary loads that replace rows behind the end by zeros in both operands.
+// do: 0 * Inf = NaN).  Each group therefore has tensor maps of its own whose rows end with the group, made on the device by
+// group_maps_kernel just before, and the TMA unit fills what lies behind with zeros in both operands.  (Bringing the last
+// 16 rows with ordinary loads instead cost a cluster-scope release and acquire per tile: 8192 rows in 16 groups, 2048 x 2048,
+// 129 us; 86 us this way.)
 #pragma once
 
 #include "runtime.h"
@@ -63,17 +65,13 @@ struct RowMaps {
 };
 
 struct RaggedParams {
-    CUtensorMap map_a;       // NT {K, F, G} box {64, 128, 1}; NN {F, K, G} box {64, 64, 1}; TN see load_columns
-    CUtensorMap map_a16;     // TN: {F, rows} box {64, 16}
+    CUtensorMap map_a;       // NT {K, F, G} box {64, 128, 1}; NN as load_columns, and G; TN load_columns
     RowMaps x;               // NT, NN {K, rows}
     CUtensorMap map_b;       // TN see load_columns
     int a_chunked, b_chunked;
-    CUtensorMap map_b16;     // TN {C, rows} box {64, 16}
     CUtensorMap map_c;       // TN: {C, F, G} box {128 bytes, 32, 1}, where rows of C are 16-byte multiples
     int tma_store;           // ... and whether it is so
-    const void* a;           // TN: the operands' addresses and row lengths, for the partial last step
-    const void* b;
-    long long lda, ldb;
+    const CUtensorMap* group_maps;      // TN: map_a and map_b of each group; nullptr: one group of all rows
     void* c;
     const int32_t* offsets;  // [groups + 1], or nullptr: one group of all rows
     int groups;
@@ -232,7 +230,7 @@ __device__ __forceinline__ __half round_to<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 round_to<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// TN: 64 rows of `chunks` times 64 columns, each chunk 64 rows of 128 bytes.  Where the rows hold whole chunks the map is
+// 64 rows of `chunks` times 64 columns, each chunk 64 rows of 128 bytes.  Where the rows hold whole chunks the map is
 // {64, rows, columns / 64} with all chunks in one box; otherwise {columns, rows} with one chunk per box (a map by chunks would
 // read past the last row's end).
 template <int CTAS>
@@ -278,8 +276,7 @@ __global__ void __launch_bounds__(ragged_threads(FORM), 1) ragged_gemm_kernel(co
         ptx::prefetch_tensormap(&p.map_a);
         if constexpr (FORM == RaggedForm::TN) {
             ptx::prefetch_tensormap(&p.map_b);
-            ptx::prefetch_tensormap(&p.map_b16);
-            ptx::prefetch_tensormap(&p.map_a16);
+            ptx::prefetch_tensormap(&p.map_c);
         } else {
             p.x.prefetch();
         }
@@ -332,25 +329,14 @@ __global__ void __launch_bounds__(ragged_threads(FORM), 1) ragged_gemm_kernel(co
             const int feature = t.feature0 + int(cta_rank) * 128;
             const int col = t.col0 + int(cta_rank) * per;
             const int blocks = FORM == RaggedForm::TN ? (t.row1 - t.row0 + RAGGED_BK - 1) / RAGGED_BK : k_blocks_row;
-            // TN: the partial step at the end of the group, 16 rows x (128 + per) columns in 16-byte units dealt out to the
-            // lanes, is fetched now and stored when its stage comes (fetched then, its latency held up every tile).
-            constexpr int UNITS = FORM != RaggedForm::TN ? 1 : CTAS == 2 ? 16 : 24;
-            uint4 tail[UNITS];
-            const int tail_rows = (t.row1 - t.row0) % 16;
-            const int units_row = 16 + per / 8;
-            if (FORM == RaggedForm::TN && tail_rows != 0) {
-#pragma unroll
-                for (int n = 0; n < UNITS; ++n) {
-                    const int i = int(lane) + 32 * n;
-                    const int r = i / units_row, q = i - r * units_row;
-                    const bool of_a = q < 16;
-                    const int x = of_a ? feature + q * 8 : col + (q - 16) * 8;
-                    tail[n] = make_uint4(0, 0, 0, 0);
-                    if (r < tail_rows && x < (of_a ? p.features : p.cols)) {
-                        const uint16_t* src = static_cast<const uint16_t*>(of_a ? p.a : p.b);
-                        tail[n] = __ldg(reinterpret_cast<const uint4*>(
-                            src + (long long)(t.row1 - tail_rows + r) * (of_a ? p.lda : p.ldb) + x));
-                    }
+            const CUtensorMap* map_a = &p.map_a;
+            const CUtensorMap* map_b = &p.map_b;
+            if (FORM == RaggedForm::TN && p.group_maps != nullptr) {
+                map_a = p.group_maps + 2 * t.group;
+                map_b = map_a + 1;
+                if (lane == 0) {
+                    ptx::tensormap_acquire(map_a);
+                    ptx::tensormap_acquire(map_b);
                 }
             }
             for (int kb = 0; kb < blocks; ++kb) {
@@ -360,15 +346,16 @@ __global__ void __launch_bounds__(ragged_threads(FORM), 1) ragged_gemm_kernel(co
                 const uint32_t b_smem = a_smem + RAGGED_A_BYTES;
                 const uint32_t full_local = ptx::smem_u32(&bar_full[stage]);
                 const uint32_t full = CTAS == 2 ? ptx::mapa(full_local, 0) : full_local;
-                uint32_t bytes;
-                bool stored = false;      // this stage holds rows written with ordinary stores
-                if constexpr (FORM != RaggedForm::TN) {
-                    bytes = RAGGED_A_BYTES + uint32_t(RowMaps::loaded(per)) * 128u;
-                    if (lane == 0) {
-                        const int k0 = kb * RAGGED_BK;
-                        if constexpr (FORM == RaggedForm::NT) {
-                            if constexpr (CTAS == 2) ptx::tma_load_3d_pair(a_smem, &p.map_a, full, k0, feature, t.group);
-                            else ptx::tma_load_3d(a_smem, &p.map_a, full, k0, feature, t.group);
+                const uint32_t bytes = RAGGED_A_BYTES + uint32_t(FORM == RaggedForm::TN ? per : RowMaps::loaded(per)) * 128u;
+                if (lane == 0) {
+                    const int k0 = kb * RAGGED_BK;
+                    if constexpr (FORM == RaggedForm::NT) {
+                        if constexpr (CTAS == 2) ptx::tma_load_3d_pair(a_smem, &p.map_a, full, k0, feature, t.group);
+                        else ptx::tma_load_3d(a_smem, &p.map_a, full, k0, feature, t.group);
+                    } else if constexpr (FORM == RaggedForm::NN) {
+                        if (p.a_chunked) {
+                            if constexpr (CTAS == 2) ptx::tma_load_4d_pair(a_smem, &p.map_a, full, 0, k0, feature / 64, t.group);
+                            else ptx::tma_load_4d(a_smem, &p.map_a, full, 0, k0, feature / 64, t.group);
                         } else {
 #pragma unroll
                             for (int j = 0; j < 2; ++j) {
@@ -378,55 +365,14 @@ __global__ void __launch_bounds__(ragged_threads(FORM), 1) ragged_gemm_kernel(co
                                     ptx::tma_load_3d(a_smem + j * 8192, &p.map_a, full, feature + j * 64, k0, t.group);
                             }
                         }
-                        p.x.template load<CTAS>(b_smem, full, k0, col, per);
+                    } else {
+                        load_columns<CTAS>(a_smem, map_a, p.a_chunked, 2, full, feature, t.row0 + k0);
+                        load_columns<CTAS>(b_smem, map_b, p.b_chunked, per / 64, full, col, t.row0 + k0);
                     }
-                } else {
-                    const int row = t.row0 + kb * RAGGED_BK;
-                    const int have = t.row1 - row;                         // rows of the group from here on
-                    const bool whole = have >= RAGGED_BK;
-                    const int steps = whole ? 4 : have / 16;               // whole steps of 16 rows
-                    const int chunks = per / 64;
-                    bytes = uint32_t(steps) * 2048u * uint32_t(2 + chunks);
-                    if (lane == 0) {
-                        // The last block goes in steps of 16 rows, chunk by chunk of 64 columns.
-                        if (whole) {
-                            load_columns<CTAS>(a_smem, &p.map_a, p.a_chunked, 2, full, feature, row);
-                            load_columns<CTAS>(b_smem, &p.map_b, p.b_chunked, chunks, full, col, row);
-                        }
-                        for (int s = 0; !whole && s < steps; ++s) {
-                            for (int j = 0; j < 2; ++j) {
-                                const uint32_t dst = a_smem + j * 8192 + s * 2048;
-                                if constexpr (CTAS == 2) ptx::tma_load_2d_pair(dst, &p.map_a16, full, feature + j * 64, row + s * 16);
-                                else ptx::tma_load_2d(dst, &p.map_a16, full, feature + j * 64, row + s * 16);
-                            }
-                            for (int j = 0; j < chunks; ++j) {
-                                const uint32_t dst = b_smem + j * 8192 + s * 2048;
-                                if constexpr (CTAS == 2) ptx::tma_load_2d_pair(dst, &p.map_b16, full, col + j * 64, row + s * 16);
-                                else ptx::tma_load_2d(dst, &p.map_b16, full, col + j * 64, row + s * 16);
-                            }
-                        }
-                    }
-                    if (!whole && have % 16 != 0) {
-#pragma unroll
-                        for (int n = 0; n < UNITS; ++n) {
-                            const int i = int(lane) + 32 * n;
-                            const int r = i / units_row, q = i - r * units_row;
-                            if (r >= 16) break;
-                            const bool of_a = q < 16;
-                            const int e = (of_a ? q : q - 16) * 8;      // first element within the CTA's columns
-                            const int k_row = steps * 16 + r;          // 128-byte swizzle: unit c of row r at c ^ (r & 7)
-                            const uint32_t dst = (of_a ? a_smem : b_smem) + uint32_t(e / 64) * 8192u + uint32_t(k_row) * 128u +
-                                                 ((uint32_t(e / 8) & 7u) ^ (uint32_t(k_row) & 7u)) * 16u;
-                            ptx::st_shared_u4(dst, tail[n].x, tail[n].y, tail[n].z, tail[n].w);
-                        }
-                        ptx::fence_proxy_async_smem();
-                        __syncwarp();
-                        stored = true;
-                    }
+                    if constexpr (FORM != RaggedForm::TN) p.x.template load<CTAS>(b_smem, full, k0, col, per);
                 }
                 if (lane == 0) {
                     if (is_leader) ptx::mbar_arrive_expect_tx(full_local, bytes);
-                    else if (stored) ptx::mbar_arrive_expect_tx_cluster(full, bytes);
                     else ptx::mbar_arrive_expect_tx_cluster_relaxed(full, bytes);
                 }
                 __syncwarp();
@@ -473,17 +419,7 @@ __global__ void __launch_bounds__(ragged_threads(FORM), 1) ragged_gemm_kernel(co
                         if (next_stage == uint32_t(p.stages)) { next_stage = 0; next_phase ^= 1u; }
                         ready = __all_sync(0xffffffffu, ptx::mbar_test(ptx::smem_u32(&bar_full[next_stage]), next_phase));
                         int steps = 4;
-                        if (FORM == RaggedForm::TN) {
-                            const int have = t.row1 - row - kb * RAGGED_BK;
-                            steps = min(4, (have + 15) / 16);
-                            // The partner wrote rows of this stage with ordinary stores before it arrived: look once more, now
-                            // acquiring what it released (at every stage that look would cost more than the MMAs).
-                            if (CTAS == 2 && have < RAGGED_BK && have % 16 != 0) {
-                                const bool seen = ptx::mbar_wait<true>(ptx::smem_u32(&bar_full[stage]), phase, wctx,
-                                                                       UMMA_TIMEOUT_MMA_FULL);
-                                if (!__all_sync(0xffffffffu, seen)) goto mma_done;
-                            }
-                        }
+                        if (FORM == RaggedForm::TN) steps = min(4, (t.row1 - row - kb * RAGGED_BK + 15) / 16);
                         if (ptx::elect_one()) {
                             const uint64_t a_stage = a_desc0 + ((stage * p.stage_bytes) >> 4);
                             const uint64_t b_stage = b_desc0 + ((stage * p.stage_bytes) >> 4);

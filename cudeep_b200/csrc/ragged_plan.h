@@ -57,4 +57,19 @@ void launch_clusters(Kernel kernel, const Params& p, long long clusters, int clu
     CB200_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
 }
 
+// A plain grid whose set-up may overlap the kernel before it (it must wait for it itself).
+template <class... Params, class... Args>
+void launch_dependent(void (*kernel)(Params...), dim3 grid, int threads, cudaStream_t stream, const Args&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(unsigned(threads), 1, 1);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = programmatic_launch_enabled() ? 1 : 0;
+    CB200_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...));
+}
+
 }  // namespace cudeep_b200
