@@ -8,6 +8,8 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 namespace cudeep_b200 {
 
 namespace {
@@ -71,113 +73,294 @@ __device__ __forceinline__ int scale_exponent(float amax) {
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float(uint32_t(e + 127) << 23); }      // -126 <= e <= 127
 
-// x / 2^e in e4m3, rounded to nearest even once (the division by a power of two is exact); NaN for what is not finite.
-__device__ __forceinline__ uint32_t e4m3(float x, float inv) {
-    const float v = x * inv;
-    const uint32_t q = __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
-    return fabsf(x) <= 3.402823466e38f ? q : 0x7fu;
+// 16 bytes of input: 4 floats or 8 16-bit values.  The block's maximum is found on the bits of the magnitudes, which order as
+// the magnitudes do with infinities and NaN on top: two instructions per word and no conversion.  A block that holds
+// something that is not finite shows it by a maximum beyond the largest finite value and takes the long way.
+template <typename T>
+struct Unit {
+    static constexpr int N = 16 / int(sizeof(T));
+    uint4 w;
+    __device__ __forceinline__ uint32_t word(int i) const { return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w; }
+    __device__ __forceinline__ float value(int j) const {
+        if constexpr (sizeof(T) == 4) {
+            return __uint_as_float(word(j));
+        } else {
+            const uint16_t h = uint16_t(word(j / 2) >> (16 * (j & 1)));
+            return to_float(*reinterpret_cast<const T*>(&h));
+        }
+    }
+    __device__ __forceinline__ uint32_t top(uint32_t m) const {      // packed for 16-bit types
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) m = max(m, word(i) & 0x7fffffffu);
+            else m = __vmaxu2(m, word(i) & 0x7fff7fffu);
+        }
+        return m;
+    }
+};
+// Magnitude bits of one value as top() packs them, and back to one value.
+template <typename T>
+__device__ __forceinline__ uint32_t unpack_top(uint32_t m) {
+    return sizeof(T) == 4 ? m : max(m & 0xffffu, m >> 16);
+}
+template <typename T>
+__device__ __forceinline__ float top_value(uint32_t bits) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(bits);
+    const uint16_t h = uint16_t(bits);
+    return to_float(*reinterpret_cast<const T*>(&h));
+}
+template <typename T>
+__device__ __forceinline__ bool top_finite(uint32_t bits) {
+    return bits < (sizeof(T) == 4 ? 0x7f800000u : std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u);
 }
 
-// Blocks of 1 x 128.  Sixteen lanes own a block, eight elements each; a warp takes two neighbouring blocks of four
-// rows at once (four independent 16-byte loads in flight per lane for 16-bit types), a CTA 32 rows x 256 columns.  The
-// scales lie [block][row], so the CTA collects its 32 x 2 scales in shared memory and writes runs of 32.
-// VEC: rows start on 16-byte boundaries; otherwise a lane takes every sixteenth element.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __restrict__ x, long long rows, int cols,
-                                                                 uint8_t* __restrict__ q, float* __restrict__ scales) {
-    __shared__ float s_scale[2][32];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int half = lane >> 4, l16 = lane & 15;
-    const int block = blockIdx.x * 2 + half;
-    const int c0 = block * FP8_BLOCK;
-    const long long row0 = (long long)blockIdx.y * 32 + warp * 4;
-    float v[4][8];
+// Four values times the inverse of the scale (exact: a power of two) in e4m3, rounded to nearest even once.
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d, float inv) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a * inv, b * inv), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c * inv, d * inv), __NV_SATFINITE, __NV_E4M3);
+    return lo | hi << 16;
+}
+// NaN's code where a value is not finite.
+__device__ __forceinline__ uint32_t nan_codes(uint32_t q, float a, float b, float c, float d) {
+    const float v[4] = {a, b, c, d};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const long long r = row0 + i;
-        const T* src = x + r * cols + c0;
-        if (VEC) {
-            if (r < rows && c0 + l16 * 8 < cols) {
-                load8(src + l16 * 8, v[i]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
-            }
+    for (int j = 0; j < 4; ++j)
+        if (!(fabsf(v[j]) <= 3.402823466e38f)) q = (q & ~(0xffu << (8 * j))) | 0x7fu << (8 * j);
+    return q;
+}
+
+// `bytes` bytes from shared memory, where they lie with the phase of dst within 4-byte words, to dst: whole words but
+// at the ends.  Whole warp; `buffer` is word-aligned.
+__device__ __forceinline__ void copy_bytes(const uint8_t* buffer, uint8_t* dst, int bytes, int lane) {
+    const int phase = int(reinterpret_cast<uintptr_t>(dst) & 3u);
+    uint8_t* base = dst - phase;
+    for (int w = lane; 4 * w < phase + bytes; w += 32) {
+        if (4 * w >= phase && 4 * w + 4 <= phase + bytes) {
+            reinterpret_cast<uint32_t*>(base)[w] = reinterpret_cast<const uint32_t*>(buffer)[w];
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = r < rows && c0 + l16 + 16 * j < cols ? to_float(src[l16 + 16 * j]) : 0.0f;
+            for (int j = 0; j < 4; ++j)
+                if (4 * w + j >= phase && 4 * w + j < phase + bytes) base[4 * w + j] = buffer[4 * w + j];
+        }
+    }
+}
+
+// Blocks of 1 x 128.  Eight lanes own a block, 16 elements each in units of 16 bytes; a warp takes four neighbouring blocks of
+// four rows, so a lane has 8 (16-bit types) or 16 independent loads under way, and a CTA 32 rows x 512 columns.  The
+// scales lie [block][row], so the CTA collects its 32 x 4 scales in shared memory and writes runs of 32.
+// 8192 x 16384 BF16, 407 MB: QROWS.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __restrict__ x, long long rows, int cols,
+                                                                 uint8_t* __restrict__ q, float* __restrict__ scales) {
+    constexpr int N = Unit<T>::N, UNITS = 16 / N;
+    __shared__ float s_scale[4][32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int sub = lane >> 3, l8 = lane & 7;
+    const int block = blockIdx.x * 4 + sub;
+    const int c0 = block * FP8_BLOCK + l8 * N;      // and 8 * N further on for each unit
+    const long long row0 = (long long)blockIdx.y * 32 + warp * 4;
+    Unit<T> u[4][UNITS];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int k = 0; k < UNITS; ++k) {
+            const int c = c0 + 8 * N * k;
+            u[i][k].w = make_uint4(0, 0, 0, 0);
+            if (row0 + i < rows && c < cols) u[i][k].w = __ldg(reinterpret_cast<const uint4*>(x + (row0 + i) * cols + c));
         }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        float amax = 0.0f;
+        uint32_t m = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, finite_abs(v[i][j]));
+        for (int k = 0; k < UNITS; ++k) m = u[i][k].top(m);
+        m = unpack_top<T>(m);
 #pragma unroll
-        for (int d = 8; d >= 1; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+        for (int d = 4; d >= 1; d >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+        const bool finite = top_finite<T>(m);
+        float amax = top_value<T>(m);
+        if (__any_sync(0xffffffffu, !finite)) {
+            amax = 0.0f;
+#pragma unroll
+            for (int k = 0; k < UNITS; ++k)
+#pragma unroll
+                for (int j = 0; j < N; ++j) amax = fmaxf(amax, finite_abs(u[i][k].value(j)));
+#pragma unroll
+            for (int d = 4; d >= 1; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+        }
         const int e = scale_exponent(amax);
         const float inv = pow2(-e);
-        if (l16 == 0) s_scale[half][warp * 4 + i] = pow2(e);
-        const long long r = row0 + i;
-        uint8_t* dst = q + r * cols + c0;
-        if (r < rows) {
-            if (VEC) {
-                if (c0 + l16 * 8 < cols) {
-                    uint2 out;
-                    out.x = e4m3(v[i][0], inv) | e4m3(v[i][1], inv) << 8 | e4m3(v[i][2], inv) << 16 | e4m3(v[i][3], inv) << 24;
-                    out.y = e4m3(v[i][4], inv) | e4m3(v[i][5], inv) << 8 | e4m3(v[i][6], inv) << 16 | e4m3(v[i][7], inv) << 24;
-                    *reinterpret_cast<uint2*>(dst + l16 * 8) = out;
-                }
-            } else {
+        if (l8 == 0) s_scale[sub][warp * 4 + i] = pow2(e);
+        if (row0 + i < rows) {
+            uint8_t* dst = q + (row0 + i) * cols + c0;
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (c0 + l16 + 16 * j < cols) dst[l16 + 16 * j] = uint8_t(e4m3(v[i][j], inv));
+            for (int k = 0; k < UNITS; ++k) {
+                if (c0 + 8 * N * k >= cols) break;
+                uint32_t out[N / 4];
+#pragma unroll
+                for (int j = 0; j < N; j += 4) {
+                    const Unit<T>& v = u[i][k];
+                    out[j / 4] = e4m3x4(v.value(j), v.value(j + 1), v.value(j + 2), v.value(j + 3), inv);
+                    if (!finite) out[j / 4] = nan_codes(out[j / 4], v.value(j), v.value(j + 1), v.value(j + 2), v.value(j + 3));
+                }
+                if constexpr (N == 8) *reinterpret_cast<uint2*>(dst + 8 * N * k) = make_uint2(out[0], out[1]);
+                else *reinterpret_cast<uint32_t*>(dst + 8 * N * k) = out[0];
             }
         }
     }
     __syncthreads();
-    if (threadIdx.x < 64) {
-        const int b = threadIdx.x >> 5;
+    if (threadIdx.x < 128) {
         const long long r = (long long)blockIdx.y * 32 + lane;
-        const int blk = blockIdx.x * 2 + b;
-        if (r < rows && (long long)blk * FP8_BLOCK < cols) scales[(long long)blk * rows + r] = s_scale[b][lane];
+        const int blk = blockIdx.x * 4 + warp;
+        if (r < rows && (long long)blk * FP8_BLOCK < cols) scales[(long long)blk * rows + r] = s_scale[warp][lane];
     }
 }
 
-// Blocks of 128 x 128, one CTA each: sixteen lanes hold a row's 128 columns, a thread 8 rows x 8 columns, so the block
-// is read once and stays in registers while its maximum is found.
-template <typename T, bool VEC>
+// The same for rows that start anywhere: a warp takes a block at a time, element by element, and the codes of its four
+// blocks of a row pass through shared memory to leave as words.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) quantize_rows_any_kernel(const T* __restrict__ x, long long rows, int cols,
+                                                                     uint8_t* __restrict__ q, float* __restrict__ scales) {
+    __shared__ float s_scale[4][32];
+    __shared__ __align__(16) uint8_t s_row[kThreads / 32][528];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int c0 = blockIdx.x * 4 * FP8_BLOCK;
+    const int width = min(4 * FP8_BLOCK, cols - c0);
+    for (int i = 0; i < 4; ++i) {
+        const long long r = (long long)blockIdx.y * 32 + warp * 4 + i;
+        if (r >= rows) break;
+        const T* src = x + r * cols + c0;
+        uint8_t* dst = q + r * cols + c0;
+        uint8_t* buffer = s_row[warp] + (reinterpret_cast<uintptr_t>(dst) & 3u);
+        float v[4][4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int c = b * FP8_BLOCK + lane + 32 * j;
+                v[b][j] = c < width ? to_float(src[c]) : 0.0f;
+            }
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            float amax = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) amax = fmaxf(amax, finite_abs(v[b][j]));
+            // Magnitudes order as their bits do.
+            amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
+            const int e = scale_exponent(amax);
+            if (lane == 0) s_scale[b][warp * 4 + i] = pow2(e);
+            uint32_t codes = e4m3x4(v[b][0], v[b][1], v[b][2], v[b][3], pow2(-e));
+            codes = nan_codes(codes, v[b][0], v[b][1], v[b][2], v[b][3]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) buffer[b * FP8_BLOCK + lane + 32 * j] = uint8_t(codes >> (8 * j));
+        }
+        __syncwarp();
+        copy_bytes(s_row[warp], dst, width, lane);
+        __syncwarp();
+    }
+    __syncthreads();
+    if (threadIdx.x < 128) {
+        const long long r = (long long)blockIdx.y * 32 + lane;
+        const int blk = blockIdx.x * 4 + warp;
+        if (r < rows && (long long)blk * FP8_BLOCK < cols) scales[(long long)blk * rows + r] = s_scale[warp][lane];
+    }
+}
+
+// Blocks of 128 x 128, one CTA each, held in registers while the block's maximum is found: eight lanes along a row of the
+// block, 32 rows at a time.
+template <typename T>
 __global__ void __launch_bounds__(kThreads) quantize_tiles_kernel(const T* __restrict__ x, long long rows, int cols,
                                                                   uint8_t* __restrict__ q, float* __restrict__ scales) {
+    constexpr int N = Unit<T>::N, UNITS = 16 / N;
     __shared__ float s_max[kThreads / 32];
-    const int l16 = threadIdx.x & 15, rr = threadIdx.x >> 4;
-    const int c0 = blockIdx.x * FP8_BLOCK;
-    const long long row0 = (long long)blockIdx.y * FP8_BLOCK + rr;
-    float v[8][8];
-    float amax = 0.0f;
+    __shared__ uint32_t s_top[kThreads / 32];
+    const int l8 = threadIdx.x & 7;
+    const int c0 = blockIdx.x * FP8_BLOCK + l8 * N;
+    const long long row0 = (long long)blockIdx.y * FP8_BLOCK + (threadIdx.x >> 3);
+    Unit<T> u[4][UNITS];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const long long r = row0 + 16 * i;
-        const T* src = x + r * cols + c0;
-        if (VEC) {
-            if (r < rows && c0 + l16 * 8 < cols) {
-                load8(src + l16 * 8, v[i]);
-            } else {
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+        for (int k = 0; k < UNITS; ++k) {
+            const long long r = row0 + 32 * i;
+            const int c = c0 + 8 * N * k;
+            u[i][k].w = make_uint4(0, 0, 0, 0);
+            if (r < rows && c < cols) u[i][k].w = __ldg(reinterpret_cast<const uint4*>(x + r * cols + c));
+        }
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int k = 0; k < UNITS; ++k) m = u[i][k].top(m);
+    m = __reduce_max_sync(0xffffffffu, unpack_top<T>(m));
+    if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) m = max(m, s_top[w]);
+    const bool finite = top_finite<T>(m);      // the same for the whole CTA
+    float amax = top_value<T>(m);
+    if (!finite) {
+        amax = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int k = 0; k < UNITS; ++k)
+#pragma unroll
+                for (int j = 0; j < N; ++j) amax = fmaxf(amax, finite_abs(u[i][k].value(j)));
+        amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
+        if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = amax;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kThreads / 32; ++w) amax = fmaxf(amax, s_max[w]);
+    }
+    const int e = scale_exponent(amax);
+    const float inv = pow2(-e);
+    if (threadIdx.x == 0) scales[(long long)blockIdx.y * gridDim.x + blockIdx.x] = pow2(e);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const long long r = row0 + 32 * i;
+        if (r >= rows) break;
+        uint8_t* dst = q + r * cols + c0;
+#pragma unroll
+        for (int k = 0; k < UNITS; ++k) {
+            if (c0 + 8 * N * k >= cols) break;
+            uint32_t out[N / 4];
+#pragma unroll
+            for (int j = 0; j < N; j += 4) {
+                const Unit<T>& v = u[i][k];
+                out[j / 4] = e4m3x4(v.value(j), v.value(j + 1), v.value(j + 2), v.value(j + 3), inv);
+                if (!finite) out[j / 4] = nan_codes(out[j / 4], v.value(j), v.value(j + 1), v.value(j + 2), v.value(j + 3));
             }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = r < rows && c0 + l16 + 16 * j < cols ? to_float(src[l16 + 16 * j]) : 0.0f;
+            if constexpr (N == 8) *reinterpret_cast<uint2*>(dst + 8 * N * k) = make_uint2(out[0], out[1]);
+            else *reinterpret_cast<uint32_t*>(dst + 8 * N * k) = out[0];
         }
     }
+}
+
+// The same for rows that start anywhere: a warp holds 16 rows, a lane every 32nd element of them, and each row's codes pass
+// through shared memory to leave as words.  4100 x 11007 FP32, 226 MB: QTILES.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) quantize_tiles_any_kernel(const T* __restrict__ x, long long rows, int cols,
+                                                                      uint8_t* __restrict__ q, float* __restrict__ scales) {
+    __shared__ float s_max[kThreads / 32];
+    __shared__ __align__(16) uint8_t s_row[kThreads / 32][4][132];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int c0 = blockIdx.x * FP8_BLOCK;
+    const int width = min(FP8_BLOCK, cols - c0);
+    const long long row0 = (long long)blockIdx.y * FP8_BLOCK + warp * 16;
+    float v[16][4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 16; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, finite_abs(v[i][j]));
+        for (int j = 0; j < 4; ++j)
+            v[i][j] = row0 + i < rows && lane + 32 * j < width ? to_float(x[(row0 + i) * cols + c0 + lane + 32 * j]) : 0.0f;
+    float amax = 0.0f;
 #pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
-    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = amax;
+    for (int i = 0; i < 16; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) amax = fmaxf(amax, finite_abs(v[i][j]));
+    amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
+    if (lane == 0) s_max[warp] = amax;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) amax = fmaxf(amax, s_max[w]);
@@ -185,27 +368,49 @@ __global__ void __launch_bounds__(kThreads) quantize_tiles_kernel(const T* __res
     const float inv = pow2(-e);
     if (threadIdx.x == 0) scales[(long long)blockIdx.y * gridDim.x + blockIdx.x] = pow2(e);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const long long r = row0 + 16 * i;
-        if (r >= rows) break;
-        uint8_t* dst = q + r * cols + c0;
-        if (VEC) {
-            if (c0 + l16 * 8 < cols) {
-                uint2 out;
-                out.x = e4m3(v[i][0], inv) | e4m3(v[i][1], inv) << 8 | e4m3(v[i][2], inv) << 16 | e4m3(v[i][3], inv) << 24;
-                out.y = e4m3(v[i][4], inv) | e4m3(v[i][5], inv) << 8 | e4m3(v[i][6], inv) << 16 | e4m3(v[i][7], inv) << 24;
-                *reinterpret_cast<uint2*>(dst + l16 * 8) = out;
-            }
-        } else {
+    for (int i0 = 0; i0 < 16; i0 += 4) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (c0 + l16 + 16 * j < cols) dst[l16 + 16 * j] = uint8_t(e4m3(v[i][j], inv));
+        for (int i = 0; i < 4; ++i) {
+            const uintptr_t dst = reinterpret_cast<uintptr_t>(q + (row0 + i0 + i) * cols + c0);
+            uint8_t* buffer = s_row[warp][i] + (dst & 3u);
+            uint32_t codes = e4m3x4(v[i0 + i][0], v[i0 + i][1], v[i0 + i][2], v[i0 + i][3], inv);
+            codes = nan_codes(codes, v[i0 + i][0], v[i0 + i][1], v[i0 + i][2], v[i0 + i][3]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) buffer[lane + 32 * j] = uint8_t(codes >> (8 * j));
         }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (row0 + i0 + i < rows) copy_bytes(s_row[warp][i], q + (row0 + i0 + i) * cols + c0, width, lane);
+        __syncwarp();
     }
 }
 
 __device__ __forceinline__ float e4m3_value(uint8_t q) {
     return __half2float(__half(__nv_cvt_fp8_to_halfraw(q, __NV_E4M3)));
+}
+
+// Eight of them, as they lie in memory.
+__device__ __forceinline__ void e4m3_values(uint2 q, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t word = i < 2 ? q.x : q.y;
+        const __half2 h = __half2(__nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t((word >> (16 * (i & 1))) & 0xffffu), __NV_E4M3));
+        const float2 f = __half22float2(h);
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+    }
+}
+
+// Eight codes of a row from column c0 on; zeros behind cols.
+template <bool VEC>
+__device__ __forceinline__ uint2 load_codes(const uint8_t* row, int c0, int cols) {
+    if (VEC) return __ldg(reinterpret_cast<const uint2*>(row + c0));
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (c0 + j < cols) w[j / 4] |= uint32_t(row[c0 + j]) << (8 * (j % 4));
+    return make_uint2(w[0], w[1]);
 }
 
 template <typename T>
@@ -221,21 +426,31 @@ __global__ void dequantize_kernel(const uint8_t* __restrict__ q, const float* __
     }
 }
 
-// Slope of the epilogue activations (tanh-form GELU) from CUDA's own expf and tanhf: the pass is bound by HBM, so the
-// accurate functions cost nothing.
-__device__ __forceinline__ float act_slope(float z, int act) {
+// Slope of the epilogue activations.  With s = sigmoid(t), t = 2 sqrt(2 / pi) (z + 0.044715 z^3): tanh-form GELU is z s, so its
+// slope is s + z s (1 - s) dt/dz; SiLU the same with t = z.  s comes from the SFU's ex2 and rcp as in the forward epilogue
+// (2 ulp; with expf and tanhf the pass was bound by arithmetic, 68 us for 8192 x 4096 instead of BACK_US).
+__device__ __forceinline__ float clamp_nan(float v, float lo, float hi) {      // keeps NaN
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(lo));
+    asm("min.NaN.f32 %0, %0, %1;" : "+f"(r) : "f"(hi));
+    return r;
+}
+
+template <int act>
+__device__ __forceinline__ float act_slope(float z) {
     if (act == EPI_RELU) return z > 0.0f ? 1.0f : 0.0f;
-    if (act == EPI_GELU) {
-        // Beyond +-30 the slope is 0 or 1 to the last bit, and z * z * z must not overflow.
-        z = fminf(fmaxf(z, -30.0f), 30.0f);
-        const float c = 0.7978845608028654f;
-        const float th = tanhf(c * (z + 0.044715f * z * z * z));
-        return 0.5f * (1.0f + th) + 0.5f * z * (1.0f - th * th) * c * (1.0f + 3.0f * 0.044715f * z * z);
-    }
-    if (act == EPI_NONE) return 1.0f;
-    const float s = 1.0f / (1.0f + expf(-z));
-    if (act == EPI_SIGMOID) return s * (1.0f - s);
-    return s > 0.0f ? s * (1.0f + z * (1.0f - s)) : 0.0f;
+    // Beyond these bounds the slope is within 1e-30 of 0 or 1; inside them no power of z and no exponential overflows.
+    constexpr float bound = act == EPI_GELU ? 10.0f : 80.0f;
+    constexpr float a = act == EPI_GELU ? 2.0f * 0.7978845608028654f : 1.0f;
+    constexpr float b = act == EPI_GELU ? a * 0.044715f : 0.0f;
+    constexpr float log2e = 1.4426950408889634f;
+    z = clamp_nan(z, -bound, bound);
+    const float z2 = z * z;
+    const float e = sfu_ex2(z * fmaf(-log2e * b, z2, -log2e * a));
+    const float s = sfu_rcp(1.0f + e);
+    const float rest = e * s;                                   // 1 - s without cancellation
+    if (act == EPI_SIGMOID) return s * rest;
+    return fmaf(z * rest * fmaf(3.0f * b, z2, a), s, s);
 }
 
 template <typename T>
@@ -249,9 +464,9 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
 // A CTA takes 256 columns and `rows_per` rows: 32 threads with eight columns each lie along a row, eight rows are worked on at
 // once.  Column sums stay in registers over the rows, are added across the eight threads of a column in a fixed order and go
 // to partial[row band][cols], which one more kernel adds up, again in order: the result does not depend on timing.
-template <typename T, bool VEC>
+template <typename T, bool VEC, int act>
 __global__ void __launch_bounds__(kThreads) act_backward_kernel(const T* __restrict__ dy, const uint8_t* __restrict__ z8,
-                                                                const float* __restrict__ zs, int act, T* __restrict__ dz,
+                                                                const float* __restrict__ zs, T* __restrict__ dz,
                                                                 long long ld_dz, float* __restrict__ partial, int rows, int cols,
                                                                 int rows_per) {
     __shared__ float s_sum[8][264];
@@ -261,6 +476,7 @@ __global__ void __launch_bounds__(kThreads) act_backward_kernel(const T* __restr
     float sum[8] = {};
     if (c0 < cols) {
         const float* s_col = zs + (long long)(c0 / FP8_BLOCK) * rows;
+#pragma unroll 4
         for (int r = blockIdx.y * rows_per + ty; r < r_end; r += 8) {
             const long long at = (long long)r * cols + c0;
             float g[8];
@@ -271,16 +487,11 @@ __global__ void __launch_bounds__(kThreads) act_backward_kernel(const T* __restr
                 for (int j = 0; j < 8; ++j) g[j] = c0 + j < cols ? to_float(dy[at + j]) : 0.0f;
             }
             if (act != EPI_NONE) {
-                uint8_t q[8];
-                if (VEC) {
-                    *reinterpret_cast<uint2*>(q) = __ldg(reinterpret_cast<const uint2*>(z8 + at));
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) q[j] = c0 + j < cols ? z8[at + j] : uint8_t(0);
-                }
+                float z[8];
+                e4m3_values(load_codes<VEC>(z8 + (long long)r * cols, c0, cols), z);
                 const float s = __ldg(s_col + r);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) g[j] *= act_slope(e4m3_value(q[j]) * s, act);
+                for (int j = 0; j < 8; ++j) g[j] *= act_slope<act>(z[j] * s);
             }
             if (!VEC) {
 #pragma unroll
@@ -305,13 +516,25 @@ __global__ void __launch_bounds__(kThreads) act_backward_kernel(const T* __restr
     }
 }
 
+// A CTA takes 32 columns, its eight warps every eighth band each; their sums are added in warp order.
 __global__ void __launch_bounds__(kThreads) add_bands_kernel(const float* __restrict__ partial, int bands, int cols,
                                                              float* __restrict__ out) {
-    const int c = blockIdx.x * kThreads + threadIdx.x;
-    if (c >= cols) return;
+    __shared__ float s_sum[8][32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int c = blockIdx.x * 32 + lane;
     float total = 0.0f;
-    for (int b = 0; b < bands; ++b) total += partial[(long long)b * cols + c];
-    out[c] = total;
+    if (c < cols) {
+#pragma unroll 4
+        for (int b = warp; b < bands; b += 8) total += partial[(long long)b * cols + c];
+    }
+    s_sum[warp][lane] = total;
+    __syncthreads();
+    if (warp == 0 && c < cols) {
+        total = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) total += s_sum[i][lane];
+        out[c] = total;
+    }
 }
 
 __global__ void __launch_bounds__(kThreads) block_tops_kernel(const float* __restrict__ scales, int rows, float* __restrict__ top) {
@@ -340,16 +563,10 @@ __global__ void __launch_bounds__(kThreads) dequantize_rows_kernel(const uint8_t
         const int b = c0 / FP8_BLOCK;
         float s = __ldg(scales + (long long)b * rows + r);
         if (top != nullptr) s /= __ldg(top + b);
-        uint8_t v[8];
-        if (VEC) {
-            *reinterpret_cast<uint2*>(v) = __ldg(reinterpret_cast<const uint2*>(q + r * cols + c0));
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = c0 + j < cols ? q[r * cols + c0 + j] : uint8_t(0);
-        }
         float f[8];
+        e4m3_values(load_codes<VEC>(q + r * cols, c0, cols), f);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = e4m3_value(v[j]) * s;
+        for (int j = 0; j < 8; ++j) f[j] *= s;
         store8(y + r * ld_y + c0, f);
     }
 }
@@ -358,7 +575,7 @@ template <typename T>
 void act_backward_typed(const T* dy, const uint8_t* z8, const float* z_scales, int act, T* dz, long long ld_dz, float* db,
                         int rows, int cols, cudaStream_t stream) {
     const bool vec = cols % 8 == 0 && reinterpret_cast<uintptr_t>(dy) % 16 == 0 && reinterpret_cast<uintptr_t>(z8) % 8 == 0;
-    const int rows_per = rows > 2048 ? 128 : 32;
+    const int rows_per = rows > 4096 ? 64 : 32;
     const int bands = (rows + rows_per - 1) / rows_per;
     CB200_REQUIRE(bands <= 65535, "too many rows");
     Scratch partial;
@@ -368,11 +585,19 @@ void act_backward_typed(const T* dy, const uint8_t* z8, const float* z_scales, i
         to = static_cast<float*>(partial.ptr);
     }
     const dim3 grid((cols + 255) / 256, bands);
-    if (vec) act_backward_kernel<T, true><<<grid, kThreads, 0, stream>>>(dy, z8, z_scales, act, dz, ld_dz, to, rows, cols, rows_per);
-    else act_backward_kernel<T, false><<<grid, kThreads, 0, stream>>>(dy, z8, z_scales, act, dz, ld_dz, to, rows, cols, rows_per);
+    auto launch = [&](auto code) {
+        constexpr int A = decltype(code)::value;
+        if (vec) act_backward_kernel<T, true, A><<<grid, kThreads, 0, stream>>>(dy, z8, z_scales, dz, ld_dz, to, rows, cols, rows_per);
+        else act_backward_kernel<T, false, A><<<grid, kThreads, 0, stream>>>(dy, z8, z_scales, dz, ld_dz, to, rows, cols, rows_per);
+    };
+    if (act == EPI_RELU) launch(std::integral_constant<int, EPI_RELU>{});
+    else if (act == EPI_GELU) launch(std::integral_constant<int, EPI_GELU>{});
+    else if (act == EPI_SILU) launch(std::integral_constant<int, EPI_SILU>{});
+    else if (act == EPI_SIGMOID) launch(std::integral_constant<int, EPI_SIGMOID>{});
+    else launch(std::integral_constant<int, EPI_NONE>{});
     CB200_CHECK_LAUNCH();
     if (to != db) {
-        add_bands_kernel<<<(cols + kThreads - 1) / kThreads, kThreads, 0, stream>>>(to, bands, cols, db);
+        add_bands_kernel<<<(cols + 31) / 32, kThreads, 0, stream>>>(to, bands, cols, db);
         CB200_CHECK_LAUNCH();
     }
 }
@@ -385,21 +610,20 @@ unsigned pass_grid(long long items) {
 
 template <typename T>
 void quantize_typed(const T* x, long long rows, int cols, int block_rows, uint8_t* q, float* scales, cudaStream_t stream) {
-    const bool vec = cols % 8 == 0 && (cols * sizeof(T)) % 16 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 &&
-                     reinterpret_cast<uintptr_t>(q) % 8 == 0;
+    // Rows of whole 16-byte units that start on their boundaries, and codes (4 or 8 to a unit) likewise.
+    const bool vec = (cols * sizeof(T)) % 16 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 &&
+                     reinterpret_cast<uintptr_t>(q) % Unit<T>::N == 0;
     const unsigned blocks = unsigned((cols + FP8_BLOCK - 1) / FP8_BLOCK);
     const int rows_per = block_rows == 1 ? 32 : FP8_BLOCK;
-    // gridDim.y holds 65535: more rows go in bands (their scales are addressed from the whole matrix's first row).
-    CB200_REQUIRE((rows + rows_per - 1) / rows_per <= 65535, "quantize_fp8: too many rows");
+    CB200_REQUIRE((rows + rows_per - 1) / rows_per <= 65535, "quantize_fp8: too many rows");      // gridDim.y
     const unsigned bands = unsigned((rows + rows_per - 1) / rows_per);
+    const dim3 grid(block_rows == 1 ? (blocks + 3) / 4 : blocks, bands);
     if (block_rows == 1) {
-        const dim3 grid((blocks + 1) / 2, bands);
-        if (vec) quantize_rows_kernel<T, true><<<grid, kThreads, 0, stream>>>(x, rows, cols, q, scales);
-        else quantize_rows_kernel<T, false><<<grid, kThreads, 0, stream>>>(x, rows, cols, q, scales);
+        if (vec) quantize_rows_kernel<T><<<grid, kThreads, 0, stream>>>(x, rows, cols, q, scales);
+        else quantize_rows_any_kernel<T><<<grid, kThreads, 0, stream>>>(x, rows, cols, q, scales);
     } else {
-        const dim3 grid(blocks, bands);
-        if (vec) quantize_tiles_kernel<T, true><<<grid, kThreads, 0, stream>>>(x, rows, cols, q, scales);
-        else quantize_tiles_kernel<T, false><<<grid, kThreads, 0, stream>>>(x, rows, cols, q, scales);
+        if (vec) quantize_tiles_kernel<T><<<grid, kThreads, 0, stream>>>(x, rows, cols, q, scales);
+        else quantize_tiles_any_kernel<T><<<grid, kThreads, 0, stream>>>(x, rows, cols, q, scales);
     }
     CB200_CHECK_LAUNCH();
 }
