@@ -129,21 +129,44 @@ __device__ __forceinline__ uint32_t nan_codes(uint32_t q, float a, float b, floa
     return q;
 }
 
-// `bytes` bytes from shared memory, where they lie with the phase of dst within 4-byte words, to dst: whole words but
-// at the ends.  Whole warp; `buffer` is word-aligned.
-__device__ __forceinline__ void copy_bytes(const uint8_t* buffer, uint8_t* dst, int bytes, int lane) {
-    const int phase = int(reinterpret_cast<uintptr_t>(dst) & 3u);
-    uint8_t* base = dst - phase;
-    for (int w = lane; 4 * w < phase + bytes; w += 32) {
-        if (4 * w >= phase && 4 * w + 4 <= phase + bytes) {
-            reinterpret_cast<uint32_t*>(base)[w] = reinterpret_cast<const uint32_t*>(buffer)[w];
-        } else {
+// A row's 128 elements of a block that start anywhere, across a warp: a lane takes every 32nd, so that loads and byte stores
+// are contiguous across the lanes.  Loads are not conditional: lanes behind the row's end read its last element and drop it
+// (a branch around each load kept the loads of a block from being under way together: 4100 x 11007 FP32 78 us instead of
+// QTILES; four neighbouring elements a lane, to store their codes as a word, were four times as many requests to L1: 100 us).
+struct RowSlice {
+    float v[4];
+    // The first `width` (1 to 128) elements of the block; zeros for a row that is not there (src then is some row that is).
+    template <typename T>
+    __device__ __forceinline__ void load(const T* src, int width, bool there, int lane) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (4 * w + j >= phase && 4 * w + j < phase + bytes) base[4 * w + j] = buffer[4 * w + j];
-        }
+        for (int j = 0; j < 4; ++j) v[j] = to_float(src[min(lane + 32 * j, width - 1)]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (!there || lane + 32 * j >= width) v[j] = 0.0f;
     }
-}
+    __device__ __forceinline__ uint32_t top(uint32_t m) const {      // as Unit::top
+#pragma unroll
+        for (int j = 0; j < 4; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+        return m;
+    }
+    __device__ __forceinline__ float finite_top(float amax) const {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) amax = fmaxf(amax, finite_abs(v[j]));
+        return amax;
+    }
+    __device__ __forceinline__ void store(uint8_t* dst, int width, int lane, float inv, bool finite) const {
+        uint32_t codes = e4m3x4(v[0], v[1], v[2], v[3], inv);
+        if (!finite) codes = nan_codes(codes, v[0], v[1], v[2], v[3]);
+        if (width == FP8_BLOCK) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) dst[lane + 32 * j] = uint8_t(codes >> (8 * j));
+            return;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (lane + 32 * j < width) dst[lane + 32 * j] = uint8_t(codes >> (8 * j));
+    }
+};
 
 // Blocks of 1 x 128.  Eight lanes own a block, 16 elements each in units of 16 bytes; a warp takes four neighbouring blocks of
 // four rows, so a lane has 8 (16-bit types) or 16 independent loads under way, and a CTA 32 rows x 512 columns.  The
@@ -216,47 +239,33 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __rest
     }
 }
 
-// The same for rows that start anywhere: a warp takes a block at a time, element by element, and the codes of its four
-// blocks of a row pass through shared memory to leave as words.
+// The same for rows that start anywhere: a warp takes four rows of a block at a time.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) quantize_rows_any_kernel(const T* __restrict__ x, long long rows, int cols,
                                                                      uint8_t* __restrict__ q, float* __restrict__ scales) {
     __shared__ float s_scale[4][32];
-    __shared__ __align__(16) uint8_t s_row[kThreads / 32][528];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int c0 = blockIdx.x * 4 * FP8_BLOCK;
-    const int width = min(4 * FP8_BLOCK, cols - c0);
-    for (int i = 0; i < 4; ++i) {
-        const long long r = (long long)blockIdx.y * 32 + warp * 4 + i;
-        if (r >= rows) break;
-        const T* src = x + r * cols + c0;
-        uint8_t* dst = q + r * cols + c0;
-        uint8_t* buffer = s_row[warp] + (reinterpret_cast<uintptr_t>(dst) & 3u);
-        float v[4][4];
+    const long long row0 = (long long)blockIdx.y * 32 + warp * 4;
+#pragma unroll 1
+    for (int b = 0; b < 4; ++b) {
+        const int c0 = (blockIdx.x * 4 + b) * FP8_BLOCK;
+        if (c0 >= cols) break;
+        const int width = min(FP8_BLOCK, cols - c0);
+        RowSlice slice[4];
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int c = b * FP8_BLOCK + lane + 32 * j;
-                v[b][j] = c < width ? to_float(src[c]) : 0.0f;
-            }
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            float amax = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) amax = fmaxf(amax, finite_abs(v[b][j]));
-            // Magnitudes order as their bits do.
-            amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
-            const int e = scale_exponent(amax);
-            if (lane == 0) s_scale[b][warp * 4 + i] = pow2(e);
-            uint32_t codes = e4m3x4(v[b][0], v[b][1], v[b][2], v[b][3], pow2(-e));
-            codes = nan_codes(codes, v[b][0], v[b][1], v[b][2], v[b][3]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) buffer[b * FP8_BLOCK + lane + 32 * j] = uint8_t(codes >> (8 * j));
+        for (int i = 0; i < 4; ++i) {
+            slice[i].load(x + min(row0 + i, rows - 1) * cols + c0, width, row0 + i < rows, lane);
         }
-        __syncwarp();
-        copy_bytes(s_row[warp], dst, width, lane);
-        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t m = __reduce_max_sync(0xffffffffu, slice[i].top(0));
+            const bool finite = top_finite<float>(m);
+            if (!finite) m = __reduce_max_sync(0xffffffffu, __float_as_uint(slice[i].finite_top(0.0f)));
+            const int e = scale_exponent(__uint_as_float(m));
+            if (lane == 0) s_scale[b][warp * 4 + i] = pow2(e);
+            const long long at = (row0 + i) * cols + c0;
+            if (row0 + i < rows) slice[i].store(q + at, width, lane, pow2(-e), finite);
+        }
     }
     __syncthreads();
     if (threadIdx.x < 128) {
@@ -337,52 +346,47 @@ __global__ void __launch_bounds__(kThreads) quantize_tiles_kernel(const T* __res
     }
 }
 
-// The same for rows that start anywhere: a warp holds 16 rows, a lane every 32nd element of them, and each row's codes pass
-// through shared memory to leave as words.  4100 x 11007 FP32, 226 MB: QTILES.
+// The same for rows that start anywhere: a warp holds eight rows.  4100 x 11007 FP32, 226 MB: QTILES.
+constexpr int kTileThreads = 512;
 template <typename T>
-__global__ void __launch_bounds__(kThreads) quantize_tiles_any_kernel(const T* __restrict__ x, long long rows, int cols,
-                                                                      uint8_t* __restrict__ q, float* __restrict__ scales) {
-    __shared__ float s_max[kThreads / 32];
-    __shared__ __align__(16) uint8_t s_row[kThreads / 32][4][132];
+__global__ void __launch_bounds__(kTileThreads) quantize_tiles_any_kernel(const T* __restrict__ x, long long rows, int cols,
+                                                                          uint8_t* __restrict__ q, float* __restrict__ scales) {
+    __shared__ uint32_t s_top[kTileThreads / 32], s_finite_top[kTileThreads / 32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int c0 = blockIdx.x * FP8_BLOCK;
     const int width = min(FP8_BLOCK, cols - c0);
-    const long long row0 = (long long)blockIdx.y * FP8_BLOCK + warp * 16;
-    float v[16][4];
+    const long long row0 = (long long)blockIdx.y * FP8_BLOCK + warp * 8;
+    RowSlice slice[8];
+    uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
+    for (int i = 0; i < 8; ++i) {
+        slice[i].load(x + min(row0 + i, rows - 1) * cols + c0, width, row0 + i < rows, lane);
+    }
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            v[i][j] = row0 + i < rows && lane + 32 * j < width ? to_float(x[(row0 + i) * cols + c0 + lane + 32 * j]) : 0.0f;
-    float amax = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) amax = fmaxf(amax, finite_abs(v[i][j]));
-    amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
-    if (lane == 0) s_max[warp] = amax;
+    for (int i = 0; i < 8; ++i) m = slice[i].top(m);
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (lane == 0) s_top[warp] = m;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) amax = fmaxf(amax, s_max[w]);
-    const int e = scale_exponent(amax);
+    for (int w = 0; w < kTileThreads / 32; ++w) m = max(m, s_top[w]);
+    const bool finite = top_finite<float>(m);      // the same for the whole CTA
+    if (!finite) {
+        float amax = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) amax = slice[i].finite_top(amax);
+        m = __reduce_max_sync(0xffffffffu, __float_as_uint(amax));
+        if (lane == 0) s_finite_top[warp] = m;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kTileThreads / 32; ++w) m = max(m, s_finite_top[w]);
+    }
+    const int e = scale_exponent(__uint_as_float(m));
     const float inv = pow2(-e);
     if (threadIdx.x == 0) scales[(long long)blockIdx.y * gridDim.x + blockIdx.x] = pow2(e);
 #pragma unroll
-    for (int i0 = 0; i0 < 16; i0 += 4) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uintptr_t dst = reinterpret_cast<uintptr_t>(q + (row0 + i0 + i) * cols + c0);
-            uint8_t* buffer = s_row[warp][i] + (dst & 3u);
-            uint32_t codes = e4m3x4(v[i0 + i][0], v[i0 + i][1], v[i0 + i][2], v[i0 + i][3], inv);
-            codes = nan_codes(codes, v[i0 + i][0], v[i0 + i][1], v[i0 + i][2], v[i0 + i][3]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) buffer[lane + 32 * j] = uint8_t(codes >> (8 * j));
-        }
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (row0 + i0 + i < rows) copy_bytes(s_row[warp][i], q + (row0 + i0 + i) * cols + c0, width, lane);
-        __syncwarp();
+    for (int i = 0; i < 8; ++i) {
+        const long long at = (row0 + i) * cols + c0;
+        if (row0 + i < rows) slice[i].store(q + at, width, lane, inv, finite);
     }
 }
 
@@ -623,7 +627,7 @@ void quantize_typed(const T* x, long long rows, int cols, int block_rows, uint8_
         else quantize_rows_any_kernel<T><<<grid, kThreads, 0, stream>>>(x, rows, cols, q, scales);
     } else {
         if (vec) quantize_tiles_kernel<T><<<grid, kThreads, 0, stream>>>(x, rows, cols, q, scales);
-        else quantize_tiles_any_kernel<T><<<grid, kThreads, 0, stream>>>(x, rows, cols, q, scales);
+        else quantize_tiles_any_kernel<T><<<grid, kTileThreads, 0, stream>>>(x, rows, cols, q, scales);
     }
     CB200_CHECK_LAUNCH();
 }
