@@ -406,14 +406,41 @@ __device__ __forceinline__ void e4m3_values(uint2 q, float (&v)[8]) {
     }
 }
 
+// Eight 16-bit values of a row from column c0 on; zeros behind cols.
+template <typename T>
+struct Unit8 {
+    uint4 w;
+    template <bool VEC>
+    __device__ __forceinline__ void load(const T* row, int c0, int cols) {
+        if (VEC) {
+            w = __ldg(reinterpret_cast<const uint4*>(row + c0));
+        } else {
+            alignas(16) T t[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                t[j] = row[min(c0 + j, cols - 1)];
+                if (c0 + j >= cols) t[j] = from_float<T>(0.0f);
+            }
+            w = *reinterpret_cast<const uint4*>(t);
+        }
+    }
+    __device__ __forceinline__ void values(float (&v)[8]) const {
+        const T* t = reinterpret_cast<const T*>(&w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = to_float(t[j]);
+    }
+};
+
 // Eight codes of a row from column c0 on; zeros behind cols.
 template <bool VEC>
 __device__ __forceinline__ uint2 load_codes(const uint8_t* row, int c0, int cols) {
     if (VEC) return __ldg(reinterpret_cast<const uint2*>(row + c0));
     uint32_t w[2] = {0, 0};
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-        if (c0 + j < cols) w[j / 4] |= uint32_t(row[c0 + j]) << (8 * (j % 4));
+    for (int j = 0; j < 8; ++j) {
+        const uint32_t code = row[min(c0 + j, cols - 1)];
+        w[j / 4] |= (c0 + j < cols ? code : 0u) << (8 * (j % 4));
+    }
     return make_uint2(w[0], w[1]);
 }
 
@@ -465,8 +492,7 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
     *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(t);
 }
 
-// A CTA takes 256 columns and `rows_per` rows: 32 threads with eight columns each lie along a row, eight rows are worked on at
-// once.  Column sums stay in registers over the rows, are added across the eight threads of a column in a fixed order and go
+// A CTA takes 256 columns and `rows_per` rows: 32 threads with eight columns each lie along a row, eight rows side by side.  Column sums stay in registers over the rows, are added across the eight threads of a column in a fixed order and go
 // to partial[row band][cols], which one more kernel adds up, again in order: the result does not depend on timing.
 template <typename T, bool VEC, int act>
 __global__ void __launch_bounds__(kThreads) act_backward_kernel(const T* __restrict__ dy, const uint8_t* __restrict__ z8,
@@ -480,31 +506,41 @@ __global__ void __launch_bounds__(kThreads) act_backward_kernel(const T* __restr
     float sum[8] = {};
     if (c0 < cols) {
         const float* s_col = zs + (long long)(c0 / FP8_BLOCK) * rows;
-#pragma unroll 4
-        for (int r = blockIdx.y * rows_per + ty; r < r_end; r += 8) {
-            const long long at = (long long)r * cols + c0;
-            float g[8];
-            if (VEC) {
-                load8(dy + at, g);
-            } else {
+        // Four rows at a time, their loads under way together (rows behind the band read its last one).
+        for (int r0 = blockIdx.y * rows_per + ty; r0 < r_end; r0 += 32) {
+            Unit8<T> g8[4];
+            uint2 z8s[4];
+            float s[4];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) g[j] = c0 + j < cols ? to_float(dy[at + j]) : 0.0f;
-            }
-            if (act != EPI_NONE) {
-                float z[8];
-                e4m3_values(load_codes<VEC>(z8 + (long long)r * cols, c0, cols), z);
-                const float s = __ldg(s_col + r);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) g[j] *= act_slope<act>(z[j] * s);
-            }
-            if (!VEC) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (c0 + j >= cols) g[j] = 0.0f;
+            for (int i = 0; i < 4; ++i) {
+                const int r = min(r0 + 8 * i, r_end - 1);
+                g8[i].template load<VEC>(dy + (long long)r * cols, c0, cols);
+                if (act != EPI_NONE) {
+                    z8s[i] = load_codes<VEC>(z8 + (long long)r * cols, c0, cols);
+                    s[i] = __ldg(s_col + r);
+                }
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sum[j] += g[j];
-            if (dz != nullptr) store8(dz + r * ld_dz + c0, g);
+            for (int i = 0; i < 4; ++i) {
+                const int r = r0 + 8 * i;
+                if (r >= r_end) break;
+                float g[8];
+                g8[i].values(g);
+                if (act != EPI_NONE) {
+                    float z[8];
+                    e4m3_values(z8s[i], z);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) g[j] *= act_slope<act>(z[j] * s[i]);
+                }
+                if (!VEC) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (c0 + j >= cols) g[j] = 0.0f;
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum[j] += g[j];
+                if (dz != nullptr) store8(dz + r * ld_dz + c0, g);
+            }
         }
     }
     if (partial == nullptr) return;
