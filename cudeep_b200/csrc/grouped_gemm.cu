@@ -32,15 +32,6 @@ __global__ void __launch_bounds__(32) group_maps_kernel(const __grid_constant__ 
 #endif
 }
 
-RaggedPlan plan_weight(int groups, int features, int cols) {
-    const int sms = device_info().num_sms;
-    RaggedPlan plan{features <= 128 ? 1 : 2, 256, 0};
-    const long long f_tiles = (features + 128 * plan.ctas - 1) / (128 * plan.ctas);
-    if (cols <= 128 || groups * f_tiles * ((cols + 255) / 256) * plan.ctas < sms) plan.tile_cols = 128;
-    plan.units = groups * f_tiles * ((cols + plan.tile_cols - 1) / plan.tile_cols);
-    return plan;
-}
-
 template <RaggedForm FORM, int CTAS, bool BF16, class OutT>
 void launch(RaggedParams& p, const RaggedPlan& plan, cudaStream_t stream) {
     const DeviceInfo& dev = device_info();
@@ -118,7 +109,7 @@ void rows_by_weight(bool nn, const void* a, long long lda, const void* w, void* 
     p.features = n;
     p.k = k;
     p.chunk_rows = RAGGED_BK;
-    const RaggedPlan plan = plan_rows(groups, rows, n);
+    const RaggedPlan plan = plan_rows(groups, rows, n, (k + RAGGED_BK - 1) / RAGGED_BK);
     if (nn) launch_rows<RaggedForm::NN>(p, plan, type, stream);
     else launch_rows<RaggedForm::NT>(p, plan, type, stream);
 }
@@ -158,7 +149,7 @@ void grouped_tn(const void* a, long long lda, const void* b, long long ldb, void
     const AlignedRows y = rows_of(a, lda, rows, m, stream);
     const AlignedRows x = rows_of(b, ldb, rows, n, stream);
     RaggedParams p{};
-    const RaggedPlan plan = plan_weight(groups, m, n);
+    const RaggedPlan plan = plan_weight(groups, rows, m, n, elem_bytes(c_type));
     p.a_chunked = encode_columns(&p.map_a, y, rows, m, 2);
     p.b_chunked = encode_columns(&p.map_b, x, rows, n, plan.tile_cols / plan.ctas / 64);
     const uint32_t c_bytes = uint32_t(elem_bytes(c_type));

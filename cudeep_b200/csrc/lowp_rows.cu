@@ -1,8 +1,13 @@
 // One-pass kernels around the 8-bit and the grouped products: padding of rows for the TMA unit, quantisation to e4m3
 // in blocks and back.  All are bound by HBM: each input is read once and each output written once.
+//
+// Each kernel waits for its predecessors itself and then lets its successor be set up, so that in a sequence of small launches (the
+// backward pass of a short batch is nine) the launches overlap.
 #include "lowp_rows.h"
 
 #include "epilogue_math.cuh"
+#include "launch_dependent.h"
+#include "sm100_ptx.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -19,6 +24,8 @@ constexpr int kThreads = 256;
 // dst[r, 0..ld) = src[r, 0..cols) followed by zeros; ld is a multiple of 16 bytes, a thread writes 16 of them.
 template <typename T>
 __global__ void pad_rows_kernel(const T* __restrict__ src, T* __restrict__ dst, long long rows, int cols, int units_row) {
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
     constexpr int V = 16 / sizeof(T);
     const long long total = rows * units_row;
     for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
@@ -175,6 +182,8 @@ struct RowSlice {
 template <typename T>
 __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __restrict__ x, long long rows, int cols,
                                                                  uint8_t* __restrict__ q, float* __restrict__ scales) {
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
     constexpr int N = Unit<T>::N, UNITS = 16 / N;
     __shared__ float s_scale[4][32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -243,6 +252,8 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __rest
 template <typename T>
 __global__ void __launch_bounds__(kThreads) quantize_rows_any_kernel(const T* __restrict__ x, long long rows, int cols,
                                                                      uint8_t* __restrict__ q, float* __restrict__ scales) {
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
     __shared__ float s_scale[4][32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long row0 = (long long)blockIdx.y * 32 + warp * 4;
@@ -280,6 +291,8 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_any_kernel(const T* __
 template <typename T>
 __global__ void __launch_bounds__(kThreads) quantize_tiles_kernel(const T* __restrict__ x, long long rows, int cols,
                                                                   uint8_t* __restrict__ q, float* __restrict__ scales) {
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
     constexpr int N = Unit<T>::N, UNITS = 16 / N;
     __shared__ float s_max[kThreads / 32];
     __shared__ uint32_t s_top[kThreads / 32];
@@ -351,6 +364,8 @@ constexpr int kTileThreads = 512;
 template <typename T>
 __global__ void __launch_bounds__(kTileThreads) quantize_tiles_any_kernel(const T* __restrict__ x, long long rows, int cols,
                                                                           uint8_t* __restrict__ q, float* __restrict__ scales) {
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
     __shared__ uint32_t s_top[kTileThreads / 32], s_finite_top[kTileThreads / 32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int c0 = blockIdx.x * FP8_BLOCK;
@@ -447,6 +462,8 @@ __device__ __forceinline__ uint2 load_codes(const uint8_t* row, int c0, int cols
 template <typename T>
 __global__ void dequantize_kernel(const uint8_t* __restrict__ q, const float* __restrict__ scales, long long rows, int cols,
                                   int block_rows, T* __restrict__ y) {
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
     const int col_blocks = (cols + FP8_BLOCK - 1) / FP8_BLOCK;
     const long long total = rows * cols;
     for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
@@ -499,6 +516,8 @@ __global__ void __launch_bounds__(kThreads) act_backward_kernel(const T* __restr
                                                                 const float* __restrict__ zs, T* __restrict__ dz,
                                                                 long long ld_dz, float* __restrict__ partial, int rows, int cols,
                                                                 int rows_per) {
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
     __shared__ float s_sum[8][264];
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
     const int c0 = blockIdx.x * 256 + tx * 8;
@@ -559,6 +578,8 @@ __global__ void __launch_bounds__(kThreads) act_backward_kernel(const T* __restr
 // A CTA takes 32 columns, its eight warps every eighth band each; their sums are added in warp order.
 __global__ void __launch_bounds__(kThreads) add_bands_kernel(const float* __restrict__ partial, int bands, int cols,
                                                              float* __restrict__ out) {
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
     __shared__ float s_sum[8][32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int c = blockIdx.x * 32 + lane;
@@ -578,6 +599,8 @@ __global__ void __launch_bounds__(kThreads) add_bands_kernel(const float* __rest
 }
 
 __global__ void __launch_bounds__(kThreads) block_tops_kernel(const float* __restrict__ scales, int rows, float* __restrict__ top) {
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
     __shared__ float s_max[kThreads / 32];
     float m = 0.0f;
     for (int r = threadIdx.x; r < rows; r += kThreads) m = fmaxf(m, finite_abs(__ldg(scales + (long long)blockIdx.x * rows + r)));
@@ -595,6 +618,8 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads) dequantize_rows_kernel(const uint8_t* __restrict__ q, const float* __restrict__ scales,
                                                                    const float* __restrict__ top, int rows, int cols,
                                                                    T* __restrict__ y, long long ld_y) {
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
     const int units = (cols + 7) / 8;
     const long long total = (long long)rows * units;
     for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
@@ -627,8 +652,8 @@ void act_backward_typed(const T* dy, const uint8_t* z8, const float* z_scales, i
     const dim3 grid((cols + 255) / 256, bands);
     auto launch = [&](auto code) {
         constexpr int A = decltype(code)::value;
-        if (vec) act_backward_kernel<T, true, A><<<grid, kThreads, 0, stream>>>(dy, z8, z_scales, dz, ld_dz, to, rows, cols, rows_per);
-        else act_backward_kernel<T, false, A><<<grid, kThreads, 0, stream>>>(dy, z8, z_scales, dz, ld_dz, to, rows, cols, rows_per);
+        if (vec) launch_dependent(act_backward_kernel<T, true, A>, dim3(grid), kThreads, stream, dy, z8, z_scales, dz, ld_dz, to, rows, cols, rows_per);
+        else launch_dependent(act_backward_kernel<T, false, A>, dim3(grid), kThreads, stream, dy, z8, z_scales, dz, ld_dz, to, rows, cols, rows_per);
     };
     if (act == EPI_RELU) launch(std::integral_constant<int, EPI_RELU>{});
     else if (act == EPI_GELU) launch(std::integral_constant<int, EPI_GELU>{});
@@ -637,7 +662,7 @@ void act_backward_typed(const T* dy, const uint8_t* z8, const float* z_scales, i
     else launch(std::integral_constant<int, EPI_NONE>{});
     CB200_CHECK_LAUNCH();
     if (to != db) {
-        add_bands_kernel<<<(cols + 31) / 32, kThreads, 0, stream>>>(to, bands, cols, db);
+        launch_dependent(add_bands_kernel, dim3((cols + 31) / 32), kThreads, stream, to, bands, cols, db);
         CB200_CHECK_LAUNCH();
     }
 }
@@ -659,11 +684,11 @@ void quantize_typed(const T* x, long long rows, int cols, int block_rows, uint8_
     const unsigned bands = unsigned((rows + rows_per - 1) / rows_per);
     const dim3 grid(block_rows == 1 ? (blocks + 3) / 4 : blocks, bands);
     if (block_rows == 1) {
-        if (vec) quantize_rows_kernel<T><<<grid, kThreads, 0, stream>>>(x, rows, cols, q, scales);
-        else quantize_rows_any_kernel<T><<<grid, kThreads, 0, stream>>>(x, rows, cols, q, scales);
+        if (vec) launch_dependent(quantize_rows_kernel<T>, dim3(grid), kThreads, stream, x, rows, cols, q, scales);
+        else launch_dependent(quantize_rows_any_kernel<T>, dim3(grid), kThreads, stream, x, rows, cols, q, scales);
     } else {
-        if (vec) quantize_tiles_kernel<T><<<grid, kThreads, 0, stream>>>(x, rows, cols, q, scales);
-        else quantize_tiles_any_kernel<T><<<grid, kTileThreads, 0, stream>>>(x, rows, cols, q, scales);
+        if (vec) launch_dependent(quantize_tiles_kernel<T>, dim3(grid), kThreads, stream, x, rows, cols, q, scales);
+        else launch_dependent(quantize_tiles_any_kernel<T>, dim3(grid), kTileThreads, stream, x, rows, cols, q, scales);
     }
     CB200_CHECK_LAUNCH();
 }
@@ -683,10 +708,10 @@ AlignedRows aligned_rows(const void* src, long long rows, int cols, int elem_siz
     out.copy = Scratch(size_t(rows) * units * 16, stream);
     out.ptr = out.copy.ptr;
     if (elem_size == 1)
-        pad_rows_kernel<uint8_t><<<pass_grid(rows * units), kThreads, 0, stream>>>(
+        launch_dependent(pad_rows_kernel<uint8_t>, dim3(pass_grid(rows * units)), kThreads, stream,
             static_cast<const uint8_t*>(src), static_cast<uint8_t*>(out.copy.ptr), rows, cols, units);
     else
-        pad_rows_kernel<uint16_t><<<pass_grid(rows * units), kThreads, 0, stream>>>(
+        launch_dependent(pad_rows_kernel<uint16_t>, dim3(pass_grid(rows * units)), kThreads, stream,
             static_cast<const uint16_t*>(src), static_cast<uint16_t*>(out.copy.ptr), rows, cols, units);
     CB200_CHECK_LAUNCH();
     return out;
@@ -703,11 +728,14 @@ void dequantize_fp8(const uint8_t* q, const float* scales, long long rows, int c
                     cudaStream_t stream) {
     const unsigned grid = pass_grid(rows * cols);
     if (y_type == TYPE_F32)
-        dequantize_kernel<<<grid, kThreads, 0, stream>>>(q, scales, rows, cols, block_rows, static_cast<float*>(y));
+        launch_dependent(dequantize_kernel<float>, dim3(grid), kThreads, stream, q, scales, rows, cols, block_rows,
+                         static_cast<float*>(y));
     else if (y_type == TYPE_F16)
-        dequantize_kernel<<<grid, kThreads, 0, stream>>>(q, scales, rows, cols, block_rows, static_cast<__half*>(y));
+        launch_dependent(dequantize_kernel<__half>, dim3(grid), kThreads, stream, q, scales, rows, cols, block_rows,
+                         static_cast<__half*>(y));
     else
-        dequantize_kernel<<<grid, kThreads, 0, stream>>>(q, scales, rows, cols, block_rows, static_cast<__nv_bfloat16*>(y));
+        launch_dependent(dequantize_kernel<__nv_bfloat16>, dim3(grid), kThreads, stream, q, scales, rows, cols, block_rows,
+                         static_cast<__nv_bfloat16*>(y));
     CB200_CHECK_LAUNCH();
 }
 
@@ -722,7 +750,7 @@ void activation_backward_fp8(const void* dy, int type, const uint8_t* z8, const 
 }
 
 void block_tops(const float* scales, int rows, int cols, float* top, cudaStream_t stream) {
-    block_tops_kernel<<<(cols + FP8_BLOCK - 1) / FP8_BLOCK, kThreads, 0, stream>>>(scales, rows, top);
+    launch_dependent(block_tops_kernel, dim3((cols + FP8_BLOCK - 1) / FP8_BLOCK), kThreads, stream, scales, rows, top);
     CB200_CHECK_LAUNCH();
 }
 
@@ -732,12 +760,12 @@ void dequantize_rows(const uint8_t* q, const float* scales, const float* top, in
     const unsigned grid = pass_grid((long long)rows * ((cols + 7) / 8));
     if (y_type == TYPE_F16) {
         __half* out = static_cast<__half*>(y);
-        if (vec) dequantize_rows_kernel<__half, true><<<grid, kThreads, 0, stream>>>(q, scales, top, rows, cols, out, ld_y);
-        else dequantize_rows_kernel<__half, false><<<grid, kThreads, 0, stream>>>(q, scales, top, rows, cols, out, ld_y);
+        if (vec) launch_dependent(dequantize_rows_kernel<__half, true>, dim3(grid), kThreads, stream, q, scales, top, rows, cols, out, ld_y);
+        else launch_dependent(dequantize_rows_kernel<__half, false>, dim3(grid), kThreads, stream, q, scales, top, rows, cols, out, ld_y);
     } else {
         __nv_bfloat16* out = static_cast<__nv_bfloat16*>(y);
-        if (vec) dequantize_rows_kernel<__nv_bfloat16, true><<<grid, kThreads, 0, stream>>>(q, scales, top, rows, cols, out, ld_y);
-        else dequantize_rows_kernel<__nv_bfloat16, false><<<grid, kThreads, 0, stream>>>(q, scales, top, rows, cols, out, ld_y);
+        if (vec) launch_dependent(dequantize_rows_kernel<__nv_bfloat16, true>, dim3(grid), kThreads, stream, q, scales, top, rows, cols, out, ld_y);
+        else launch_dependent(dequantize_rows_kernel<__nv_bfloat16, false>, dim3(grid), kThreads, stream, q, scales, top, rows, cols, out, ld_y);
     }
     CB200_CHECK_LAUNCH();
 }

@@ -1,7 +1,11 @@
 // Tile choice and launch shared by the ragged and the 8-bit products.
 #pragma once
 
+#include "launch_dependent.h"
 #include "umma_gemm.cuh"
+
+#include <algorithm>
+#include <cmath>
 
 namespace cudeep_b200 {
 
@@ -11,22 +15,62 @@ struct RaggedPlan {
     long long units;      // most tiles there can be, whatever the group sizes
 };
 
-// Rows of `groups` groups, `rows` in all, on the columns of the tiles.
-inline RaggedPlan plan_rows(int groups, int rows, int features) {
+// An SM takes in about 41 bytes of operands a cycle from L2, 20 from HBM (measured: 16 KB boxes, all SMs loading), and a K
+// block of 128 bytes per row costs two cycles of MMAs per column on 128 lanes.
+constexpr double PLAN_L2_BYTES = 41.0, PLAN_HBM_BYTES = 20.0, PLAN_MMA_CYCLES = 2.0;
+
+// Rows of `groups` groups, `rows` in all, on the columns of the tiles; `blocks` K blocks.  Sizes of the groups are not known
+// here, so the cost of each choice is that of groups of equal size: waves of tiles, each its K blocks at the slower of
+// loads and MMAs and a start and an end that nothing hides.  Weights that only one tile of a group reads come from HBM.
+inline RaggedPlan plan_rows(int groups, int rows, int features, int blocks) {
     const int sms = device_info().num_sms;
-    RaggedPlan plan{features <= 128 ? 1 : 2, 256, 0};
-    const long long f_tiles = (features + 128 * plan.ctas - 1) / (128 * plan.ctas);
     const int used = groups < rows ? groups : rows;
-    for (int tile = 256; tile >= 32; tile /= 2) {
-        plan.tile_cols = tile;
-        // Each group that has rows ends in a partial tile: half a tile on average.
-        const long long expected = f_tiles * (rows / tile + (used + 1) / 2);
-        if (expected * plan.ctas >= sms) break;
+    const double size = double(rows) / used;
+    RaggedPlan best{2, 256, 0};
+    double best_cost = 1e30;
+    for (int ctas = 2; ctas >= 1; --ctas) {
+        const long long f_tiles = (features + 128 * ctas - 1) / (128 * ctas);
+        for (int tile = 256; tile >= 32; tile /= 2) {
+            const int per_group = int((size + tile - 1) / tile);
+            const int width = int((size / per_group + 16 * ctas - 1) / (16 * ctas)) * 16 * ctas;
+            // Uneven groups: the last tile of a group is half empty on average.
+            const double tiles = double(f_tiles) * (groups == 1 ? per_group : used * (size / tile > 1 ? size / tile + 0.5 : 1.0));
+            const double waves = std::ceil(tiles * ctas / sms);
+            const double loads = 16384.0 / (per_group == 1 ? PLAN_HBM_BYTES : PLAN_L2_BYTES) + width / ctas * 128 / PLAN_L2_BYTES;
+            const double cost = waves * (blocks * std::max(loads, PLAN_MMA_CYCLES * width) + 2500.0 + 8.0 * width);
+            if (cost < 0.97 * best_cost) {
+                best_cost = cost;
+                best = RaggedPlan{ctas, tile, 0};
+            }
+        }
     }
     const int most = (rows + 31) / 32 * 32;
-    if (plan.tile_cols > most) plan.tile_cols = most;
-    plan.units = f_tiles * (rows / plan.tile_cols + used);
-    return plan;
+    if (best.tile_cols > most) best.tile_cols = most;
+    best.units = (features + 128ll * best.ctas - 1) / (128 * best.ctas) * (rows / best.tile_cols + used);
+    return best;
+}
+
+// Gradients of `groups` matrices: tiles of features x cols, summed over `rows` rows of all groups.  C leaves while the next
+// tile is summed, at about 30 bytes a cycle and SM.
+inline RaggedPlan plan_weight(int groups, int rows, int features, int cols, int c_bytes) {
+    const int sms = device_info().num_sms;
+    const double blocks = std::ceil(double(rows) / groups / 64);
+    RaggedPlan best{2, 256, 0};
+    double best_cost = 1e30;
+    for (int ctas = 2; ctas >= 1; --ctas) {
+        for (int tile = 256; tile >= 128; tile /= 2) {
+            const long long tiles = (features + 128ll * ctas - 1) / (128 * ctas) * ((cols + tile - 1) / tile) * groups;
+            const double waves = std::ceil(double(tiles) * ctas / sms);
+            const double loads = (16384.0 + tile / ctas * 128) / PLAN_L2_BYTES;
+            const double sums = blocks * std::max(loads, PLAN_MMA_CYCLES * tile), out = 128.0 * tile * c_bytes / 30.0;
+            const double cost = waves * std::max(sums + 500.0, out) + std::min(sums, out) + 2500.0;
+            if (cost < 0.97 * best_cost) {
+                best_cost = cost;
+                best = RaggedPlan{ctas, tile, tiles};
+            }
+        }
+    }
+    return best;
 }
 
 template <class Kernel, class Params>
@@ -55,21 +99,6 @@ void launch_clusters(Kernel kernel, const Params& p, long long clusters, int clu
     cfg.attrs = attr;
     cfg.numAttrs = unsigned(count);
     CB200_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
-}
-
-// A plain grid whose set-up may overlap the kernel before it (it must wait for it itself).
-template <class... Params, class... Args>
-void launch_dependent(void (*kernel)(Params...), dim3 grid, int threads, cudaStream_t stream, const Args&... args) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(unsigned(threads), 1, 1);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = programmatic_launch_enabled() ? 1 : 0;
-    CB200_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...));
 }
 
 }  // namespace cudeep_b200
