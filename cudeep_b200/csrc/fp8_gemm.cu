@@ -5,6 +5,7 @@
 #include "fp8_rows.cuh"
 #include "ragged_plan.h"
 
+#include <algorithm>
 #include <map>
 #include <mutex>
 #include <utility>
@@ -16,6 +17,7 @@ namespace {
 struct FewPlan {
     int step;       // features per tile
     int split;      // CTAs per tile, each with a range of K
+    double cost;    // cycles
 };
 
 // Clusters of `size` CTAs, an SM each, that the device runs at once: fewer than SMs / size, as a cluster lies within one
@@ -47,24 +49,24 @@ int resident_clusters(int size) {
     return known[key] = count < 1 ? 1 : count;
 }
 
-// The cheapest of all steps and splits by what an SM's stream of operands costs, in cycles: 20 bytes of weights a cycle (they
-// come from HBM), 40 of rows (from L2, read by every tile), and fixed costs of a wave and of adding up a split tile.
+// The cheapest of all steps and splits by what an SM's stream of operands costs, in cycles: weights that one tile reads come
+// from HBM, what several tiles read from L2; and fixed costs of a wave and of adding up a split tile.
 FewPlan plan_few(int rows, int features, int k) {
     const int blocks = (k + FP8_BK - 1) / FP8_BK;
-    const int loaded = RowMaps::loaded((rows + 15) / 16 * 16);
-    FewPlan best{128, 1};
-    double best_cost = 1e30;
+    const int row_tiles = (rows + FP8F_MAX_ROWS - 1) / FP8F_MAX_ROWS;
+    const int tile_rows = rows < FP8F_MAX_ROWS ? rows : FP8F_MAX_ROWS;
+    const int loaded = RowMaps::loaded((tile_rows + 15) / 16 * 16);
+    FewPlan best{128, 1, 1e30};
     for (int step = 128; step >= 64; step -= 16) {
         for (int split = 1; split <= 8; split *= 2) {
             if (split > 1 && blocks < 4 * split) break;      // four blocks of K for each CTA at least
-            const long long tiles = (features + step - 1) / step, resident = resident_clusters(split);
+            const long long tiles = (long long)((features + step - 1) / step) * row_tiles, resident = resident_clusters(split);
             const long long waves = (tiles + resident - 1) / resident;
-            const double per_block = step * 128 / 20.0 + loaded * 128 / 40.0;
-            const double cost = waves * ((blocks + split - 1) / split * per_block + 3000.0 + (split > 1 ? 2000.0 + 20.0 * rows : 0.0));
-            if (cost < best_cost * 0.98) {
-                best_cost = cost;
-                best = FewPlan{step, split};
-            }
+            const double loads = step * 128 / (row_tiles == 1 ? PLAN_HBM_BYTES : PLAN_L2_BYTES) + loaded * 128 / PLAN_L2_BYTES;
+            const double sums = 200.0 + 4.0 * tile_rows;      // taking a block's accumulators out
+            const double cost = waves * ((blocks + split - 1) / split * std::max(loads, sums) + 4000.0 +
+                                         (split > 1 ? 2000.0 + 20.0 * tile_rows : 0.0));
+            if (cost < best.cost * 0.98) best = FewPlan{step, split, cost};
         }
     }
     return best;
@@ -75,12 +77,14 @@ void launch_few(Fp8FewParams& p, cudaStream_t stream) {
     const DeviceInfo& dev = device_info();
     CB200_REQUIRE(dev.cc_major == 10, "8-bit products need an sm_100 device");
     p.w_bytes = FORM == RaggedForm::NT ? uint32_t(p.step) * 128u : RAGGED_A_BYTES;
-    p.stage_bytes = RAGGED_A_BYTES + uint32_t(RowMaps::loaded((p.rows + 15) / 16 * 16)) * 128u;
+    p.stage_bytes = RAGGED_A_BYTES + uint32_t(RowMaps::loaded(((p.rows < FP8F_MAX_ROWS ? p.rows : FP8F_MAX_ROWS) + 15) / 16 * 16)) * 128u;
     const int fit = int(FP8F_SMEM_BUDGET / p.stage_bytes);
     p.stages = fit < FP8F_MAX_STAGES ? fit : FP8F_MAX_STAGES;
     p.status = dev.status_word;
     p.wait_limit_ns = 2000000000ull;
-    const long long tiles = (p.features + p.step - 1) / p.step;
+    p.f_tiles = (p.features + p.step - 1) / p.step;
+    p.tile_rows = p.rows < FP8F_MAX_ROWS ? p.rows : FP8F_MAX_ROWS;
+    const long long tiles = (long long)p.f_tiles * ((p.rows + FP8F_MAX_ROWS - 1) / FP8F_MAX_ROWS);
     CB200_TRACE("fp8 %s tcgen05, features on lanes: rows=%d features=%d k=%d stages=%d tiles=%lld step=%d split=%d",
                 FORM == RaggedForm::NT ? "nt" : "nn", p.rows, p.features, p.k, p.stages, tiles, p.step,
                 p.split);
@@ -117,6 +121,15 @@ bool narrow_tiles(int m, int n) {
     return (long long)((m + 255) / 256) * ((n + 127) / 128) <= device_info().num_sms / 2;
 }
 
+// Cycles of the product with the rows on the lanes, as plan_few counts them: a block's 32 KB of operands, or 24 KB of a
+// narrow tile's, and the sums of a finished tile, which nothing hides.
+double cost_by_rows(int m, int n, int k, bool narrow) {
+    const int blocks = (k + FP8_BK - 1) / FP8_BK, pairs = device_info().num_sms / 2;
+    const long long tiles = (long long)((m + 255) / 256) * (narrow ? (n + 127) / 128 : (n + 255) / 256);
+    const double waves = double((tiles + pairs - 1) / pairs);
+    return waves * (blocks * (narrow ? 24576.0 : 32768.0) / PLAN_L2_BYTES + (narrow ? 1500.0 : 3000.0)) + 4000.0;
+}
+
 template <RaggedForm FORM, class OutT>
 void launch_by_rows(Fp8RowsParams& p, bool narrow, cudaStream_t stream) {
     if constexpr (FORM == RaggedForm::NT) {
@@ -150,11 +163,12 @@ void product(const uint8_t* x, const float* x_scales, const uint8_t* w, const fl
         p.features = n;
         p.k = k;
     };
-    if (m > FP8F_MAX_ROWS) {
+    const bool narrow = !nn && narrow_tiles(m, n);
+    const FewPlan few = plan_few(m, n, k);
+    if (m > FP8F_MAX_ROWS && cost_by_rows(m, n, k, narrow) < few.cost) {
         Fp8RowsParams p{};
         fill(p);
         encode_tensor_map_u8(&p.map_x, xr.ptr, 2, x_dims, x_strides, box, TmaSwizzle::B128);
-        const bool narrow = !nn && narrow_tiles(m, n);
         if (narrow) {
             const uint32_t w_box[2] = {128, 64};
             encode_tensor_map_u8(&p.map_w, wr.ptr, 2, w_dims, w_strides, w_box, TmaSwizzle::B128);
@@ -165,11 +179,10 @@ void product(const uint8_t* x, const float* x_scales, const uint8_t* w, const fl
     } else {
         Fp8FewParams p{};
         fill(p);
-        const FewPlan plan = plan_few(m, n, k);
-        p.step = plan.step;
-        p.split = plan.split;
+        p.step = few.step;
+        p.split = few.split;
         if (!nn) {
-            const uint32_t w_box[2] = {128, uint32_t(plan.step)};
+            const uint32_t w_box[2] = {128, uint32_t(few.step)};
             encode_tensor_map_u8(&p.map_w, wr.ptr, 2, w_dims, w_strides, w_box, TmaSwizzle::B128);
         }
         for (uint32_t i = 0; i < 5; ++i) {

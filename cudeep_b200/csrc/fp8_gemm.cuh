@@ -66,11 +66,11 @@ __device__ __forceinline__ void fp8_activation(float (&v)[N], const Fp8Activatio
     }
 }
 
-// ---- few rows -----------------------------------------------------------------------------------------------------------------
+// ---- few tiles ----------------------------------------------------------------------------------------------------------------
 
-// For up to 128 rows the FEATURES lie on the 128 lanes and the rows on the columns: the width of the MMA follows the number
-// of rows, and a CTA streams its 128 features' weights once, which is all such a product costs.  One tile per CTA; where the
-// features make fewer tiles than the device has SMs, a cluster of up to eight CTAs shares a tile, each with a range of K,
+// For few rows (and for few features, whatever the rows) the FEATURES lie on the 128 lanes and up to 128 rows on the columns:
+// the width of the MMA follows the number of rows, and a CTA streams its features' weights once, which is all that a product
+// of a few rows costs.  One tile per CTA; where there are fewer tiles than the device has SMs, a cluster of up to eight CTAs shares a tile, each with a range of K,
 // and adds the parts up through distributed shared memory in rank order.  A tile may take fewer than 128 features (the last
 // lanes then idle), so that the tiles fill the SMs: 16384 features are 128 tiles of 128, but 147 of 112.
 //
@@ -95,7 +95,9 @@ struct Fp8FewParams {
     int act;
     void* c;
     int rows;
+    int tile_rows;           // rows per tile, up to 128
     int features;
+    int f_tiles;
     int k;
     int split;               // CTAs per tile
     int step;                // features per tile, a multiple of 16 up to 128
@@ -128,10 +130,13 @@ __global__ void __launch_bounds__(FP8F_THREADS, 1) fp8_few_kernel(const __grid_c
 
     const int split = p.split;
     const uint32_t rank = split > 1 ? ptx::cluster_ctarank() : 0u;
-    const int feature0 = int(blockIdx.x) / split * p.step;
+    const int tile = int(blockIdx.x) / split;
+    const int feature0 = tile % p.f_tiles * p.step;
+    const int row0 = tile / p.f_tiles * p.tile_rows;
+    const int rows = min(p.tile_rows, p.rows - row0);      // of this tile
     const int f_end = min(p.features, feature0 + p.step);
-    const int umma_n = (p.rows + 15) / 16 * 16;
-    const int buf_cols = (p.rows + 31) / 32 * 32;
+    const int umma_n = (rows + 15) / 16 * 16;
+    const int buf_cols = (rows + 31) / 32 * 32;
     const int buffers = min(FP8F_MAX_BUFFERS, 512 / buf_cols);
     const int all_blocks = (p.k + FP8_BK - 1) / FP8_BK;
     const int share = (all_blocks + split - 1) / split;
@@ -184,7 +189,7 @@ __global__ void __launch_bounds__(FP8F_THREADS, 1) fp8_few_kernel(const __grid_c
                 ptx::mbar_arrive_expect_tx(full, bytes);
                 const int k0 = (kb0 + kb) * FP8_BK;
                 ptx::tma_load_2d(a_smem, &p.map_w, full, A_MN ? feature0 : k0, A_MN ? k0 : feature0);
-                p.x.template load<1>(a_smem + RAGGED_A_BYTES, full, k0, 0, umma_n);
+                p.x.template load<1>(a_smem + RAGGED_A_BYTES, full, k0, row0, umma_n);
                 if (++stage == uint32_t(p.stages)) { stage = 0; phase ^= 1u; }
             }
         }
@@ -220,7 +225,7 @@ __global__ void __launch_bounds__(FP8F_THREADS, 1) fp8_few_kernel(const __grid_c
     } else {
         // ------------------------------------------------------------ sums
         float* mine = &factors[warp - 2][0][0];
-        const float* xs = p.x_scales + (long long)kb0 * p.rows + c_begin;
+        const float* xs = p.x_scales + (long long)kb0 * p.rows + row0 + c_begin;
         // A tile's features may belong to two blocks of scales; lanes behind the last feature take some that exist.
         const float* ws = p.w_scales + (min(feature, p.features - 1) / 128) * p.ws_feature + kb0 * p.ws_k;
         float px[4][2], pw[4];
@@ -229,7 +234,7 @@ __global__ void __launch_bounds__(FP8F_THREADS, 1) fp8_few_kernel(const __grid_c
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int c = int(lane) + 32 * i;
-                x[i] = kb < blocks && c < c_count && c_begin + c < p.rows ? __ldg(xs + (long long)kb * p.rows + c) : 0.0f;
+                x[i] = kb < blocks && c < c_count && c_begin + c < rows ? __ldg(xs + (long long)kb * p.rows + c) : 0.0f;
             }
         };
 #pragma unroll
@@ -278,11 +283,11 @@ __global__ void __launch_bounds__(FP8F_THREADS, 1) fp8_few_kernel(const __grid_c
             }
         }
         const Fp8Activation act(p.act);
-        const int stored = min(c_count, p.rows - c_begin);
+        const int stored = min(c_count, rows - c_begin);
         if (split == 1) {
             if (feature < f_end) {
                 const float bias = p.bias != nullptr ? __ldg(p.bias + feature) : 0.0f;
-                OutT* dst = static_cast<OutT*>(p.c) + (long long)c_begin * p.features + feature;
+                OutT* dst = static_cast<OutT*>(p.c) + (long long)(row0 + c_begin) * p.features + feature;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     if (16 * i < stored) {
@@ -319,12 +324,12 @@ __global__ void __launch_bounds__(FP8F_THREADS, 1) fp8_few_kernel(const __grid_c
 #pragma unroll
             for (int j = 0; j < 4; ++j) bias[j] = p.bias != nullptr && f + j < f_end ? __ldg(p.bias + f + j) : 0.0f;
             const int step = split * FP8F_EPI_WARPS;
-            for (int c = int(rank) + split * int(warp - 2); c < p.rows; c += 2 * step) {
+            for (int c = int(rank) + split * int(warp - 2); c < rows; c += 2 * step) {
                 float v[2][4] = {};
                 for (int s = 0; s < split; ++s) {
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const int cc = c + i * step < p.rows ? c + i * step : c;
+                        const int cc = c + i * step < rows ? c + i * step : c;
                         const float4 q = ptx::ld_cluster_v4(
                             ptx::mapa(smem_base + (uint32_t(cc) * 128u + uint32_t(f_in)) * 4u, uint32_t(s)));
                         v[i][0] += q.x;
@@ -335,11 +340,11 @@ __global__ void __launch_bounds__(FP8F_THREADS, 1) fp8_few_kernel(const __grid_c
                 }
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    if (c + i * step >= p.rows) break;
+                    if (c + i * step >= rows) break;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) v[i][j] += bias[j];
                     fp8_activation(v[i], act);
-                    OutT* dst = static_cast<OutT*>(p.c) + (long long)(c + i * step) * p.features + f;
+                    OutT* dst = static_cast<OutT*>(p.c) + (long long)(row0 + c + i * step) * p.features + f;
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         if (f + j < f_end) dst[j] = round_to<OutT>(v[i][j]);

@@ -77,7 +77,7 @@ void rows_by_weight(bool nn, const void* a, long long lda, const void* w, void* 
                     int n, int k, cudaStream_t stream) {
     const AlignedRows x = rows_of(a, lda, rows, k, stream);
     const int w_cols = nn ? n : k, w_rows = nn ? k : n;
-    const AlignedRows wt = aligned_rows(w, (long long)groups * w_rows, w_cols, 2, stream);
+    const AlignedRows wt = aligned_rows(w, (long long)groups * w_rows, w_cols, 2, stream, offsets, w_rows);
     RaggedParams p{};
     {
         const uint64_t row_bytes = uint64_t(wt.ld) * 2, group_bytes = row_bytes * uint64_t(w_rows);

@@ -22,19 +22,29 @@ namespace {
 constexpr int kThreads = 256;
 
 // dst[r, 0..ld) = src[r, 0..cols) followed by zeros; ld is a multiple of 16 bytes, a thread writes 16 of them.
+// With offsets, rows_group rows belong to each group, and those of groups without rows in their turn (the weights of experts
+// that have no token) are left out.
 template <typename T>
-__global__ void pad_rows_kernel(const T* __restrict__ src, T* __restrict__ dst, long long rows, int cols, int units_row) {
+__global__ void pad_rows_kernel(const T* __restrict__ src, T* __restrict__ dst, long long rows, int cols, int units_row,
+                                const int32_t* __restrict__ offsets, int rows_group) {
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
     constexpr int V = 16 / sizeof(T);
     const long long total = rows * units_row;
     for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
         const long long r = i / units_row;
+        if (offsets != nullptr) {
+            const int g = int(r / rows_group);
+            if (__ldg(offsets + g + 1) <= __ldg(offsets + g)) continue;
+        }
         const int c0 = int(i - r * units_row) * V;
-        const T* s = src + r * cols + c0;
+        const T* s = src + r * cols;
         alignas(16) T v[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = c0 + j < cols ? s[j] : T(0);
+        for (int j = 0; j < V; ++j) v[j] = s[min(c0 + j, cols - 1)];      // no branch: all loads under way together
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (c0 + j >= cols) v[j] = T(0);
         reinterpret_cast<uint4*>(dst)[i] = *reinterpret_cast<const uint4*>(v);
     }
 }
@@ -695,7 +705,8 @@ void quantize_typed(const T* x, long long rows, int cols, int block_rows, uint8_
 
 }  // namespace
 
-AlignedRows aligned_rows(const void* src, long long rows, int cols, int elem_size, cudaStream_t stream) {
+AlignedRows aligned_rows(const void* src, long long rows, int cols, int elem_size, cudaStream_t stream, const int32_t* offsets,
+                         int rows_group) {
     AlignedRows out;
     const int per_unit = 16 / elem_size;
     if (cols % per_unit == 0 && reinterpret_cast<uintptr_t>(src) % 16 == 0) {
@@ -709,10 +720,10 @@ AlignedRows aligned_rows(const void* src, long long rows, int cols, int elem_siz
     out.ptr = out.copy.ptr;
     if (elem_size == 1)
         launch_dependent(pad_rows_kernel<uint8_t>, dim3(pass_grid(rows * units)), kThreads, stream,
-            static_cast<const uint8_t*>(src), static_cast<uint8_t*>(out.copy.ptr), rows, cols, units);
+            static_cast<const uint8_t*>(src), static_cast<uint8_t*>(out.copy.ptr), rows, cols, units, offsets, rows_group);
     else
         launch_dependent(pad_rows_kernel<uint16_t>, dim3(pass_grid(rows * units)), kThreads, stream,
-            static_cast<const uint16_t*>(src), static_cast<uint16_t*>(out.copy.ptr), rows, cols, units);
+            static_cast<const uint16_t*>(src), static_cast<uint16_t*>(out.copy.ptr), rows, cols, units, offsets, rows_group);
     CB200_CHECK_LAUNCH();
     return out;
 }

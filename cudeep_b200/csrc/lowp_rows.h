@@ -17,8 +17,10 @@ struct AlignedRows {
     long long ld = 0;      // elements between rows
     Scratch copy;          // holds ptr where the caller's matrix had to be copied
 };
-// The caller's matrix itself where it qualifies, else a copy with zero-padded rows.
-AlignedRows aligned_rows(const void* src, long long rows, int cols, int elem_size, cudaStream_t stream);
+// The caller's matrix itself where it qualifies, else a copy with zero-padded rows.  With `offsets` (device), rows_group rows belong
+// to each of their groups, and groups without rows need not be copied.
+AlignedRows aligned_rows(const void* src, long long rows, int cols, int elem_size, cudaStream_t stream,
+                         const int32_t* offsets = nullptr, int rows_group = 1);
 
 // q = e4m3(x / s), s a power of two for each block of 128 columns and block_rows (1 or 128) rows.
 void quantize_fp8(const void* x, int x_type, long long rows, int cols, int block_rows, uint8_t* q, float* scales,

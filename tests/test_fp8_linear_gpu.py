@@ -56,7 +56,7 @@ def check(torch, got, want, bound):
 
 
 SHAPES = [(1, 64, 64), (3, 128, 128), (16, 256, 384), (33, 130, 300), (100, 77, 1001), (129, 520, 128), (257, 256, 256),
-          (300, 1000, 520), (512, 384, 2048), (16, 256, 4096), (7, 4200, 4200), (128, 300, 2000)]
+          (300, 1000, 520), (512, 384, 2048), (16, 256, 4096), (7, 4200, 4200), (128, 300, 2000), (809, 104, 3000), (1119, 117, 536)]
 
 
 @pytest.mark.parametrize("out", ["f32", "f16", "bf16"])
