@@ -67,6 +67,7 @@ PROTOTYPES = {
     "cudeep_b200_matmul_bf16": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
     "cudeep_b200_matmul_f16_tuned": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                                              ctypes.c_uint32, ctypes.c_uint32, c_void_p]),
+    "cudeep_b200_cast": (c_int, [c_void_p, c_int, c_void_p, c_int, ctypes.c_longlong, _stream]),
     "cudeep_b200_quantize_fp8": (c_int, [c_void_p, c_int, ctypes.c_longlong, c_int, c_int, c_void_p, c_void_p,
                                          _stream]),
     "cudeep_b200_dequantize_fp8": (c_int, [c_void_p, c_void_p, ctypes.c_longlong, c_int, c_int, c_void_p, c_int,

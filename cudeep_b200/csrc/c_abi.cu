@@ -204,6 +204,14 @@ int cudeep_b200_matmul_f16_tuned(const void* A, const void* B, float* C, int M, 
     });
 }
 
+int cudeep_b200_cast(const void* src, int src_type, void* dst, int dst_type, long long count,
+                     cudeep_b200_stream_t stream) {
+    return guarded([&] {
+        cudeep::kernels::launch_cast(src, as_element_type(src_type), dst, as_element_type(dst_type), count,
+                                     as_stream(stream));
+    });
+}
+
 int cudeep_b200_quantize_fp8(const void* x, int x_type, long long rows, int cols, int block_rows, void* q,
                              float* scales, cudeep_b200_stream_t stream) {
     return guarded([&] {

@@ -106,6 +106,7 @@ void rows_by_weight(bool nn, const void* a, long long lda, const void* w, void* 
     p.offsets = offsets;
     p.groups = groups;
     p.rows = rows;
+    p.share = rows;
     p.features = n;
     p.k = k;
     p.chunk_rows = RAGGED_BK;
@@ -148,18 +149,43 @@ void grouped_tn(const void* a, long long lda, const void* b, long long ldb, void
                 const int32_t* offsets, int groups, int rows, int m, int n, const float* col_scale, cudaStream_t stream) {
     const AlignedRows y = rows_of(a, lda, rows, m, stream);
     const AlignedRows x = rows_of(b, ldb, rows, n, stream);
+    RaggedPlan plan = plan_weight(groups, rows, m, n, elem_bytes(c_type));
+    // One gradient of few tiles and many rows: `parts` ranges of the rows as groups of their own, summed in FP32 and added up
+    // in order by a pass of their own (4112 rows, 701 x 1740: TNSPLIT).
+    int parts = 1;
+    if (offsets == nullptr) {
+        for (int p = 2; p <= 16 && rows >= 512 * p; p *= 2) {
+            RaggedPlan split = plan_weight(p, rows, m, n, 4);
+            split.cost += 5000.0 + 8.0 * p * m * n / (device_info().num_sms * PLAN_HBM_BYTES);
+            if (split.cost < 0.95 * plan.cost) {
+                plan = split;
+                parts = p;
+            }
+        }
+    }
+    Scratch sums;
+    void* out = c;
+    int out_type = c_type;
+    long long ldc = n;
+    if (parts > 1) {
+        ldc = (n + 3) / 4 * 4;
+        sums = Scratch(size_t(parts) * m * ldc * sizeof(float), stream);
+        out = sums.ptr;
+        out_type = TYPE_F32;
+    }
     RaggedParams p{};
-    const RaggedPlan plan = plan_weight(groups, rows, m, n, elem_bytes(c_type));
+    p.groups = parts > 1 ? parts : groups;
+    p.share = parts > 1 ? ((rows + parts - 1) / parts + RAGGED_BK - 1) / RAGGED_BK * RAGGED_BK : rows;
     p.a_chunked = encode_columns(&p.map_a, y, rows, m, 2);
     p.b_chunked = encode_columns(&p.map_b, x, rows, n, plan.tile_cols / plan.ctas / 64);
-    const uint32_t c_bytes = uint32_t(elem_bytes(c_type));
-    p.tma_store = (size_t(n) * c_bytes) % 16 == 0 && reinterpret_cast<uintptr_t>(c) % 16 == 0;
+    const uint32_t c_bytes = uint32_t(elem_bytes(out_type));
+    p.tma_store = (size_t(ldc) * c_bytes) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
     if (p.tma_store) {
-        const uint64_t dims[3] = {uint64_t(n), uint64_t(m), uint64_t(groups)};
-        const uint64_t strides[2] = {uint64_t(n) * c_bytes, uint64_t(n) * c_bytes * uint64_t(m)};
+        const uint64_t dims[3] = {uint64_t(n), uint64_t(m), uint64_t(p.groups)};
+        const uint64_t strides[2] = {uint64_t(ldc) * c_bytes, uint64_t(ldc) * c_bytes * uint64_t(m)};
         const uint32_t box[3] = {128 / c_bytes, 32, 1};
-        if (c_type == TYPE_F32) encode_tensor_map(&p.map_c, static_cast<const float*>(c), 3, dims, strides, box, TmaSwizzle::B128);
-        else encode_tensor_map_f16(&p.map_c, c, 3, dims, strides, box, TmaSwizzle::B128);
+        if (out_type == TYPE_F32) encode_tensor_map(&p.map_c, static_cast<const float*>(out), 3, dims, strides, box, TmaSwizzle::B128);
+        else encode_tensor_map_f16(&p.map_c, out, 3, dims, strides, box, TmaSwizzle::B128);
     }
     Scratch maps;
     if (offsets != nullptr) {
@@ -168,9 +194,9 @@ void grouped_tn(const void* a, long long lda, const void* b, long long ldb, void
         launch_dependent(group_maps_kernel, dim3(unsigned(groups)), 32, stream, p.map_a, p.map_b, offsets, rows,
                          static_cast<CUtensorMap*>(maps.ptr));
     }
-    p.c = c;
+    p.c = out;
+    p.ldc = ldc;
     p.offsets = offsets;
-    p.groups = groups;
     p.rows = rows;
     p.features = m;
     p.cols = n;
@@ -178,14 +204,15 @@ void grouped_tn(const void* a, long long lda, const void* b, long long ldb, void
     // The tensor core's accumulation loses about 2.4e-9 relative per row summed (it truncates), so a gradient in
     // single precision is summed over 2048 rows at a time, added up with rounding in the epilogue; a 16-bit one
     // (2e-3 from its own rounding) in one go.
-    p.chunk_rows = c_type == TYPE_F32 ? 2048 : (rows + RAGGED_BK - 1) / RAGGED_BK * RAGGED_BK;
+    p.chunk_rows = out_type == TYPE_F32 ? 2048 : (rows + RAGGED_BK - 1) / RAGGED_BK * RAGGED_BK;
     if (type == TYPE_BF16) {
-        if (plan.ctas == 2) launch_weight<2, true>(p, plan, c_type, stream);
-        else launch_weight<1, true>(p, plan, c_type, stream);
+        if (plan.ctas == 2) launch_weight<2, true>(p, plan, out_type, stream);
+        else launch_weight<1, true>(p, plan, out_type, stream);
     } else {
-        if (plan.ctas == 2) launch_weight<2, false>(p, plan, c_type, stream);
-        else launch_weight<1, false>(p, plan, c_type, stream);
+        if (plan.ctas == 2) launch_weight<2, false>(p, plan, out_type, stream);
+        else launch_weight<1, false>(p, plan, out_type, stream);
     }
+    if (parts > 1) add_parts(static_cast<const float*>(out), parts, m, n, ldc, c, c_type, stream);
 }
 
 }  // namespace cudeep_b200

@@ -50,6 +50,16 @@ int checked_epilogue(GemmEpilogue epilogue) {
 
 }  // namespace
 
+void launch_cast(const void* src, ElementType src_type, void* dst, ElementType dst_type, long long count, cudaStream_t stream) {
+    const int st = checked_type(src_type), dt = checked_type(dst_type);
+    CB200_REQUIRE(src != nullptr && dst != nullptr, "cast: null pointer");
+    CB200_REQUIRE(count >= 0, "cast: count must not be negative");
+    check_element_address(src, cudeep_b200::elem_bytes(st), "src");
+    check_element_address(dst, cudeep_b200::elem_bytes(dt), "dst");
+    if (count == 0) return;
+    cudeep_b200::cast(src, st, dst, dt, count, stream);
+}
+
 void launch_quantize_fp8(const void* x, ElementType type, long long rows, int cols, Fp8Block block, void* q, float* scales,
                          cudaStream_t stream) {
     const int t = checked_type(type), b = checked_block(block);

@@ -21,31 +21,68 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// dst[r, 0..ld) = src[r, 0..cols) followed by zeros; ld is a multiple of 16 bytes, a thread writes 16 of them.
-// With offsets, rows_group rows belong to each group, and those of groups without rows in their turn (the weights of experts
-// that have no token) are left out.
-template <typename T>
-__global__ void pad_rows_kernel(const T* __restrict__ src, T* __restrict__ dst, long long rows, int cols, int units_row,
-                                const int32_t* __restrict__ offsets, int rows_group) {
+// dst[r, 0..ld) = src[r, 0..row_bytes) followed by zeros, in bytes; ld is a multiple of 16 and dst aligned to it.  A warp takes 512
+// bytes of a row, a lane every 32nd word of the result, shifted together from the two aligned words of the source that hold it (loads
+// byte by byte ran at 2 TB/s, 16 bytes a lane at a quarter of the requests' width).  Words that reach over the matrix's
+// ends are put together from bytes.  With offsets, rows_group rows belong to each group, and those of groups without
+// rows in their turn (the weights of experts that have no token) are left out.
+__global__ void __launch_bounds__(kThreads) pad_rows_kernel(const uint8_t* __restrict__ src, uint8_t* __restrict__ dst,
+                                                            long long rows, int row_bytes, int ld,
+                                                            const int32_t* __restrict__ offsets, int rows_group) {
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
-    constexpr int V = 16 / sizeof(T);
-    const long long total = rows * units_row;
-    for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
-        const long long r = i / units_row;
-        if (offsets != nullptr) {
-            const int g = int(r / rows_group);
-            if (__ldg(offsets + g + 1) <= __ldg(offsets + g)) continue;
+    const int lane = threadIdx.x & 31;
+    const long long r = blockIdx.x * (long long)(kThreads / 32) + (threadIdx.x >> 5);
+    if (r >= rows) return;
+    if (offsets != nullptr) {
+        const int g = int(r / rows_group);
+        if (__ldg(offsets + g + 1) <= __ldg(offsets + g)) return;
+    }
+    const uint8_t* row = src + r * row_bytes;
+    const uint8_t* end = src + rows * row_bytes;
+    const int shift = int(reinterpret_cast<uintptr_t>(row) & 3u);
+    const uint32_t* words = reinterpret_cast<const uint32_t*>(row - shift);
+    uint32_t* out = reinterpret_cast<uint32_t*>(dst + r * ld);
+    const int count = ld / 4;
+    // Words that hold bytes outside the matrix (its first, its last) are put together from bytes.
+    const int last = (row_bytes + shift - 1) / 4;      // word of the row's last byte
+    const int from = row - shift >= src ? 0 : 1;
+    const int to = row - shift + 4 * last + 4 <= end ? last : last - 1;
+    auto word_of_bytes = [&](int w) {
+        uint32_t v = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int at = 4 * w + i - shift;
+            if (at >= 0 && at < row_bytes) v |= uint32_t(row[at]) << (8 * i);
         }
-        const int c0 = int(i - r * units_row) * V;
-        const T* s = src + r * cols;
-        alignas(16) T v[V];
+        return v;
+    };
+    const int w0 = int(blockIdx.y) * 128;
+    uint32_t lo[4], hi[4];
+    if (from <= to) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = s[min(c0 + j, cols - 1)];      // no branch: all loads under way together
+        for (int j = 0; j < 4; ++j) {
+            const int w = w0 + lane + 32 * j;
+            lo[j] = __ldg(words + max(from, min(w, to)));
+            hi[j] = __ldg(words + max(from, min(w + 1, to)));
+        }
+    }
+    if (from != 0 || to != last) {
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (c0 + j >= cols) v[j] = T(0);
-        reinterpret_cast<uint4*>(dst)[i] = *reinterpret_cast<const uint4*>(v);
+        for (int j = 0; j < 4; ++j) {
+            const int w = w0 + lane + 32 * j;
+            if (w < from || w > to) lo[j] = word_of_bytes(w);
+            if (w + 1 < from || w + 1 > to) hi[j] = word_of_bytes(w + 1);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int w = w0 + lane + 32 * j;
+        if (w >= count) break;
+        const int left = row_bytes - 4 * w;      // bytes of the row from this word on
+        uint32_t v = __funnelshift_r(lo[j], hi[j], 8 * shift);
+        if (left < 4) v = left <= 0 ? 0u : v & (0xffffffffu >> (8 * (4 - left)));
+        out[w] = v;
     }
 }
 
@@ -677,6 +714,40 @@ void act_backward_typed(const T* dy, const uint8_t* z8, const float* z_scales, i
     }
 }
 
+template <typename T>
+__global__ void __launch_bounds__(kThreads) add_parts_kernel(const float* __restrict__ part, int parts, int m, int n, long long ld,
+                                                             T* __restrict__ out) {
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
+    const long long units = ld / 4, total = m * units;
+    for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
+        float4 sum = __ldg(reinterpret_cast<const float4*>(part) + i);
+        for (int p = 1; p < parts; ++p) {
+            const float4 v = __ldg(reinterpret_cast<const float4*>(part) + p * total + i);
+            sum.x += v.x;
+            sum.y += v.y;
+            sum.z += v.z;
+            sum.w += v.w;
+        }
+        const long long r = i / units;
+        const int c = int(i - r * units) * 4;
+        T* dst = out + r * n + c;
+        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (c + j < n) dst[j] = from_float<T>(v[j]);
+    }
+}
+
+template <typename S, typename D>
+__global__ void __launch_bounds__(kThreads) cast_kernel(const S* __restrict__ src, D* __restrict__ dst, long long count) {
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
+#pragma unroll 4
+    for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < count; i += (long long)gridDim.x * blockDim.x)
+        dst[i] = from_float<D>(to_float(src[i]));
+}
+
 unsigned pass_grid(long long items) {
     const long long most = 16ll * device_info().num_sms;
     const long long want = (items + kThreads - 1) / kThreads;
@@ -718,12 +789,11 @@ AlignedRows aligned_rows(const void* src, long long rows, int cols, int elem_siz
     out.ld = (long long)units * per_unit;
     out.copy = Scratch(size_t(rows) * units * 16, stream);
     out.ptr = out.copy.ptr;
-    if (elem_size == 1)
-        launch_dependent(pad_rows_kernel<uint8_t>, dim3(pass_grid(rows * units)), kThreads, stream,
-            static_cast<const uint8_t*>(src), static_cast<uint8_t*>(out.copy.ptr), rows, cols, units, offsets, rows_group);
-    else
-        launch_dependent(pad_rows_kernel<uint16_t>, dim3(pass_grid(rows * units)), kThreads, stream,
-            static_cast<const uint16_t*>(src), static_cast<uint16_t*>(out.copy.ptr), rows, cols, units, offsets, rows_group);
+    CB200_REQUIRE((rows + 7) / 8 <= 2147483647ll && (units + 31) / 32 <= 65535, "matrix too large");      // the grid
+    const dim3 grid(unsigned((rows + kThreads / 32 - 1) / (kThreads / 32)), unsigned((units + 31) / 32));
+    launch_dependent(pad_rows_kernel, grid, kThreads, stream,
+                     static_cast<const uint8_t*>(src), static_cast<uint8_t*>(out.copy.ptr), rows, cols * elem_size,
+                     units * 16, offsets, rows_group);
     CB200_CHECK_LAUNCH();
     return out;
 }
@@ -779,6 +849,31 @@ void dequantize_rows(const uint8_t* q, const float* scales, const float* top, in
         else launch_dependent(dequantize_rows_kernel<__nv_bfloat16, false>, dim3(grid), kThreads, stream, q, scales, top, rows, cols, out, ld_y);
     }
     CB200_CHECK_LAUNCH();
+}
+
+void add_parts(const float* part, int parts, int m, int n, long long ld, void* out, int type, cudaStream_t stream) {
+    const unsigned grid = pass_grid(m * (ld / 4));
+    if (type == TYPE_F32)
+        launch_dependent(add_parts_kernel<float>, dim3(grid), kThreads, stream, part, parts, m, n, ld, static_cast<float*>(out));
+    else if (type == TYPE_F16)
+        launch_dependent(add_parts_kernel<__half>, dim3(grid), kThreads, stream, part, parts, m, n, ld, static_cast<__half*>(out));
+    else
+        launch_dependent(add_parts_kernel<__nv_bfloat16>, dim3(grid), kThreads, stream, part, parts, m, n, ld,
+                         static_cast<__nv_bfloat16*>(out));
+}
+
+void cast(const void* src, int src_type, void* dst, int dst_type, long long count, cudaStream_t stream) {
+    const unsigned grid = pass_grid(count);
+    auto from = [&](auto* s) {
+        using S = std::remove_pointer_t<decltype(s)>;
+        const S* in = static_cast<const S*>(src);
+        if (dst_type == TYPE_F32) launch_dependent(cast_kernel<S, float>, dim3(grid), kThreads, stream, in, static_cast<float*>(dst), count);
+        else if (dst_type == TYPE_F16) launch_dependent(cast_kernel<S, __half>, dim3(grid), kThreads, stream, in, static_cast<__half*>(dst), count);
+        else launch_dependent(cast_kernel<S, __nv_bfloat16>, dim3(grid), kThreads, stream, in, static_cast<__nv_bfloat16*>(dst), count);
+    };
+    if (src_type == TYPE_F32) from(static_cast<float*>(nullptr));
+    else if (src_type == TYPE_F16) from(static_cast<__half*>(nullptr));
+    else from(static_cast<__nv_bfloat16*>(nullptr));
 }
 
 }  // namespace cudeep_b200

@@ -22,6 +22,9 @@ struct AlignedRows {
 AlignedRows aligned_rows(const void* src, long long rows, int cols, int elem_size, cudaStream_t stream,
                          const int32_t* offsets = nullptr, int rows_group = 1);
 
+// dst = src, rounded to dst_type.
+void cast(const void* src, int src_type, void* dst, int dst_type, long long count, cudaStream_t stream);
+
 // q = e4m3(x / s), s a power of two for each block of 128 columns and block_rows (1 or 128) rows.
 void quantize_fp8(const void* x, int x_type, long long rows, int cols, int block_rows, uint8_t* q, float* scales,
                   cudaStream_t stream);
@@ -39,5 +42,8 @@ void activation_backward_fp8(const void* dy, int type, const uint8_t* z8, const 
 void block_tops(const float* scales, int rows, int cols, float* top, cudaStream_t stream);
 void dequantize_rows(const uint8_t* q, const float* scales, const float* top, int rows, int cols, void* y, long long ld_y,
                      int y_type, cudaStream_t stream);
+
+// out[m, n] = sum over `parts` of part[parts][m][ld], in order, rounded to `type`.  ld is a multiple of 4.
+void add_parts(const float* part, int parts, int m, int n, long long ld, void* out, int type, cudaStream_t stream);
 
 }  // namespace cudeep_b200

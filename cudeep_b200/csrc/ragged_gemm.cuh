@@ -34,7 +34,7 @@ enum class RaggedForm { NT, NN, TN };
 constexpr int RAGGED_MAX_GROUPS = 1024;
 constexpr int RAGGED_BK = 64;                        // 16-bit elements per K block = one 128-byte swizzle row
 // Epilogue warps: with four, a gradient tile of 512 summed rows took longer to leave than to compute.
-__host__ __device__ constexpr int ragged_epilogue_warps(RaggedForm form) { return form == RaggedForm::TN ? 8 : 4; }
+__host__ __device__ constexpr int ragged_epilogue_warps(RaggedForm) { return 8; }
 __host__ __device__ constexpr int ragged_threads(RaggedForm form) { return 64 + 32 * ragged_epilogue_warps(form); }
 constexpr uint32_t RAGGED_STAGING_BYTES = 8 * 2 * 4096;   // TN: two blocks of 32 rows x 128 bytes per epilogue warp
 constexpr uint32_t RAGGED_A_BYTES = 128 * 128;       // one CTA's features of a K block
@@ -73,7 +73,9 @@ struct RaggedParams {
     int tma_store;           // ... and whether it is so
     const CUtensorMap* group_maps;      // TN: map_a and map_b of each group; nullptr: one group of all rows
     void* c;
-    const int32_t* offsets;  // [groups + 1], or nullptr: one group of all rows
+    long long ldc;           // TN: elements between rows of C
+    const int32_t* offsets;  // [groups + 1], or nullptr: `share` rows each, a multiple of 64 unless there is one group
+    int share;
     int groups;
     int rows;                // rows of X (and of Y)
     int features;            // F
@@ -186,9 +188,10 @@ __device__ __forceinline__ void write_block(uint32_t block, uint32_t lane, T* ds
     __syncwarp();
 }
 
-// One warp: the row range of each group, brought into [0, rows], and the number of tiles before it.  col_tiles >= 0:
+// One warp: the row range of each group, brought into [0, rows] (without offsets: `share` rows each), and the number of tiles
+// before it.  col_tiles >= 0:
 // column tiles of every group (TN); otherwise -col_tiles is the number of a group's rows that a tile takes.
-__device__ __forceinline__ void group_tables(const int32_t* offsets, int groups, int rows, int f_tiles, int col_tiles,
+__device__ __forceinline__ void group_tables(const int32_t* offsets, int groups, int rows, int share, int f_tiles, int col_tiles,
                                              int* group_rows, int* group_start, uint32_t* status) {
     const int lane = int(threadIdx.x & 31);
     int carry = 0;
@@ -197,7 +200,7 @@ __device__ __forceinline__ void group_tables(const int32_t* offsets, int groups,
         const int g = base + lane;
         int tiles = 0;
         if (g < groups) {
-            int lo = 0, hi = rows;
+            int lo = min(rows, g * share), hi = min(rows, (g + 1) * share);
             if (offsets != nullptr) {
                 lo = __ldg(offsets + g);
                 hi = __ldg(offsets + g + 1);
@@ -298,7 +301,7 @@ __global__ void __launch_bounds__(ragged_threads(FORM), 1) ragged_gemm_kernel(co
     const int f_tiles = (p.features + 128 * CTAS - 1) / (128 * CTAS);
     const int c_tiles_tn = FORM == RaggedForm::TN ? (p.cols + p.tile_cols - 1) / p.tile_cols : 0;
     if (warp == 0)
-        group_tables(p.offsets, p.groups, p.rows, f_tiles, FORM == RaggedForm::TN ? c_tiles_tn : -p.tile_cols, group_rows,
+        group_tables(p.offsets, p.groups, p.rows, p.share, f_tiles, FORM == RaggedForm::TN ? c_tiles_tn : -p.tile_cols, group_rows,
                      group_start, p.status);
     ptx::tc_fence_before();
     __syncthreads();
@@ -513,8 +516,8 @@ __global__ void __launch_bounds__(ragged_threads(FORM), 1) ragged_gemm_kernel(co
                             } else {
                                 __syncwarp();
                                 OutT* dst = static_cast<OutT*>(p.c) +
-                                            ((long long)t.group * p.features + feature_w) * p.cols + t.col0 + c0;
-                                write_block<OutT>(block, lane, dst, p.cols, min(32, p.features - feature_w), c_end - c0, add);
+                                            ((long long)t.group * p.features + feature_w) * p.ldc + t.col0 + c0;
+                                write_block<OutT>(block, lane, dst, p.ldc, min(32, p.features - feature_w), c_end - c0, add);
                             }
                         }
                     }
@@ -538,14 +541,16 @@ __global__ void __launch_bounds__(ragged_threads(FORM), 1) ragged_gemm_kernel(co
                 ptx::tc_fence_after();
                 const uint32_t t_row = tmem_base + acc * 256u + ((quarter * 32u) << 16);
                 OutT* dst = static_cast<OutT*>(p.c) + (long long)t.col0 * p.features + feature;
-                for (int c = 0; c < t.col_count; c += 32) {
+                const int c_half = (t.umma_n / 2 + 31) / 32 * 32;      // warps 6..9 take the second half of the columns
+                const int c_begin = (int(warp - 2) >> 2) * c_half, c_end = min(t.col_count, c_begin + c_half);
+                for (int c = c_begin; c < c_end; c += 32) {
                     uint32_t r[32];
                     ptx::tmem_ld_32x32(t_row + c, r);
                     ptx::tmem_ld_wait();
                     if (feature < p.features) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j)
-                            if (c + j < t.col_count)
+                            if (c + j < c_end)
                                 dst[(long long)(c + j) * p.features] = round_to<OutT>(__uint_as_float(r[j]));
                     }
                 }

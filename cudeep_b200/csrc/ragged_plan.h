@@ -13,6 +13,7 @@ struct RaggedPlan {
     int ctas;             // CTAs per tile
     int tile_cols;        // columns of a tile at most
     long long units;      // most tiles there can be, whatever the group sizes
+    double cost;          // estimate in cycles
 };
 
 // An SM takes in about 41 bytes of operands a cycle from L2, 20 from HBM (measured: 16 KB boxes, all SMs loading), and a K
@@ -26,8 +27,7 @@ inline RaggedPlan plan_rows(int groups, int rows, int features, int blocks) {
     const int sms = device_info().num_sms;
     const int used = groups < rows ? groups : rows;
     const double size = double(rows) / used;
-    RaggedPlan best{2, 256, 0};
-    double best_cost = 1e30;
+    RaggedPlan best{2, 256, 0, 1e30};
     for (int ctas = 2; ctas >= 1; --ctas) {
         const long long f_tiles = (features + 128 * ctas - 1) / (128 * ctas);
         for (int tile = 256; tile >= 32; tile /= 2) {
@@ -38,10 +38,7 @@ inline RaggedPlan plan_rows(int groups, int rows, int features, int blocks) {
             const double waves = std::ceil(tiles * ctas / sms);
             const double loads = 16384.0 / (per_group == 1 ? PLAN_HBM_BYTES : PLAN_L2_BYTES) + width / ctas * 128 / PLAN_L2_BYTES;
             const double cost = waves * (blocks * std::max(loads, PLAN_MMA_CYCLES * width) + 2500.0 + 8.0 * width);
-            if (cost < 0.97 * best_cost) {
-                best_cost = cost;
-                best = RaggedPlan{ctas, tile, 0};
-            }
+            if (cost < 0.97 * best.cost) best = RaggedPlan{ctas, tile, 0, cost};
         }
     }
     const int most = (rows + 31) / 32 * 32;
@@ -55,8 +52,7 @@ inline RaggedPlan plan_rows(int groups, int rows, int features, int blocks) {
 inline RaggedPlan plan_weight(int groups, int rows, int features, int cols, int c_bytes) {
     const int sms = device_info().num_sms;
     const double blocks = std::ceil(double(rows) / groups / 64);
-    RaggedPlan best{2, 256, 0};
-    double best_cost = 1e30;
+    RaggedPlan best{2, 256, 0, 1e30};
     for (int ctas = 2; ctas >= 1; --ctas) {
         for (int tile = 256; tile >= 128; tile /= 2) {
             const long long tiles = (features + 128ll * ctas - 1) / (128 * ctas) * ((cols + tile - 1) / tile) * groups;
@@ -64,10 +60,7 @@ inline RaggedPlan plan_weight(int groups, int rows, int features, int cols, int 
             const double loads = (16384.0 + tile / ctas * 128) / PLAN_L2_BYTES;
             const double sums = blocks * std::max(loads, PLAN_MMA_CYCLES * tile), out = 128.0 * tile * c_bytes / 30.0;
             const double cost = waves * std::max(sums + 500.0, out) + std::min(sums, out) + 2500.0;
-            if (cost < 0.97 * best_cost) {
-                best_cost = cost;
-                best = RaggedPlan{ctas, tile, tiles};
-            }
+            if (cost < 0.97 * best.cost) best = RaggedPlan{ctas, tile, tiles, cost};
         }
     }
     return best;

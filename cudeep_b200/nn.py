@@ -9,6 +9,9 @@ all on the forward path:
   * Sequential.forward folds an activation module that directly follows a Linear or Conv2d into
     that layer's epilogue (the unfused result is the same function applied as a separate pass).
 Training (autograd, optimisers) is outside this library's scope.
+
+Additions: LinearFp8, the same layer on 8-bit products, and GroupedLinear, one weight for each of several row groups
+(experts); both give the gradients of their products.
 """
 from __future__ import annotations
 
@@ -16,6 +19,7 @@ from typing import Optional
 
 import numpy as np
 
+from . import lowp
 from .tensor import DType, Tensor, conv2d, linear
 
 
@@ -110,6 +114,82 @@ class Linear(Module):
 
     def forward(self, x, activation=None):
         return linear(x, self._parameters["weight"], self._parameters.get("bias"), activation)
+
+
+class _Prepared:
+    """What a layer makes of its weight before it is used, kept until the parameter is replaced (load_state_dict).  A weight
+    changed in place is not noticed: call the layer's refresh()."""
+
+    def __init__(self):
+        self.of = self.value = None
+
+    def get(self, parameter, make):
+        if self.of is not parameter:
+            self.value, self.of = make(parameter), parameter
+        return self.value
+
+
+class LinearFp8(Linear):
+    """Linear on 8-bit products: x is quantised in blocks of 1 x 128 at each call, the weight once in blocks of 128 x 128.
+    x is float32 or bfloat16 [rows, in_features]; the result has its type.  Parameters as Linear's, in float32."""
+
+    def __init__(self, in_features, out_features, bias=True):
+        super().__init__(in_features, out_features, bias)
+        self._weight8 = _Prepared()
+
+    def refresh(self) -> None:
+        self._weight8 = _Prepared()
+
+    def weight_fp8(self) -> lowp.Fp8Tensor:
+        return self._weight8.get(self._parameters["weight"], lambda w: lowp.quantize_fp8(w, tiles=True))
+
+    def forward(self, x, activation=None):
+        return lowp.linear_fp8(lowp.quantize_fp8(x), self.weight_fp8(), self._parameters.get("bias"), activation,
+                               x.dtype())
+
+    def forward_saved(self, x, activation=None):
+        """(y, saved) for `backward`: y as forward's, saved holds x and, with an activation, the pre-activation in 8 bits.
+        Without an activation nothing but the codes that the product reads anyway is kept."""
+        x8 = lowp.quantize_fp8(x)
+        bias = self._parameters.get("bias")
+        z = lowp.linear_fp8(x8, self.weight_fp8(), bias, None, DType.float32 if activation else x.dtype())
+        if activation is None:
+            return z, (x8, None, None)
+        y = getattr(z, activation)()
+        return y.to(x.dtype()), (x8, lowp.quantize_fp8(z), activation)
+
+    def backward(self, grad, saved):
+        """(dx, dweight, dbias) in float32 for bfloat16 `grad` of y and what forward_saved kept; the product for dx takes the
+        weight in bfloat16."""
+        x8, z8, activation = saved
+        dx, dw, db = lowp.linear_backward_saved(grad, x8, self._parameters["weight"].to(DType.bfloat16), z8, activation,
+                                                DType.float32)
+        return dx.to(DType.float32), dw, (db if "bias" in self._parameters else None)
+
+
+class GroupedLinear(Module):
+    """y[r] = x[r] W[g]^T for the rows of each group g: the experts' products of a mixture of experts.  x is bfloat16
+    [rows, in_features] with the rows of a group next to each other, offsets an int32 Tensor of groups + 1 row numbers.  The
+    parameter is float32 [groups, out_features, in_features]; the products take it in bfloat16."""
+
+    def __init__(self, groups, in_features, out_features):
+        super().__init__()
+        self.groups, self.in_features, self.out_features = groups, in_features, out_features
+        self.register_parameter("weight", Tensor.randn([groups, out_features, in_features]))
+        self._weight16 = _Prepared()
+
+    def refresh(self) -> None:
+        self._weight16 = _Prepared()
+
+    def weight_bf16(self) -> Tensor:
+        return self._weight16.get(self._parameters["weight"], lambda w: w.to(DType.bfloat16))
+
+    def forward(self, x, offsets):
+        return lowp.grouped_linear(x, self.weight_bf16(), offsets)
+
+    def backward(self, grad, x, offsets):
+        """(dx in bfloat16, dweight in float32)."""
+        return lowp.grouped_linear_backward(grad, x, self.weight_bf16(), offsets)
 
 
 class Conv2d(Module):

@@ -22,14 +22,30 @@ from . import _lib
 
 
 class DType(enum.Enum):
-    """Element types (include/cudeep/common.cuh:10-14)."""
+    """Element types: the reference's (include/cudeep/common.cuh:10-14), then those of the low-precision products."""
     float16 = 0
     float32 = 1
     float64 = 2
+    bfloat16 = 3
+    float8_e4m3 = 4
+    int32 = 5
 
 
 _NP = {DType.float32: np.float32, DType.float64: np.float64}
+# Types that only the functions of lowp.py and the copies to and from the host take.
+_LOW = {DType.bfloat16: 2, DType.float8_e4m3: 1, DType.int32: 4}
+# CUDEEP_B200_TYPE_* codes of the C ABI.
+_TYPE_CODE = {DType.float32: 0, DType.bfloat16: 2}
 EPILOGUE = {None: 0, "none": 0, "relu": 1, "gelu": 2, "silu": 3, "sigmoid": 4}
+
+
+def _e4m3_values() -> np.ndarray:
+    """The value of each of the 256 codes of e4m3."""
+    code = np.arange(256)
+    e, m = (code >> 3) & 15, code & 7
+    v = np.where(e == 0, np.ldexp(m / 8.0, -6), np.ldexp(1 + m / 8.0, e - 7))
+    v = np.where((code & 127) == 127, np.nan, v)
+    return np.where(code >= 128, -v, v).astype(np.float32)
 
 
 def _epilogue_code(act) -> int:
@@ -75,8 +91,8 @@ class Tensor:
         self._shape = [int(s) for s in shape]
         if any(s < 0 for s in self._shape):
             raise RuntimeError("Tensor: negative extent")
-        if dtype not in _NP:
-            raise RuntimeError("Tensor: only float32 and float64 are supported on this path")
+        if dtype not in _NP and dtype not in _LOW:
+            raise RuntimeError("Tensor: float16 tensors are not supported on this path")
         self._dtype = dtype
         self._strides = list(_strides) if _strides is not None else _contiguous_strides(self._shape)
         self._storage = _storage if _storage is not None else _Storage(self.nbytes())
@@ -115,7 +131,13 @@ class Tensor:
         return n
 
     def itemsize(self) -> int:
+        if self._dtype in _LOW:
+            return _LOW[self._dtype]
         return 4 if self._dtype == DType.float32 else 8
+
+    def _require_plain(self, what: str) -> None:
+        if self._dtype not in _NP:
+            raise RuntimeError(f"{what}: float32 or float64 tensor expected, got {self._dtype.name}")
 
     def nbytes(self) -> int:
         return self.numel() * self.itemsize()
@@ -145,6 +167,8 @@ class Tensor:
     def randn(shape, dtype: DType = DType.float32, seed: Optional[int] = None) -> "Tensor":
         """Standard-normal values.  The reference draws them with a time-seeded cuRAND generator
         (src/tensor.cu:158-206); here they come from NumPy so that a seed reproduces them."""
+        if dtype not in _NP:
+            raise RuntimeError(f"randn: float32 or float64 expected, got {dtype.name}")
         rng = np.random.default_rng(seed)
         return Tensor.from_numpy(rng.standard_normal(tuple(shape)).astype(_NP[dtype]))
 
@@ -155,6 +179,8 @@ class Tensor:
             dtype = DType.float32
         elif arr.dtype == np.float64:
             dtype = DType.float64
+        elif arr.dtype == np.int32:
+            dtype = DType.int32
         else:
             raise RuntimeError("Unsupported numpy dtype")
         arr = np.ascontiguousarray(arr)
@@ -165,14 +191,33 @@ class Tensor:
         return t
 
     def numpy(self) -> np.ndarray:
+        """Host copy; bfloat16 and float8_e4m3 come as the float32 values they stand for."""
         src = self if self.is_contiguous() else self.contiguous()
-        out = np.empty(tuple(self._shape), dtype=_NP[self._dtype])
+        raw = {DType.bfloat16: np.uint16, DType.float8_e4m3: np.uint8, DType.int32: np.int32}
+        out = np.empty(tuple(self._shape), dtype=_NP.get(self._dtype) or raw[self._dtype])
         if out.nbytes:
             lib = _lib.load()
             if self.stream is not None:
                 _lib.check(lib.cudeep_b200_stream_synchronize(self.stream))
             _lib.check(lib.cudeep_b200_memcpy_d2h(out.ctypes.data_as(ctypes.c_void_p), src._storage.ptr,
                                                   out.nbytes, None))
+        if self._dtype == DType.bfloat16:
+            return (out.astype(np.uint32) << 16).view(np.float32)
+        if self._dtype == DType.float8_e4m3:
+            return _e4m3_values()[out]
+        return out
+
+    def to(self, dtype: DType) -> "Tensor":
+        """The same values as float32 or bfloat16 (rounded to nearest even)."""
+        if self._dtype == dtype:
+            return self
+        if self._dtype not in _TYPE_CODE or dtype not in _TYPE_CODE:
+            raise RuntimeError(f"to: no conversion from {self._dtype.name} to {dtype.name}")
+        src = self if self.is_contiguous() else self.contiguous()
+        out = Tensor(self._shape, dtype)
+        out.stream = self.stream
+        _lib.check(_lib.load().cudeep_b200_cast(src._storage.ptr, _TYPE_CODE[self._dtype], out._storage.ptr,
+                                                _TYPE_CODE[dtype], self.numel(), self.stream))
         return out
 
     # ---- views and copies ----------------------------------------------------------------
@@ -210,6 +255,8 @@ class Tensor:
     def contiguous(self) -> "Tensor":
         if self.is_contiguous():
             return self
+        if self.itemsize() not in (4, 8):
+            raise RuntimeError(f"contiguous: {self._dtype.name} tensors cannot be re-laid")
         out = Tensor(self._shape, self._dtype)
         out.stream = self.stream
         nd = self.ndim()
@@ -222,6 +269,7 @@ class Tensor:
     def fill_(self, value: float) -> "Tensor":
         if not self.is_contiguous():
             raise RuntimeError("fill_: tensor must be contiguous")
+        self._require_plain("fill_")
         lib = _lib.load()
         fn = lib.cudeep_b200_fill_f32 if self._dtype == DType.float32 else lib.cudeep_b200_fill_f64
         _lib.check(fn(self._storage.ptr, float(value), self.numel(), self.stream))
@@ -245,6 +293,7 @@ class Tensor:
             raise RuntimeError("matmul: inner dimensions do not match")
         if not (self.is_contiguous() and other.is_contiguous()):
             raise RuntimeError("matmul requires contiguous tensors")
+        self._require_plain("matmul")
         m, k = self._shape
         n = other._shape[1]
         out = Tensor([m, n], self._dtype)
@@ -315,6 +364,7 @@ def broadcast_add(matrix: Tensor, row: Tensor) -> Tensor:
     """out[i, j] = matrix[i, j] + row[j]  (module.cpp:664-694)."""
     if matrix.ndim() != 2 or row.numel() != matrix.shape()[1] or matrix.dtype() != row.dtype():
         raise RuntimeError("broadcast_add: expected [rows, cols] + [cols] of one dtype")
+    matrix._require_plain("broadcast_add")
     m = matrix if matrix.is_contiguous() else matrix.contiguous()
     r = row if row.is_contiguous() else row.contiguous()
     out = Tensor(matrix.shape(), matrix.dtype())
@@ -341,6 +391,7 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation=
         raise RuntimeError("linear: dtype mismatch")
     if bias is not None and bias.numel() != weight.shape()[0]:
         raise RuntimeError("linear: bias must have out_features elements")
+    x._require_plain("linear")
     act = _epilogue_code(activation)
     xc = x if x.is_contiguous() else x.contiguous()
     wc = weight if weight.is_contiguous() else weight.contiguous()
@@ -371,6 +422,7 @@ def conv2d(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, stride=(1, 
         raise RuntimeError("conv2d: channel mismatch")
     if x.dtype() != weight.dtype() or (bias is not None and bias.dtype() != x.dtype()):
         raise RuntimeError("conv2d: dtype mismatch")
+    x._require_plain("conv2d")
     (sh, sw), (ph, pw) = _pair(stride), _pair(padding)
     n, c, h, w = x.shape()
     oc, _, kh, kw = weight.shape()

@@ -16,6 +16,10 @@ enum class ElementType : int { F32 = 0, F16 = 1, BF16 = 2 };
 // (weights).  Scales lie [column block][row] and [row block][column block].
 enum class Fp8Block : int { Row = 1, Tile = 128 };
 
+// dst = src in another element type, rounded to nearest even.
+void launch_cast(const void* src, ElementType src_type, void* dst, ElementType dst_type, long long count,
+                 cudaStream_t stream = nullptr);
+
 void launch_quantize_fp8(const void* x, ElementType type, long long rows, int cols, Fp8Block block, void* q, float* scales,
                          cudaStream_t stream = nullptr);
 void launch_dequantize_fp8(const void* q, const float* scales, long long rows, int cols, Fp8Block block, void* y,

@@ -156,6 +156,10 @@ int cudeep_b200_gemm_tf32_tuned(const float* A, const float* B, int b_is_nk, flo
 #define CUDEEP_B200_TYPE_F16 1
 #define CUDEEP_B200_TYPE_BF16 2
 
+/* dst = src in another of these types, rounded to nearest even. */
+int cudeep_b200_cast(const void* src, int src_type, void* dst, int dst_type, long long count,
+                     cudeep_b200_stream_t stream);
+
 /* q[rows, cols] = x / scale in 8-bit floating point (e4m3: 4 exponent bits, 3 of mantissa, largest
  * 448, no infinities), rounded to nearest even, with one scale for each block of 128 columns and
  * block_rows = 1 (activations) or 128 (weights) rows:
