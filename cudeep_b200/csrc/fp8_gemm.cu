@@ -3,6 +3,7 @@
 
 #include "fp8_gemm.cuh"
 #include "fp8_rows.cuh"
+#include "fp8_scaled.cuh"
 #include "ragged_plan.h"
 
 #include <algorithm>
@@ -92,18 +93,22 @@ void launch_few(Fp8FewParams& p, cudaStream_t stream) {
                     FP8F_SMEM_BUDGET + 1024, stream);
 }
 
+template <class OutT, class Params>
+void set_output(Params& p) {
+    p.tma_store = (size_t(p.features) * sizeof(OutT)) % 16 == 0 && reinterpret_cast<uintptr_t>(p.c) % 16 == 0;
+    if (!p.tma_store) return;
+    const uint64_t dims[2] = {uint64_t(p.features), uint64_t(p.rows)};
+    const uint64_t strides[1] = {uint64_t(p.features) * sizeof(OutT)};
+    const uint32_t box[2] = {uint32_t(128 / sizeof(OutT)), 32};
+    if (sizeof(OutT) == 4) encode_tensor_map(&p.map_c, static_cast<const float*>(p.c), 2, dims, strides, box, TmaSwizzle::B128);
+    else encode_tensor_map_f16(&p.map_c, p.c, 2, dims, strides, box, TmaSwizzle::B128);
+}
+
 template <RaggedForm FORM, int BN, class OutT>
 void launch_by_rows_bn(Fp8RowsParams& p, cudaStream_t stream) {
     const DeviceInfo& dev = device_info();
     CB200_REQUIRE(dev.cc_major == 10, "8-bit products need an sm_100 device");
-    p.tma_store = (size_t(p.features) * sizeof(OutT)) % 16 == 0 && reinterpret_cast<uintptr_t>(p.c) % 16 == 0;
-    if (p.tma_store) {
-        const uint64_t dims[2] = {uint64_t(p.features), uint64_t(p.rows)};
-        const uint64_t strides[1] = {uint64_t(p.features) * sizeof(OutT)};
-        const uint32_t box[2] = {uint32_t(128 / sizeof(OutT)), 32};
-        if (sizeof(OutT) == 4) encode_tensor_map(&p.map_c, static_cast<const float*>(p.c), 2, dims, strides, box, TmaSwizzle::B128);
-        else encode_tensor_map_f16(&p.map_c, p.c, 2, dims, strides, box, TmaSwizzle::B128);
-    }
+    set_output<OutT>(p);
     p.status = dev.status_word;
     p.wait_limit_ns = 2000000000ull;
     p.tiles_m = (p.rows + 255) / 256;
@@ -114,6 +119,49 @@ void launch_by_rows_bn(Fp8RowsParams& p, cudaStream_t stream) {
                 FORM == RaggedForm::NT ? "nt" : "nn", p.rows, p.features, p.k, BN, FP8R_STAGES, clusters,
                 p.tma_store ? "bulk-tensor" : "rows");
     launch_clusters(fp8_rows_kernel<FORM, BN, OutT>, p, clusters, 2, FP8R_THREADS, FP8R_SMEM_BYTES, FP8R_SMEM_BYTES, stream);
+}
+
+// The scales applied by the tensor core, and behind it fp8_rows.cuh's kernel, which runs if they were not all powers of two.
+template <RaggedForm FORM, class OutT>
+void launch_scaled(Fp8RowsParams& rows_form, cudaStream_t stream) {
+    const DeviceInfo& dev = device_info();
+    CB200_REQUIRE(dev.cc_major == 10, "8-bit products need an sm_100 device");
+    Fp8ScaledParams p{};
+    p.map_x = rows_form.map_x;
+    p.map_w = rows_form.map_w;
+    p.bias = rows_form.bias;
+    p.act = rows_form.act;
+    p.c = rows_form.c;
+    p.rows = rows_form.rows;
+    p.features = rows_form.features;
+    p.k = rows_form.k;
+    p.tiles_m = (p.rows + 255) / 256;
+    p.tiles_n = (p.features + 255) / 256;
+    p.chunk_blocks = sizeof(OutT) == 4 ? 2048 / FP8_BK : 16384 / FP8_BK;
+    p.status = dev.status_word;
+    p.wait_limit_ns = 2000000000ull;
+    const int k_blocks = (p.k + FP8_BK - 1) / FP8_BK;
+    const size_t x_words = size_t(k_blocks) * p.tiles_m * 2 * 128, w_words = size_t(k_blocks) * p.tiles_n * 2 * 128;
+    Scratch packed((x_words + w_words + SCALE_FLAGS) * 4, stream);
+    uint32_t* xs = static_cast<uint32_t*>(packed.ptr);
+    uint32_t* ws = xs + x_words;
+    uint32_t* odd = ws + w_words;
+    p.odd_scales = rows_form.odd_scales = odd;
+    const uint32_t xs_box[2] = {16, 32}, ws_box[2] = {16, 64};
+    const uint64_t strides[1] = {16}, xs_dims[2] = {16, x_words / 4}, ws_dims[2] = {16, w_words / 4};
+    encode_tensor_map_u8(&p.map_xs, xs, 2, xs_dims, strides, xs_box, TmaSwizzle::None);
+    encode_tensor_map_u8(&p.map_ws, ws, 2, ws_dims, strides, ws_box, TmaSwizzle::None);
+    launch_dependent(pack_scales_kernel, dim3(SCALE_FLAGS), 256, stream, rows_form.x_scales, p.rows, 2 * p.tiles_m,
+                     rows_form.w_scales, (p.features + 127) / 128, 2 * p.tiles_n, rows_form.ws_feature, rows_form.ws_k, k_blocks, xs,
+                     ws, odd);
+    set_output<OutT>(p);
+    const long long tiles = (long long)p.tiles_m * p.tiles_n;
+    const long long clusters = tiles < dev.num_sms / 2 ? tiles : dev.num_sms / 2;
+    CB200_TRACE("fp8 %s tcgen05, scales in the MMA: rows=%d features=%d k=%d tile=256x256 stages=%d clusters=%lld store=%s",
+                FORM == RaggedForm::NT ? "nt" : "nn", p.rows, p.features, p.k, FP8S_STAGES, clusters,
+                p.tma_store ? "bulk-tensor" : "rows");
+    launch_clusters(fp8_scaled_kernel<FORM, OutT>, p, clusters, 2, FP8R_THREADS, FP8S_SMEM_BYTES, FP8S_SMEM_BYTES, stream);
+    launch_by_rows_bn<FORM, 256, OutT>(rows_form, stream);
 }
 
 // Tiles of 256 rows x 256 features; of 128 features where even those do not outnumber the pairs of SMs.
@@ -130,8 +178,13 @@ double cost_by_rows(int m, int n, int k, bool narrow) {
     return waves * (blocks * (narrow ? 24576.0 : 32768.0) / PLAN_L2_BYTES + (narrow ? 1500.0 : 3000.0)) + 4000.0;
 }
 
+// Packing the scales and a kernel that finds nothing to do cost about 5 us: the scaled form is for products of 40 us and more by the
+// estimate above.
+constexpr double SCALED_FROM_CYCLES = 75000.0;
+
 template <RaggedForm FORM, class OutT>
-void launch_by_rows(Fp8RowsParams& p, bool narrow, cudaStream_t stream) {
+void launch_by_rows(Fp8RowsParams& p, bool narrow, bool scaled, cudaStream_t stream) {
+    if (scaled) return launch_scaled<FORM, OutT>(p, stream);
     if constexpr (FORM == RaggedForm::NT) {
         if (narrow) return launch_by_rows_bn<FORM, 128, OutT>(p, stream);
     }
@@ -165,7 +218,9 @@ void product(const uint8_t* x, const float* x_scales, const uint8_t* w, const fl
     };
     const bool narrow = !nn && narrow_tiles(m, n);
     const FewPlan few = plan_few(m, n, k);
-    if (m > FP8F_MAX_ROWS && cost_by_rows(m, n, k, narrow) < few.cost) {
+    const double rows_cost = cost_by_rows(m, n, k, narrow);
+    if (m > FP8F_MAX_ROWS && rows_cost < few.cost) {
+        const bool scaled = !narrow && rows_cost >= SCALED_FROM_CYCLES;
         Fp8RowsParams p{};
         fill(p);
         encode_tensor_map_u8(&p.map_x, xr.ptr, 2, x_dims, x_strides, box, TmaSwizzle::B128);
@@ -173,9 +228,9 @@ void product(const uint8_t* x, const float* x_scales, const uint8_t* w, const fl
             const uint32_t w_box[2] = {128, 64};
             encode_tensor_map_u8(&p.map_w, wr.ptr, 2, w_dims, w_strides, w_box, TmaSwizzle::B128);
         }
-        if (y_type == TYPE_F32) launch_by_rows<FORM, float>(p, narrow, stream);
-        else if (y_type == TYPE_F16) launch_by_rows<FORM, __half>(p, narrow, stream);
-        else launch_by_rows<FORM, __nv_bfloat16>(p, narrow, stream);
+        if (y_type == TYPE_F32) launch_by_rows<FORM, float>(p, narrow, scaled, stream);
+        else if (y_type == TYPE_F16) launch_by_rows<FORM, __half>(p, narrow, scaled, stream);
+        else launch_by_rows<FORM, __nv_bfloat16>(p, narrow, scaled, stream);
     } else {
         Fp8FewParams p{};
         fill(p);

@@ -25,6 +25,13 @@ constexpr uint32_t FP8R_STAGING_BYTES = 8 * 4096;      // 32 rows x 128 bytes pe
 constexpr int FP8R_STAGES = 6;
 constexpr uint32_t FP8R_SMEM_BYTES = FP8R_STAGES * FP8R_STAGE_BYTES + FP8R_STAGING_BYTES + 1024;
 
+constexpr int SCALE_FLAGS = 256;      // CTAs of pack_scales_kernel (fp8_scaled.cuh), each with a word of its own
+
+// Whether any word is set; all threads of the CTA.
+__device__ __forceinline__ bool any_odd_scales(const uint32_t* flags) {
+    return __syncthreads_or(threadIdx.x < SCALE_FLAGS ? int(__ldg(flags + threadIdx.x)) : 0) != 0;
+}
+
 struct Fp8RowsParams {
     CUtensorMap map_x;       // {K, rows} box {128, 128}
     CUtensorMap map_w;       // NT {K, F} box {128, BN / 2}; NN {F, K} box {128, 128}
@@ -40,6 +47,7 @@ struct Fp8RowsParams {
     int features;
     int k;
     int tiles_m, tiles_n;
+    const uint32_t* odd_scales;      // nullptr, or SCALE_FLAGS words: run only if one of them is set
     uint32_t* status;
     unsigned long long wait_limit_ns;
 };
@@ -48,6 +56,46 @@ template <int REGS>
 __device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS)); }
 template <int REGS>
 __device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS)); }
+
+// A warp's 32 rows x BN / 2 features: bias, activation, and out through its staging block.
+template <int BN, class OutT, class Params>
+__device__ __forceinline__ void store_tile(const Params& p, float (&acc)[BN / 64][32], const Fp8Activation& act, uint32_t staging,
+                                           uint32_t lane, int row0, int feature0) {
+    constexpr int COLS = 128 / sizeof(OutT);          // columns of a staged block: 128 bytes per row
+#pragma unroll
+    for (int i = 0; i < BN / 64; ++i) {
+        if (p.bias != nullptr) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+                const int f = feature0 + 32 * i + j;
+                acc[i][j] += __ldg(p.bias + min(f, p.features - 1));
+            }
+        }
+        fp8_activation(acc[i], act);
+        const int c0 = 32 * i / COLS * COLS;          // first column of the staged block this chunk belongs to
+        if (32 * i == c0) {
+            if (lane == 0) ptx::bulk_wait_group_read<0>();      // the block's last store has read it
+            __syncwarp();
+        }
+        stage_block<OutT>(staging, lane, 32 * i - c0, acc[i]);
+        if (32 * (i + 1) - c0 == COLS) {              // the block is full
+            const int f0 = feature0 + c0;
+            if (p.tma_store) {
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0 && row0 < p.rows && f0 < p.features) {
+                    ptx::tma_store_2d(&p.map_c, staging, f0, row0);
+                    ptx::bulk_commit_group();
+                }
+            } else {
+                // Rows of C that are no 16-byte multiples: the warp writes them one by one.
+                __syncwarp();
+                OutT* dst = static_cast<OutT*>(p.c) + (long long)row0 * p.features + f0;
+                write_block<OutT>(staging, lane, dst, p.features, min(32, p.rows - row0), p.features - f0, false);
+            }
+        }
+    }
+}
 
 template <RaggedForm FORM, int BN, class OutT>
 __global__ void __launch_bounds__(FP8R_THREADS, 1) fp8_rows_kernel(const __grid_constant__ Fp8RowsParams p) {
@@ -58,6 +106,10 @@ __global__ void __launch_bounds__(FP8R_THREADS, 1) fp8_rows_kernel(const __grid_
     constexpr int CHUNKS = BN / 32;      // of 16 columns, per epilogue warp (half of the tile's columns)
     constexpr uint32_t TX_BYTES = 2 * 16384 + BN * 128;
 
+    if (p.odd_scales != nullptr) {
+        ptx::grid_dependency_wait();
+        if (!any_odd_scales(p.odd_scales)) return;      // the tensor core has applied these scales itself
+    }
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bar_full[FP8R_STAGES];
     __shared__ __align__(8) uint64_t bar_empty[FP8R_STAGES];
@@ -243,40 +295,7 @@ __global__ void __launch_bounds__(FP8R_THREADS, 1) fp8_rows_kernel(const __grid_
                 ++it;
               }
             }
-            constexpr int COLS = 128 / sizeof(OutT);          // columns of a staged block: 128 bytes per row
-#pragma unroll
-            for (int i = 0; i < BN / 64; ++i) {
-                if (p.bias != nullptr) {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        const int f = feature0 + 32 * i + j;
-                        acc[i][j] += __ldg(p.bias + min(f, p.features - 1));
-                    }
-                }
-                fp8_activation(acc[i], act);
-                const int c0 = 32 * i / COLS * COLS;          // first column of the staged block this chunk belongs to
-                if (32 * i == c0) {
-                    if (lane == 0) ptx::bulk_wait_group_read<0>();      // the block's last store has read it
-                    __syncwarp();
-                }
-                stage_block<OutT>(staging, lane, 32 * i - c0, acc[i]);
-                if (32 * (i + 1) - c0 == COLS) {              // the block is full
-                    const int f0 = feature0 + c0;
-                    if (p.tma_store) {
-                        ptx::fence_proxy_async_smem();
-                        __syncwarp();
-                        if (lane == 0 && row0 < p.rows && f0 < p.features) {
-                            ptx::tma_store_2d(&p.map_c, staging, f0, row0);
-                            ptx::bulk_commit_group();
-                        }
-                    } else {
-                        // Rows of C that are no 16-byte multiples: the warp writes them one by one.
-                        __syncwarp();
-                        OutT* dst = static_cast<OutT*>(p.c) + (long long)row0 * p.features + f0;
-                        write_block<OutT>(staging, lane, dst, p.features, min(32, p.rows - row0), p.features - f0, false);
-                    }
-                }
-            }
+            store_tile<BN, OutT>(p, acc, act, staging, lane, row0, feature0);
         }
     epilogue_done:
         __syncwarp();

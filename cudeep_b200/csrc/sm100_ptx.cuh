@@ -439,6 +439,26 @@ __device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t a_desc, uint64
             : : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
 }
 
+// kind::mxf8f6f4: 8-bit operands with a power-of-two scale (UE8M0) for each row and 32 elements of K, read from tensor memory.
+template <int CTAS>
+__device__ __forceinline__ void umma_mxf8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t scale_a_tmem, uint32_t scale_b_tmem, uint32_t accumulate) {
+    static_assert(CTAS == 2, "pairs only");
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%5], [%6], p;\n\t"
+        "}\n"
+        : : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(scale_a_tmem), "r"(scale_b_tmem)
+        : "memory");
+}
+// 32 rows of 16 bytes from shared memory (no swizzle, 8-row groups 128 bytes apart) to four columns of tensor memory, the same in
+// each quarter of the lanes; in both CTAs of the pair, each from its own shared memory.  Ordered with the thread's MMAs.
+__device__ __forceinline__ void tmem_cp_32x128b_pair(uint32_t taddr, uint64_t smem_desc) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(smem_desc) : "memory");
+}
+
 // Make `bar` (a shared::cluster address; a plain CTA-local shared address is
 // valid too) complete one arrival once all MMAs issued so far have finished.
 template <int CTAS>
@@ -513,6 +533,12 @@ __host__ __device__ constexpr uint32_t idesc_f16(int m, int n, int a_mn_major, i
 // The same for kind::f8f6f4 with e4m3 A and B (format 0), FP32 accumulate.
 __host__ __device__ constexpr uint32_t idesc_e4m3(int m, int n, int a_mn_major, int b_mn_major) {
     return idesc_f16(m, n, a_mn_major, b_mn_major, 0);
+}
+
+// kind::mxf8f6f4 with e4m3 A and B and UE8M0 scales (bit 23), scale bytes 0 of their words: the fields of idesc_f16 otherwise.
+__host__ __device__ constexpr uint32_t idesc_mxf8(int m, int n, int a_mn_major, int b_mn_major) {
+    return (uint32_t(a_mn_major) << 15) | (uint32_t(b_mn_major) << 16) | (uint32_t(n >> 3) << 17) | (1u << 23) |
+           (uint32_t(m >> 4) << 24);
 }
 
 }  // namespace ptx
