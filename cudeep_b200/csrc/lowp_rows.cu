@@ -13,6 +13,7 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <algorithm>
 #include <type_traits>
 
 namespace cudeep_b200 {
@@ -186,7 +187,7 @@ __device__ __forceinline__ uint32_t nan_codes(uint32_t q, float a, float b, floa
 // A row's 128 elements of a block that start anywhere, across a warp: a lane takes every 32nd, so that loads and byte stores
 // are contiguous across the lanes.  Loads are not conditional: lanes behind the row's end read its last element and drop it
 // (a branch around each load kept the loads of a block from being under way together: 4100 x 11007 FP32 78 us instead of
-// QTILES; four neighbouring elements a lane, to store their codes as a word, were four times as many requests to L1: 100 us).
+// 50 us; four neighbouring elements a lane, to store their codes as a word, were four times as many requests to L1: 100 us).
 struct RowSlice {
     float v[4];
     // The first `width` (1 to 128) elements of the block; zeros for a row that is not there (src then is some row that is).
@@ -225,19 +226,20 @@ struct RowSlice {
 // Blocks of 1 x 128.  Eight lanes own a block, 16 elements each in units of 16 bytes; a warp takes four neighbouring blocks of
 // four rows, so a lane has 8 (16-bit types) or 16 independent loads under way, and a CTA 32 rows x 512 columns.  The
 // scales lie [block][row], so the CTA collects its 32 x 4 scales in shared memory and writes runs of 32.
-// 8192 x 16384 BF16, 407 MB: QROWS.
+// 8192 x 16384 BF16, 407 MB: 61 us.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __restrict__ x, long long rows, int cols,
-                                                                 uint8_t* __restrict__ q, float* __restrict__ scales) {
+                                                                 int grid_cols, uint8_t* __restrict__ q, float* __restrict__ scales) {
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
+    const int bx = int(blockIdx.x % unsigned(grid_cols)), by = int(blockIdx.x / unsigned(grid_cols));
     constexpr int N = Unit<T>::N, UNITS = 16 / N;
     __shared__ float s_scale[4][32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int sub = lane >> 3, l8 = lane & 7;
-    const int block = blockIdx.x * 4 + sub;
+    const int block = bx * 4 + sub;
     const int c0 = block * FP8_BLOCK + l8 * N;      // and 8 * N further on for each unit
-    const long long row0 = (long long)blockIdx.y * 32 + warp * 4;
+    const long long row0 = (long long)by * 32 + warp * 4;
     Unit<T> u[4][UNITS];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -289,8 +291,8 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __rest
     }
     __syncthreads();
     if (threadIdx.x < 128) {
-        const long long r = (long long)blockIdx.y * 32 + lane;
-        const int blk = blockIdx.x * 4 + warp;
+        const long long r = (long long)by * 32 + lane;
+        const int blk = bx * 4 + warp;
         if (r < rows && (long long)blk * FP8_BLOCK < cols) scales[(long long)blk * rows + r] = s_scale[warp][lane];
     }
 }
@@ -298,15 +300,16 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __rest
 // The same for rows that start anywhere: a warp takes four rows of a block at a time.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) quantize_rows_any_kernel(const T* __restrict__ x, long long rows, int cols,
-                                                                     uint8_t* __restrict__ q, float* __restrict__ scales) {
+                                                                     int grid_cols, uint8_t* __restrict__ q, float* __restrict__ scales) {
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
+    const int bx = int(blockIdx.x % unsigned(grid_cols)), by = int(blockIdx.x / unsigned(grid_cols));
     __shared__ float s_scale[4][32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const long long row0 = (long long)blockIdx.y * 32 + warp * 4;
+    const long long row0 = (long long)by * 32 + warp * 4;
 #pragma unroll 1
     for (int b = 0; b < 4; ++b) {
-        const int c0 = (blockIdx.x * 4 + b) * FP8_BLOCK;
+        const int c0 = (bx * 4 + b) * FP8_BLOCK;
         if (c0 >= cols) break;
         const int width = min(FP8_BLOCK, cols - c0);
         RowSlice slice[4];
@@ -327,8 +330,8 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_any_kernel(const T* __
     }
     __syncthreads();
     if (threadIdx.x < 128) {
-        const long long r = (long long)blockIdx.y * 32 + lane;
-        const int blk = blockIdx.x * 4 + warp;
+        const long long r = (long long)by * 32 + lane;
+        const int blk = bx * 4 + warp;
         if (r < rows && (long long)blk * FP8_BLOCK < cols) scales[(long long)blk * rows + r] = s_scale[warp][lane];
     }
 }
@@ -337,15 +340,16 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_any_kernel(const T* __
 // block, 32 rows at a time.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) quantize_tiles_kernel(const T* __restrict__ x, long long rows, int cols,
-                                                                  uint8_t* __restrict__ q, float* __restrict__ scales) {
+                                                                  int grid_cols, uint8_t* __restrict__ q, float* __restrict__ scales) {
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
+    const int bx = int(blockIdx.x % unsigned(grid_cols)), by = int(blockIdx.x / unsigned(grid_cols));
     constexpr int N = Unit<T>::N, UNITS = 16 / N;
     __shared__ float s_max[kThreads / 32];
     __shared__ uint32_t s_top[kThreads / 32];
     const int l8 = threadIdx.x & 7;
-    const int c0 = blockIdx.x * FP8_BLOCK + l8 * N;
-    const long long row0 = (long long)blockIdx.y * FP8_BLOCK + (threadIdx.x >> 3);
+    const int c0 = bx * FP8_BLOCK + l8 * N;
+    const long long row0 = (long long)by * FP8_BLOCK + (threadIdx.x >> 3);
     Unit<T> u[4][UNITS];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -384,7 +388,7 @@ __global__ void __launch_bounds__(kThreads) quantize_tiles_kernel(const T* __res
     }
     const int e = scale_exponent(amax);
     const float inv = pow2(-e);
-    if (threadIdx.x == 0) scales[(long long)blockIdx.y * gridDim.x + blockIdx.x] = pow2(e);
+    if (threadIdx.x == 0) scales[(long long)by * grid_cols + bx] = pow2(e);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const long long r = row0 + 32 * i;
@@ -406,18 +410,19 @@ __global__ void __launch_bounds__(kThreads) quantize_tiles_kernel(const T* __res
     }
 }
 
-// The same for rows that start anywhere: a warp holds eight rows.  4100 x 11007 FP32, 226 MB: QTILES.
+// The same for rows that start anywhere: a warp holds eight rows.  4100 x 11007 FP32, 226 MB: 50 us.
 constexpr int kTileThreads = 512;
 template <typename T>
 __global__ void __launch_bounds__(kTileThreads) quantize_tiles_any_kernel(const T* __restrict__ x, long long rows, int cols,
-                                                                          uint8_t* __restrict__ q, float* __restrict__ scales) {
+                                                                          int grid_cols, uint8_t* __restrict__ q, float* __restrict__ scales) {
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
+    const int bx = int(blockIdx.x % unsigned(grid_cols)), by = int(blockIdx.x / unsigned(grid_cols));
     __shared__ uint32_t s_top[kTileThreads / 32], s_finite_top[kTileThreads / 32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int c0 = blockIdx.x * FP8_BLOCK;
+    const int c0 = bx * FP8_BLOCK;
     const int width = min(FP8_BLOCK, cols - c0);
-    const long long row0 = (long long)blockIdx.y * FP8_BLOCK + warp * 8;
+    const long long row0 = (long long)by * FP8_BLOCK + warp * 8;
     RowSlice slice[8];
     uint32_t m = 0;
 #pragma unroll
@@ -444,7 +449,7 @@ __global__ void __launch_bounds__(kTileThreads) quantize_tiles_any_kernel(const 
     }
     const int e = scale_exponent(__uint_as_float(m));
     const float inv = pow2(-e);
-    if (threadIdx.x == 0) scales[(long long)blockIdx.y * gridDim.x + blockIdx.x] = pow2(e);
+    if (threadIdx.x == 0) scales[(long long)by * grid_cols + bx] = pow2(e);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const long long at = (row0 + i) * cols + c0;
@@ -523,7 +528,7 @@ __global__ void dequantize_kernel(const uint8_t* __restrict__ q, const float* __
 
 // Slope of the epilogue activations.  With s = sigmoid(t), t = 2 sqrt(2 / pi) (z + 0.044715 z^3): tanh-form GELU is z s, so its
 // slope is s + z s (1 - s) dt/dz; SiLU the same with t = z.  s comes from the SFU's ex2 and rcp as in the forward epilogue
-// (2 ulp; with expf and tanhf the pass was bound by arithmetic, 68 us for 8192 x 4096 instead of BACK_US).
+// (2 ulp; with expf and tanhf the pass was bound by arithmetic, 68 us for 8192 x 4096 instead of 34 us with the bands' sums).
 __device__ __forceinline__ float clamp_nan(float v, float lo, float hi) {      // keeps NaN
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(lo));
@@ -596,7 +601,8 @@ __global__ void __launch_bounds__(kThreads) act_backward_kernel(const T* __restr
                     float z[8];
                     e4m3_values(z8s[i], z);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) g[j] *= act_slope<act>(z[j] * s[i]);
+                    for (int j = 0; j < 8; ++j)      // rounded before the sum, whether dz is stored or not
+                        g[j] = __fmul_rn(g[j], act_slope<act>(z[j] * s[i]));
                 }
                 if (!VEC) {
 #pragma unroll
@@ -687,9 +693,10 @@ template <typename T>
 void act_backward_typed(const T* dy, const uint8_t* z8, const float* z_scales, int act, T* dz, long long ld_dz, float* db,
                         int rows, int cols, cudaStream_t stream) {
     const bool vec = cols % 8 == 0 && reinterpret_cast<uintptr_t>(dy) % 16 == 0 && reinterpret_cast<uintptr_t>(z8) % 8 == 0;
-    const int rows_per = rows > 4096 ? 64 : 32;
+    // Bands of the grid's second dimension (at most 65535); 64 rows keep the last wave of CTAs full for large matrices.
+    const int least = (rows / 65535 + 32) / 32 * 32;
+    const int rows_per = std::max(rows > 4096 ? 64 : 32, least);
     const int bands = (rows + rows_per - 1) / rows_per;
-    CB200_REQUIRE(bands <= 65535, "too many rows");
     Scratch partial;
     float* to = db;
     if (db != nullptr && bands > 1) {
@@ -761,15 +768,17 @@ void quantize_typed(const T* x, long long rows, int cols, int block_rows, uint8_
                      reinterpret_cast<uintptr_t>(q) % Unit<T>::N == 0;
     const unsigned blocks = unsigned((cols + FP8_BLOCK - 1) / FP8_BLOCK);
     const int rows_per = block_rows == 1 ? 32 : FP8_BLOCK;
-    CB200_REQUIRE((rows + rows_per - 1) / rows_per <= 65535, "quantize_fp8: too many rows");      // gridDim.y
-    const unsigned bands = unsigned((rows + rows_per - 1) / rows_per);
-    const dim3 grid(block_rows == 1 ? (blocks + 3) / 4 : blocks, bands);
+    // One grid dimension, neighbours along a row first.
+    const int grid_cols = int(block_rows == 1 ? (blocks + 3) / 4 : blocks);
+    const long long ctas = (rows + rows_per - 1) / rows_per * grid_cols;
+    CB200_REQUIRE(ctas <= 2147483647ll, "quantize_fp8: matrix too large");
+    const dim3 grid{unsigned(ctas)};
     if (block_rows == 1) {
-        if (vec) launch_dependent(quantize_rows_kernel<T>, dim3(grid), kThreads, stream, x, rows, cols, q, scales);
-        else launch_dependent(quantize_rows_any_kernel<T>, dim3(grid), kThreads, stream, x, rows, cols, q, scales);
+        if (vec) launch_dependent(quantize_rows_kernel<T>, grid, kThreads, stream, x, rows, cols, grid_cols, q, scales);
+        else launch_dependent(quantize_rows_any_kernel<T>, grid, kThreads, stream, x, rows, cols, grid_cols, q, scales);
     } else {
-        if (vec) launch_dependent(quantize_tiles_kernel<T>, dim3(grid), kThreads, stream, x, rows, cols, q, scales);
-        else launch_dependent(quantize_tiles_any_kernel<T>, dim3(grid), kTileThreads, stream, x, rows, cols, q, scales);
+        if (vec) launch_dependent(quantize_tiles_kernel<T>, grid, kThreads, stream, x, rows, cols, grid_cols, q, scales);
+        else launch_dependent(quantize_tiles_any_kernel<T>, grid, kTileThreads, stream, x, rows, cols, grid_cols, q, scales);
     }
     CB200_CHECK_LAUNCH();
 }

@@ -149,7 +149,7 @@ int cudeep_b200_gemm_tf32_tuned(const float* A, const float* B, int b_is_nk, flo
 /* No counterpart in the reference: the products of low-precision Linear layers and of layers whose
  * rows are split among experts.  All matrices are row-major and contiguous; any base address that
  * suits its element type and any row length is taken (rows that are not 16-byte multiples are first
- * copied to a padded temporary).  Zero rows are a valid size. */
+ * copied to a padded temporary).  Zero rows are a valid size.  Results must not overlap operands. */
 
 /* Element types of the operands passed as void pointers. */
 #define CUDEEP_B200_TYPE_F32 0
@@ -191,7 +191,8 @@ int cudeep_b200_linear_backward_data_fp8(const void* dy, const float* dy_scales,
  *   dx[M,K] = dz * W,   dw[N,K] = dz^T * x,   db[N] = column sums of dz (FP32).
  * type is that of dy, W and dx, F16 or BF16; dw has it or is F32.  dx, dw and db may each be NULL, and
  * then so may what only they need; z8 is not read without an activation.  dz is rounded to `type`
- * before the products, db is not. */
+ * before the products, db is not.  x enters dw without rounding if its scales are powers of two
+ * (cudeep_b200_quantize_fp8's are), else rounded to `type`. */
 int cudeep_b200_linear_backward_saved_fp8(const void* dy, int type, const void* x8, const float* x_scales,
                                           const void* z8, const float* z_scales, int epilogue,
                                           const void* W, void* dx, void* dw, int dw_type, float* db, int M,

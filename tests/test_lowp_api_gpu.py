@@ -349,7 +349,11 @@ def test_offsets_beyond_32_bits(dev):
     tail, tail_s = x8[-300:].contiguous(), xs[:, -300:].contiguous()
     dev.check(lib.cudeep_b200_linear_forward_fp8(p(tail), p(tail_s), p(w8), p(ws), None, p(last), 2, 300, n, k, 0, None))
     assert dev.sync_status() == 0
-    assert torch.equal(y[-300:], last)
+    # The large product and the small one sum in different orders.  All terms are positive, so each FP32 sum is within
+    # (128 + 2) * 2^-23 = 2^-15.9 of the exact value, far below bfloat16's half step: the two roundings of values that near can
+    # only be equal or neighbours, 2^-7 of the value apart.
+    assert ((y[-300:].double() - last.double()).abs() <= 2.0 ** -7 * last.double()).all()
+    last = y[-300:].clone()
     q = torch.empty(m, n, dtype=torch.uint8, device=dev.dev)
     s = torch.empty(-(-n // 128), m, device=dev.dev)
     dev.check(lib.cudeep_b200_quantize_fp8(p(y), 2, m, n, 1, p(q), p(s), None))
@@ -370,6 +374,59 @@ def test_offsets_beyond_32_bits(dev):
     assert (out[-300:].double() - want).norm() <= 2.0 ** -8 * want.norm() and bool((out[:-300] == 0).all())
     want = dy[-300:].double().t() @ last.double()
     assert (dw.double() - want).norm() <= 1e-5 * want.norm()
+
+
+def test_gradients_asked_for_one_by_one(dev):
+    torch = dev.torch
+    m, n, k = 150, 72, 200
+    gen = torch.Generator(device=dev.dev).manual_seed(9)
+    dy, w = torch.randn(m, n, generator=gen, device=dev.dev).bfloat16(), torch.randn(n, k, generator=gen, device=dev.dev).bfloat16()
+    x8, z8 = (torch.randint(0, 120, (m, d), generator=gen, device=dev.dev, dtype=torch.int32).to(torch.uint8) for d in (k, n))
+    xs, zs = torch.full((2, m), 0.125, device=dev.dev), torch.full((1, m), 0.02, device=dev.dev)
+    lib, p = dev.lib, dev.ptr
+    for act in (0, 3):
+        z = (p(z8), p(zs)) if act else (None, None)
+        make = lambda: [torch.full(s, 7.0, dtype=t, device=dev.dev) for s, t in      # noqa: E731
+                        (((m, k), torch.bfloat16), ((n, k), torch.bfloat16), ((n,), torch.float32))]
+        whole = make()
+        dev.check(lib.cudeep_b200_linear_backward_saved_fp8(p(dy), 2, p(x8), p(xs), *z, act, p(w), p(whole[0]), p(whole[1]), 2,
+                                                            p(whole[2]), m, n, k, None))
+        for i in range(3):
+            part = make()
+            dx, dw, db = (p(part[j]) if j == i else None for j in range(3))
+            dev.check(lib.cudeep_b200_linear_backward_saved_fp8(
+                p(dy), 2, p(x8) if dw else None, p(xs) if dw else None, *z, act, p(w) if dx else None, dx, dw, 2, db, m, n, k,
+                None))
+            assert dev.sync_status() == 0
+            for j in range(3):
+                assert torch.equal(part[j], whole[j]) if j == i else bool((part[j] == 7).all())
+
+
+def test_many_rows(dev):
+    """More rows than a grid's second dimension holds bands."""
+    torch = dev.torch
+    m, n = 5_000_001, 64
+    x = torch.randn(m, n, device=dev.dev).bfloat16()
+    lib, p = dev.lib, dev.ptr
+    for block_rows in (1, 128):
+        q, s = torch.empty(m, n, dtype=torch.uint8, device=dev.dev), torch.empty(m if block_rows == 1 else -(-m // 128), device=dev.dev)
+        dev.check(lib.cudeep_b200_quantize_fp8(p(x), 2, m, n, block_rows, p(q), p(s), None))
+        part = x[-129:].contiguous()      # the last block of 128 rows begins at a multiple of 128: 5000001 = 39062 * 128 + 65
+        if block_rows == 128:
+            part = x[-65:].contiguous()
+        r = part.shape[0]
+        q1, s1 = torch.empty(r, n, dtype=torch.uint8, device=dev.dev), torch.empty(r if block_rows == 1 else 1, device=dev.dev)
+        dev.check(lib.cudeep_b200_quantize_fp8(p(part), 2, r, n, block_rows, p(q1), p(s1), None))
+        assert dev.sync_status() == 0
+        assert torch.equal(q[-r:], q1) and torch.equal(s[-s1.numel():], s1)
+    z8, zs = torch.full((m, n), 0x38, dtype=torch.uint8, device=dev.dev), torch.ones(m, device=dev.dev)
+    db = torch.empty(n, device=dev.dev)
+    dev.check(lib.cudeep_b200_linear_backward_saved_fp8(p(x), 2, None, None, p(z8), p(zs), 1, None, None, None, 2, p(db), m, n, 8,
+                                                        None))
+    assert dev.sync_status() == 0
+    want = x.double().sum(0)
+    # FP32 sums of 5e6 terms in bands: each band and the sum of the bands may lose 2^-24 of the magnitudes per addition.
+    assert ((db.double() - want).abs() <= (300 + 80000 / 8) * 2.0 ** -24 * x.double().abs().sum(0)).all()
 
 
 def test_nan_codes_and_infinities(dev):
