@@ -96,6 +96,25 @@ def test_quantize_borders(dev, block_rows):
     assert torch.equal(q, want_q)
 
 
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("lead,shift", [(0, 0), (0, 1), (4, 0), (8, 4), (3, 2)])
+def test_quantize_odd_rows_at_any_address(dev, block_rows, lead, shift):
+    """Rows whose starts take all phases within a word, from bases that suit vectors and from others."""
+    torch = dev.torch
+    rows, cols = 131, 389
+    for t in (torch.float32, torch.bfloat16):
+        buf = torch.randn(rows * cols + lead, device=dev.dev).to(t)
+        x = buf[lead:].view(rows, cols)
+        out = torch.full((rows * cols + 64,), 0xAA, dtype=torch.uint8, device=dev.dev)
+        scales = dev.empty((4, rows) if block_rows == 1 else (2, 4))
+        dev.check(dev.lib.cudeep_b200_quantize_fp8(dev.ptr(x), 0 if t == torch.float32 else 2, rows, cols, block_rows,
+                                                   ctypes.c_void_p(out.data_ptr() + 16 + shift), dev.ptr(scales), None))
+        want_q, want_s = reference(torch, x, block_rows)
+        start, end = 16 + shift, 16 + shift + rows * cols
+        assert torch.equal(out[start:end].view(rows, cols), want_q) and torch.equal(scales, want_s)
+        assert bool((out[:start] == 0xAA).all()) and bool((out[end:] == 0xAA).all())
+
+
 def test_quantize_unaligned_base_and_neighbours(dev):
     """A matrix that starts one element into a buffer; bytes around the result stay as they were."""
     torch = dev.torch
