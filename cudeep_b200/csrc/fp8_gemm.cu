@@ -178,9 +178,10 @@ double cost_by_rows(int m, int n, int k, bool narrow) {
     return waves * (blocks * (narrow ? 24576.0 : 32768.0) / PLAN_L2_BYTES + (narrow ? 1500.0 : 3000.0)) + 4000.0;
 }
 
-// Packing the scales and a kernel that finds nothing to do cost about 5 us: the scaled form is for products of 40 us and more by the
-// estimate above.
-constexpr double SCALED_FROM_CYCLES = 75000.0;
+// Packing the scales and a kernel that finds nothing to do cost about 5 us, which products of an estimated 50000 cycles and more
+// make good: 2048 x 4096 x 4096 (61000) takes 35.3 us so and 36.9 by rows, 4096 x 1024 -> 8192 (70000) 37.0 and 40.8, but
+// 2047 x 5000 -> 1672 (39000) 38.3 and 35.0.
+constexpr double SCALED_FROM_CYCLES = 50000.0;
 
 template <RaggedForm FORM, class OutT>
 void launch_by_rows(Fp8RowsParams& p, bool narrow, bool scaled, cudaStream_t stream) {

@@ -70,14 +70,14 @@ __device__ __forceinline__ void fp8_activation(float (&v)[N], const Fp8Activatio
 
 // For few rows (and for few features, whatever the rows) the FEATURES lie on the 128 lanes and up to 128 rows on the columns:
 // the width of the MMA follows the number of rows, and a CTA streams its features' weights once, which is all that a product
-// of a few rows costs.  One tile per CTA; where there are fewer tiles than the device has SMs, a cluster of up to eight CTAs shares a tile, each with a range of K,
-// and adds the parts up through distributed shared memory in rank order.  A tile may take fewer than 128 features (the last
+// of a few rows costs.  One tile per CTA; where there are fewer tiles than the device has SMs, a cluster of up to eight CTAs
+// shares a tile, each with a range of K, and adds the parts up through distributed shared memory in rank order.  A tile may take fewer than 128 features (the last
 // lanes then idle), so that the tiles fill the SMs: 16384 features are 128 tiles of 128, but 147 of 112.
 //
 // The factors xs * ws change along the columns here: each epilogue warp fetches those of its columns four blocks ahead and
 // reads them back from shared memory.  With so few columns TMEM holds up to eight accumulators, so the tensor core runs
 // ahead of the sums by that many blocks (two accumulators and factors one block ahead: 16 rows, 4096 -> 16384 took 35 us, 
-// every block waiting for its factors; now FEW_US us).
+// every block waiting for its factors; now 17 us).
 constexpr int FP8F_MAX_ROWS = 128;
 constexpr int FP8F_EPI_WARPS = 8;
 constexpr int FP8F_THREADS = 64 + 32 * FP8F_EPI_WARPS;

@@ -145,7 +145,8 @@ def slope64(torch, z, name):
 @pytest.mark.parametrize("dw_type", ["same", "f32"])
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("act", sorted(ACTS))
-@pytest.mark.parametrize("m,n,k", [(1, 64, 64), (40, 130, 72), (333, 77, 101), (300, 256, 384), (2500, 64, 136)])
+@pytest.mark.parametrize("m,n,k", [(1, 64, 64), (40, 130, 72), (333, 77, 101), (300, 256, 384), (2500, 64, 136), (1100, 512, 512),
+                                   (150, 2600, 1900)])
 def test_backward_saved(dev, m, n, k, act, dtype, dw_type):
     """dz is rounded to the type first (eps / 2 of it): that much of the sum of magnitudes joins the products' bounds."""
     torch = dev.torch
