@@ -78,13 +78,13 @@ void launch_few(Fp8FewParams& p, cudaStream_t stream) {
     const DeviceInfo& dev = device_info();
     CB200_REQUIRE(dev.cc_major == 10, "8-bit products need an sm_100 device");
     p.w_bytes = FORM == RaggedForm::NT ? uint32_t(p.step) * 128u : RAGGED_A_BYTES;
-    p.stage_bytes = RAGGED_A_BYTES + uint32_t(RowMaps::loaded(((p.rows < FP8F_MAX_ROWS ? p.rows : FP8F_MAX_ROWS) + 15) / 16 * 16)) * 128u;
+    p.tile_rows = p.rows < FP8F_MAX_ROWS ? p.rows : FP8F_MAX_ROWS;
+    p.stage_bytes = RAGGED_A_BYTES + uint32_t(RowMaps::loaded((p.tile_rows + 15) / 16 * 16)) * 128u;
     const int fit = int(FP8F_SMEM_BUDGET / p.stage_bytes);
     p.stages = fit < FP8F_MAX_STAGES ? fit : FP8F_MAX_STAGES;
     p.status = dev.status_word;
     p.wait_limit_ns = 2000000000ull;
     p.f_tiles = (p.features + p.step - 1) / p.step;
-    p.tile_rows = p.rows < FP8F_MAX_ROWS ? p.rows : FP8F_MAX_ROWS;
     const long long tiles = (long long)p.f_tiles * ((p.rows + FP8F_MAX_ROWS - 1) / FP8F_MAX_ROWS);
     CB200_TRACE("fp8 %s tcgen05, features on lanes: rows=%d features=%d k=%d stages=%d tiles=%lld step=%d split=%d",
                 FORM == RaggedForm::NT ? "nt" : "nn", p.rows, p.features, p.k, p.stages, tiles, p.step,
@@ -94,12 +94,12 @@ void launch_few(Fp8FewParams& p, cudaStream_t stream) {
 }
 
 template <class OutT, class Params>
-void set_output(Params& p) {
+void set_output(Params& p, uint32_t box_rows) {
     p.tma_store = (size_t(p.features) * sizeof(OutT)) % 16 == 0 && reinterpret_cast<uintptr_t>(p.c) % 16 == 0;
     if (!p.tma_store) return;
     const uint64_t dims[2] = {uint64_t(p.features), uint64_t(p.rows)};
     const uint64_t strides[1] = {uint64_t(p.features) * sizeof(OutT)};
-    const uint32_t box[2] = {uint32_t(128 / sizeof(OutT)), 32};
+    const uint32_t box[2] = {uint32_t(128 / sizeof(OutT)), box_rows};
     if (sizeof(OutT) == 4) encode_tensor_map(&p.map_c, static_cast<const float*>(p.c), 2, dims, strides, box, TmaSwizzle::B128);
     else encode_tensor_map_f16(&p.map_c, p.c, 2, dims, strides, box, TmaSwizzle::B128);
 }
@@ -108,7 +108,7 @@ template <RaggedForm FORM, int BN, class OutT>
 void launch_by_rows_bn(Fp8RowsParams& p, cudaStream_t stream) {
     const DeviceInfo& dev = device_info();
     CB200_REQUIRE(dev.cc_major == 10, "8-bit products need an sm_100 device");
-    set_output<OutT>(p);
+    set_output<OutT>(p, 32);
     p.status = dev.status_word;
     p.wait_limit_ns = 2000000000ull;
     p.tiles_m = (p.rows + 255) / 256;
@@ -154,7 +154,7 @@ void launch_scaled(Fp8RowsParams& rows_form, cudaStream_t stream) {
     launch_dependent(pack_scales_kernel, dim3(SCALE_FLAGS), 256, stream, rows_form.x_scales, p.rows, 2 * p.tiles_m,
                      rows_form.w_scales, (p.features + 127) / 128, 2 * p.tiles_n, rows_form.ws_feature, rows_form.ws_k, k_blocks, xs,
                      ws, odd);
-    set_output<OutT>(p);
+    set_output<OutT>(p, 16);
     const long long tiles = (long long)p.tiles_m * p.tiles_n;
     const long long clusters = tiles < dev.num_sms / 2 ? tiles : dev.num_sms / 2;
     CB200_TRACE("fp8 %s tcgen05, scales in the MMA: rows=%d features=%d k=%d tile=256x256 stages=%d clusters=%lld store=%s",

@@ -20,9 +20,11 @@ constexpr int FP8R_THREADS = 384;               // three groups of four warps
 // Registers per thread: 384 * 168 at launch; 128 * 56 + 256 * 216 = 62464 <= 64512 afterwards.
 constexpr int FP8R_REGS_FEW = 56;
 constexpr int FP8R_REGS_MANY = 216;
-constexpr uint32_t FP8R_STAGE_BYTES = 2 * 128 * 128;
+constexpr int FP8R_ATOMS = 2;                     // K blocks per stage
+constexpr uint32_t FP8R_ATOM_BYTES = 2 * 128 * 128;
+constexpr uint32_t FP8R_STAGE_BYTES = FP8R_ATOMS * FP8R_ATOM_BYTES;
 constexpr uint32_t FP8R_STAGING_BYTES = 8 * 4096;      // 32 rows x 128 bytes per epilogue warp
-constexpr int FP8R_STAGES = 6;
+constexpr int FP8R_STAGES = 3;
 constexpr uint32_t FP8R_SMEM_BYTES = FP8R_STAGES * FP8R_STAGE_BYTES + FP8R_STAGING_BYTES + 1024;
 
 constexpr int SCALE_FLAGS = 256;      // CTAs of pack_scales_kernel (fp8_scaled.cuh), each with a word of its own
@@ -57,41 +59,43 @@ __device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.
 template <int REGS>
 __device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS)); }
 
-// A warp's 32 rows x BN / 2 features: bias, activation, and out through its staging block.
-template <int BN, class OutT, class Params>
+// A warp's 32 rows x BN / 2 features: bias, activation, and out through its staging block of ROWS x 128 bytes (the box of map_c).
+template <int BN, class OutT, int ROWS, class Params>
 __device__ __forceinline__ void store_tile(const Params& p, float (&acc)[BN / 64][32], const Fp8Activation& act, uint32_t staging,
                                            uint32_t lane, int row0, int feature0) {
-    constexpr int COLS = 128 / sizeof(OutT);          // columns of a staged block: 128 bytes per row
+    constexpr int COLS = 128 / sizeof(OutT);          // columns of a staged block
+    constexpr int CHUNKS = COLS / 32;                 // of 32 columns
 #pragma unroll
-    for (int i = 0; i < BN / 64; ++i) {
-        if (p.bias != nullptr) {
+    for (int i0 = 0; i0 < BN / 64; i0 += CHUNKS) {
+        const int f0 = feature0 + 32 * i0;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-                const int f = feature0 + 32 * i + j;
-                acc[i][j] += __ldg(p.bias + min(f, p.features - 1));
+        for (int i = i0; i < i0 + CHUNKS; ++i) {
+            if (p.bias != nullptr) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) acc[i][j] += __ldg(p.bias + min(feature0 + 32 * i + j, p.features - 1));
             }
+            fp8_activation(acc[i], act);
         }
-        fp8_activation(acc[i], act);
-        const int c0 = 32 * i / COLS * COLS;          // first column of the staged block this chunk belongs to
-        if (32 * i == c0) {
+#pragma unroll
+        for (int r0 = 0; r0 < 32; r0 += ROWS) {
             if (lane == 0) ptx::bulk_wait_group_read<0>();      // the block's last store has read it
             __syncwarp();
-        }
-        stage_block<OutT>(staging, lane, 32 * i - c0, acc[i]);
-        if (32 * (i + 1) - c0 == COLS) {              // the block is full
-            const int f0 = feature0 + c0;
+            if (ROWS == 32 || int(lane) / ROWS == r0 / ROWS) {
+#pragma unroll
+                for (int i = i0; i < i0 + CHUNKS; ++i) stage_block<OutT>(staging, lane % ROWS, 32 * (i - i0), acc[i]);
+            }
             if (p.tma_store) {
                 ptx::fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0 && row0 < p.rows && f0 < p.features) {
-                    ptx::tma_store_2d(&p.map_c, staging, f0, row0);
+                if (lane == 0 && row0 + r0 < p.rows && f0 < p.features) {
+                    ptx::tma_store_2d(&p.map_c, staging, f0, row0 + r0);
                     ptx::bulk_commit_group();
                 }
             } else {
                 // Rows of C that are no 16-byte multiples: the warp writes them one by one.
                 __syncwarp();
-                OutT* dst = static_cast<OutT*>(p.c) + (long long)row0 * p.features + f0;
-                write_block<OutT>(staging, lane, dst, p.features, min(32, p.rows - row0), p.features - f0, false);
+                OutT* dst = static_cast<OutT*>(p.c) + (long long)(row0 + r0) * p.features + f0;
+                write_block<OutT>(staging, lane, dst, p.features, min(ROWS, p.rows - row0 - r0), p.features - f0, false);
             }
         }
     }
@@ -104,7 +108,7 @@ __global__ void __launch_bounds__(FP8R_THREADS, 1) fp8_rows_kernel(const __grid_
     constexpr bool B_MN = FORM == RaggedForm::NN;
     static_assert(BN == 256 || (BN == 128 && !B_MN), "a row of features in a box is one 128-byte swizzle row");
     constexpr int CHUNKS = BN / 32;      // of 16 columns, per epilogue warp (half of the tile's columns)
-    constexpr uint32_t TX_BYTES = 2 * 16384 + BN * 128;
+    constexpr uint32_t TX_BYTES = FP8R_ATOMS * (2 * 16384 + BN * 128);
 
     if (p.odd_scales != nullptr) {
         ptx::grid_dependency_wait();
@@ -169,16 +173,19 @@ __global__ void __launch_bounds__(FP8R_THREADS, 1) fp8_rows_kernel(const __grid_
                     raster_coords(u, p.tiles_m, p.tiles_n, 8, tm, tn);
                     const int row = (tm * 2 + int(cta_rank)) * 128;
                     const int feature = tn * BN + int(cta_rank) * (BN / 2);
-                    for (int kb = 0; kb < k_blocks; ++kb) {
+                    for (int kb = 0; kb < k_blocks; kb += FP8R_ATOMS) {
                         if (!ptx::mbar_wait(ptx::smem_u32(&bar_empty[stage]), phase ^ 1u, wctx, UMMA_TIMEOUT_PRODUCER))
                             goto producer_done;
-                        const uint32_t a_smem = smem_base + stage * FP8R_STAGE_BYTES;
                         const uint32_t full_local = ptx::smem_u32(&bar_full[stage]);
                         if (is_leader) ptx::mbar_arrive_expect_tx(full_local, TX_BYTES);
                         const uint32_t full = ptx::mapa(full_local, 0);
-                        const int k0 = kb * FP8_BK;
-                        ptx::tma_load_2d_pair(a_smem, &p.map_x, full, k0, row);
-                        ptx::tma_load_2d_pair(a_smem + 16384, &p.map_w, full, B_MN ? feature : k0, B_MN ? k0 : feature);
+#pragma unroll
+                        for (int a = 0; a < FP8R_ATOMS; ++a) {      // a block behind the last one loads as zeros
+                            const uint32_t a_smem = smem_base + stage * FP8R_STAGE_BYTES + a * FP8R_ATOM_BYTES;
+                            const int k0 = (kb + a) * FP8_BK;
+                            ptx::tma_load_2d_pair(a_smem, &p.map_x, full, k0, row);
+                            ptx::tma_load_2d_pair(a_smem + 16384, &p.map_w, full, B_MN ? feature : k0, B_MN ? k0 : feature);
+                        }
                         if (++stage == FP8R_STAGES) { stage = 0; phase ^= 1u; }
                     }
                 }
@@ -196,29 +203,32 @@ __global__ void __launch_bounds__(FP8R_THREADS, 1) fp8_rows_kernel(const __grid_
             for (int u = first_unit; u < num_units; u += unit_stride) {
                 for (int kb = 0; kb < k_blocks; ++kb, ++it) {
                     const uint32_t acc = it & 1;
-                    if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&bar_full[stage]), phase, wctx,
-                                                                UMMA_TIMEOUT_MMA_FULL)))
+                    const uint32_t atom = uint32_t(kb) % FP8R_ATOMS;
+                    if (atom == 0 && !__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&bar_full[stage]), phase, wctx,
+                                                                             UMMA_TIMEOUT_MMA_FULL)))
                         goto mma_done;
                     if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&bar_acc_empty[acc]), ((it >> 1) & 1) ^ 1u,
                                                                 wctx, UMMA_TIMEOUT_MMA_ACC)))
                         goto mma_done;
                     ptx::tc_fence_after();
+                    const bool stage_done = atom + 1 == FP8R_ATOMS || kb + 1 == k_blocks;
                     if (ptx::elect_one()) {
-                        const uint64_t a_stage = a_desc0 + ((stage * FP8R_STAGE_BYTES) >> 4);
-                        const uint64_t b_stage = b_desc0 + ((stage * FP8R_STAGE_BYTES) >> 4);
+                        const uint64_t offset = (stage * FP8R_STAGE_BYTES + atom * FP8R_ATOM_BYTES) >> 4;
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
-                            ptx::umma_f8<2>(tmem_base + acc * 256u, a_stage + ((kk * 32u) >> 4),
-                                            b_stage + ((kk * B_KSTEP) >> 4), idesc, kk != 0);
+                            ptx::umma_f8<2>(tmem_base + acc * 256u, a_desc0 + offset + ((kk * 32u) >> 4),
+                                            b_desc0 + offset + ((kk * B_KSTEP) >> 4), idesc, kk != 0);
                         const uint32_t accf_local = ptx::smem_u32(&bar_acc_full[acc]);
                         ptx::umma_commit<2>(accf_local);
                         ptx::umma_commit<2>(ptx::mapa(accf_local, 1));
-                        const uint32_t empty_local = ptx::smem_u32(&bar_empty[stage]);
-                        ptx::umma_commit<2>(empty_local);
-                        ptx::umma_commit<2>(ptx::mapa(empty_local, 1));
+                        if (stage_done) {
+                            const uint32_t empty_local = ptx::smem_u32(&bar_empty[stage]);
+                            ptx::umma_commit<2>(empty_local);
+                            ptx::umma_commit<2>(ptx::mapa(empty_local, 1));
+                        }
                     }
                     __syncwarp();
-                    if (++stage == FP8R_STAGES) { stage = 0; phase ^= 1u; }
+                    if (stage_done && ++stage == FP8R_STAGES) { stage = 0; phase ^= 1u; }
                 }
             }
         mma_done:
@@ -295,7 +305,7 @@ __global__ void __launch_bounds__(FP8R_THREADS, 1) fp8_rows_kernel(const __grid_
                 ++it;
               }
             }
-            store_tile<BN, OutT>(p, acc, act, staging, lane, row0, feature0);
+            store_tile<BN, OutT, 32>(p, acc, act, staging, lane, row0, feature0);
         }
     epilogue_done:
         __syncwarp();

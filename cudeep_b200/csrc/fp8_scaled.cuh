@@ -17,16 +17,18 @@
 
 namespace cudeep_b200 {
 
-constexpr int FP8S_STAGES = 5;
-constexpr uint32_t FP8S_SCALE_BYTES = 3 * 512;         // of a stage: 128 rows, 256 features
-constexpr uint32_t FP8S_SMEM_BYTES = FP8S_STAGES * (FP8R_STAGE_BYTES + FP8S_SCALE_BYTES) + FP8R_STAGING_BYTES + 1024;
+constexpr int FP8S_STAGES = 3;
+constexpr uint32_t FP8S_SCALE_BYTES = 3 * 512;         // of a K block: 128 rows, 256 features
+constexpr uint32_t FP8S_STAGING_BYTES = 8 * 2048;      // 16 rows x 128 bytes per epilogue warp: what three stages of two blocks leave
+constexpr uint32_t FP8S_SMEM_BYTES =
+    FP8S_STAGES * (FP8R_STAGE_BYTES + FP8R_ATOMS * FP8S_SCALE_BYTES) + FP8S_STAGING_BYTES + 1024;
 
 struct Fp8ScaledParams {
     CUtensorMap map_x;       // {K, rows} box {128, 128}
     CUtensorMap map_w;       // NT {K, F}, NN {F, K}: box {128, 128}
     CUtensorMap map_xs;      // packed scales {16, 32 * tiles of 128 rows * K blocks}, box {16, 32}
     CUtensorMap map_ws;      // ... of W, box {16, 64}
-    CUtensorMap map_c;
+    CUtensorMap map_c;       // {F, rows} box {128 bytes, 16}
     const float* bias;
     int act;
     void* c;
@@ -94,7 +96,7 @@ __global__ void __launch_bounds__(FP8R_THREADS, 1) fp8_scaled_kernel(const __gri
     const bool is_leader = cta_rank == 0;
     const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t smem_staging = smem_base + FP8S_STAGES * FP8R_STAGE_BYTES;      // swizzled blocks: 1024-byte aligned
-    const uint32_t smem_scales = smem_staging + FP8R_STAGING_BYTES;
+    const uint32_t smem_scales = smem_staging + FP8S_STAGING_BYTES;
     ptx::WaitCtx wctx{&abort_flag, p.status, p.wait_limit_ns};
 
     if (threadIdx.x == 0) {
@@ -140,20 +142,25 @@ __global__ void __launch_bounds__(FP8R_THREADS, 1) fp8_scaled_kernel(const __gri
                     raster_coords(u, p.tiles_m, p.tiles_n, 8, tm, tn);
                     const int row = (tm * 2 + int(cta_rank)) * 128;
                     const int feature = tn * 256 + int(cta_rank) * 128;
-                    for (int kb = 0; kb < k_blocks; ++kb) {
+                    for (int kb = 0; kb < k_blocks; kb += FP8R_ATOMS) {
                         if (!ptx::mbar_wait(ptx::smem_u32(&bar_empty[stage]), phase ^ 1u, wctx, UMMA_TIMEOUT_PRODUCER))
                             goto producer_done;
-                        const uint32_t a_smem = smem_base + stage * FP8R_STAGE_BYTES;
-                        const uint32_t s_smem = smem_scales + stage * FP8S_SCALE_BYTES;
                         const uint32_t full_local = ptx::smem_u32(&bar_full[stage]);
-                        if (is_leader) ptx::mbar_arrive_expect_tx(full_local, 2 * (FP8R_STAGE_BYTES + FP8S_SCALE_BYTES));
+                        if (is_leader)
+                            ptx::mbar_arrive_expect_tx(full_local, 2 * (FP8R_STAGE_BYTES + FP8R_ATOMS * FP8S_SCALE_BYTES));
                         const uint32_t full = ptx::mapa(full_local, 0);
-                        const int k0 = kb * FP8_BK;
-                        ptx::tma_load_2d_pair(a_smem, &p.map_x, full, k0, row);
-                        ptx::tma_load_2d_pair(a_smem + 16384, &p.map_w, full, B_MN ? feature : k0, B_MN ? k0 : feature);
-                        // Each CTA needs the scales of its own rows and of all 256 features.
-                        ptx::tma_load_2d_pair(s_smem, &p.map_xs, full, 0, (kb * 2 * p.tiles_m + tm * 2 + int(cta_rank)) * 32);
-                        ptx::tma_load_2d_pair(s_smem + 512, &p.map_ws, full, 0, (kb * 2 * p.tiles_n + tn * 2) * 32);
+#pragma unroll
+                        for (int a = 0; a < FP8R_ATOMS; ++a) {      // a block behind the last one loads as zeros
+                            const uint32_t a_smem = smem_base + stage * FP8R_STAGE_BYTES + a * FP8R_ATOM_BYTES;
+                            const uint32_t s_smem = smem_scales + (stage * FP8R_ATOMS + a) * FP8S_SCALE_BYTES;
+                            const int k0 = (kb + a) * FP8_BK;
+                            ptx::tma_load_2d_pair(a_smem, &p.map_x, full, k0, row);
+                            ptx::tma_load_2d_pair(a_smem + 16384, &p.map_w, full, B_MN ? feature : k0, B_MN ? k0 : feature);
+                            // Each CTA needs the scales of its own rows and of all 256 features.
+                            ptx::tma_load_2d_pair(s_smem, &p.map_xs, full, 0,
+                                                  ((kb + a) * 2 * p.tiles_m + tm * 2 + int(cta_rank)) * 32);
+                            ptx::tma_load_2d_pair(s_smem + 512, &p.map_ws, full, 0, ((kb + a) * 2 * p.tiles_n + tn * 2) * 32);
+                        }
                         if (++stage == FP8S_STAGES) { stage = 0; phase ^= 1u; }
                     }
                 }
@@ -173,38 +180,42 @@ __global__ void __launch_bounds__(FP8R_THREADS, 1) fp8_scaled_kernel(const __gri
                 for (int kb = 0; kb < k_blocks; ++kb) {
                     const bool first = kb % p.chunk_blocks == 0;
                     const bool last = kb + 1 == k_blocks || (kb + 1) % p.chunk_blocks == 0;
-                    if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&bar_full[stage]), phase, wctx,
-                                                                UMMA_TIMEOUT_MMA_FULL)))
+                    const uint32_t atom = uint32_t(kb) % FP8R_ATOMS;
+                    const bool stage_done = atom + 1 == FP8R_ATOMS || kb + 1 == k_blocks;
+                    if (atom == 0 && !__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&bar_full[stage]), phase, wctx,
+                                                                             UMMA_TIMEOUT_MMA_FULL)))
                         goto mma_done;
                     if (first && !__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&bar_acc_empty), (it & 1) ^ 1u, wctx,
                                                                          UMMA_TIMEOUT_MMA_ACC)))
                         goto mma_done;
                     ptx::tc_fence_after();
                     if (ptx::elect_one()) {
-                        const uint64_t a_stage = a_desc0 + ((stage * FP8R_STAGE_BYTES) >> 4);
-                        const uint64_t b_stage = b_desc0 + ((stage * FP8R_STAGE_BYTES) >> 4);
-                        const uint64_t s_stage = s_desc0 + ((stage * FP8S_SCALE_BYTES) >> 4);
-                        // Columns 256 on: 4 for the scales of the rows, 8 for those of the features; each stage its own.
-                        const uint32_t s_tmem = tmem_base + 256u + stage * 16u;
-                        ptx::tmem_cp_32x128b_pair(s_tmem, s_stage);
-                        ptx::tmem_cp_32x128b_pair(s_tmem + 4, s_stage + (512u >> 4));
-                        ptx::tmem_cp_32x128b_pair(s_tmem + 8, s_stage + (1024u >> 4));
+                        const uint64_t offset = (stage * FP8R_STAGE_BYTES + atom * FP8R_ATOM_BYTES) >> 4;
+                        const uint64_t s_block = s_desc0 + (((stage * FP8R_ATOMS + atom) * FP8S_SCALE_BYTES) >> 4);
+                        // Columns 256 on: 4 for the scales of the rows, 8 for those of the features; each block of the ring its own.
+                        const uint32_t s_tmem = tmem_base + 256u + (stage * FP8R_ATOMS + atom) * 16u;
+                        ptx::tmem_cp_32x128b_pair(s_tmem, s_block);
+                        ptx::tmem_cp_32x128b_pair(s_tmem + 4, s_block + (512u >> 4));
+                        ptx::tmem_cp_32x128b_pair(s_tmem + 8, s_block + (1024u >> 4));
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
-                            ptx::umma_mxf8<2>(tmem_base, a_stage + ((kk * 32u) >> 4), b_stage + ((kk * B_KSTEP) >> 4), idesc, s_tmem,
-                                              s_tmem + 4, !(first && kk == 0));
+                            ptx::umma_mxf8<2>(tmem_base, a_desc0 + offset + ((kk * 32u) >> 4),
+                                              b_desc0 + offset + ((kk * B_KSTEP) >> 4), idesc, s_tmem, s_tmem + 4,
+                                              !(first && kk == 0));
                         if (last) {
                             const uint32_t accf_local = ptx::smem_u32(&bar_acc_full);
                             ptx::umma_commit<2>(accf_local);
                             ptx::umma_commit<2>(ptx::mapa(accf_local, 1));
                         }
-                        const uint32_t empty_local = ptx::smem_u32(&bar_empty[stage]);
-                        ptx::umma_commit<2>(empty_local);
-                        ptx::umma_commit<2>(ptx::mapa(empty_local, 1));
+                        if (stage_done) {
+                            const uint32_t empty_local = ptx::smem_u32(&bar_empty[stage]);
+                            ptx::umma_commit<2>(empty_local);
+                            ptx::umma_commit<2>(ptx::mapa(empty_local, 1));
+                        }
                     }
                     __syncwarp();
                     if (last) ++it;
-                    if (++stage == FP8S_STAGES) { stage = 0; phase ^= 1u; }
+                    if (stage_done && ++stage == FP8S_STAGES) { stage = 0; phase ^= 1u; }
                 }
             }
         mma_done:
@@ -216,7 +227,7 @@ __global__ void __launch_bounds__(FP8R_THREADS, 1) fp8_scaled_kernel(const __gri
         // ------------------------------------------------------------ sums and epilogue
         const uint32_t quarter = warp & 3u;
         const int half = int(warp - 4) >> 2;
-        const uint32_t staging = smem_staging + (warp - 4) * 4096u;
+        const uint32_t staging = smem_staging + (warp - 4) * 2048u;
         const uint32_t t_row = tmem_base + uint32_t(half) * 128u + ((quarter * 32u) << 16);
         const Fp8Activation act(p.act);
         uint32_t it = 0;
@@ -255,7 +266,7 @@ __global__ void __launch_bounds__(FP8R_THREADS, 1) fp8_scaled_kernel(const __gri
                     for (int j = 0; j < 16; ++j) acc[i >> 1][(i & 1) * 16 + j] += __uint_as_float(r[i & 1][j]);
                 }
             }
-            store_tile<256, OutT>(p, acc, act, staging, lane, row0, feature0);
+            store_tile<256, OutT, 16>(p, acc, act, staging, lane, row0, feature0);
         }
     epilogue_done:
         __syncwarp();

@@ -37,15 +37,19 @@ void launch(RaggedParams& p, const RaggedPlan& plan, cudaStream_t stream) {
     const DeviceInfo& dev = device_info();
     CB200_REQUIRE(dev.cc_major == 10, "grouped products need an sm_100 device");
     p.tile_cols = plan.tile_cols;
-    p.stage_bytes = RAGGED_A_BYTES + uint32_t(RowMaps::loaded(plan.tile_cols / CTAS)) * 128u;
-    const uint32_t staging_bytes = FORM == RaggedForm::TN ? RAGGED_STAGING_BYTES : 0u;
-    const int fit = int((RAGGED_SMEM_BUDGET - staging_bytes) / p.stage_bytes);
+    p.atom_bytes = RAGGED_A_BYTES + uint32_t(RowMaps::loaded(plan.tile_cols / CTAS)) * 128u;
+    const uint32_t fixed = (FORM == RaggedForm::TN ? RAGGED_STAGING_BYTES : 0u) + ragged_table_bytes(p.groups);
+    // As many K blocks to a stage, and so to a barrier, as leave three stages; more than two gain nothing.
+    p.atoms = int((RAGGED_SMEM_BUDGET - fixed) / 3 / p.atom_bytes);
+    p.atoms = p.atoms < 1 ? 1 : p.atoms > 2 ? 2 : p.atoms;
+    p.stage_bytes = p.atoms * p.atom_bytes;
+    const int fit = int((RAGGED_SMEM_BUDGET - fixed) / p.stage_bytes);
     p.stages = fit < RAGGED_MAX_STAGES ? fit : RAGGED_MAX_STAGES;
     p.status = dev.status_word;
     p.wait_limit_ns = 2000000000ull;
     long long clusters = dev.num_sms / CTAS;
     if (clusters > plan.units) clusters = plan.units;
-    const uint32_t smem_bytes = uint32_t(p.stages) * p.stage_bytes + staging_bytes + 1024;
+    const uint32_t smem_bytes = uint32_t(p.stages) * p.stage_bytes + fixed + 1024;
     CB200_TRACE("grouped %s %s tcgen05: rows=%d groups=%d features=%d %s=%d tile=%dx%d stages=%d clusters=%lld",
                 FORM == RaggedForm::NT ? "nt" : FORM == RaggedForm::NN ? "nn" : "tn", BF16 ? "bf16" : "f16", p.rows, p.groups,
                 p.features, FORM == RaggedForm::TN ? "cols" : "k", FORM == RaggedForm::TN ? p.cols : p.k, 128 * CTAS,

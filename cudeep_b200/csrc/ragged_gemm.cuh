@@ -36,10 +36,14 @@ constexpr int RAGGED_BK = 64;                        // 16-bit elements per K bl
 // Epilogue warps: with four, a gradient tile of 512 summed rows took longer to leave than to compute.
 __host__ __device__ constexpr int ragged_epilogue_warps(RaggedForm) { return 8; }
 __host__ __device__ constexpr int ragged_threads(RaggedForm form) { return 64 + 32 * ragged_epilogue_warps(form); }
-constexpr uint32_t RAGGED_STAGING_BYTES = 8 * 2 * 4096;   // TN: two blocks of 32 rows x 128 bytes per epilogue warp
+// TN: a block of 32 rows x 128 bytes for each epilogue warp.  A second one would cost the third stage of two K blocks (8192 x
+// 4096 x 4096: 232 us instead of 211).
+constexpr uint32_t RAGGED_STAGING_BYTES = 8 * 4096;
+// First and last row of each group, and the tiles before it, behind everything else in shared memory.
+__host__ __device__ constexpr uint32_t ragged_table_bytes(int groups) { return uint32_t(3 * groups + 1) * 4u; }
 constexpr uint32_t RAGGED_A_BYTES = 128 * 128;       // one CTA's features of a K block
 constexpr int RAGGED_MAX_STAGES = 12;
-constexpr uint32_t RAGGED_SMEM_BUDGET = 232448 - 1024 - 13 * 1024;   // minus alignment slack, group tables and barriers
+constexpr uint32_t RAGGED_SMEM_BUDGET = 232448 - 1024 - 512;   // minus alignment slack and barriers
 constexpr uint32_t UMMA_BAD_OFFSETS = 6;             // status word: the offsets decrease or leave [0, rows]
 
 // Rows of a matrix as K blocks of 128 bytes.  One box brings all rows that a CTA stages for a tile, up to 128, rounded up to a
@@ -84,6 +88,9 @@ struct RaggedParams {
     int tile_cols;           // columns of a tile at most: rows of a group (NT, NN) or C (TN); <= 256
     int stages;
     uint32_t stage_bytes;
+    // K blocks per stage, atom_bytes apart.  Two to a barrier instead of one: 8192 x 4096 x 4096 nt 214 -> 187 us.
+    int atoms;
+    uint32_t atom_bytes;
     int chunk_rows;          // TN: rows summed in the tensor core's accumulator before they are added into C
     const float* col_scale;  // TN: nullptr, or a factor for each 128 columns of C
     uint32_t* status;
@@ -264,14 +271,15 @@ __global__ void __launch_bounds__(ragged_threads(FORM), 1) ragged_gemm_kernel(co
     __shared__ __align__(8) uint64_t bar_acc_empty[2];
     __shared__ uint32_t tmem_base_holder;
     __shared__ uint32_t abort_flag;
-    __shared__ int group_rows[2 * RAGGED_MAX_GROUPS];      // first and last row of each group
-    __shared__ int group_start[RAGGED_MAX_GROUPS + 1];     // tiles before each group
 
     const uint32_t warp = threadIdx.x >> 5;
     const uint32_t lane = threadIdx.x & 31;
     const uint32_t cta_rank = CTAS == 2 ? ptx::cluster_ctarank() : 0u;
     const bool is_leader = cta_rank == 0;
     const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
+    int* group_rows = reinterpret_cast<int*>(smem_raw + (smem_base - ptx::smem_u32(smem_raw)) +
+                                             uint32_t(p.stages) * p.stage_bytes + (FORM == RaggedForm::TN ? RAGGED_STAGING_BYTES : 0u));
+    int* group_start = group_rows + 2 * p.groups;
     ptx::WaitCtx wctx{&abort_flag, p.status, p.wait_limit_ns};
 
     if (threadIdx.x == 0) {
@@ -342,39 +350,43 @@ __global__ void __launch_bounds__(ragged_threads(FORM), 1) ragged_gemm_kernel(co
                     ptx::tensormap_acquire(map_b);
                 }
             }
-            for (int kb = 0; kb < blocks; ++kb) {
+            for (int kb = 0; kb < blocks; kb += p.atoms) {
                 const bool ok = ptx::mbar_wait(ptx::smem_u32(&bar_empty[stage]), phase ^ 1u, wctx, UMMA_TIMEOUT_PRODUCER);
                 if (!__all_sync(0xffffffffu, ok)) goto producer_done;
-                const uint32_t a_smem = smem_base + stage * p.stage_bytes;
-                const uint32_t b_smem = a_smem + RAGGED_A_BYTES;
                 const uint32_t full_local = ptx::smem_u32(&bar_full[stage]);
                 const uint32_t full = CTAS == 2 ? ptx::mapa(full_local, 0) : full_local;
-                const uint32_t bytes = RAGGED_A_BYTES + uint32_t(FORM == RaggedForm::TN ? per : RowMaps::loaded(per)) * 128u;
+                const uint32_t atom = RAGGED_A_BYTES + uint32_t(FORM == RaggedForm::TN ? per : RowMaps::loaded(per)) * 128u;
                 if (lane == 0) {
-                    const int k0 = kb * RAGGED_BK;
-                    if constexpr (FORM == RaggedForm::NT) {
-                        if constexpr (CTAS == 2) ptx::tma_load_3d_pair(a_smem, &p.map_a, full, k0, feature, t.group);
-                        else ptx::tma_load_3d(a_smem, &p.map_a, full, k0, feature, t.group);
-                    } else if constexpr (FORM == RaggedForm::NN) {
-                        if (p.a_chunked) {
-                            if constexpr (CTAS == 2) ptx::tma_load_4d_pair(a_smem, &p.map_a, full, 0, k0, feature / 64, t.group);
-                            else ptx::tma_load_4d(a_smem, &p.map_a, full, 0, k0, feature / 64, t.group);
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 2; ++j) {
+                    // Blocks behind the last one load as zeros or are not multiplied.
+                    for (int a = 0; a < p.atoms; ++a) {
+                        const uint32_t a_smem = smem_base + stage * p.stage_bytes + a * p.atom_bytes;
+                        const uint32_t b_smem = a_smem + RAGGED_A_BYTES;
+                        const int k0 = (kb + a) * RAGGED_BK;
+                        if constexpr (FORM == RaggedForm::NT) {
+                            if constexpr (CTAS == 2) ptx::tma_load_3d_pair(a_smem, &p.map_a, full, k0, feature, t.group);
+                            else ptx::tma_load_3d(a_smem, &p.map_a, full, k0, feature, t.group);
+                        } else if constexpr (FORM == RaggedForm::NN) {
+                            if (p.a_chunked) {
                                 if constexpr (CTAS == 2)
-                                    ptx::tma_load_3d_pair(a_smem + j * 8192, &p.map_a, full, feature + j * 64, k0, t.group);
+                                    ptx::tma_load_4d_pair(a_smem, &p.map_a, full, 0, k0, feature / 64, t.group);
                                 else
-                                    ptx::tma_load_3d(a_smem + j * 8192, &p.map_a, full, feature + j * 64, k0, t.group);
+                                    ptx::tma_load_4d(a_smem, &p.map_a, full, 0, k0, feature / 64, t.group);
+                            } else {
+#pragma unroll
+                                for (int j = 0; j < 2; ++j) {
+                                    if constexpr (CTAS == 2)
+                                        ptx::tma_load_3d_pair(a_smem + j * 8192, &p.map_a, full, feature + j * 64, k0, t.group);
+                                    else
+                                        ptx::tma_load_3d(a_smem + j * 8192, &p.map_a, full, feature + j * 64, k0, t.group);
+                                }
                             }
+                        } else {
+                            load_columns<CTAS>(a_smem, map_a, p.a_chunked, 2, full, feature, t.row0 + k0);
+                            load_columns<CTAS>(b_smem, map_b, p.b_chunked, per / 64, full, col, t.row0 + k0);
                         }
-                    } else {
-                        load_columns<CTAS>(a_smem, map_a, p.a_chunked, 2, full, feature, t.row0 + k0);
-                        load_columns<CTAS>(b_smem, map_b, p.b_chunked, per / 64, full, col, t.row0 + k0);
+                        if constexpr (FORM != RaggedForm::TN) p.x.template load<CTAS>(b_smem, full, k0, col, per);
                     }
-                    if constexpr (FORM != RaggedForm::TN) p.x.template load<CTAS>(b_smem, full, k0, col, per);
-                }
-                if (lane == 0) {
+                    const uint32_t bytes = uint32_t(p.atoms) * atom;
                     if (is_leader) ptx::mbar_arrive_expect_tx(full_local, bytes);
                     else ptx::mbar_arrive_expect_tx_cluster_relaxed(full, bytes);
                 }
@@ -412,7 +424,7 @@ __global__ void __launch_bounds__(ragged_threads(FORM), 1) ragged_gemm_kernel(co
                     ptx::tc_fence_after();
                     const uint32_t d_tmem = tmem_base + acc * 256u;
                     bool ready = __all_sync(0xffffffffu, ptx::mbar_test(ptx::smem_u32(&bar_full[stage]), phase));
-                    for (int kb = 0; kb < blocks; ++kb) {
+                    for (int kb = 0; kb < blocks; kb += p.atoms) {
                         if (!ready &&
                             !__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&bar_full[stage]), phase, wctx,
                                                                     UMMA_TIMEOUT_MMA_FULL)))
@@ -421,21 +433,25 @@ __global__ void __launch_bounds__(ragged_threads(FORM), 1) ragged_gemm_kernel(co
                         uint32_t next_stage = stage + 1, next_phase = phase;
                         if (next_stage == uint32_t(p.stages)) { next_stage = 0; next_phase ^= 1u; }
                         ready = __all_sync(0xffffffffu, ptx::mbar_test(ptx::smem_u32(&bar_full[next_stage]), next_phase));
-                        int steps = 4;
-                        if (FORM == RaggedForm::TN) steps = min(4, (t.row1 - row - kb * RAGGED_BK + 15) / 16);
                         if (ptx::elect_one()) {
                             const uint64_t a_stage = a_desc0 + ((stage * p.stage_bytes) >> 4);
                             const uint64_t b_stage = b_desc0 + ((stage * p.stage_bytes) >> 4);
+                            for (int a = 0; a < p.atoms; ++a) {
+                                int steps = kb + a < blocks ? 4 : 0;
+                                if (FORM == RaggedForm::TN)
+                                    steps = max(0, min(steps, (t.row1 - row - (kb + a) * RAGGED_BK + 15) / 16));
+                                const uint64_t offset = (a * p.atom_bytes) >> 4;
 #pragma unroll
-                            for (int kk = 0; kk < 4; ++kk)
-                                if (kk < steps)
-                                    ptx::umma_f16<CTAS>(d_tmem, a_stage + ((kk * (A_MN ? KSTEP_MN : KSTEP_K)) >> 4),
-                                                        b_stage + ((kk * (B_MN ? KSTEP_MN : KSTEP_K)) >> 4), idesc,
-                                                        (kb | kk) != 0);
+                                for (int kk = 0; kk < 4; ++kk)
+                                    if (kk < steps)
+                                        ptx::umma_f16<CTAS>(d_tmem, a_stage + offset + ((kk * (A_MN ? KSTEP_MN : KSTEP_K)) >> 4),
+                                                            b_stage + offset + ((kk * (B_MN ? KSTEP_MN : KSTEP_K)) >> 4), idesc,
+                                                            (kb | a | kk) != 0);
+                            }
                             const uint32_t empty_local = ptx::smem_u32(&bar_empty[stage]);
                             ptx::umma_commit<CTAS>(empty_local);
                             if constexpr (CTAS == 2) ptx::umma_commit<CTAS>(ptx::mapa(empty_local, 1));
-                            if (kb + 1 == blocks) {
+                            if (kb + p.atoms >= blocks) {
                                 const uint32_t accf_local = ptx::smem_u32(&bar_acc_full[acc]);
                                 ptx::umma_commit<CTAS>(accf_local);
                                 if constexpr (CTAS == 2) ptx::umma_commit<CTAS>(ptx::mapa(accf_local, 1));
@@ -456,7 +472,6 @@ __global__ void __launch_bounds__(ragged_threads(FORM), 1) ragged_gemm_kernel(co
     } else {
         // ------------------------------------------------------------ epilogue
         const uint32_t quarter = warp & 3u;
-        uint32_t block_turn = 0;      // TN
         int it = 0;
         for (int u = first_unit; u < num_units; u += unit_stride) {
             const RaggedTile t = walk.at(u);
@@ -465,7 +480,8 @@ __global__ void __launch_bounds__(ragged_threads(FORM), 1) ragged_gemm_kernel(co
                 // later chunks of an FP32 gradient by a tensor reduction, an FP32 addition in L2; each element has this one
                 // writer, in order), or, where rows of C are no 16-byte multiples, row by row.
                 const int feature_w = t.feature0 + int(cta_rank) * 128 + int(quarter) * 32;
-                const uint32_t staging = smem_base + uint32_t(p.stages) * p.stage_bytes + (warp - 2) * 8192u;
+                const uint32_t staging =
+                    smem_base + uint32_t(p.stages) * p.stage_bytes + (warp - 2) * 4096u;
                 constexpr int COLS = 128 / sizeof(OutT);
                 const int c_begin = (int(warp - 2) >> 2) * (t.umma_n / 2);      // warps 6..9 take the second half of the columns
                 const int c_end = min(t.col_count, c_begin + t.umma_n / 2);
@@ -482,7 +498,6 @@ __global__ void __launch_bounds__(ragged_threads(FORM), 1) ragged_gemm_kernel(co
                     if (add && lane == 0) ptx::bulk_wait_group<0>();      // the chunk before has arrived in C
                     __syncwarp();
                     const uint32_t t_row = tmem_base + acc * 256u + ((quarter * 32u) << 16);
-                    uint32_t block = staging;
                     for (int c = c_begin; c < c_end; c += 32) {
                         uint32_t r[32];
                         if (any) {
@@ -494,30 +509,28 @@ __global__ void __launch_bounds__(ragged_threads(FORM), 1) ragged_gemm_kernel(co
                         }
                         const float scale = p.col_scale != nullptr ? __ldg(p.col_scale + (t.col0 + c) / 128) : 1.0f;
                         const int c0 = c / COLS * COLS;
-                        if (c == c0) {      // the two blocks take turns: the store before the last has read this one
-                            block = staging + (block_turn++ & 1u) * 4096u;
-                            if (lane == 0) ptx::bulk_wait_group_read<1>();
+                        if (c == c0) {      // the last store has read the block
+                            if (lane == 0) ptx::bulk_wait_group_read<0>();
                             __syncwarp();
                         }
                         float v[32];
 #pragma unroll
                         for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) * scale;
-                        stage_block<OutT>(block, lane, c - c0, v);
+                        stage_block<OutT>(staging, lane, c - c0, v);
                         if (c + 32 - c0 == COLS || c + 32 >= c_end) {
                             if (p.tma_store) {
                                 ptx::fence_proxy_async_smem();
                                 __syncwarp();
-                                if (lane == 0) {
-                                    if (feature_w >= p.features) {      // nothing to write, but a group of stores all the same
-                                    } else if (add) ptx::tma_reduce_add_3d(&p.map_c, block, t.col0 + c0, feature_w, t.group);
-                                    else ptx::tma_store_3d(&p.map_c, block, t.col0 + c0, feature_w, t.group);
+                                if (lane == 0 && feature_w < p.features) {
+                                    if (add) ptx::tma_reduce_add_3d(&p.map_c, staging, t.col0 + c0, feature_w, t.group);
+                                    else ptx::tma_store_3d(&p.map_c, staging, t.col0 + c0, feature_w, t.group);
                                     ptx::bulk_commit_group();
                                 }
                             } else {
                                 __syncwarp();
                                 OutT* dst = static_cast<OutT*>(p.c) +
                                             ((long long)t.group * p.features + feature_w) * p.ldc + t.col0 + c0;
-                                write_block<OutT>(block, lane, dst, p.ldc, min(32, p.features - feature_w), c_end - c0, add);
+                                write_block<OutT>(staging, lane, dst, p.ldc, min(32, p.features - feature_w), c_end - c0, add);
                             }
                         }
                     }
