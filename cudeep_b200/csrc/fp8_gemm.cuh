@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(FP8F_THREADS, 1) fp8_few_kernel(const __grid_c
                     if (16 * i < c_count) {
                         uint32_t r[16];
                         ptx::tmem_ld_32x16(t_row + 16 * i, r);
-                        ptx::tmem_ld_wait();
+                        ptx::tmem_ld_wait(r);
 #pragma unroll
                         for (int j = 0; j < 16; j += 4) {
                             const float4 sc = *reinterpret_cast<const float4*>(f + 16 * i + j);

@@ -267,43 +267,43 @@ __global__ void __launch_bounds__(FP8R_THREADS, 1) fp8_rows_kernel(const __grid_
 #pragma unroll 1
             for (int kb4 = 0; kb4 < k_blocks; kb4 += 4) {
 #pragma unroll
-              for (int d = 0; d < 4; ++d) {
-                const int kb = kb4 + d;
-                if (kb >= k_blocks) break;
-                const float s = px[d] * pw[d];
-                if (kb + 4 < k_blocks) {
-                    px[d] = __ldg(xs + (long long)(kb + 4) * p.rows);
-                    pw[d] = __ldg(ws + (kb + 4) * p.ws_k);
-                }
-                const uint32_t buf = it & 1;
-                const bool ok = ptx::mbar_wait(ptx::smem_u32(&bar_acc_full[buf]), (it >> 1) & 1, wctx, UMMA_TIMEOUT_EPILOGUE);
-                if (!__all_sync(0xffffffffu, ok)) goto epilogue_done;
-                ptx::tc_fence_after();
-                const uint32_t t_row = tmem_base + buf * 256u + uint32_t(half) * uint32_t(BN / 2) + ((quarter * 32u) << 16);
-                uint32_t r[2][16];
-                ptx::tmem_ld_32x16(t_row, r[0]);
+                for (int d = 0; d < 4; ++d) {
+                    const int kb = kb4 + d;
+                    if (kb >= k_blocks) break;
+                    const float s = px[d] * pw[d];
+                    if (kb + 4 < k_blocks) {
+                        px[d] = __ldg(xs + (long long)(kb + 4) * p.rows);
+                        pw[d] = __ldg(ws + (kb + 4) * p.ws_k);
+                    }
+                    const uint32_t buf = it & 1;
+                    const bool ok = ptx::mbar_wait(ptx::smem_u32(&bar_acc_full[buf]), (it >> 1) & 1, wctx, UMMA_TIMEOUT_EPILOGUE);
+                    if (!__all_sync(0xffffffffu, ok)) goto epilogue_done;
+                    ptx::tc_fence_after();
+                    const uint32_t t_row = tmem_base + buf * 256u + uint32_t(half) * uint32_t(BN / 2) + ((quarter * 32u) << 16);
+                    uint32_t r[2][16];
+                    ptx::tmem_ld_32x16(t_row, r[0]);
 #pragma unroll
-                for (int i = 0; i < CHUNKS; ++i) {
-                    ptx::tmem_ld_wait();
-                    if (i + 1 < CHUNKS) {
-                        ptx::tmem_ld_32x16(t_row + 16 * (i + 1), r[(i + 1) & 1]);
-                    } else {
-                        ptx::tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) {
-                            const uint32_t e = ptx::smem_u32(&bar_acc_empty[buf]);
-                            if (is_leader) ptx::mbar_arrive(e);
-                            else ptx::mbar_arrive_cluster_relaxed(ptx::mapa(e, 0));
+                    for (int i = 0; i < CHUNKS; ++i) {
+                        ptx::tmem_ld_wait(r[i & 1]);
+                        if (i + 1 < CHUNKS) {
+                            ptx::tmem_ld_32x16(t_row + 16 * (i + 1), r[(i + 1) & 1]);
+                        } else {
+                            ptx::tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) {
+                                const uint32_t e = ptx::smem_u32(&bar_acc_empty[buf]);
+                                if (is_leader) ptx::mbar_arrive(e);
+                                else ptx::mbar_arrive_cluster_relaxed(ptx::mapa(e, 0));
+                            }
+                        }
+#pragma unroll
+                        for (int j = 0; j < 16; j += 2) {
+                            float* sum = &acc[i >> 1][(i & 1) * 16 + j];
+                            fma2(sum[0], sum[1], r[i & 1][j], r[i & 1][j + 1], s, s);
                         }
                     }
-#pragma unroll
-                    for (int j = 0; j < 16; j += 2) {
-                        float* sum = &acc[i >> 1][(i & 1) * 16 + j];
-                        fma2(sum[0], sum[1], r[i & 1][j], r[i & 1][j + 1], s, s);
-                    }
+                    ++it;
                 }
-                ++it;
-              }
             }
             store_tile<BN, OutT, 32>(p, acc, act, staging, lane, row0, feature0);
         }

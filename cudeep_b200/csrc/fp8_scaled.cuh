@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(FP8R_THREADS, 1) fp8_scaled_kernel(const __gri
                 ptx::tmem_ld_32x16(t_row, r[0]);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    ptx::tmem_ld_wait();
+                    ptx::tmem_ld_wait(r[i & 1]);
                     if (i < 7) {
                         ptx::tmem_ld_32x16(t_row + 16 * (i + 1), r[(i + 1) & 1]);
                     } else {

@@ -54,7 +54,7 @@ void launch(RaggedParams& p, const RaggedPlan& plan, cudaStream_t stream) {
                 FORM == RaggedForm::NT ? "nt" : FORM == RaggedForm::NN ? "nn" : "tn", BF16 ? "bf16" : "f16", p.rows, p.groups,
                 p.features, FORM == RaggedForm::TN ? "cols" : "k", FORM == RaggedForm::TN ? p.cols : p.k, 128 * CTAS,
                 plan.tile_cols, p.stages, clusters);
-    launch_clusters(ragged_gemm_kernel<FORM, CTAS, BF16, OutT>, p, clusters, CTAS, ragged_threads(FORM), smem_bytes,
+    launch_clusters(ragged_gemm_kernel<FORM, CTAS, BF16, OutT>, p, clusters, CTAS, RAGGED_THREADS, smem_bytes,
                     RAGGED_SMEM_BUDGET + 1024, stream);
 }
 

@@ -33,9 +33,9 @@ enum class RaggedForm { NT, NN, TN };
 
 constexpr int RAGGED_MAX_GROUPS = 1024;
 constexpr int RAGGED_BK = 64;                        // 16-bit elements per K block = one 128-byte swizzle row
-// Epilogue warps: with four, a gradient tile of 512 summed rows took longer to leave than to compute.
-__host__ __device__ constexpr int ragged_epilogue_warps(RaggedForm) { return 8; }
-__host__ __device__ constexpr int ragged_threads(RaggedForm form) { return 64 + 32 * ragged_epilogue_warps(form); }
+// With four epilogue warps a gradient tile of 512 summed rows took longer to leave than to compute.
+constexpr int RAGGED_EPI_WARPS = 8;
+constexpr int RAGGED_THREADS = 64 + 32 * RAGGED_EPI_WARPS;
 // TN: a block of 32 rows x 128 bytes for each epilogue warp.  A second one would cost the third stage of two K blocks (8192 x
 // 4096 x 4096: 232 us instead of 211).
 constexpr uint32_t RAGGED_STAGING_BYTES = 8 * 4096;
@@ -196,8 +196,8 @@ __device__ __forceinline__ void write_block(uint32_t block, uint32_t lane, T* ds
 }
 
 // One warp: the row range of each group, brought into [0, rows] (without offsets: `share` rows each), and the number of tiles
-// before it.  col_tiles >= 0:
-// column tiles of every group (TN); otherwise -col_tiles is the number of a group's rows that a tile takes.
+// before it.  col_tiles >= 0: column tiles of every group (TN); otherwise -col_tiles is the number of a group's rows that a
+// tile takes.
 __device__ __forceinline__ void group_tables(const int32_t* offsets, int groups, int rows, int share, int f_tiles, int col_tiles,
                                              int* group_rows, int* group_start, uint32_t* status) {
     const int lane = int(threadIdx.x & 31);
@@ -207,10 +207,13 @@ __device__ __forceinline__ void group_tables(const int32_t* offsets, int groups,
         const int g = base + lane;
         int tiles = 0;
         if (g < groups) {
-            int lo = min(rows, g * share), hi = min(rows, (g + 1) * share);
+            int lo, hi;
             if (offsets != nullptr) {
                 lo = __ldg(offsets + g);
                 hi = __ldg(offsets + g + 1);
+            } else {
+                lo = int(min((long long)rows, (long long)g * share));
+                hi = int(min((long long)rows, (long long)(g + 1) * share));
             }
             const int lo_in = min(max(lo, 0), rows), hi_in = min(max(hi, lo_in), rows);
             bad = bad || lo_in != lo || hi_in != hi;      // nothing is read or written outside the matrices
@@ -258,7 +261,7 @@ __device__ __forceinline__ void load_columns(uint32_t dst, const CUtensorMap* ma
 }
 
 template <RaggedForm FORM, int CTAS, bool BF16, class OutT>
-__global__ void __launch_bounds__(ragged_threads(FORM), 1) ragged_gemm_kernel(const __grid_constant__ RaggedParams p) {
+__global__ void __launch_bounds__(RAGGED_THREADS, 1) ragged_gemm_kernel(const __grid_constant__ RaggedParams p) {
 #if defined(__CUDA_ARCH_FEAT_SM100_ALL) || defined(__CUDA_ARCH_FEAT_SM101_ALL) || \
     defined(__CUDA_ARCH_FEAT_SM103_ALL)
     constexpr bool A_MN = FORM != RaggedForm::NT;
@@ -297,7 +300,7 @@ __global__ void __launch_bounds__(ragged_threads(FORM), 1) ragged_gemm_kernel(co
         }
         for (int a = 0; a < 2; ++a) {
             ptx::mbar_init(ptx::smem_u32(&bar_acc_full[a]), 1);
-            ptx::mbar_init(ptx::smem_u32(&bar_acc_empty[a]), ragged_epilogue_warps(FORM) * CTAS);
+            ptx::mbar_init(ptx::smem_u32(&bar_acc_empty[a]), RAGGED_EPI_WARPS * CTAS);
         }
         ptx::fence_mbar_init();
     }
@@ -502,7 +505,7 @@ __global__ void __launch_bounds__(ragged_threads(FORM), 1) ragged_gemm_kernel(co
                         uint32_t r[32];
                         if (any) {
                             ptx::tmem_ld_32x32(t_row + c, r);
-                            ptx::tmem_ld_wait();
+                            ptx::tmem_ld_wait(r);
                         } else {
 #pragma unroll
                             for (int j = 0; j < 32; ++j) r[j] = 0u;
@@ -559,7 +562,7 @@ __global__ void __launch_bounds__(ragged_threads(FORM), 1) ragged_gemm_kernel(co
                 for (int c = c_begin; c < c_end; c += 32) {
                     uint32_t r[32];
                     ptx::tmem_ld_32x32(t_row + c, r);
-                    ptx::tmem_ld_wait();
+                    ptx::tmem_ld_wait(r);
                     if (feature < p.features) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j)

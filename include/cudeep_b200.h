@@ -45,8 +45,9 @@ int cudeep_b200_version(void);
 const char* cudeep_b200_last_error(void);
 
 /* Reads the current device's kernel status word into *status (0 = no kernel
- * abandoned a wait; 1..4 name the pipeline role that timed out) and clears it
- * when `clear` is non-zero.  Synchronises the device. */
+ * abandoned a wait; 1..5 name the pipeline role that timed out, 6 says that a
+ * grouped product met bad offsets) and clears it when `clear` is non-zero.
+ * Synchronises the device. */
 int cudeep_b200_device_status(int clear, uint32_t* status);
 
 /* ---- matmul (device pointers) -------------------------------------------------------- */
