@@ -24,6 +24,12 @@ __device__ __forceinline__ float sfu_rcp(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float clamp_nan(float v, float lo, float hi) {      // keeps NaN
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(lo));
+    asm("min.NaN.f32 %0, %0, %1;" : "+f"(r) : "f"(hi));
+    return r;
+}
 __device__ __forceinline__ float act_sigmoid(float x) {
     return sfu_rcp(1.0f + sfu_ex2(-1.4426950408889634f * x));
 }

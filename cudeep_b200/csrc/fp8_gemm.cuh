@@ -32,15 +32,19 @@ __device__ __forceinline__ void fma2(float& d0, float& d1, uint32_t a0, uint32_t
 // The epilogue's activations as one formula, y = g * sigmoid(a z + b z^3), g = z (GELU in its tanh form, SiLU) or 1
 // (sigmoid), with log2(e) folded into a and b.  Two values share one reciprocal, 1 / d0 = d1 / (d0 d1): the SFU is what bounds
 // an epilogue that activates 128 values a thread, and this takes three of its operations per pair instead of four.  The
-// exponents are held below 60 so that d0 d1 stays finite (sigmoid = 2^-60 there instead of less); fminf also keeps a NaN
-// from its neighbour, and the factor g carries it on.
+// exponents are held below 60 so that d0 d1 stays finite (sigmoid = 2^-60 there instead of less); g is held above -64, so
+// that no z however low makes more of that than 2^-54.  fminf also keeps a NaN from its neighbour, and the factor g carries
+// it on.  Where the formula has no cubic term b is a negligible number of the right sign instead of 0: 0 * Inf is NaN.
 struct Fp8Activation {
     int act;
     float a, b;
+    float g_lo, g_hi;
     __device__ __forceinline__ explicit Fp8Activation(int act_) : act(act_) {
         const float c = act == EPI_GELU ? 2.0f * 0.7978845608028654f : 1.0f;
         a = -1.4426950408889634f * c;
-        b = act == EPI_GELU ? a * 0.044715f : 0.0f;
+        b = act == EPI_GELU ? a * 0.044715f : -1e-37f;
+        g_lo = act == EPI_SIGMOID ? 1.0f : -64.0f;
+        g_hi = act == EPI_SIGMOID ? 1.0f : __int_as_float(0x7f800000);
     }
 };
 
@@ -50,33 +54,32 @@ __device__ __forceinline__ void fp8_activation(float (&v)[N], const Fp8Activatio
     if (f.act == EPI_NONE) return;
     if (f.act == EPI_RELU) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) v[j] = fmaxf(v[j], 0.0f);
+        for (int j = 0; j < N; ++j) v[j] = fmaxf(v[j], 0.0f);      // as the other epilogues' ReLU, which drops NaN
         return;
     }
-    const bool gate = f.act != EPI_SIGMOID;
 #pragma unroll
     for (int j = 0; j < N; j += 2) {
         const float x0 = v[j], x1 = v[j + 1];
         const float d0 = 1.0f + sfu_ex2(fminf(x0 * fmaf(f.b * x0, x0, f.a), 60.0f));
         const float d1 = 1.0f + sfu_ex2(fminf(x1 * fmaf(f.b * x1, x1, f.a), 60.0f));
         const float r = sfu_rcp(d0 * d1);
-        const float g0 = gate || x0 != x0 ? x0 : 1.0f, g1 = gate || x1 != x1 ? x1 : 1.0f;
-        v[j] = g0 * (d1 * r);
-        v[j + 1] = g1 * (d0 * r);
+        v[j] = clamp_nan(x0, f.g_lo, f.g_hi) * (d1 * r);
+        v[j + 1] = clamp_nan(x1, f.g_lo, f.g_hi) * (d0 * r);
     }
 }
 
 // ---- few tiles ----------------------------------------------------------------------------------------------------------------
 
-// For few rows (and for few features, whatever the rows) the FEATURES lie on the 128 lanes and up to 128 rows on the columns:
-// the width of the MMA follows the number of rows, and a CTA streams its features' weights once, which is all that a product
-// of a few rows costs.  One tile per CTA; where there are fewer tiles than the device has SMs, a cluster of up to eight CTAs
-// shares a tile, each with a range of K, and adds the parts up through distributed shared memory in rank order.  A tile may take fewer than 128 features (the last
-// lanes then idle), so that the tiles fill the SMs: 16384 features are 128 tiles of 128, but 147 of 112.
+// For few rows (and for few features, whatever the rows) the FEATURES lie on the 128 lanes and up to 128 rows on the
+// columns: the width of the MMA follows the number of rows, and a CTA streams its features' weights once, which is all that
+// a product of a few rows costs.  One tile per CTA; where there are fewer tiles than the device has SMs, a cluster of up to
+// eight CTAs shares a tile, each with a range of K, and adds the parts up through distributed shared memory in rank order.
+// A tile may take fewer than 128 features (the last lanes then idle), so that the tiles fill the SMs: 16384 features are 128
+// tiles of 128, but 147 of 112.
 //
 // The factors xs * ws change along the columns here: each epilogue warp fetches those of its columns four blocks ahead and
 // reads them back from shared memory.  With so few columns TMEM holds up to eight accumulators, so the tensor core runs
-// ahead of the sums by that many blocks (two accumulators and factors one block ahead: 16 rows, 4096 -> 16384 took 35 us, 
+// ahead of the sums by that many blocks (two accumulators and factors one block ahead: 16 rows, 4096 -> 16384 took 35 us,
 // every block waiting for its factors; now 17 us).
 constexpr int FP8F_MAX_ROWS = 128;
 constexpr int FP8F_EPI_WARPS = 8;

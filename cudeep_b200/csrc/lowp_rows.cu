@@ -1,8 +1,8 @@
 // One-pass kernels around the 8-bit and the grouped products: padding of rows for the TMA unit, quantisation to e4m3
 // in blocks and back.  All are bound by HBM: each input is read once and each output written once.
 //
-// Each kernel waits for its predecessors itself and then lets its successor be set up, so that in a sequence of small launches (the
-// backward pass of a short batch is nine) the launches overlap.
+// Each kernel waits for its predecessors itself and then lets its successor be set up, so that in a sequence of small
+// launches (the backward pass of a short batch is nine) the launches overlap.
 #include "lowp_rows.h"
 
 #include "epilogue_math.cuh"
@@ -22,11 +22,11 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// dst[r, 0..ld) = src[r, 0..row_bytes) followed by zeros, in bytes; ld is a multiple of 16 and dst aligned to it.  A warp takes 512
-// bytes of a row, a lane every 32nd word of the result, shifted together from the two aligned words of the source that hold it (loads
-// byte by byte ran at 2 TB/s, 16 bytes a lane at a quarter of the requests' width).  Words that reach over the matrix's
-// ends are put together from bytes.  With offsets, rows_group rows belong to each group, and those of groups without
-// rows in their turn (the weights of experts that have no token) are left out.
+// dst[r, 0..ld) = src[r, 0..row_bytes) followed by zeros, in bytes; ld is a multiple of 16 and dst aligned to it.  A warp
+// takes 512 bytes of a row, a lane every 32nd word of the result, shifted together from the two aligned words of the source
+// that hold it (loads byte by byte ran at 2 TB/s, 16 bytes a lane at a quarter of the requests' width).  Words that reach
+// over the matrix's ends are put together from bytes.  With offsets, rows_group rows belong to each group, and those of
+// groups without rows in their turn (the weights of experts that have no token) are left out.
 __global__ void __launch_bounds__(kThreads) pad_rows_kernel(const uint8_t* __restrict__ src, uint8_t* __restrict__ dst,
                                                             long long rows, int row_bytes, int ld,
                                                             const int32_t* __restrict__ offsets, int rows_group) {
@@ -529,13 +529,6 @@ __global__ void dequantize_kernel(const uint8_t* __restrict__ q, const float* __
 // Slope of the epilogue activations.  With s = sigmoid(t), t = 2 sqrt(2 / pi) (z + 0.044715 z^3): tanh-form GELU is z s, so its
 // slope is s + z s (1 - s) dt/dz; SiLU the same with t = z.  s comes from the SFU's ex2 and rcp as in the forward epilogue
 // (2 ulp; with expf and tanhf the pass was bound by arithmetic, 68 us for 8192 x 4096 instead of 34 us with the bands' sums).
-__device__ __forceinline__ float clamp_nan(float v, float lo, float hi) {      // keeps NaN
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(lo));
-    asm("min.NaN.f32 %0, %0, %1;" : "+f"(r) : "f"(hi));
-    return r;
-}
-
 template <int act>
 __device__ __forceinline__ float act_slope(float z) {
     if (act == EPI_RELU) return z > 0.0f ? 1.0f : 0.0f;
@@ -561,8 +554,9 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
     *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(t);
 }
 
-// A CTA takes 256 columns and `rows_per` rows: 32 threads with eight columns each lie along a row, eight rows side by side.  Column sums stay in registers over the rows, are added across the eight threads of a column in a fixed order and go
-// to partial[row band][cols], which one more kernel adds up, again in order: the result does not depend on timing.
+// A CTA takes 256 columns and `rows_per` rows: 32 threads with eight columns each lie along a row, eight rows side by side.
+// Column sums stay in registers over the rows, are added across the eight threads of a column in a fixed order and go to
+// partial[row band][cols], which one more kernel adds up, again in order: the result does not depend on timing.
 template <typename T, bool VEC, int act>
 __global__ void __launch_bounds__(kThreads) act_backward_kernel(const T* __restrict__ dy, const uint8_t* __restrict__ z8,
                                                                 const float* __restrict__ zs, T* __restrict__ dz,

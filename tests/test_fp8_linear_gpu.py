@@ -178,3 +178,44 @@ def test_backward_saved(dev, m, n, k, act, dtype, dw_type):
     if dtype == "f16":
         lost = (xs.amax(1).double() * 2.0 ** -25).repeat_interleave(128)[None, :k].expand(m, k)
     check(torch, dw, dz.t() @ x, rounded.t() @ x.abs() + dz.abs().t() @ lost + m * 2.0 ** -23 * (dz.abs().t() @ x.abs()))
+
+
+@pytest.mark.parametrize("act", sorted(ACTS))
+@pytest.mark.parametrize("m,n,k", [(4, 256, 256), (4, 300, 4096), (1100, 4096, 512), (300, 520, 256), (4096, 4096, 2048)])
+def test_activations_of_infinities_huge_values_and_nan(dev, act, m, n, k):
+    """Features of one sign each, so that a row's pre-activation is +-s: infinite, huge, NaN or moderate by the row.
+
+    Below z = -64 the activated values are within 2^-54 of their limit 0 (sigmoid: 2^-60); everything here is a sum of equal
+    terms that are powers of two times 448, whose FP32 sums lose at most the tolerance of the other tests."""
+    torch = dev.torch
+    x8 = torch.full((m, k), 0x38, device=dev.dev, dtype=torch.uint8)      # 1.0
+    w8 = torch.full((n, k), 0x7E, device=dev.dev, dtype=torch.uint8)      # 448
+    w8[1::2] = 0xFE
+    xs = torch.full((-(-k // 128), m), 2.0 ** -36, device=dev.dev)
+    xs[:, 0] = 2.0 ** 100
+    xs[:, 1] = 2.0 ** 80
+    x8[2, k // 2] = 0x7F      # NaN
+    ws = torch.full((-(-n // 128), -(-k // 128)), 2.0 ** 20, device=dev.dev)
+    y = torch.zeros((m, n), device=dev.dev)
+    dev.check(dev.lib.cudeep_b200_linear_forward_fp8(dev.ptr(x8), dev.ptr(xs), dev.ptr(w8), dev.ptr(ws), None, dev.ptr(y), 0,
+                                                     m, n, k, ACTS[act], None))
+    assert dev.sync_status() == 0
+    up, down = y[:, 0::2], y[:, 1::2]
+    inf = float("inf")
+    if act == "relu":      # drops NaN, as the framework's other epilogues
+        assert (y[2] == 0).all() and not y.isnan().any()
+    else:
+        assert y[2].isnan().all() and y.isnan().sum().item() == n
+    if act == "sigmoid":
+        assert (up[:2] == 1).all()
+    else:
+        assert (up[0] == inf).all()
+        assert ((up[1].double() / (448.0 * k * 2.0 ** 100) - 1).abs() <= (128 + k // 128) * 2.0 ** -23 + 2.0 ** -20).all()
+    if act == "none":
+        assert (down[0] == -inf).all() and (down[1] == -up[1, :1]).all()
+    else:
+        assert (down[:2].abs() <= 2.0 ** -54).all()
+    z = 448.0 * k * 2.0 ** -16 * torch.ones(n, device=dev.dev, dtype=torch.float64)
+    bound = 1.13 * (128 + k // 128) * 2.0 ** -23 * z + 2.0 ** -20 * z.clamp(min=1)
+    z[1::2] *= -1
+    check(torch, y[3:], act64(torch, z, act).expand(m - 3, n), bound)
