@@ -43,9 +43,7 @@ def _dense(t: Tensor, what: str, dtype: Optional[DType] = None) -> Tensor:
 
 
 def _like(ref: Tensor, shape, dtype: DType) -> Tensor:
-    out = Tensor(shape, dtype)
-    out.stream = ref.stream
-    return out
+    return Tensor(shape, dtype, _stream=ref.stream)
 
 
 def _ptr(t: Optional[Tensor]):

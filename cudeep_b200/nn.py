@@ -19,8 +19,10 @@ from typing import Optional
 
 import numpy as np
 
-from . import lowp
-from .tensor import DType, Tensor, conv2d, linear
+from . import _lib, lowp
+from .tensor import DType, Tensor, _epilogue_code, conv2d, linear
+
+_ACTIVATIONS = (None, "relu", "gelu", "silu", "sigmoid")     # by epilogue code
 
 
 class Parameter(Tensor):
@@ -118,15 +120,30 @@ class Linear(Module):
 
 class _Prepared:
     """What a layer makes of its weight before it is used, kept until the parameter is replaced (load_state_dict).  A weight
-    changed in place is not noticed: call the layer's refresh()."""
+    changed in place is not noticed: call the layer's refresh().  It is made on the parameter's stream and finished before
+    any stream uses it; once other streams have, they are waited for before its memory goes back to the pool."""
 
     def __init__(self):
         self.of = self.value = None
+        self.used_elsewhere = False
 
-    def get(self, parameter, make):
+    def get(self, parameter, make, stream):
         if self.of is not parameter:
+            self.drop()
             self.value, self.of = make(parameter), parameter
+            _lib.check(_lib.load().cudeep_b200_stream_synchronize(parameter.stream))
+        if _handle(stream) != _handle(parameter.stream):
+            self.used_elsewhere = True
         return self.value
+
+    def drop(self):
+        if self.used_elsewhere:
+            _lib.check(_lib.load().cudeep_b200_device_synchronize())
+        self.__init__()
+
+
+def _handle(stream):
+    return getattr(stream, "value", stream) or 0
 
 
 class LinearFp8(Linear):
@@ -138,21 +155,23 @@ class LinearFp8(Linear):
         self._weight8 = _Prepared()
 
     def refresh(self) -> None:
-        self._weight8 = _Prepared()
+        self._weight8.drop()
 
-    def weight_fp8(self) -> lowp.Fp8Tensor:
-        return self._weight8.get(self._parameters["weight"], lambda w: lowp.quantize_fp8(w, tiles=True))
+    def weight_fp8(self, stream=None) -> lowp.Fp8Tensor:
+        """The weight as the products on `stream` take it."""
+        return self._weight8.get(self._parameters["weight"], lambda w: lowp.quantize_fp8(w, tiles=True), stream)
 
     def forward(self, x, activation=None):
-        return lowp.linear_fp8(lowp.quantize_fp8(x), self.weight_fp8(), self._parameters.get("bias"), activation,
+        return lowp.linear_fp8(lowp.quantize_fp8(x), self.weight_fp8(x.stream), self._parameters.get("bias"), activation,
                                x.dtype())
 
     def forward_saved(self, x, activation=None):
         """(y, saved) for `backward`: y as forward's, saved holds x and, with an activation, the pre-activation in 8 bits.
         Without an activation nothing but the codes that the product reads anyway is kept."""
+        activation = _ACTIVATIONS[_epilogue_code(activation)]
         x8 = lowp.quantize_fp8(x)
         bias = self._parameters.get("bias")
-        z = lowp.linear_fp8(x8, self.weight_fp8(), bias, None, DType.float32 if activation else x.dtype())
+        z = lowp.linear_fp8(x8, self.weight_fp8(x.stream), bias, None, DType.float32 if activation else x.dtype())
         if activation is None:
             return z, (x8, None, None)
         y = getattr(z, activation)()
@@ -162,8 +181,8 @@ class LinearFp8(Linear):
         """(dx, dweight, dbias) in float32 for bfloat16 `grad` of y and what forward_saved kept; the product for dx takes the
         weight in bfloat16."""
         x8, z8, activation = saved
-        dx, dw, db = lowp.linear_backward_saved(grad, x8, self._parameters["weight"].to(DType.bfloat16), z8, activation,
-                                                DType.float32)
+        weight = self._parameters["weight"]._cast_on(DType.bfloat16, grad.stream)
+        dx, dw, db = lowp.linear_backward_saved(grad, x8, weight, z8, activation, DType.float32)
         return dx.to(DType.float32), dw, (db if "bias" in self._parameters else None)
 
 
@@ -179,17 +198,18 @@ class GroupedLinear(Module):
         self._weight16 = _Prepared()
 
     def refresh(self) -> None:
-        self._weight16 = _Prepared()
+        self._weight16.drop()
 
-    def weight_bf16(self) -> Tensor:
-        return self._weight16.get(self._parameters["weight"], lambda w: w.to(DType.bfloat16))
+    def weight_bf16(self, stream=None) -> Tensor:
+        """The weight as the products on `stream` take it."""
+        return self._weight16.get(self._parameters["weight"], lambda w: w.to(DType.bfloat16), stream)
 
     def forward(self, x, offsets):
-        return lowp.grouped_linear(x, self.weight_bf16(), offsets)
+        return lowp.grouped_linear(x, self.weight_bf16(x.stream), offsets)
 
     def backward(self, grad, x, offsets):
         """(dx in bfloat16, dweight in float32)."""
-        return lowp.grouped_linear_backward(grad, x, self.weight_bf16(), offsets)
+        return lowp.grouped_linear_backward(grad, x, self.weight_bf16(x.stream), offsets)
 
 
 class Conv2d(Module):
@@ -255,7 +275,7 @@ class Sequential(Module):
             m = mods[i]
             nxt = mods[i + 1] if i + 1 < len(mods) else None
             if (self.fuse and isinstance(m, (Linear, Conv2d)) and isinstance(nxt, _Activation)
-                    and x.dtype() == DType.float32):
+                    and (x.dtype() == DType.float32 or isinstance(m, LinearFp8))):
                 x = m.forward(x, activation=nxt.name)
                 i += 2
             else:

@@ -87,7 +87,8 @@ class _Storage:
 
 
 class Tensor:
-    def __init__(self, shape: Sequence[int], dtype: DType = DType.float32, *, _storage=None, _strides=None):
+    def __init__(self, shape: Sequence[int], dtype: DType = DType.float32, *, _storage=None, _strides=None,
+                 _stream=None):
         self._shape = [int(s) for s in shape]
         if any(s < 0 for s in self._shape):
             raise RuntimeError("Tensor: negative extent")
@@ -95,7 +96,9 @@ class Tensor:
             raise RuntimeError("Tensor: float16 tensors are not supported on this path")
         self._dtype = dtype
         self._strides = list(_strides) if _strides is not None else _contiguous_strides(self._shape)
-        self._storage = _storage if _storage is not None else _Storage(self.nbytes())
+        if _storage is None:
+            _storage = _Storage(self.nbytes()) if _stream is None else _Storage(self.nbytes(), _stream)
+        self._storage = _storage
         self._stream = getattr(self._storage, "stream", None)
 
     @property
@@ -209,15 +212,16 @@ class Tensor:
 
     def to(self, dtype: DType) -> "Tensor":
         """The same values as float32 or bfloat16 (rounded to nearest even)."""
-        if self._dtype == dtype:
-            return self
+        return self if self._dtype == dtype else self._cast_on(dtype, self.stream)
+
+    def _cast_on(self, dtype: DType, stream) -> "Tensor":
+        """A copy as `to` makes it, for use on `stream`."""
         if self._dtype not in _TYPE_CODE or dtype not in _TYPE_CODE:
             raise RuntimeError(f"to: no conversion from {self._dtype.name} to {dtype.name}")
         src = self if self.is_contiguous() else self.contiguous()
-        out = Tensor(self._shape, dtype)
-        out.stream = self.stream
+        out = Tensor(self._shape, dtype, _stream=stream)
         _lib.check(_lib.load().cudeep_b200_cast(src._storage.ptr, _TYPE_CODE[self._dtype], out._storage.ptr,
-                                                _TYPE_CODE[dtype], self.numel(), self.stream))
+                                                _TYPE_CODE[dtype], self.numel(), stream))
         return out
 
     # ---- views and copies ----------------------------------------------------------------

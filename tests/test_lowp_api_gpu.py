@@ -137,6 +137,69 @@ def test_grouped_layer_is_adjoint(cd):
         start += s
 
 
+def test_activation_by_name_code_or_none(cd):
+    rng = np.random.default_rng(4)
+    x = cd.Tensor.from_numpy(rng.standard_normal((5, 96)).astype(np.float32))
+    layer = cd.nn.LinearFp8(96, 40)
+    plain = layer.forward_saved(x)
+    for none in ("none", 0):
+        y, saved = layer.forward_saved(x, none)
+        assert np.array_equal(y.numpy(), plain[0].numpy()) and saved[1] is None
+        dy = cd.Tensor.from_numpy(rng.standard_normal((5, 40)).astype(np.float32)).to(cd.DType.bfloat16)
+        for a, b in zip(layer.backward(dy, saved), layer.backward(dy, plain[1])):
+            assert np.array_equal(a.numpy(), b.numpy())
+    assert np.array_equal(layer.forward_saved(x, 3)[0].numpy(), layer.forward_saved(x, "silu")[0].numpy())
+    for bad in ("tanh", 5):
+        with pytest.raises(RuntimeError, match="unknown"):
+            layer.forward_saved(x, bad)
+
+
+def test_sequential_of_bfloat16_rows(cd):
+    """LinearFp8 takes the activation behind it into its epilogue whatever the type of x."""
+    rng = np.random.default_rng(6)
+    x = cd.Tensor.from_numpy(rng.standard_normal((33, 96)).astype(np.float32)).to(cd.DType.bfloat16)
+    a, b = cd.nn.LinearFp8(96, 160), cd.nn.LinearFp8(160, 40)
+    y = cd.nn.Sequential(a, cd.nn.SiLU(), b)(x)
+    assert y.dtype() == cd.DType.bfloat16
+    assert np.array_equal(y.numpy(), b(a(x, "silu")).numpy())
+
+
+def test_layers_on_a_stream_of_their_own(cd):
+    """The first use of a weight, its replacement and the gradients on another stream than the parameter's, while the
+    parameter's stream is busy: as on one stream, bit for bit."""
+    rng = np.random.default_rng(5)
+    m, n, k, groups = 260, 392, 520, 3
+    x32 = rng.standard_normal((m, k)).astype(np.float32)
+    dy32 = rng.standard_normal((m, n)).astype(np.float32)
+    offsets = cd.Tensor.from_numpy(np.array([0, 100, 100, m], np.int32))
+    weights = [(rng.standard_normal((n, k)) / 20).astype(np.float32) for _ in range(2)]
+    experts = [(rng.standard_normal((groups, n, k)) / 20).astype(np.float32) for _ in range(2)]
+    busy = cd.Tensor.ones([4096, 4096])
+
+    def run(stream):
+        linear, grouped, got = cd.nn.LinearFp8(k, n), cd.nn.GroupedLinear(groups, k, n), []
+        for w, e in zip(weights, experts):
+            linear.load_state_dict({"weight": w})
+            grouped.load_state_dict({"weight": e})
+            x = cd.Tensor.from_numpy(x32)
+            dy = cd.Tensor.from_numpy(dy32)
+            if stream is not None:
+                x.set_stream(stream)
+                dy.set_stream(stream)
+                for _ in range(4):
+                    busy.matmul(busy)
+            x16, dy16 = x.to(cd.DType.bfloat16), dy.to(cd.DType.bfloat16)
+            y, saved = linear.forward_saved(x, "gelu")
+            out = [y, *linear.backward(dy16, saved), grouped(x16, offsets), *grouped.backward(dy16, x16, offsets)]
+            linear.refresh()
+            grouped.refresh()
+            got.append([t.numpy() for t in out])
+        return got
+
+    for a, b in zip(run(None), run(cd.Stream())):
+        assert all(np.array_equal(p, q) for p, q in zip(a, b))
+
+
 # ---- streams, graphs, repeats ----------------------------------------------------------------------------------------------
 
 
