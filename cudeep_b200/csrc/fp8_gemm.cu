@@ -198,8 +198,8 @@ void product(const uint8_t* x, const float* x_scales, const uint8_t* w, const fl
              int y_type, int m, int n, int k, int act, cudaStream_t stream) {
     constexpr bool nn = FORM == RaggedForm::NN;
     const int w_cols = nn ? n : k, w_rows = nn ? k : n;
-    const AlignedRows xr = aligned_rows(x, m, k, 1, stream);
-    const AlignedRows wr = aligned_rows(w, w_rows, w_cols, 1, stream);
+    const PreparedRows operands = prepare_rows({x, m, k, 1}, {w, w_rows, w_cols, 1}, {}, stream);
+    const AlignedRows &xr = operands.a, &wr = operands.b;
     const uint32_t box[2] = {128, 128};
     const uint64_t w_dims[2] = {uint64_t(w_cols), uint64_t(w_rows)}, w_strides[1] = {uint64_t(wr.ld)};
     const uint64_t x_dims[2] = {uint64_t(k), uint64_t(m)}, x_strides[1] = {uint64_t(xr.ld)};

@@ -69,19 +69,12 @@ void launch_rows(RaggedParams& p, const RaggedPlan& plan, int type, cudaStream_t
     }
 }
 
-AlignedRows rows_of(const void* src, long long ld, int rows, int cols, cudaStream_t stream) {
-    if (ld == 0) return aligned_rows(src, rows, cols, 2, stream);
-    AlignedRows out;
-    out.ptr = src;
-    out.ld = ld;
-    return out;
-}
-
-void rows_by_weight(bool nn, const void* a, long long lda, const void* w, void* c, int type, const int32_t* offsets, int groups, int rows,
-                    int n, int k, cudaStream_t stream) {
-    const AlignedRows x = rows_of(a, lda, rows, k, stream);
+void rows_by_weight(bool nn, const void* a, long long lda, const void* w, long long ldw, void* c, int type, const int32_t* offsets,
+                    int groups, int rows, int n, int k, cudaStream_t stream) {
     const int w_cols = nn ? n : k, w_rows = nn ? k : n;
-    const AlignedRows wt = aligned_rows(w, (long long)groups * w_rows, w_cols, 2, stream, offsets, w_rows);
+    const PreparedRows operands = prepare_rows({a, rows, k, 2, lda}, {w, (long long)groups * w_rows, w_cols, 2, ldw, offsets, w_rows},
+                                               {}, stream);
+    const AlignedRows &x = operands.a, &wt = operands.b;
     RaggedParams p{};
     {
         const uint64_t row_bytes = uint64_t(wt.ld) * 2, group_bytes = row_bytes * uint64_t(w_rows);
@@ -141,18 +134,18 @@ void launch_weight(RaggedParams& p, const RaggedPlan& plan, int c_type, cudaStre
 
 void grouped_nt(const void* a, const void* w, void* c, int type, const int32_t* offsets, int groups, int rows, int n, int k,
                 cudaStream_t stream) {
-    rows_by_weight(false, a, 0, w, c, type, offsets, groups, rows, n, k, stream);
+    rows_by_weight(false, a, 0, w, 0, c, type, offsets, groups, rows, n, k, stream);
 }
 
-void grouped_nn(const void* a, long long lda, const void* w, void* c, int type, const int32_t* offsets, int groups, int rows,
-                int n, int k, cudaStream_t stream) {
-    rows_by_weight(true, a, lda, w, c, type, offsets, groups, rows, n, k, stream);
+void grouped_nn(const void* a, long long lda, const void* w, long long ldw, void* c, int type, const int32_t* offsets, int groups,
+                int rows, int n, int k, cudaStream_t stream) {
+    rows_by_weight(true, a, lda, w, ldw, c, type, offsets, groups, rows, n, k, stream);
 }
 
 void grouped_tn(const void* a, long long lda, const void* b, long long ldb, void* c, int type, int c_type,
                 const int32_t* offsets, int groups, int rows, int m, int n, const float* col_scale, cudaStream_t stream) {
-    const AlignedRows y = rows_of(a, lda, rows, m, stream);
-    const AlignedRows x = rows_of(b, ldb, rows, n, stream);
+    const PreparedRows operands = prepare_rows({a, rows, m, 2, lda}, {b, rows, n, 2, ldb}, {}, stream);
+    const AlignedRows &y = operands.a, &x = operands.b;
     RaggedPlan plan = plan_weight(groups, rows, m, n, elem_bytes(c_type));
     // One gradient of few tiles and many rows: `parts` ranges of the rows as groups of their own, summed in FP32 and added up
     // in order by a pass of their own (8192 rows, 512 x 512: 50 us in one range, 18 us so).

@@ -97,7 +97,7 @@ void launch_grouped_matmul_nn(const void* A, const void* B, void* C, ElementType
     check_grouped(A, B, C, offsets, groups, rows, N, K);
     check_element_address(C, 2, "C");
     if (rows == 0) return;
-    cudeep_b200::grouped_nn(A, 0, B, C, t, offsets, groups, rows, N, K, stream);
+    cudeep_b200::grouped_nn(A, 0, B, 0, C, t, offsets, groups, rows, N, K, stream);
 }
 
 void launch_grouped_matmul_tn(const void* A, const void* B, void* C, ElementType type, ElementType c_type,
@@ -168,38 +168,40 @@ void launch_linear_backward_saved_fp8(const void* dy, ElementType type, const vo
         if (db != nullptr) CB200_CUDA(cudaMemsetAsync(db, 0, size_t(N) * sizeof(float), stream));
         return;
     }
+    // W, and dy where the products read it themselves, as the TMA unit reads them.  And x as a 16-bit operand: q * s is exact in
+    // BF16 for the power-of-two scales of quantize_fp8; FP16 has too few exponents for that, so there each column block is
+    // taken relative to its largest scale (products below 2^-24 of that are lost) and the result is multiplied by it.
+    Scratch top_buf;
+    ScaleTops tops;
+    if (dw != nullptr && t == TYPE_F16) {
+        top_buf = Scratch(size_t((K + FP8_BLOCK - 1) / FP8_BLOCK) * sizeof(float), stream);
+        tops = ScaleTops{x_scales, M, K, static_cast<float*>(top_buf.ptr)};
+    }
+    const bool products = dx != nullptr || dw != nullptr;
+    const PreparedRows operands = prepare_rows({dx != nullptr ? W : nullptr, N, K, 2},
+                                               {act == EPI_NONE && products ? dy : nullptr, M, N, 2}, tops, stream);
     // dz goes to the tensor cores in dy's type: both products take it as an operand next to 16-bit W and x.  db is summed
     // from its FP32 values.
-    const void* dz = dy;
-    long long ld_dz = 0;      // contiguous, of any row length
+    const void* dz = operands.b.ptr;
+    long long ld_dz = operands.b.ld;
     Scratch dz_buf;
+    ColumnSums sums;
     if (act != EPI_NONE) {
-        if (dx != nullptr || dw != nullptr) {
+        if (products) {
             ld_dz = (N + 63) / 64 * 64;      // whole 128-byte rows of a box
             dz_buf = Scratch(size_t(M) * ld_dz * 2, stream);
             dz = dz_buf.ptr;
         }
-        activation_backward_fp8(dy, t, static_cast<const uint8_t*>(z8), z_scales, act, dz_buf.ptr, ld_dz, db, M, N, stream);
+        sums = activation_backward_fp8(dy, t, static_cast<const uint8_t*>(z8), z_scales, act, dz_buf.ptr, ld_dz, db, M, N, stream);
     } else if (db != nullptr) {
-        activation_backward_fp8(dy, t, nullptr, nullptr, act, nullptr, 0, db, M, N, stream);
+        sums = activation_backward_fp8(dy, t, nullptr, nullptr, act, nullptr, 0, db, M, N, stream);
     }
-    if (dx != nullptr) grouped_nn(dz, ld_dz, W, dx, t, nullptr, 1, M, K, N, stream);
-    if (dw != nullptr) {
-        // x as a 16-bit operand.  q * s is exact in BF16 for the power-of-two scales of quantize_fp8; FP16 has too few
-        // exponents for that, so there each column block is taken relative to its largest scale (products below
-        // 2^-24 of that are lost) and the result is multiplied by it.
-        const long long ld_x = (K + 63) / 64 * 64;
-        Scratch x_buf(size_t(M) * ld_x * 2, stream);
-        Scratch top_buf;
-        float* top = nullptr;
-        if (t == TYPE_F16) {
-            top_buf = Scratch(size_t((K + FP8_BLOCK - 1) / FP8_BLOCK) * sizeof(float), stream);
-            top = static_cast<float*>(top_buf.ptr);
-            block_tops(x_scales, M, K, top, stream);
-        }
-        dequantize_rows(static_cast<const uint8_t*>(x8), x_scales, top, M, K, x_buf.ptr, ld_x, t, stream);
-        grouped_tn(dz, ld_dz, x_buf.ptr, ld_x, dw, t, wt, nullptr, 1, M, N, K, top, stream);
-    }
+    if (dx != nullptr) grouped_nn(dz, ld_dz, operands.a.ptr, operands.a.ld, dx, t, nullptr, 1, M, K, N, stream);
+    if (dw == nullptr) return finish_sums(sums, stream);
+    const long long ld_x = (K + 63) / 64 * 64;
+    Scratch x_buf(size_t(M) * ld_x * 2, stream);
+    dequantize_rows(static_cast<const uint8_t*>(x8), x_scales, tops.top, M, K, x_buf.ptr, ld_x, t, sums, stream);
+    grouped_tn(dz, ld_dz, x_buf.ptr, ld_x, dw, t, wt, nullptr, 1, M, N, K, tops.top, stream);
 }
 
 }  // namespace kernels

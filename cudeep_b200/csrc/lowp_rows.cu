@@ -22,22 +22,34 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// The work of a CTA in prepare_kernel for one matrix to pad.
+struct PadJob {
+    const uint8_t* src;
+    uint8_t* dst;
+    long long rows;
+    int row_bytes, ld;
+    const int32_t* offsets;
+    int rows_group;
+    unsigned chunks;      // of 512 bytes, in a row of the result
+    unsigned blocks;      // CTAs
+};
+
 // dst[r, 0..ld) = src[r, 0..row_bytes) followed by zeros, in bytes; ld is a multiple of 16 and dst aligned to it.  A warp
 // takes 512 bytes of a row, a lane every 32nd word of the result, shifted together from the two aligned words of the source
 // that hold it (loads byte by byte ran at 2 TB/s, 16 bytes a lane at a quarter of the requests' width).  Words that reach
 // over the matrix's ends are put together from bytes.  With offsets, rows_group rows belong to each group, and those of
 // groups without rows in their turn (the weights of experts that have no token) are left out.
-__global__ void __launch_bounds__(kThreads) pad_rows_kernel(const uint8_t* __restrict__ src, uint8_t* __restrict__ dst,
-                                                            long long rows, int row_bytes, int ld,
-                                                            const int32_t* __restrict__ offsets, int rows_group) {
-    ptx::grid_dependency_wait();
-    ptx::grid_launch_dependents();
+__device__ __forceinline__ void pad_rows(const PadJob& job, unsigned block) {
+    const uint8_t* __restrict__ src = job.src;
+    uint8_t* __restrict__ dst = job.dst;
+    const long long rows = job.rows;
+    const int row_bytes = job.row_bytes, ld = job.ld;
     const int lane = threadIdx.x & 31;
-    const long long r = blockIdx.x * (long long)(kThreads / 32) + (threadIdx.x >> 5);
+    const long long r = block / job.chunks * (long long)(kThreads / 32) + (threadIdx.x >> 5);
     if (r >= rows) return;
-    if (offsets != nullptr) {
-        const int g = int(r / rows_group);
-        if (__ldg(offsets + g + 1) <= __ldg(offsets + g)) return;
+    if (job.offsets != nullptr) {
+        const int g = int(r / job.rows_group);
+        if (__ldg(job.offsets + g + 1) <= __ldg(job.offsets + g)) return;
     }
     const uint8_t* row = src + r * row_bytes;
     const uint8_t* end = src + rows * row_bytes;
@@ -58,7 +70,7 @@ __global__ void __launch_bounds__(kThreads) pad_rows_kernel(const uint8_t* __res
         }
         return v;
     };
-    const int w0 = int(blockIdx.y) * 128;
+    const int w0 = int(block % job.chunks) * 128;
     uint32_t lo[4], hi[4];
     if (from <= to) {
 #pragma unroll
@@ -622,54 +634,85 @@ __global__ void __launch_bounds__(kThreads) act_backward_kernel(const T* __restr
     }
 }
 
+// Column sums that still lie in bands of rows.
+struct Bands {
+    const float* partial;      // [bands][cols]
+    int bands, cols;
+    float* out;
+    unsigned blocks;           // CTAs: one for 32 columns
+};
+
 // A CTA takes 32 columns, its eight warps every eighth band each; their sums are added in warp order.
-__global__ void __launch_bounds__(kThreads) add_bands_kernel(const float* __restrict__ partial, int bands, int cols,
-                                                             float* __restrict__ out) {
-    ptx::grid_dependency_wait();
-    ptx::grid_launch_dependents();
+__device__ __forceinline__ void add_bands(const Bands& p, unsigned block) {
     __shared__ float s_sum[8][32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int c = blockIdx.x * 32 + lane;
+    const int c = int(block) * 32 + lane;
     float total = 0.0f;
-    if (c < cols) {
+    if (c < p.cols) {
 #pragma unroll 4
-        for (int b = warp; b < bands; b += 8) total += partial[(long long)b * cols + c];
+        for (int b = warp; b < p.bands; b += 8) total += p.partial[(long long)b * p.cols + c];
     }
     s_sum[warp][lane] = total;
     __syncthreads();
-    if (warp == 0 && c < cols) {
+    if (warp == 0 && c < p.cols) {
         total = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) total += s_sum[i][lane];
-        out[c] = total;
+        p.out[c] = total;
     }
 }
 
-__global__ void __launch_bounds__(kThreads) block_tops_kernel(const float* __restrict__ scales, int rows, float* __restrict__ top) {
+__global__ void __launch_bounds__(kThreads) add_bands_kernel(const __grid_constant__ Bands p) {
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
+    add_bands(p, blockIdx.x);
+}
+
+__device__ __forceinline__ void block_top(const float* __restrict__ scales, int rows, float* __restrict__ top, unsigned block) {
     __shared__ float s_max[kThreads / 32];
     float m = 0.0f;
-    for (int r = threadIdx.x; r < rows; r += kThreads) m = fmaxf(m, finite_abs(__ldg(scales + (long long)blockIdx.x * rows + r)));
+    for (int r = threadIdx.x; r < rows; r += kThreads) m = fmaxf(m, finite_abs(__ldg(scales + (long long)block * rows + r)));
 #pragma unroll
     for (int d = 16; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
     if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) m = fmaxf(m, s_max[w]);
-    if (threadIdx.x == 0) top[blockIdx.x] = m > 0.0f ? m : 1.0f;
+    if (threadIdx.x == 0) top[block] = m > 0.0f ? m : 1.0f;
 }
 
-// Eight elements per thread, zeros behind cols up to the next multiple of eight.
+// What a product needs before it, in one launch: each launch costs the host about 2 us, more than a small one of these takes
+// (a grouped product of 64 rows with both operands to pad occupies the host for 11.6 us with a launch for each and 8.7 us so).
+struct PrepareParams {
+    PadJob pad[2];
+    const float* scales;
+    int scale_rows;
+    float* top;
+};
+__global__ void __launch_bounds__(kThreads) prepare_kernel(const __grid_constant__ PrepareParams p) {
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
+    unsigned block = blockIdx.x;
+    if (block < p.pad[0].blocks) return pad_rows(p.pad[0], block);
+    block -= p.pad[0].blocks;
+    if (block < p.pad[1].blocks) return pad_rows(p.pad[1], block);
+    block_top(p.scales, p.scale_rows, p.top, block - p.pad[1].blocks);
+}
+
+// Eight elements per thread, zeros behind cols up to the next multiple of eight.  The first CTAs add up column sums instead, of
+// the pass before it (a launch less).
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads) dequantize_rows_kernel(const uint8_t* __restrict__ q, const float* __restrict__ scales,
                                                                    const float* __restrict__ top, int rows, int cols,
-                                                                   T* __restrict__ y, long long ld_y) {
+                                                                   T* __restrict__ y, long long ld_y,
+                                                                   const __grid_constant__ Bands sums) {
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
+    if (blockIdx.x < sums.blocks) return add_bands(sums, blockIdx.x);
+    const unsigned block = blockIdx.x - sums.blocks, blocks = gridDim.x - sums.blocks;
     const int units = (cols + 7) / 8;
     const long long total = (long long)rows * units;
-    for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
+    for (long long i = block * (long long)blockDim.x + threadIdx.x; i < total; i += (long long)blocks * blockDim.x) {
         const long long r = i / units;
         const int c0 = int(i - r * units) * 8;
         const int b = c0 / FP8_BLOCK;
@@ -684,18 +727,21 @@ __global__ void __launch_bounds__(kThreads) dequantize_rows_kernel(const uint8_t
 }
 
 template <typename T>
-void act_backward_typed(const T* dy, const uint8_t* z8, const float* z_scales, int act, T* dz, long long ld_dz, float* db,
-                        int rows, int cols, cudaStream_t stream) {
+ColumnSums act_backward_typed(const T* dy, const uint8_t* z8, const float* z_scales, int act, T* dz, long long ld_dz, float* db,
+                              int rows, int cols, cudaStream_t stream) {
     const bool vec = cols % 8 == 0 && reinterpret_cast<uintptr_t>(dy) % 16 == 0 && reinterpret_cast<uintptr_t>(z8) % 8 == 0;
     // Bands of the grid's second dimension (at most 65535); 64 rows keep the last wave of CTAs full for large matrices.
     const int least = (rows / 65535 + 32) / 32 * 32;
     const int rows_per = std::max(rows > 4096 ? 64 : 32, least);
     const int bands = (rows + rows_per - 1) / rows_per;
-    Scratch partial;
+    ColumnSums sums;
     float* to = db;
     if (db != nullptr && bands > 1) {
-        partial = Scratch(size_t(bands) * cols * sizeof(float), stream);
-        to = static_cast<float*>(partial.ptr);
+        sums.partial = Scratch(size_t(bands) * cols * sizeof(float), stream);
+        sums.bands = bands;
+        sums.cols = cols;
+        sums.out = db;
+        to = static_cast<float*>(sums.partial.ptr);
     }
     const dim3 grid((cols + 255) / 256, bands);
     auto launch = [&](auto code) {
@@ -709,10 +755,18 @@ void act_backward_typed(const T* dy, const uint8_t* z8, const float* z_scales, i
     else if (act == EPI_SIGMOID) launch(std::integral_constant<int, EPI_SIGMOID>{});
     else launch(std::integral_constant<int, EPI_NONE>{});
     CB200_CHECK_LAUNCH();
-    if (to != db) {
-        launch_dependent(add_bands_kernel, dim3((cols + 31) / 32), kThreads, stream, to, bands, cols, db);
-        CB200_CHECK_LAUNCH();
-    }
+    return sums;
+}
+
+// The part of a pass over `sums`; none without any.
+Bands bands_of(const ColumnSums& sums) {
+    Bands p{};
+    p.partial = static_cast<const float*>(sums.partial.ptr);
+    p.bands = sums.bands;
+    p.cols = sums.cols;
+    p.out = sums.out;
+    p.blocks = sums.out != nullptr ? unsigned((sums.cols + 31) / 32) : 0u;
+    return p;
 }
 
 template <typename T>
@@ -779,24 +833,38 @@ void quantize_typed(const T* x, long long rows, int cols, int block_rows, uint8_
 
 }  // namespace
 
-AlignedRows aligned_rows(const void* src, long long rows, int cols, int elem_size, cudaStream_t stream, const int32_t* offsets,
-                         int rows_group) {
-    AlignedRows out;
-    const int per_unit = 16 / elem_size;
-    if (cols % per_unit == 0 && reinterpret_cast<uintptr_t>(src) % 16 == 0) {
-        out.ptr = src;
-        out.ld = cols;
-        return out;
+PreparedRows prepare_rows(const RowsRequest& a, const RowsRequest& b, const ScaleTops& tops, cudaStream_t stream) {
+    PreparedRows out;
+    PrepareParams p{};
+    long long blocks = 0;
+    auto add = [&](const RowsRequest& m, AlignedRows& to, PadJob& job) {
+        if (m.src == nullptr) return;
+        const int per_unit = 16 / m.elem_size;
+        if (m.ld != 0 || (m.cols % per_unit == 0 && reinterpret_cast<uintptr_t>(m.src) % 16 == 0)) {
+            to.ptr = m.src;
+            to.ld = m.ld != 0 ? m.ld : m.cols;
+            return;
+        }
+        const int units = (m.cols + per_unit - 1) / per_unit;
+        to.ld = (long long)units * per_unit;
+        to.copy = Scratch(size_t(m.rows) * units * 16, stream);
+        to.ptr = to.copy.ptr;
+        const long long chunks = (units + 31) / 32, ctas = (m.rows + kThreads / 32 - 1) / (kThreads / 32) * chunks;
+        CB200_REQUIRE(ctas <= 1000000000ll, "matrix too large");      // two of them in a grid
+        job = PadJob{static_cast<const uint8_t*>(m.src), static_cast<uint8_t*>(to.copy.ptr), m.rows, m.cols * m.elem_size, units * 16,
+                     m.offsets, m.rows_group, unsigned(chunks), unsigned(ctas)};
+        blocks += ctas;
+    };
+    add(a, out.a, p.pad[0]);
+    add(b, out.b, p.pad[1]);
+    if (tops.top != nullptr) {
+        p.scales = tops.scales;
+        p.scale_rows = tops.rows;
+        p.top = tops.top;
+        blocks += (tops.cols + FP8_BLOCK - 1) / FP8_BLOCK;
     }
-    const int units = (cols + per_unit - 1) / per_unit;
-    out.ld = (long long)units * per_unit;
-    out.copy = Scratch(size_t(rows) * units * 16, stream);
-    out.ptr = out.copy.ptr;
-    CB200_REQUIRE((rows + 7) / 8 <= 2147483647ll && (units + 31) / 32 <= 65535, "matrix too large");      // the grid
-    const dim3 grid(unsigned((rows + kThreads / 32 - 1) / (kThreads / 32)), unsigned((units + 31) / 32));
-    launch_dependent(pad_rows_kernel, grid, kThreads, stream,
-                     static_cast<const uint8_t*>(src), static_cast<uint8_t*>(out.copy.ptr), rows, cols * elem_size,
-                     units * 16, offsets, rows_group);
+    if (blocks == 0) return out;
+    launch_dependent(prepare_kernel, dim3(unsigned(blocks)), kThreads, stream, p);
     CB200_CHECK_LAUNCH();
     return out;
 }
@@ -823,33 +891,35 @@ void dequantize_fp8(const uint8_t* q, const float* scales, long long rows, int c
     CB200_CHECK_LAUNCH();
 }
 
-void activation_backward_fp8(const void* dy, int type, const uint8_t* z8, const float* z_scales, int act, void* dz,
-                             long long ld_dz, float* db, int rows, int cols, cudaStream_t stream) {
+ColumnSums activation_backward_fp8(const void* dy, int type, const uint8_t* z8, const float* z_scales, int act, void* dz,
+                                   long long ld_dz, float* db, int rows, int cols, cudaStream_t stream) {
     if (type == TYPE_F16)
-        act_backward_typed(static_cast<const __half*>(dy), z8, z_scales, act, static_cast<__half*>(dz), ld_dz, db, rows, cols,
-                           stream);
-    else
-        act_backward_typed(static_cast<const __nv_bfloat16*>(dy), z8, z_scales, act, static_cast<__nv_bfloat16*>(dz), ld_dz, db,
-                           rows, cols, stream);
+        return act_backward_typed(static_cast<const __half*>(dy), z8, z_scales, act, static_cast<__half*>(dz), ld_dz, db, rows,
+                                  cols, stream);
+    return act_backward_typed(static_cast<const __nv_bfloat16*>(dy), z8, z_scales, act, static_cast<__nv_bfloat16*>(dz), ld_dz, db,
+                              rows, cols, stream);
 }
 
-void block_tops(const float* scales, int rows, int cols, float* top, cudaStream_t stream) {
-    launch_dependent(block_tops_kernel, dim3((cols + FP8_BLOCK - 1) / FP8_BLOCK), kThreads, stream, scales, rows, top);
+void finish_sums(const ColumnSums& sums, cudaStream_t stream) {
+    const Bands p = bands_of(sums);
+    if (p.blocks == 0) return;
+    launch_dependent(add_bands_kernel, dim3(p.blocks), kThreads, stream, p);
     CB200_CHECK_LAUNCH();
 }
 
 void dequantize_rows(const uint8_t* q, const float* scales, const float* top, int rows, int cols, void* y, long long ld_y,
-                     int y_type, cudaStream_t stream) {
+                     int y_type, const ColumnSums& sums, cudaStream_t stream) {
+    const Bands bands = bands_of(sums);
     const bool vec = cols % 8 == 0 && reinterpret_cast<uintptr_t>(q) % 8 == 0;
-    const unsigned grid = pass_grid((long long)rows * ((cols + 7) / 8));
+    const unsigned grid = bands.blocks + pass_grid((long long)rows * ((cols + 7) / 8));
     if (y_type == TYPE_F16) {
         __half* out = static_cast<__half*>(y);
-        if (vec) launch_dependent(dequantize_rows_kernel<__half, true>, dim3(grid), kThreads, stream, q, scales, top, rows, cols, out, ld_y);
-        else launch_dependent(dequantize_rows_kernel<__half, false>, dim3(grid), kThreads, stream, q, scales, top, rows, cols, out, ld_y);
+        if (vec) launch_dependent(dequantize_rows_kernel<__half, true>, dim3(grid), kThreads, stream, q, scales, top, rows, cols, out, ld_y, bands);
+        else launch_dependent(dequantize_rows_kernel<__half, false>, dim3(grid), kThreads, stream, q, scales, top, rows, cols, out, ld_y, bands);
     } else {
         __nv_bfloat16* out = static_cast<__nv_bfloat16*>(y);
-        if (vec) launch_dependent(dequantize_rows_kernel<__nv_bfloat16, true>, dim3(grid), kThreads, stream, q, scales, top, rows, cols, out, ld_y);
-        else launch_dependent(dequantize_rows_kernel<__nv_bfloat16, false>, dim3(grid), kThreads, stream, q, scales, top, rows, cols, out, ld_y);
+        if (vec) launch_dependent(dequantize_rows_kernel<__nv_bfloat16, true>, dim3(grid), kThreads, stream, q, scales, top, rows, cols, out, ld_y, bands);
+        else launch_dependent(dequantize_rows_kernel<__nv_bfloat16, false>, dim3(grid), kThreads, stream, q, scales, top, rows, cols, out, ld_y, bands);
     }
     CB200_CHECK_LAUNCH();
 }

@@ -17,10 +17,28 @@ struct AlignedRows {
     long long ld = 0;      // elements between rows
     Scratch copy;          // holds ptr where the caller's matrix had to be copied
 };
-// The caller's matrix itself where it qualifies, else a copy with zero-padded rows.  With `offsets` (device), rows_group rows belong
-// to each of their groups, and groups without rows need not be copied.
-AlignedRows aligned_rows(const void* src, long long rows, int cols, int elem_size, cudaStream_t stream,
-                         const int32_t* offsets = nullptr, int rows_group = 1);
+// A matrix that is wanted so; src may be nullptr.  With `offsets` (device), rows_group rows belong to each of their groups, and
+// groups without rows need not be copied.
+struct RowsRequest {
+    const void* src = nullptr;
+    long long rows = 0;
+    int cols = 0;
+    int elem_size = 1;
+    long long ld = 0;      // nonzero: its rows qualify already, that many elements apart
+    const int32_t* offsets = nullptr;
+    int rows_group = 1;
+};
+// top[b] = the largest finite scale of column block b; nothing with top == nullptr.
+struct ScaleTops {
+    const float* scales = nullptr;      // [block][rows]
+    int rows = 0, cols = 0;
+    float* top = nullptr;
+};
+struct PreparedRows {
+    AlignedRows a, b;
+};
+// The callers' matrices themselves where they qualify, else copies with zero-padded rows; all that is to be done in one launch.
+PreparedRows prepare_rows(const RowsRequest& a, const RowsRequest& b, const ScaleTops& tops, cudaStream_t stream);
 
 // dst = src, rounded to dst_type.
 void cast(const void* src, int src_type, void* dst, int dst_type, long long count, cudaStream_t stream);
@@ -32,16 +50,21 @@ void quantize_fp8(const void* x, int x_type, long long rows, int cols, int block
 void dequantize_fp8(const uint8_t* q, const float* scales, long long rows, int cols, int block_rows, void* y, int y_type,
                     cudaStream_t stream);
 
-
+// Column sums on their way: of each band of rows, to be added up by finish_sums or along with dequantize_rows.
+struct ColumnSums {
+    Scratch partial;
+    int bands = 0, cols = 0;
+    float* out = nullptr;      // nullptr: nothing is left to do
+};
 // dz = dy * act'(z8 * z_scales), rounded to dy's type, rows ld_dz elements apart (zeros behind cols); dz may be nullptr.
-// db[cols] = column sums of dz before its rounding; db may be nullptr.  type: TYPE_F16 or TYPE_BF16.
-void activation_backward_fp8(const void* dy, int type, const uint8_t* z8, const float* z_scales, int act, void* dz,
-                             long long ld_dz, float* db, int rows, int cols, cudaStream_t stream);
-// y = q * (s / top[b]) in a 16-bit type, rows ld_y elements apart, for blocks of 1 x 128; top[b] = the largest finite
-// scale of column block b.  With top == nullptr: y = q * s.
-void block_tops(const float* scales, int rows, int cols, float* top, cudaStream_t stream);
+// db[cols] = column sums of dz before its rounding, once the result is finished; db may be nullptr.  type: TYPE_F16 or TYPE_BF16.
+ColumnSums activation_backward_fp8(const void* dy, int type, const uint8_t* z8, const float* z_scales, int act, void* dz,
+                                   long long ld_dz, float* db, int rows, int cols, cudaStream_t stream);
+void finish_sums(const ColumnSums& sums, cudaStream_t stream);
+// y = q * (s / top[b]) in a 16-bit type, rows ld_y elements apart, for blocks of 1 x 128; with top == nullptr: y = q * s.
+// Finishes `sums` as well.
 void dequantize_rows(const uint8_t* q, const float* scales, const float* top, int rows, int cols, void* y, long long ld_y,
-                     int y_type, cudaStream_t stream);
+                     int y_type, const ColumnSums& sums, cudaStream_t stream);
 
 // out[m, n] = sum over `parts` of part[parts][m][ld], in order, rounded to `type`.  ld is a multiple of 4.
 void add_parts(const float* part, int parts, int m, int n, long long ld, void* out, int type, cudaStream_t stream);
