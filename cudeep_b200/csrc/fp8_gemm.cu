@@ -7,9 +7,6 @@
 #include "ragged_plan.h"
 
 #include <algorithm>
-#include <map>
-#include <mutex>
-#include <utility>
 
 namespace cudeep_b200 {
 
@@ -21,33 +18,9 @@ struct FewPlan {
     double cost;    // cycles
 };
 
-// Clusters of `size` CTAs, an SM each, that the device runs at once: fewer than SMs / size, as a cluster lies within one
-// part of the chip.  (148 CTAs as 37 clusters of four took two turns: 1 row, 4096 -> 4096 13.2 us, 128 CTAs 8.1 us.)
-int resident_clusters(int size) {
-    static std::mutex mu;
-    static std::map<std::pair<int, int>, int> known;
-    const DeviceInfo& dev = device_info();
-    if (size == 1) return dev.num_sms;
-    std::lock_guard<std::mutex> lock(mu);
-    const auto key = std::make_pair(dev.device, size);
-    const auto at = known.find(key);
-    if (at != known.end()) return at->second;
-    auto kernel = fp8_few_kernel<RaggedForm::NT, float>;
-    ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), FP8F_SMEM_BUDGET + 1024);
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(unsigned(size), 1, 1);
-    cfg.blockDim = dim3(FP8F_THREADS, 1, 1);
-    cfg.dynamicSmemBytes = FP8F_SMEM_BUDGET + 1024;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = unsigned(size);
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    int count = 0;
-    CB200_CUDA(cudaOccupancyMaxActiveClusters(&count, kernel, &cfg));
-    return known[key] = count < 1 ? 1 : count;
+int few_clusters(int size) {
+    return resident_clusters(reinterpret_cast<const void*>(fp8_few_kernel<RaggedForm::NT, float>), size, FP8F_THREADS,
+                             FP8F_SMEM_BUDGET + 1024);
 }
 
 // The cheapest of all steps and splits by what an SM's stream of operands costs, in cycles: weights that one tile reads come
@@ -61,7 +34,7 @@ FewPlan plan_few(int rows, int features, int k) {
     for (int step = 128; step >= 64; step -= 16) {
         for (int split = 1; split <= 8; split *= 2) {
             if (split > 1 && blocks < 4 * split) break;      // four blocks of K for each CTA at least
-            const long long tiles = (long long)((features + step - 1) / step) * row_tiles, resident = resident_clusters(split);
+            const long long tiles = (long long)((features + step - 1) / step) * row_tiles, resident = few_clusters(split);
             const long long waves = (tiles + resident - 1) / resident;
             const double loads = step * 128 / (row_tiles == 1 ? PLAN_HBM_BYTES : PLAN_L2_BYTES) + loaded * 128 / PLAN_L2_BYTES;
             const double sums = 200.0 + 4.0 * tile_rows;      // taking a block's accumulators out

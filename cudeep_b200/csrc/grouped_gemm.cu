@@ -47,14 +47,15 @@ void launch(RaggedParams& p, const RaggedPlan& plan, cudaStream_t stream) {
     p.stages = fit < RAGGED_MAX_STAGES ? fit : RAGGED_MAX_STAGES;
     p.status = dev.status_word;
     p.wait_limit_ns = 2000000000ull;
-    long long clusters = dev.num_sms / CTAS;
+    p.split = plan.split;
+    long long clusters = plan.split > 1 ? plan.units : dev.num_sms / CTAS;
     if (clusters > plan.units) clusters = plan.units;
     const uint32_t smem_bytes = uint32_t(p.stages) * p.stage_bytes + fixed + 1024;
-    CB200_TRACE("grouped %s %s tcgen05: rows=%d groups=%d features=%d %s=%d tile=%dx%d stages=%d clusters=%lld",
+    CB200_TRACE("grouped %s %s tcgen05: rows=%d groups=%d features=%d %s=%d tile=%dx%d split=%d stages=%d clusters=%lld",
                 FORM == RaggedForm::NT ? "nt" : FORM == RaggedForm::NN ? "nn" : "tn", BF16 ? "bf16" : "f16", p.rows, p.groups,
                 p.features, FORM == RaggedForm::TN ? "cols" : "k", FORM == RaggedForm::TN ? p.cols : p.k, 128 * CTAS,
-                plan.tile_cols, p.stages, clusters);
-    launch_clusters(ragged_gemm_kernel<FORM, CTAS, BF16, OutT>, p, clusters, CTAS, RAGGED_THREADS, smem_bytes,
+                plan.tile_cols, plan.split, p.stages, clusters);
+    launch_clusters(ragged_gemm_kernel<FORM, CTAS, BF16, OutT>, p, clusters, CTAS * plan.split, RAGGED_THREADS, smem_bytes,
                     RAGGED_SMEM_BUDGET + 1024, stream);
 }
 
@@ -107,7 +108,10 @@ void rows_by_weight(bool nn, const void* a, long long lda, const void* w, long l
     p.features = n;
     p.k = k;
     p.chunk_rows = RAGGED_BK;
-    const RaggedPlan plan = plan_rows(groups, rows, n, (k + RAGGED_BK - 1) / RAGGED_BK);
+    const RaggedPlan plan = plan_rows(groups, rows, n, (k + RAGGED_BK - 1) / RAGGED_BK, [](int size) {
+        return resident_clusters(reinterpret_cast<const void*>(ragged_gemm_kernel<RaggedForm::NT, 1, true, __nv_bfloat16>), size,
+                                 RAGGED_THREADS, RAGGED_SMEM_BUDGET + 1024);
+    });
     if (nn) launch_rows<RaggedForm::NN>(p, plan, type, stream);
     else launch_rows<RaggedForm::NT>(p, plan, type, stream);
 }

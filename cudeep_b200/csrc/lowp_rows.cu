@@ -48,7 +48,7 @@ __device__ __forceinline__ void pad_rows(const PadJob& job, unsigned block) {
     const long long r = block / job.chunks * (long long)(kThreads / 32) + (threadIdx.x >> 5);
     if (r >= rows) return;
     if (job.offsets != nullptr) {
-        const int g = int(r / job.rows_group);
+        const int g = rows <= 0x7fffffff ? int(unsigned(r) / unsigned(job.rows_group)) : int(r / job.rows_group);
         if (__ldg(job.offsets + g + 1) <= __ldg(job.offsets + g)) return;
     }
     const uint8_t* row = src + r * row_bytes;

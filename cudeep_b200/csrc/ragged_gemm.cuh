@@ -85,6 +85,9 @@ struct RaggedParams {
     int features;            // F
     int cols;                // TN: C
     int k;                   // NT, NN: length of the sums
+    // NT, NN of single CTAs: CTAs per tile, a cluster, each with a range of the sums' blocks.  More than one only where every
+    // cluster has one tile at most.
+    int split;
     int tile_cols;           // columns of a tile at most: rows of a group (NT, NN) or C (TN); <= 256
     int stages;
     uint32_t stage_bytes;
@@ -308,6 +311,9 @@ __global__ void __launch_bounds__(RAGGED_THREADS, 1) ragged_gemm_kernel(const __
         ptx::tmem_alloc<CTAS>(ptx::smem_u32(&tmem_base_holder), 512);
         ptx::tmem_relinquish<CTAS>();
     }
+    constexpr bool SPLITS = FORM != RaggedForm::TN && CTAS == 1;
+    const int split = SPLITS ? p.split : 1;
+    const int split_rank = SPLITS && split > 1 ? int(ptx::cluster_ctarank()) : 0;
     ptx::grid_dependency_wait();      // the offsets may come from the kernel before
     const int f_tiles = (p.features + 128 * CTAS - 1) / (128 * CTAS);
     const int c_tiles_tn = FORM == RaggedForm::TN ? (p.cols + p.tile_cols - 1) / p.tile_cols : 0;
@@ -324,11 +330,16 @@ __global__ void __launch_bounds__(RAGGED_THREADS, 1) ragged_gemm_kernel(const __
     const uint32_t tmem_base = tmem_base_holder;
     ptx::grid_launch_dependents();
 
-    const int unit_stride = gridDim.x / CTAS;
-    const int first_unit = blockIdx.x / CTAS;
+    const int first_unit = int(blockIdx.x) / (CTAS * split);
     RaggedWalk<FORM, CTAS> walk{group_rows, group_start, p.groups, f_tiles, c_tiles_tn, p.tile_cols, p.features, p.cols};
     const int num_units = walk.total();
-    const int k_blocks_row = FORM == RaggedForm::TN ? 0 : (p.k + RAGGED_BK - 1) / RAGGED_BK;
+    // A split tile is its cluster's only one (with bad offsets there may be more tiles: those are left out).
+    const int unit_stride = split > 1 ? num_units : int(gridDim.x) / CTAS;
+    // Blocks of this CTA's sums, k_first on; a split tile's last CTAs may have none.
+    const int k_blocks_all = FORM == RaggedForm::TN ? 0 : (p.k + RAGGED_BK - 1) / RAGGED_BK;
+    const int k_share = split > 1 ? ((k_blocks_all + split - 1) / split + p.atoms - 1) / p.atoms * p.atoms : k_blocks_all;
+    const int k_first = min(k_blocks_all, split_rank * k_share);
+    const int k_blocks_row = min(k_share, k_blocks_all - k_first);
     // TN: blocks of a chunk of the group's rows that starts at `row`.
     auto chunk_blocks = [&](const RaggedTile& t, int row) {
         return (min(p.chunk_rows, t.row1 - row) + RAGGED_BK - 1) / RAGGED_BK;
@@ -364,7 +375,7 @@ __global__ void __launch_bounds__(RAGGED_THREADS, 1) ragged_gemm_kernel(const __
                     for (int a = 0; a < p.atoms; ++a) {
                         const uint32_t a_smem = smem_base + stage * p.stage_bytes + a * p.atom_bytes;
                         const uint32_t b_smem = a_smem + RAGGED_A_BYTES;
-                        const int k0 = (kb + a) * RAGGED_BK;
+                        const int k0 = (k_first + kb + a) * RAGGED_BK;
                         if constexpr (FORM == RaggedForm::NT) {
                             if constexpr (CTAS == 2) ptx::tma_load_3d_pair(a_smem, &p.map_a, full, k0, feature, t.group);
                             else ptx::tma_load_3d(a_smem, &p.map_a, full, k0, feature, t.group);
@@ -551,14 +562,37 @@ __global__ void __launch_bounds__(RAGGED_THREADS, 1) ragged_gemm_kernel(const __
                 } while (row < t.row1);
             } else {
                 const int feature = t.feature0 + int(cta_rank) * 128 + int(quarter) * 32 + int(lane);
+                const int c_half = (t.umma_n / 2 + 31) / 32 * 32;      // warps 6..9 take the second half of the columns
+                const int c_begin = (int(warp - 2) >> 2) * c_half, c_end = min(t.col_count, c_begin + c_half);
                 const uint32_t acc = it & 1;
+                if (SPLITS && split > 1) {
+                    // The stage ring is idle once the last MMA is done: it takes this CTA's part, [column][128 features].
+                    const uint32_t part = smem_base + (quarter * 32u + lane) * 4u;
+                    if (k_blocks_row > 0) {
+                        const bool ok = ptx::mbar_wait(ptx::smem_u32(&bar_acc_full[0]), 0, wctx, UMMA_TIMEOUT_EPILOGUE);
+                        if (!__all_sync(0xffffffffu, ok)) goto epilogue_done;
+                        ptx::tc_fence_after();
+                    }
+                    for (int c = c_begin; c < c_end; c += 32) {
+                        uint32_t r[32];
+                        if (k_blocks_row > 0) {
+                            ptx::tmem_ld_32x32(tmem_base + ((quarter * 32u) << 16) + c, r);
+                            ptx::tmem_ld_wait(r);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) r[j] = 0u;
+                        }
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (c + j < c_end) ptx::st_shared_f32(part + uint32_t(c + j) * 512u, __uint_as_float(r[j]));
+                    }
+                    continue;
+                }
                 const bool ok = ptx::mbar_wait(ptx::smem_u32(&bar_acc_full[acc]), (it >> 1) & 1, wctx, UMMA_TIMEOUT_EPILOGUE);
                 if (!__all_sync(0xffffffffu, ok)) goto epilogue_done;
                 ptx::tc_fence_after();
                 const uint32_t t_row = tmem_base + acc * 256u + ((quarter * 32u) << 16);
                 OutT* dst = static_cast<OutT*>(p.c) + (long long)t.col0 * p.features + feature;
-                const int c_half = (t.umma_n / 2 + 31) / 32 * 32;      // warps 6..9 take the second half of the columns
-                const int c_begin = (int(warp - 2) >> 2) * c_half, c_end = min(t.col_count, c_begin + c_half);
                 for (int c = c_begin; c < c_end; c += 32) {
                     uint32_t r[32];
                     ptx::tmem_ld_32x32(t_row + c, r);
@@ -585,6 +619,36 @@ __global__ void __launch_bounds__(RAGGED_THREADS, 1) ragged_gemm_kernel(const __
         if (CTAS == 2) ptx::cluster_arrive();
         if (FORM == RaggedForm::TN && lane == 0) ptx::bulk_wait_group_read<0>();      // bulk stores still read shared memory
         __syncwarp();
+    }
+
+    if constexpr (SPLITS) {
+        if (split > 1) {
+            __syncwarp();
+            ptx::cluster_arrive();
+            ptx::cluster_wait();
+            if (warp >= 2 && first_unit < num_units) {
+                // Rank r finishes columns r, r + split, ...: a warp a column, four features a lane, the parts in rank order.
+                const RaggedTile t = walk.at(first_unit);
+                const int f = t.feature0 + 4 * int(lane);
+                for (int c = split_rank + split * int(warp - 2); c < t.col_count; c += split * RAGGED_EPI_WARPS) {
+                    float v[4] = {};
+                    for (int r = 0; r < split; ++r) {
+                        const float4 q = ptx::ld_cluster_v4(ptx::mapa(smem_base + uint32_t(c) * 512u + lane * 16u, uint32_t(r)));
+                        v[0] += q.x;
+                        v[1] += q.y;
+                        v[2] += q.z;
+                        v[3] += q.w;
+                    }
+                    OutT* dst = static_cast<OutT*>(p.c) + (long long)(t.col0 + c) * p.features + f;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (f + j < p.features) dst[j] = round_to<OutT>(v[j]);
+                }
+            }
+            __syncwarp();
+            ptx::cluster_arrive();      // nobody leaves while its part may still be read
+            ptx::cluster_wait();
+        }
     }
 
     // ---------------------------------------------------------------- teardown

@@ -6,6 +6,9 @@
 
 #include <algorithm>
 #include <cmath>
+#include <map>
+#include <mutex>
+#include <tuple>
 
 namespace cudeep_b200 {
 
@@ -14,19 +17,55 @@ struct RaggedPlan {
     int tile_cols;        // columns of a tile at most
     long long units;      // most tiles there can be, whatever the group sizes
     double cost;          // estimate in cycles
+    int split = 1;        // CTAs that share a tile of one CTA, each with a range of the sums
 };
 
 // An SM takes in about 41 bytes of operands a cycle from L2, 20 from HBM (measured: 16 KB boxes, all SMs loading), and a K
 // block of 128 bytes per row costs two cycles of MMAs per column on 128 lanes.
 constexpr double PLAN_L2_BYTES = 41.0, PLAN_HBM_BYTES = 20.0, PLAN_MMA_CYCLES = 2.0;
 
+// Clusters of `size` CTAs of a kernel, an SM each, that the device runs at once: fewer than SMs / size, as a cluster lies within
+// one part of the chip.  (148 CTAs as 37 clusters of four took two turns: 1 row, 4096 -> 4096 in 8 bits 13.2 us, 128 CTAs
+// 8.1 us.)
+inline int resident_clusters(const void* kernel, int size, int threads, size_t smem_bytes) {
+    static std::mutex mu;
+    static std::map<std::tuple<int, const void*, int>, int> known;
+    const DeviceInfo& dev = device_info();
+    if (size == 1) return dev.num_sms;
+    std::lock_guard<std::mutex> lock(mu);
+    const auto key = std::make_tuple(dev.device, kernel, size);
+    const auto at = known.find(key);
+    if (at != known.end()) return at->second;
+    ensure_dynamic_smem(kernel, int(smem_bytes));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(size), 1, 1);
+    cfg.blockDim = dim3(unsigned(threads), 1, 1);
+    cfg.dynamicSmemBytes = smem_bytes;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = unsigned(size);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int count = 0;
+    CB200_CUDA(cudaOccupancyMaxActiveClusters(&count, kernel, &cfg));
+    return known[key] = count < 1 ? 1 : count;
+}
+
 // Rows of `groups` groups, `rows` in all, on the columns of the tiles; `blocks` K blocks.  Sizes of the groups are not known
 // here, so the cost of each choice is that of groups of equal size: waves of tiles, each its K blocks at the slower of
 // loads and MMAs and a start and an end that nothing hides.  Weights that only one tile of a group reads come from HBM.
-inline RaggedPlan plan_rows(int groups, int rows, int features, int blocks) {
+//
+// Where there are few tiles (a token or two for each expert), clusters share them, if each cluster then has one at most
+// (7 rows of 31 groups, 4096 -> 208: 23.4 us with a CTA to a tile, 7.8 us with eight; 1 row, 4096 -> 4096: 23.1 and 10.0 us).
+// clusters(size): how many the device runs at once.
+template <class Clusters>
+RaggedPlan plan_rows(int groups, int rows, int features, int blocks, Clusters clusters) {
     const int sms = device_info().num_sms;
     const int used = groups < rows ? groups : rows;
     const double size = double(rows) / used;
+    const int most = (rows + 31) / 32 * 32;
     RaggedPlan best{2, 256, 0, 1e30};
     for (int ctas = 2; ctas >= 1; --ctas) {
         const long long f_tiles = (features + 128 * ctas - 1) / (128 * ctas);
@@ -39,9 +78,14 @@ inline RaggedPlan plan_rows(int groups, int rows, int features, int blocks) {
             const double loads = 16384.0 / (per_group == 1 ? PLAN_HBM_BYTES : PLAN_L2_BYTES) + width / ctas * 128 / PLAN_L2_BYTES;
             const double cost = waves * (blocks * std::max(loads, PLAN_MMA_CYCLES * width) + 2500.0 + 8.0 * width);
             if (cost < 0.97 * best.cost) best = RaggedPlan{ctas, tile, 0, cost};
+            if (ctas == 2 || tile > 128) continue;      // the parts of a tile lie in the stages' memory
+            for (int split = 2; split <= 8 && blocks >= 4 * split; split *= 2) {
+                if (f_tiles * (rows / std::min(tile, most) + used) > clusters(split)) break;
+                const double shared = (blocks + split - 1) / split * std::max(loads, PLAN_MMA_CYCLES * width) + 4500.0 + 28.0 * width;
+                if (shared < 0.97 * best.cost) best = RaggedPlan{ctas, tile, 0, shared, split};
+            }
         }
     }
-    const int most = (rows + 31) / 32 * 32;
     if (best.tile_cols > most) best.tile_cols = most;
     best.units = (features + 128ll * best.ctas - 1) / (128 * best.ctas) * (rows / best.tile_cols + used);
     return best;

@@ -105,3 +105,52 @@ def test_tn(dev, sizes, n, k, dtype, out):
         r = slice(off[g], off[g + 1])
         a, b = dy[r].double(), x[r].double()
         close(torch, dw[g], a.t() @ b, a.abs().t() @ b.abs(), max(1, sizes[g]))
+
+
+# Few tiles of long sums: clusters of CTAs share them, each with a range of K.
+FEW = [
+    ([1], 64, 4096),
+    ([3, 0, 2, 1], 130, 2050),
+    ([20, 0, 13], 256, 1600),
+    ([100], 300, 1100),
+    ([0, 1, 0, 0, 2] + [0] * 20 + [1, 0, 3, 0, 0, 1], 208, 4091),
+    ([5, 6], 512, 520),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("sizes,features,k", FEW)
+def test_few_tiles_of_long_sums(dev, sizes, features, k, dtype):
+    """nt sums over k, nn the transposed weight over k: as the other sizes, and the same bits again."""
+    torch = dev.torch
+    t = {"f16": torch.float16, "bf16": torch.bfloat16}[dtype]
+    rows, off, offsets, x, w, _ = make(dev, sizes, features, k, t, 4, lead=1)
+    wt = w.transpose(1, 2).contiguous()
+    for name, weight in (("nt", w), ("nn", wt)):
+        results = []
+        for _ in range(2):
+            y = torch.full((rows, features), 7.0, dtype=t, device=dev.dev)
+            call(dev, name, dev.ptr(x), dev.ptr(weight), dev.ptr(y), TYPES[dtype], dev.ptr(offsets), len(sizes), rows, features, k,
+                 None)
+            results.append(y)
+        y = results[0]
+        assert torch.equal(y, results[1])
+        assert bool((y[:off[0]] == 7).all()) and bool((y[off[-1]:] == 7).all())
+        for g in range(len(sizes)):
+            r = slice(off[g], off[g + 1])
+            a, b = x[r].double(), w[g].double()
+            close(torch, y[r], a @ b.t(), a.abs() @ b.abs().t(), k)
+
+
+def test_few_tiles_with_bad_offsets(dev):
+    """Ranges that overlap make more tiles than the rows can have: reported, and nothing outside the matrix is written."""
+    torch = dev.torch
+    rows, n, k, groups = 4, 128, 4096, 12
+    x = torch.ones(rows, k, dtype=torch.bfloat16, device=dev.dev)
+    w = torch.ones(groups, n, k, dtype=torch.bfloat16, device=dev.dev)
+    offsets = torch.tensor([0, 4] * 6 + [0], dtype=torch.int32, device=dev.dev)
+    y = torch.full((rows + 8, n), 7.0, dtype=torch.bfloat16, device=dev.dev)
+    dev.check(dev.lib.cudeep_b200_grouped_matmul_nt(dev.ptr(x), dev.ptr(w), dev.ptr(y[4]), 2, dev.ptr(offsets), groups, rows, n, k,
+                                                    None))
+    assert dev.sync_status() == 6
+    assert bool((y[:4] == 7).all()) and bool((y[8:] == 7).all())
