@@ -2,7 +2,7 @@
 // in blocks and back.  All are bound by HBM: each input is read once and each output written once.
 //
 // Each kernel waits for its predecessors itself and then lets its successor be set up, so that in a sequence of small
-// launches (the backward pass of a short batch is nine) the launches overlap.
+// launches (the backward pass of a short batch is five) the launches overlap.
 #include "lowp_rows.h"
 
 #include "epilogue_math.cuh"
