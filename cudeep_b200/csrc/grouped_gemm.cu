@@ -76,7 +76,12 @@ void rows_by_weight(bool nn, const void* a, long long lda, const void* w, long l
     const PreparedRows operands = prepare_rows({a, rows, k, 2, lda}, {w, (long long)groups * w_rows, w_cols, 2, ldw, offsets, w_rows},
                                                {}, stream);
     const AlignedRows &x = operands.a, &wt = operands.b;
+    const RaggedPlan plan = plan_rows(groups, rows, n, (k + RAGGED_BK - 1) / RAGGED_BK, nn ? 128 : 64, [](int size) {
+        return resident_clusters(reinterpret_cast<const void*>(ragged_gemm_kernel<RaggedForm::NT, 1, true, __nv_bfloat16>), size,
+                                 RAGGED_THREADS, RAGGED_SMEM_BUDGET + 1024);
+    });
     RaggedParams p{};
+    p.step = plan.step;
     {
         const uint64_t row_bytes = uint64_t(wt.ld) * 2, group_bytes = row_bytes * uint64_t(w_rows);
         p.a_chunked = nn && wt.ld >= (w_cols + 63) / 64 * 64;
@@ -88,7 +93,7 @@ void rows_by_weight(bool nn, const void* a, long long lda, const void* w, long l
         } else {
             const uint64_t dims[3] = {uint64_t(w_cols), uint64_t(w_rows), uint64_t(groups)};
             const uint64_t strides[2] = {row_bytes, group_bytes};
-            const uint32_t box[3] = {64, nn ? 64u : 128u, 1};
+            const uint32_t box[3] = {64, nn ? 64u : uint32_t(plan.step), 1};
             encode_tensor_map_f16(&p.map_a, wt.ptr, 3, dims, strides, box, TmaSwizzle::B128);
         }
     }
@@ -108,10 +113,6 @@ void rows_by_weight(bool nn, const void* a, long long lda, const void* w, long l
     p.features = n;
     p.k = k;
     p.chunk_rows = RAGGED_BK;
-    const RaggedPlan plan = plan_rows(groups, rows, n, (k + RAGGED_BK - 1) / RAGGED_BK, [](int size) {
-        return resident_clusters(reinterpret_cast<const void*>(ragged_gemm_kernel<RaggedForm::NT, 1, true, __nv_bfloat16>), size,
-                                 RAGGED_THREADS, RAGGED_SMEM_BUDGET + 1024);
-    });
     if (nn) launch_rows<RaggedForm::NN>(p, plan, type, stream);
     else launch_rows<RaggedForm::NT>(p, plan, type, stream);
 }
@@ -177,6 +178,7 @@ void grouped_tn(const void* a, long long lda, const void* b, long long ldb, void
     RaggedParams p{};
     p.groups = parts > 1 ? parts : groups;
     p.share = parts > 1 ? ((rows + parts - 1) / parts + RAGGED_BK - 1) / RAGGED_BK * RAGGED_BK : rows;
+    p.step = 128;
     p.a_chunked = encode_columns(&p.map_a, y, rows, m, 2);
     p.b_chunked = encode_columns(&p.map_b, x, rows, n, plan.tile_cols / plan.ctas / 64);
     const uint32_t c_bytes = uint32_t(elem_bytes(out_type));

@@ -88,6 +88,7 @@ struct RaggedParams {
     // NT, NN of single CTAs: CTAs per tile, a cluster, each with a range of the sums' blocks.  More than one only where every
     // cluster has one tile at most.
     int split;
+    int step;                // features of a CTA's tile: 128; NT of single CTAs 64 to 128 (the last lanes then idle)
     int tile_cols;           // columns of a tile at most: rows of a group (NT, NN) or C (TN); <= 256
     int stages;
     uint32_t stage_bytes;
@@ -114,7 +115,7 @@ template <RaggedForm FORM, int CTAS>
 struct RaggedWalk {
     const int* off;
     const int* start;
-    int groups, f_tiles, c_tiles_tn, tile_cols, features, cols;
+    int groups, f_tiles, c_tiles_tn, tile_cols, features, cols, step;
     int g = 0;
 
     __device__ __forceinline__ int total() const { return start[groups]; }
@@ -142,7 +143,7 @@ struct RaggedWalk {
             t.col_count = min(share, t.row1 - t.col0);
             t.umma_n = max(unit, (t.col_count + unit - 1) / unit * unit);
         }
-        t.feature0 = ft * 128 * CTAS;
+        t.feature0 = ft * step * CTAS;
         return t;
     }
 };
@@ -315,7 +316,9 @@ __global__ void __launch_bounds__(RAGGED_THREADS, 1) ragged_gemm_kernel(const __
     const int split = SPLITS ? p.split : 1;
     const int split_rank = SPLITS && split > 1 ? int(ptx::cluster_ctarank()) : 0;
     ptx::grid_dependency_wait();      // the offsets may come from the kernel before
-    const int f_tiles = (p.features + 128 * CTAS - 1) / (128 * CTAS);
+    constexpr bool STEPS = FORM == RaggedForm::NT && CTAS == 1;
+    const int step = STEPS ? p.step : 128;
+    const int f_tiles = (p.features + step * CTAS - 1) / (step * CTAS);
     const int c_tiles_tn = FORM == RaggedForm::TN ? (p.cols + p.tile_cols - 1) / p.tile_cols : 0;
     if (warp == 0)
         group_tables(p.offsets, p.groups, p.rows, p.share, f_tiles, FORM == RaggedForm::TN ? c_tiles_tn : -p.tile_cols, group_rows,
@@ -331,7 +334,7 @@ __global__ void __launch_bounds__(RAGGED_THREADS, 1) ragged_gemm_kernel(const __
     ptx::grid_launch_dependents();
 
     const int first_unit = int(blockIdx.x) / (CTAS * split);
-    RaggedWalk<FORM, CTAS> walk{group_rows, group_start, p.groups, f_tiles, c_tiles_tn, p.tile_cols, p.features, p.cols};
+    RaggedWalk<FORM, CTAS> walk{group_rows, group_start, p.groups, f_tiles, c_tiles_tn, p.tile_cols, p.features, p.cols, step};
     const int num_units = walk.total();
     // A split tile is its cluster's only one (with bad offsets there may be more tiles: those are left out).
     const int unit_stride = split > 1 ? num_units : int(gridDim.x) / CTAS;
@@ -369,7 +372,7 @@ __global__ void __launch_bounds__(RAGGED_THREADS, 1) ragged_gemm_kernel(const __
                 if (!__all_sync(0xffffffffu, ok)) goto producer_done;
                 const uint32_t full_local = ptx::smem_u32(&bar_full[stage]);
                 const uint32_t full = CTAS == 2 ? ptx::mapa(full_local, 0) : full_local;
-                const uint32_t atom = RAGGED_A_BYTES + uint32_t(FORM == RaggedForm::TN ? per : RowMaps::loaded(per)) * 128u;
+                const uint32_t atom = (STEPS ? uint32_t(step) * 128u : RAGGED_A_BYTES) + uint32_t(FORM == RaggedForm::TN ? per : RowMaps::loaded(per)) * 128u;
                 if (lane == 0) {
                     // Blocks behind the last one load as zeros or are not multiplied.
                     for (int a = 0; a < p.atoms; ++a) {
@@ -562,6 +565,7 @@ __global__ void __launch_bounds__(RAGGED_THREADS, 1) ragged_gemm_kernel(const __
                 } while (row < t.row1);
             } else {
                 const int feature = t.feature0 + int(cta_rank) * 128 + int(quarter) * 32 + int(lane);
+                const int f_end = STEPS ? min(p.features, t.feature0 + step) : p.features;
                 const int c_half = (t.umma_n / 2 + 31) / 32 * 32;      // warps 6..9 take the second half of the columns
                 const int c_begin = (int(warp - 2) >> 2) * c_half, c_end = min(t.col_count, c_begin + c_half);
                 const uint32_t acc = it & 1;
@@ -597,7 +601,7 @@ __global__ void __launch_bounds__(RAGGED_THREADS, 1) ragged_gemm_kernel(const __
                     uint32_t r[32];
                     ptx::tmem_ld_32x32(t_row + c, r);
                     ptx::tmem_ld_wait(r);
-                    if (feature < p.features) {
+                    if (feature < f_end) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j)
                             if (c + j < c_end)
@@ -629,7 +633,7 @@ __global__ void __launch_bounds__(RAGGED_THREADS, 1) ragged_gemm_kernel(const __
             if (warp >= 2 && first_unit < num_units) {
                 // Rank r finishes columns r, r + split, ...: a warp a column, four features a lane, the parts in rank order.
                 const RaggedTile t = walk.at(first_unit);
-                const int f = t.feature0 + 4 * int(lane);
+                const int f = t.feature0 + 4 * int(lane), f_end = STEPS ? min(p.features, t.feature0 + step) : p.features;
                 for (int c = split_rank + split * int(warp - 2); c < t.col_count; c += split * RAGGED_EPI_WARPS) {
                     float v[4] = {};
                     for (int r = 0; r < split; ++r) {
@@ -642,7 +646,7 @@ __global__ void __launch_bounds__(RAGGED_THREADS, 1) ragged_gemm_kernel(const __
                     OutT* dst = static_cast<OutT*>(p.c) + (long long)(t.col0 + c) * p.features + f;
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        if (f + j < p.features) dst[j] = round_to<OutT>(v[j]);
+                        if (f + j < f_end) dst[j] = round_to<OutT>(v[j]);
                 }
             }
             __syncwarp();

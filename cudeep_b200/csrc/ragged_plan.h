@@ -18,6 +18,7 @@ struct RaggedPlan {
     long long units;      // most tiles there can be, whatever the group sizes
     double cost;          // estimate in cycles
     int split = 1;        // CTAs that share a tile of one CTA, each with a range of the sums
+    int step = 128;       // features of a CTA's tile
 };
 
 // An SM takes in about 41 bytes of operands a cycle from L2, 20 from HBM (measured: 16 KB boxes, all SMs loading), and a K
@@ -60,34 +61,42 @@ inline int resident_clusters(const void* kernel, int size, int threads, size_t s
 // Where there are few tiles (a token or two for each expert), clusters share them, if each cluster then has one at most
 // (7 rows of 31 groups, 4096 -> 208: 23.4 us with a CTA to a tile, 7.8 us with eight; 1 row, 4096 -> 4096: 23.1 and 10.0 us).
 // clusters(size): how many the device runs at once.
+//
+// Tiles of a single CTA that take all rows of a group may have fewer than 128 features, least_step at least, where that makes
+// fuller waves (64 rows of 16 groups, 1024 -> 4096: 512 tiles of 128 are four waves on 148 SMs, and so are 592 of 112: 27.2 us
+// and 26.0 us).
 template <class Clusters>
-RaggedPlan plan_rows(int groups, int rows, int features, int blocks, Clusters clusters) {
+RaggedPlan plan_rows(int groups, int rows, int features, int blocks, int least_step, Clusters clusters) {
     const int sms = device_info().num_sms;
     const int used = groups < rows ? groups : rows;
     const double size = double(rows) / used;
     const int most = (rows + 31) / 32 * 32;
     RaggedPlan best{2, 256, 0, 1e30};
-    for (int ctas = 2; ctas >= 1; --ctas) {
-        const long long f_tiles = (features + 128 * ctas - 1) / (128 * ctas);
-        for (int tile = 256; tile >= 32; tile /= 2) {
-            const int per_group = int((size + tile - 1) / tile);
-            const int width = int((size / per_group + 16 * ctas - 1) / (16 * ctas)) * 16 * ctas;
-            // Uneven groups: the last tile of a group is half empty on average.
-            const double tiles = double(f_tiles) * (groups == 1 ? per_group : used * (size / tile > 1 ? size / tile + 0.5 : 1.0));
-            const double waves = std::ceil(tiles * ctas / sms);
-            const double loads = 16384.0 / (per_group == 1 ? PLAN_HBM_BYTES : PLAN_L2_BYTES) + width / ctas * 128 / PLAN_L2_BYTES;
-            const double cost = waves * (blocks * std::max(loads, PLAN_MMA_CYCLES * width) + 2500.0 + 8.0 * width);
-            if (cost < 0.97 * best.cost) best = RaggedPlan{ctas, tile, 0, cost};
-            if (ctas == 2 || tile > 128) continue;      // the parts of a tile lie in the stages' memory
-            for (int split = 2; split <= 8 && blocks >= 4 * split; split *= 2) {
-                if (f_tiles * (rows / std::min(tile, most) + used) > clusters(split)) break;
-                const double shared = (blocks + split - 1) / split * std::max(loads, PLAN_MMA_CYCLES * width) + 4500.0 + 28.0 * width;
-                if (shared < 0.97 * best.cost) best = RaggedPlan{ctas, tile, 0, shared, split};
-            }
+    int fit[3] = {-1, -1, -1};
+    auto consider = [&](int ctas, int step, int tile) {
+        const long long f_tiles = (features + (long long)step * ctas - 1) / (step * ctas);
+        const int per_group = int((size + tile - 1) / tile);
+        const int width = int((size / per_group + 16 * ctas - 1) / (16 * ctas)) * 16 * ctas;
+        // Uneven groups: the last tile of a group is half empty on average.
+        const double tiles = double(f_tiles) * (groups == 1 ? per_group : used * (size / tile > 1 ? size / tile + 0.5 : 1.0));
+        const double waves = std::ceil(tiles * ctas / sms);
+        const double loads = step * 128 / (per_group == 1 ? PLAN_HBM_BYTES : PLAN_L2_BYTES) + width / ctas * 128 / PLAN_L2_BYTES;
+        const double cost = waves * (blocks * std::max(loads, PLAN_MMA_CYCLES * width) + 2500.0 + 8.0 * width);
+        if (cost < 0.97 * best.cost) best = RaggedPlan{ctas, tile, 0, cost, 1, step};
+        if (ctas == 2 || tile > 128) return;      // the parts of a tile lie in the stages' memory
+        for (int split = 2; split <= 8 && blocks >= 4 * split; split *= 2) {
+            int& count = fit[split == 2 ? 0 : split == 4 ? 1 : 2];
+            if (count < 0) count = clusters(split);
+            if (f_tiles * (rows / std::min(tile, most) + used) > count) break;
+            const double shared = (blocks + split - 1) / split * std::max(loads, PLAN_MMA_CYCLES * width) + 4500.0 + 28.0 * width;
+            if (shared < 0.97 * best.cost) best = RaggedPlan{ctas, tile, 0, shared, split, step};
         }
-    }
+    };
+    for (int tile = 256; tile >= 32; tile /= 2) consider(2, 128, tile);
+    for (int step = 128; step >= least_step; step -= 16)
+        for (int tile = 256; tile >= 32 && (step == 128 || tile >= size); tile /= 2) consider(1, step, tile);
     if (best.tile_cols > most) best.tile_cols = most;
-    best.units = (features + 128ll * best.ctas - 1) / (128 * best.ctas) * (rows / best.tile_cols + used);
+    best.units = (features + (long long)best.step * best.ctas - 1) / (best.step * best.ctas) * (rows / best.tile_cols + used);
     return best;
 }
 

@@ -107,7 +107,7 @@ def test_tn(dev, sizes, n, k, dtype, out):
         close(torch, dw[g], a.t() @ b, a.abs().t() @ b.abs(), max(1, sizes[g]))
 
 
-# Few tiles of long sums: clusters of CTAs share them, each with a range of K.
+# Few tiles of long sums: clusters of CTAs share them, each with a range of K; and few rows for each of many groups.
 FEW = [
     ([1], 64, 4096),
     ([3, 0, 2, 1], 130, 2050),
@@ -115,6 +115,9 @@ FEW = [
     ([100], 300, 1100),
     ([0, 1, 0, 0, 2] + [0] * 20 + [1, 0, 3, 0, 0, 1], 208, 4091),
     ([5, 6], 512, 520),
+    ([1] * 37, 520, 192),        # tiles of fewer than 128 features
+    ([4, 0, 9] * 5, 1000, 256),
+    ([2] * 70, 300, 72),
 ]
 
 
