@@ -35,6 +35,7 @@ __device__ __forceinline__ void fma2(float& d0, float& d1, uint32_t a0, uint32_t
 // exponents are held below 60 so that d0 d1 stays finite (sigmoid = 2^-60 there instead of less); g is held above -64, so
 // that no z however low makes more of that than 2^-54.  fminf also keeps a NaN from its neighbour, and the factor g carries
 // it on.  Where the formula has no cubic term b is a negligible number of the right sign instead of 0: 0 * Inf is NaN.
+// The two bounds of g cost 8192 x 4096 -> 16384 with GELU 440 -> 441.5 us (417 without an activation).
 struct Fp8Activation {
     int act;
     float a, b;
