@@ -29,13 +29,15 @@ __device__ __forceinline__ void fma2(float& d0, float& d1, uint32_t a0, uint32_t
         : "+f"(d0), "+f"(d1) : "r"(a0), "r"(a1), "f"(s0), "f"(s1));
 }
 
-// The epilogue's activations as one formula, y = g * sigmoid(a z + b z^3), g = z (GELU in its tanh form, SiLU) or 1
-// (sigmoid), with log2(e) folded into a and b.  Two values share one reciprocal, 1 / d0 = d1 / (d0 d1): the SFU is what bounds
-// an epilogue that activates 128 values a thread, and this takes three of its operations per pair instead of four.  The
-// exponents are held below 60 so that d0 d1 stays finite (sigmoid = 2^-60 there instead of less); g is held above -64, so
-// that no z however low makes more of that than 2^-54.  fminf also keeps a NaN from its neighbour, and the factor g carries
-// it on.  Where the formula has no cubic term b is a negligible number of the right sign instead of 0: 0 * Inf is NaN.
-// The two bounds of g cost 8192 x 4096 -> 16384 with GELU 440 -> 441.5 us (417 without an activation).
+// The epilogue's activations as one formula, y = g * sigmoid(t), g = z (GELU in its tanh form, SiLU) or 1 (sigmoid), with
+// -t log2(e) = u = z (a + b z^2).  sigmoid = 1 / d, d = 1 + 2^u, and two values share one reciprocal, 1 / d0 = d1 / (d0 d1): the
+// SFU is what bounds an epilogue that activates 128 values a thread, and this takes three of its operations per pair instead
+// of four.  u is held below 126, where sigmoid is FP32's least normal number, 2^-126, and so that d0 d1 stays finite d1 is
+// taken times 2^-126: the product then lies between 2^-126 and 2^126, and one more multiplication per pair takes that out of
+// 1 / d1: 8192 x 4096 -> 16384 with GELU 469.3 us in bursts, 467.6 us with u held below 60 and no factors.  (The sign of u
+// instead, sigmoid = 2^-u / (1 + 2^-u) for positive u, costs three operations a value, 482 us.)  g is held above -128, so that no z however low makes more of 2^-126 than 2^-119.
+// fminf also keeps a NaN from its neighbour, and the factor g carries it on.  Where the formula has no cubic term b is a
+// negligible number of the right sign instead of 0: 0 * Inf is NaN.
 struct Fp8Activation {
     int act;
     float a, b;
@@ -44,7 +46,7 @@ struct Fp8Activation {
         const float c = act == EPI_GELU ? 2.0f * 0.7978845608028654f : 1.0f;
         a = -1.4426950408889634f * c;
         b = act == EPI_GELU ? a * 0.044715f : -1e-37f;
-        g_lo = act == EPI_SIGMOID ? 1.0f : -64.0f;
+        g_lo = act == EPI_SIGMOID ? 1.0f : -128.0f;
         g_hi = act == EPI_SIGMOID ? 1.0f : __int_as_float(0x7f800000);
     }
 };
@@ -58,14 +60,15 @@ __device__ __forceinline__ void fp8_activation(float (&v)[N], const Fp8Activatio
         for (int j = 0; j < N; ++j) v[j] = fmaxf(v[j], 0.0f);      // as the other epilogues' ReLU, which drops NaN
         return;
     }
+    constexpr float least = 1.17549435e-38f;      // 2^-126
 #pragma unroll
     for (int j = 0; j < N; j += 2) {
         const float x0 = v[j], x1 = v[j + 1];
-        const float d0 = 1.0f + sfu_ex2(fminf(x0 * fmaf(f.b * x0, x0, f.a), 60.0f));
-        const float d1 = 1.0f + sfu_ex2(fminf(x1 * fmaf(f.b * x1, x1, f.a), 60.0f));
+        const float d0 = 1.0f + sfu_ex2(fminf(x0 * fmaf(f.b * x0, x0, f.a), 126.0f));
+        const float d1 = fmaf(sfu_ex2(fminf(x1 * fmaf(f.b * x1, x1, f.a), 126.0f)), least, least);
         const float r = sfu_rcp(d0 * d1);
         v[j] = clamp_nan(x0, f.g_lo, f.g_hi) * (d1 * r);
-        v[j + 1] = clamp_nan(x1, f.g_lo, f.g_hi) * (d0 * r);
+        v[j + 1] = clamp_nan(x1, f.g_lo, f.g_hi) * ((d0 * r) * least);
     }
 }
 
