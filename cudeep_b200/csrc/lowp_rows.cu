@@ -544,8 +544,9 @@ __global__ void dequantize_kernel(const uint8_t* __restrict__ q, const float* __
 template <int act>
 __device__ __forceinline__ float act_slope(float z) {
     if (act == EPI_RELU) return z > 0.0f ? 1.0f : 0.0f;
-    // Beyond these bounds the slope is within 1e-30 of 0 or 1; inside them no power of z and no exponential overflows.
-    constexpr float bound = act == EPI_GELU ? 10.0f : 80.0f;
+    // At these bounds e reaches 2^126, so s (or 1 - s) FP32's least normal number, 2^-126; beyond them the slope differs from 0 or
+    // 1 by no more than that times z dt/dz.  Inside them no power of z and no exponential overflows.
+    constexpr float bound = act == EPI_GELU ? 10.0f : 87.33f;
     constexpr float a = act == EPI_GELU ? 2.0f * 0.7978845608028654f : 1.0f;
     constexpr float b = act == EPI_GELU ? a * 0.044715f : 0.0f;
     constexpr float log2e = 1.4426950408889634f;

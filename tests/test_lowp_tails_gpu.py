@@ -1,4 +1,4 @@
-"""Activations of the 8-bit products far below zero, against the same formulas in 64 bits."""
+"""Activations and their slopes far from zero, against the same formulas in 64 bits."""
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -63,3 +63,34 @@ def test_activations_far_below_zero(dev, act, m, n, k, out):
     assert not y.isnan().any()
     assert (err[normal] <= (rel * want.abs())[normal]).all()
     assert (y.double().abs()[~normal] <= (z.abs().clamp(min=1) * 2.0 ** -126 * 1.01)[~normal]).all()
+
+
+@pytest.mark.parametrize("act", sorted(ACTS))
+def test_slopes_far_from_zero(dev, act):
+    """db of a single row is the slope itself: s + z s (1 - s) dt/dz (sigmoid: s (1 - s)), each term as far off as s is, the
+    second with two roundings and an s more."""
+    torch = dev.torch
+    n = 4096
+    codes = torch.arange(256, device=dev.dev).repeat(n // 256)
+    z8 = torch.where(codes % 128 == 127, codes - 1, codes).to(torch.uint8).reshape(1, n).contiguous()
+    zs = torch.exp2(torch.arange(n // 128, device=dev.dev).float() % 12 - 9).reshape(n // 128, 1).contiguous()
+    z = z8.view(torch.float8_e4m3fn).double() * zs.double().repeat_interleave(128)[None]
+    dy = torch.ones(1, n, dtype=torch.bfloat16, device=dev.dev)
+    db = torch.full((n,), float("nan"), device=dev.dev)
+    dev.check(dev.lib.cudeep_b200_linear_backward_saved_fp8(dev.ptr(dy), 2, None, None, dev.ptr(z8), dev.ptr(zs), ACTS[act], None,
+                                                            None, None, 2, dev.ptr(db), 1, n, 8, None))
+    assert dev.sync_status() == 0
+    t, dt = exponent64(torch, z, act)
+    s, rest = torch.sigmoid(t), torch.sigmoid(-t)
+    first, second = (0 * z, s * rest) if act == "sigmoid" else (s, z * s * rest * dt)
+    least = torch.minimum(s, rest) if act == "sigmoid" else s
+    normal = least >= 2.0 ** -126 * 1.001
+    assert bool((z < -50).any()) and bool((~normal).any())
+    err = (db[None].double() - (first + second)).abs()
+    bound = 2 * relative_bound(torch, t) * (first.abs() + second.abs())
+    # sigmoid's complement below the least normal number may be off by that much, and so the terms it multiplies.
+    bound = bound + (z.abs() * dt).clamp(min=1) * (rest < 2.0 ** -126 * 1.001) * 2.0 ** -126 * 1.01
+    assert not db.isnan().any()
+    assert (err[normal] <= bound[normal]).all()
+    tail = ((z.abs() * dt + 1) * 2.0 ** -126 * 1.01)
+    assert (db[None].double().abs()[~normal] <= tail[~normal]).all()
