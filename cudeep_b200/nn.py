@@ -119,17 +119,19 @@ class Linear(Module):
 
 
 class _Prepared:
-    """What a layer makes of its weight before it is used, kept until the parameter is replaced (load_state_dict).  A weight
-    changed in place is not noticed: call the layer's refresh().  It is made on the parameter's stream and finished before
-    any stream uses it; once other streams have, they are waited for before its memory goes back to the pool."""
+    """What a layer makes of its weight before it is used, kept until the parameter is replaced (load_state_dict) or changed in
+    place through a Tensor (fill_, zero_, also of another Tensor of the same memory).  What the library cannot see, values
+    written to the parameter's address, needs a call of the layer's refresh().  It is made on the parameter's stream and finished
+    before any stream uses it; once other streams have, they are waited for before its memory goes back to the pool."""
 
     def __init__(self):
-        self.of = self.value = None
+        self.of = self.version = self.value = None
         self.used_elsewhere = False
 
     def get(self, parameter, make, stream):
-        if self.of is not parameter:
+        if self.of is not parameter or self.version != parameter._storage.version:
             self.drop()
+            self.version = parameter._storage.version
             self.value, self.of = make(parameter), parameter
             _lib.check(_lib.load().cudeep_b200_stream_synchronize(parameter.stream))
         if _handle(stream) != _handle(parameter.stream):
@@ -155,6 +157,7 @@ class LinearFp8(Linear):
         self._weight8 = _Prepared()
 
     def refresh(self) -> None:
+        """After writing to the parameter's address: the next call takes its new values."""
         self._weight8.drop()
 
     def weight_fp8(self, stream=None) -> lowp.Fp8Tensor:
@@ -198,6 +201,7 @@ class GroupedLinear(Module):
         self._weight16 = _Prepared()
 
     def refresh(self) -> None:
+        """After writing to the parameter's address: the next call takes its new values."""
         self._weight16.drop()
 
     def weight_bf16(self, stream=None) -> Tensor:

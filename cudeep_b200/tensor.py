@@ -70,11 +70,12 @@ def _contiguous_strides(shape: Sequence[int]) -> list[int]:
 class _Storage:
     """A pool block, returned to the pool when the last view of it goes away.  `stream` is the
     stream its tensor last worked on: the pool lets other streams have the block only after
-    that stream has drained."""
+    that stream has drained.  `version` counts the calls that changed its values in place."""
 
     def __init__(self, nbytes: int, stream=None):
         self.ptr = ctypes.c_void_p()
         self.stream = stream
+        self.version = 0
         _lib.check(_lib.load().cudeep_b200_pool_alloc_on_stream(max(int(nbytes), 1), stream,
                                                                 ctypes.byref(self.ptr)))
 
@@ -277,6 +278,7 @@ class Tensor:
         lib = _lib.load()
         fn = lib.cudeep_b200_fill_f32 if self._dtype == DType.float32 else lib.cudeep_b200_fill_f64
         _lib.check(fn(self._storage.ptr, float(value), self.numel(), self.stream))
+        self._storage.version += 1
         return self
 
     def zero_(self) -> "Tensor":

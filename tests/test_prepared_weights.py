@@ -1,0 +1,92 @@
+"""The weights that LinearFp8 and GroupedLinear prepare: when they are made anew, and when their memory may be used again.  On the
+CPU, with a library that does nothing but note the calls it gets."""
+import itertools
+
+import pytest
+
+
+class FakeLib:
+    """Every function succeeds; `calls` lists (name, arguments).  Allocations get numbers of their own."""
+
+    def __init__(self):
+        self.calls = []
+        self.hooks = {}
+        self.addresses = itertools.count(0x1000, 0x1000)
+
+    def __getattr__(self, name):
+        if not name.startswith("cudeep_b200_"):
+            raise AttributeError(name)
+        name = name[len("cudeep_b200_"):]
+
+        def call(*args):
+            if name == "pool_alloc_on_stream":
+                args[2]._obj.value = next(self.addresses)
+            self.calls.append((name, tuple(getattr(a, "value", a) for a in args)))
+            if name in self.hooks:
+                self.hooks[name]()
+            return 0
+        return call
+
+    def count(self, name):
+        return sum(c[0] == name for c in self.calls)
+
+    def freed(self, address):
+        """Position of the call that frees a block; None if there is none."""
+        return next((i for i, (n, a) in enumerate(self.calls) if n == "pool_free_on_stream" and a[0] == address), None)
+
+
+@pytest.fixture()
+def fake(monkeypatch):
+    from cudeep_b200 import _lib
+    lib = FakeLib()
+    monkeypatch.setattr(_lib, "load", lambda: lib)
+    return lib
+
+
+@pytest.fixture()
+def cd():
+    import cudeep_b200
+    return cudeep_b200
+
+
+SIDE = 0x51DE
+
+
+def layer_and_call(cd, kind):
+    D = cd.DType
+    if kind == "linear":
+        layer = cd.nn.LinearFp8(128, 64)
+        call = lambda x: layer(x)      # noqa: E731
+        make, x = "quantize_fp8", cd.Tensor([4, 128])
+        held = lambda: [layer.weight_fp8().data, layer.weight_fp8().scales]      # noqa: E731
+        per_call = 1      # x is quantised too
+    else:
+        layer = cd.nn.GroupedLinear(2, 128, 64)
+        offsets = cd.Tensor([3], D.int32)
+        call = lambda x: layer(x, offsets)      # noqa: E731
+        make, x = "cast", cd.Tensor([4, 128], D.bfloat16)
+        held = lambda: [layer.weight_bf16()]      # noqa: E731
+        per_call = 0
+    return layer, call, make, x, held, per_call
+
+
+@pytest.mark.parametrize("kind", ["linear", "grouped"])
+def test_made_again_after_a_change_in_place(cd, fake, kind):
+    layer, call, make, x, _, per_call = layer_and_call(cd, kind)
+    call(x)
+    call(x)
+    assert fake.count(make) == 1 + 2 * per_call
+    for change in (lambda w: w.fill_(0.5), lambda w: w.zero_(), lambda w: w.reshape([-1]).fill_(2.0)):
+        before = fake.count(make)
+        change(layer._parameters["weight"])
+        call(x)
+        call(x)
+        assert fake.count(make) - before == 1 + 2 * per_call
+    # Through the tensor that the parameter shares its memory with.
+    own = cd.Tensor.zeros(layer._parameters["weight"].shape())
+    layer.register_parameter("weight", own)
+    call(x)
+    before = fake.count(make)
+    own.fill_(3.0)
+    call(x)
+    assert fake.count(make) - before == 1 + per_call
