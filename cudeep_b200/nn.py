@@ -122,11 +122,11 @@ class _Prepared:
     """What a layer makes of its weight before it is used, kept until the parameter is replaced (load_state_dict) or changed in
     place through a Tensor (fill_, zero_, also of another Tensor of the same memory).  What the library cannot see, values
     written to the parameter's address, needs a call of the layer's refresh().  It is made on the parameter's stream and finished
-    before any stream uses it; once other streams have, they are waited for before its memory goes back to the pool."""
+    before any stream uses it; once other streams have, they are waited for before its memory goes back to the pool, whether the
+    layer lets go of it last or a caller."""
 
     def __init__(self):
-        self.of = self.version = self.value = None
-        self.used_elsewhere = False
+        self.drop()
 
     def get(self, parameter, make, stream):
         if self.of is not parameter or self.version != parameter._storage.version:
@@ -134,18 +134,23 @@ class _Prepared:
             self.version = parameter._storage.version
             self.value, self.of = make(parameter), parameter
             _lib.check(_lib.load().cudeep_b200_stream_synchronize(parameter.stream))
-        if _handle(stream) != _handle(parameter.stream):
-            self.used_elsewhere = True
+        for t in (self.value.data, self.value.scales) if isinstance(self.value, lowp.Fp8Tensor) else (self.value,):
+            _used_on(t, stream)
         return self.value
 
     def drop(self):
-        if self.used_elsewhere:
-            _lib.check(_lib.load().cudeep_b200_device_synchronize())
-        self.__init__()
+        self.of = self.version = self.value = None
 
 
 def _handle(stream):
     return getattr(stream, "value", stream) or 0
+
+
+def _used_on(t, stream):
+    """t, which the layer holds and a kernel on `stream` reads: its memory outlives that, should the layer go first."""
+    if t is not None and _handle(stream) != _handle(t.stream):
+        t._storage.shared = True
+    return t
 
 
 class LinearFp8(Linear):
@@ -164,17 +169,18 @@ class LinearFp8(Linear):
         """The weight as the products on `stream` take it."""
         return self._weight8.get(self._parameters["weight"], lambda w: lowp.quantize_fp8(w, tiles=True), stream)
 
+    def _bias(self, stream):
+        return _used_on(self._parameters.get("bias"), stream)
+
     def forward(self, x, activation=None):
-        return lowp.linear_fp8(lowp.quantize_fp8(x), self.weight_fp8(x.stream), self._parameters.get("bias"), activation,
-                               x.dtype())
+        return lowp.linear_fp8(lowp.quantize_fp8(x), self.weight_fp8(x.stream), self._bias(x.stream), activation, x.dtype())
 
     def forward_saved(self, x, activation=None):
         """(y, saved) for `backward`: y as forward's, saved holds x and, with an activation, the pre-activation in 8 bits.
         Without an activation nothing but the codes that the product reads anyway is kept."""
         activation = _ACTIVATIONS[_epilogue_code(activation)]
         x8 = lowp.quantize_fp8(x)
-        bias = self._parameters.get("bias")
-        z = lowp.linear_fp8(x8, self.weight_fp8(x.stream), bias, None, DType.float32 if activation else x.dtype())
+        z = lowp.linear_fp8(x8, self.weight_fp8(x.stream), self._bias(x.stream), None, DType.float32 if activation else x.dtype())
         if activation is None:
             return z, (x8, None, None)
         y = getattr(z, activation)()
@@ -184,7 +190,7 @@ class LinearFp8(Linear):
         """(dx, dweight, dbias) in float32 for bfloat16 `grad` of y and what forward_saved kept; the product for dx takes the
         weight in bfloat16."""
         x8, z8, activation = saved
-        weight = self._parameters["weight"]._cast_on(DType.bfloat16, grad.stream)
+        weight = _used_on(self._parameters["weight"], grad.stream)._cast_on(DType.bfloat16, grad.stream)
         dx, dw, db = lowp.linear_backward_saved(grad, x8, weight, z8, activation, DType.float32)
         return dx.to(DType.float32), dw, (db if "bias" in self._parameters else None)
 

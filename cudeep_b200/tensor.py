@@ -70,11 +70,14 @@ def _contiguous_strides(shape: Sequence[int]) -> list[int]:
 class _Storage:
     """A pool block, returned to the pool when the last view of it goes away.  `stream` is the
     stream its tensor last worked on: the pool lets other streams have the block only after
-    that stream has drained.  `version` counts the calls that changed its values in place."""
+    that stream has drained.  `shared` says that other streams have used it besides; the device
+    is waited for then, whoever lets go of it last.  `version` counts the calls that changed its
+    values in place."""
 
     def __init__(self, nbytes: int, stream=None):
         self.ptr = ctypes.c_void_p()
         self.stream = stream
+        self.shared = False
         self.version = 0
         _lib.check(_lib.load().cudeep_b200_pool_alloc_on_stream(max(int(nbytes), 1), stream,
                                                                 ctypes.byref(self.ptr)))
@@ -82,7 +85,10 @@ class _Storage:
     def __del__(self):
         try:
             if self.ptr:
-                _lib.load().cudeep_b200_pool_free_on_stream(self.ptr, self.stream)
+                lib = _lib.load()
+                if self.shared:
+                    lib.cudeep_b200_device_synchronize()
+                lib.cudeep_b200_pool_free_on_stream(self.ptr, self.stream)
         except Exception:
             pass
 

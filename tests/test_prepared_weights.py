@@ -1,5 +1,6 @@
 """The weights that LinearFp8 and GroupedLinear prepare: when they are made anew, and when their memory may be used again.  On the
 CPU, with a library that does nothing but note the calls it gets."""
+import gc
 import itertools
 
 import pytest
@@ -90,3 +91,60 @@ def test_made_again_after_a_change_in_place(cd, fake, kind):
     own.fill_(3.0)
     call(x)
     assert fake.count(make) - before == 1 + per_call
+
+
+@pytest.mark.parametrize("how", ["refresh", "replace", "change", "delete", "delete_after_taking_it"])
+@pytest.mark.parametrize("kind", ["linear", "grouped"])
+def test_other_streams_are_waited_for_before_the_memory_goes_back(cd, fake, kind, how):
+    layer, call, _, x, held, _ = layer_and_call(cd, kind)
+    x.set_stream(SIDE)
+    call(x)
+    addresses = [t.data_ptr() for t in held()]
+    assert addresses and all(fake.freed(a) is None for a in addresses)
+    start = len(fake.calls)
+    if how == "refresh":
+        layer.refresh()
+    elif how == "replace":
+        layer.register_parameter("weight", cd.Tensor.zeros(layer._parameters["weight"].shape()))
+        call(x)
+    elif how == "change":
+        layer._parameters["weight"].fill_(1.0)
+        call(x)
+    else:
+        if how == "delete_after_taking_it":      # a caller still holds the prepared weight when the layer goes
+            taken = held()
+            del held, call, layer
+            gc.collect()
+            assert all(fake.freed(a) is None for a in addresses)
+            del taken
+        else:
+            del held, call, layer
+        gc.collect()
+    for a in addresses:
+        at = fake.freed(a)
+        assert at is not None
+        assert any(n == "device_synchronize" for n, _ in fake.calls[start:at])
+
+
+@pytest.mark.parametrize("kind", ["linear", "grouped"])
+def test_one_stream_is_not_waited_for(cd, fake, kind):
+    layer, call, _, x, held, _ = layer_and_call(cd, kind)
+    call(x)
+    addresses = [t.data_ptr() for t in held()]
+    layer.refresh()
+    assert all(fake.freed(a) is not None for a in addresses) and fake.count("device_synchronize") == 0
+
+
+def test_the_other_parameters_of_the_layer_too(cd, fake):
+    """The bias of the product and the weight that the gradient takes are read on the caller's stream."""
+    D = cd.DType
+    layer, x, grad = cd.nn.LinearFp8(128, 64), cd.Tensor([4, 128]), cd.Tensor([4, 64], D.bfloat16)
+    x.set_stream(SIDE)
+    grad.set_stream(SIDE)
+    layer.backward(grad, layer.forward_saved(x)[1])
+    addresses = [p.data_ptr() for p in layer.parameters()]
+    start = len(fake.calls)
+    del layer
+    gc.collect()
+    for a in addresses:
+        assert any(n == "device_synchronize" for n, _ in fake.calls[start:fake.freed(a)])
