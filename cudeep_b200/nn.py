@@ -15,6 +15,7 @@ Additions: LinearFp8, the same layer on 8-bit products, and GroupedLinear, one w
 """
 from __future__ import annotations
 
+import threading
 from typing import Optional
 
 import numpy as np
@@ -126,20 +127,25 @@ class _Prepared:
     layer lets go of it last or a caller."""
 
     def __init__(self):
-        self.drop()
+        self.lock = threading.Lock()      # making a value waits for the device, and other threads run meanwhile
+        self.of = self.version = self.value = None
 
     def get(self, parameter, make, stream):
-        if self.of is not parameter or self.version != parameter._storage.version:
-            self.drop()
-            self.version = parameter._storage.version
-            self.value, self.of = make(parameter), parameter
-            _lib.check(_lib.load().cudeep_b200_stream_synchronize(parameter.stream))
-        for t in (self.value.data, self.value.scales) if isinstance(self.value, lowp.Fp8Tensor) else (self.value,):
+        with self.lock:
+            if self.of is not parameter or self.version != parameter._storage.version:
+                self.of = self.value = None
+                self.version = parameter._storage.version
+                value = make(parameter)
+                _lib.check(_lib.load().cudeep_b200_stream_synchronize(parameter.stream))
+                self.value, self.of = value, parameter
+            value = self.value
+        for t in (value.data, value.scales) if isinstance(value, lowp.Fp8Tensor) else (value,):
             _used_on(t, stream)
-        return self.value
+        return value
 
     def drop(self):
-        self.of = self.version = self.value = None
+        with self.lock:
+            self.of = self.version = self.value = None
 
 
 def _handle(stream):

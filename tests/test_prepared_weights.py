@@ -2,6 +2,7 @@
 CPU, with a library that does nothing but note the calls it gets."""
 import gc
 import itertools
+import threading
 
 import pytest
 
@@ -148,3 +149,40 @@ def test_the_other_parameters_of_the_layer_too(cd, fake):
     gc.collect()
     for a in addresses:
         assert any(n == "device_synchronize" for n, _ in fake.calls[start:fake.freed(a)])
+
+
+@pytest.mark.parametrize("kind", ["linear", "grouped"])
+def test_refresh_while_another_thread_prepares(cd, fake, kind):
+    """The other thread comes in while this one waits for the weight to be made (which lets go of the interpreter's lock)."""
+    layer, call, _, x, held, _ = layer_and_call(cd, kind)
+    others = []
+
+    def come_in():
+        if not others:
+            others.append(threading.Thread(target=layer.refresh))
+            others[0].start()
+            others[0].join(0.5)      # it may have to wait for this thread
+
+    fake.hooks["stream_synchronize"] = come_in
+    call(x)                          # takes the prepared weight, whichever
+    assert all(t is not None for t in held())
+    others[0].join(10)
+    assert not others[0].is_alive()
+
+
+@pytest.mark.parametrize("kind", ["linear", "grouped"])
+def test_a_weight_that_could_not_be_made_is_not_kept(cd, fake, kind):
+    """An error while preparing it leaves nothing behind, and the next call prepares it again."""
+    layer, call, make, x, held, _ = layer_and_call(cd, kind)
+
+    def fail():
+        raise RuntimeError("planted")
+
+    fake.hooks["stream_synchronize"] = fail
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="planted"):
+            call(x)
+    del fake.hooks["stream_synchronize"]
+    before = fake.count(make)
+    call(x)
+    assert fake.count(make) > before and all(t is not None for t in held())
