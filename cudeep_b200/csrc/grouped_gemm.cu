@@ -32,7 +32,7 @@ __global__ void __launch_bounds__(32) group_maps_kernel(const __grid_constant__ 
 #endif
 }
 
-template <RaggedForm FORM, int CTAS, bool BF16, class OutT>
+template <RaggedForm FORM, int CTAS, bool BF16, class OutT, bool WIDE = false>
 void launch(RaggedParams& p, const RaggedPlan& plan, cudaStream_t stream) {
     const DeviceInfo& dev = device_info();
     CB200_REQUIRE(dev.cc_major == 10, "grouped products need an sm_100 device");
@@ -55,7 +55,7 @@ void launch(RaggedParams& p, const RaggedPlan& plan, cudaStream_t stream) {
                 FORM == RaggedForm::NT ? "nt" : FORM == RaggedForm::NN ? "nn" : "tn", BF16 ? "bf16" : "f16", p.rows, p.groups,
                 p.features, FORM == RaggedForm::TN ? "cols" : "k", FORM == RaggedForm::TN ? p.cols : p.k, 128 * CTAS,
                 plan.tile_cols, plan.split, p.stages, clusters);
-    launch_clusters(ragged_gemm_kernel<FORM, CTAS, BF16, OutT>, p, clusters, CTAS * plan.split, RAGGED_THREADS, smem_bytes,
+    launch_clusters(ragged_gemm_kernel<FORM, CTAS, BF16, OutT, WIDE>, p, clusters, CTAS * plan.split, RAGGED_THREADS, smem_bytes,
                     RAGGED_SMEM_BUDGET + 1024, stream);
 }
 
@@ -128,11 +128,11 @@ int encode_columns(CUtensorMap* map, const AlignedRows& m, int rows, int cols, i
     return chunked ? 1 : 0;
 }
 
-template <int CTAS, bool BF16>
+template <int CTAS, bool BF16, bool WIDE = false>
 void launch_weight(RaggedParams& p, const RaggedPlan& plan, int c_type, cudaStream_t stream) {
-    if (c_type == TYPE_F32) launch<RaggedForm::TN, CTAS, BF16, float>(p, plan, stream);
+    if (c_type == TYPE_F32) launch<RaggedForm::TN, CTAS, BF16, float, WIDE>(p, plan, stream);
     else if constexpr (BF16) launch<RaggedForm::TN, CTAS, BF16, __nv_bfloat16>(p, plan, stream);
-    else launch<RaggedForm::TN, CTAS, BF16, __half>(p, plan, stream);
+    else launch<RaggedForm::TN, CTAS, BF16, __half, WIDE>(p, plan, stream);
 }
 
 }  // namespace
@@ -148,7 +148,8 @@ void grouped_nn(const void* a, long long lda, const void* w, long long ldw, void
 }
 
 void grouped_tn(const void* a, long long lda, const void* b, long long ldb, void* c, int type, int c_type,
-                const int32_t* offsets, int groups, int rows, int m, int n, const float* col_scale, cudaStream_t stream) {
+                const int32_t* offsets, int groups, int rows, int m, int n, const float* col_scale, const WideOperands& wide,
+                cudaStream_t stream) {
     const PreparedRows operands = prepare_rows({a, rows, m, 2, lda}, {b, rows, n, 2, ldb}, {}, stream);
     const AlignedRows &y = operands.a, &x = operands.b;
     RaggedPlan plan = plan_weight(groups, rows, m, n, elem_bytes(c_type));
@@ -181,6 +182,20 @@ void grouped_tn(const void* a, long long lda, const void* b, long long ldb, void
     p.step = 128;
     p.a_chunked = encode_columns(&p.map_a, y, rows, m, 2);
     p.b_chunked = encode_columns(&p.map_b, x, rows, n, plan.tile_cols / plan.ctas / 64);
+    int most_rows = rows;
+    if (wide.wide != nullptr) {
+        CB200_REQUIRE(type == TYPE_F16 && offsets == nullptr && rows <= (1 << 29), "operands in two parts: FP16, one group of 2^29 rows");
+        p.wide = wide.wide;
+        p.wide_blocks = wide.blocks;
+        p.part_rows = (rows + RAGGED_BK - 1) / RAGGED_BK * RAGGED_BK;
+        p.wide_share = parts > 1 ? 2 * p.share : 2 * p.part_rows;
+        most_rows = 2 * p.part_rows;
+        const uint64_t row_bytes = uint64_t(wide.ld_parts) * 2;
+        const uint64_t dims[4] = {64, uint64_t(rows), uint64_t((m + 63) / 64), 2};
+        const uint64_t strides[3] = {row_bytes, 128, row_bytes * uint64_t(rows)};
+        const uint32_t box[4] = {64, 64, 2, 1};
+        encode_tensor_map_f16(&p.map_parts, wide.parts, 4, dims, strides, box, TmaSwizzle::B128);
+    }
     const uint32_t c_bytes = uint32_t(elem_bytes(out_type));
     p.tma_store = (size_t(ldc) * c_bytes) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
     if (p.tma_store) {
@@ -207,12 +222,16 @@ void grouped_tn(const void* a, long long lda, const void* b, long long ldb, void
     // The tensor core's accumulation loses about 2.4e-9 relative per row summed (it truncates), so a gradient in
     // single precision is summed over 2048 rows at a time, added up with rounding in the epilogue; a 16-bit one
     // (2e-3 from its own rounding) in one go.
-    p.chunk_rows = out_type == TYPE_F32 ? 2048 : (rows + RAGGED_BK - 1) / RAGGED_BK * RAGGED_BK;
+    p.chunk_rows = out_type == TYPE_F32 ? 2048 : (most_rows + RAGGED_BK - 1) / RAGGED_BK * RAGGED_BK;
+    const bool pairs = plan.ctas == 2;
     if (type == TYPE_BF16) {
-        if (plan.ctas == 2) launch_weight<2, true>(p, plan, out_type, stream);
+        if (pairs) launch_weight<2, true>(p, plan, out_type, stream);
         else launch_weight<1, true>(p, plan, out_type, stream);
+    } else if (wide.wide != nullptr) {
+        if (pairs) launch_weight<2, false, true>(p, plan, out_type, stream);
+        else launch_weight<1, false, true>(p, plan, out_type, stream);
     } else {
-        if (plan.ctas == 2) launch_weight<2, false>(p, plan, out_type, stream);
+        if (pairs) launch_weight<2, false>(p, plan, out_type, stream);
         else launch_weight<1, false>(p, plan, out_type, stream);
     }
     if (parts > 1) add_parts(static_cast<const float*>(out), parts, m, n, ldc, c, c_type, stream);

@@ -110,7 +110,7 @@ void launch_grouped_matmul_tn(const void* A, const void* B, void* C, ElementType
         CB200_CUDA(cudaMemsetAsync(C, 0, size_t(groups) * M * N * cudeep_b200::elem_bytes(ct), stream));
         return;
     }
-    cudeep_b200::grouped_tn(A, 0, B, 0, C, t, ct, offsets, groups, rows, M, N, nullptr, stream);
+    cudeep_b200::grouped_tn(A, 0, B, 0, C, t, ct, offsets, groups, rows, M, N, nullptr, {}, stream);
 }
 
 void launch_linear_forward_fp8(const void* x, const float* x_scales, const void* W, const float* w_scales, const float* bias,
@@ -169,13 +169,17 @@ void launch_linear_backward_saved_fp8(const void* dy, ElementType type, const vo
         return;
     }
     // W, and dy where the products read it themselves, as the TMA unit reads them.  And x as a 16-bit operand: q * s is exact in
-    // BF16 for the power-of-two scales of quantize_fp8; FP16 has too few exponents for that, so there each column block is
-    // taken relative to its largest scale (products below 2^-24 of that are lost) and the result is multiplied by it.
+    // BF16 for the power-of-two scales of quantize_fp8.  FP16 has fewer exponents: there each column block is taken relative to
+    // its largest scale, by which the result is multiplied, exact too while the scales of a block lie within 2^15 of each other.
+    // Where they do not (rows of zeros, whose scale is 1, next to small values; a row far larger than the others) the device
+    // takes x in BF16, and dz, rounded to FP16 as ever, as the sum of two BF16 matrices: two products, and nothing is lost.
     Scratch top_buf;
     ScaleTops tops;
     if (dw != nullptr && t == TYPE_F16) {
-        top_buf = Scratch(size_t((K + FP8_BLOCK - 1) / FP8_BLOCK) * sizeof(float), stream);
-        tops = ScaleTops{x_scales, M, K, static_cast<float*>(top_buf.ptr)};
+        tops = ScaleTops{x_scales, M, K};
+        top_buf = Scratch(size_t(tops.blocks()) * (sizeof(float) + sizeof(uint32_t)), stream);
+        tops.top = static_cast<float*>(top_buf.ptr);
+        tops.wide = reinterpret_cast<uint32_t*>(tops.top + tops.blocks());
     }
     const bool products = dx != nullptr || dw != nullptr;
     const PreparedRows operands = prepare_rows({dx != nullptr ? W : nullptr, N, K, 2},
@@ -199,9 +203,18 @@ void launch_linear_backward_saved_fp8(const void* dy, ElementType type, const vo
     if (dx != nullptr) grouped_nn(dz, ld_dz, operands.a.ptr, operands.a.ld, dx, t, nullptr, 1, M, K, N, stream);
     if (dw == nullptr) return finish_sums(sums, stream);
     const long long ld_x = (K + 63) / 64 * 64;
-    Scratch x_buf(size_t(M) * ld_x * 2, stream);
-    dequantize_rows(static_cast<const uint8_t*>(x8), x_scales, tops.top, M, K, x_buf.ptr, ld_x, t, sums, stream);
-    grouped_tn(dz, ld_dz, x_buf.ptr, ld_x, dw, t, wt, nullptr, 1, M, N, K, tops.top, stream);
+    const long long ld_parts = (N + 63) / 64 * 64;
+    const size_t x_bytes = size_t(M) * ld_x * 2, parts_bytes = t == TYPE_F16 ? size_t(M) * ld_parts * 4 : 0;
+    Scratch x_buf(x_bytes + parts_bytes, stream);
+    SplitRequest split;
+    WideOperands wide;
+    if (t == TYPE_F16) {
+        void* parts = static_cast<uint8_t*>(x_buf.ptr) + x_bytes;
+        split = SplitRequest{dz, ld_dz, N, parts, ld_parts};
+        wide = WideOperands{tops.wide, tops.blocks(), parts, ld_parts};
+    }
+    dequantize_rows(static_cast<const uint8_t*>(x8), x_scales, tops, M, K, x_buf.ptr, ld_x, t, sums, split, stream);
+    grouped_tn(dz, ld_dz, x_buf.ptr, ld_x, dw, t, wt, nullptr, 1, M, N, K, tops.top, wide, stream);
 }
 
 }  // namespace kernels

@@ -5,6 +5,7 @@
 // launches (the backward pass of a short batch is five) the launches overlap.
 #include "lowp_rows.h"
 
+#include "device_flags.cuh"
 #include "epilogue_math.cuh"
 #include "launch_dependent.h"
 #include "sm100_ptx.cuh"
@@ -669,17 +670,38 @@ __global__ void __launch_bounds__(kThreads) add_bands_kernel(const __grid_consta
     add_bands(p, blockIdx.x);
 }
 
-__device__ __forceinline__ void block_top(const float* __restrict__ scales, int rows, float* __restrict__ top, unsigned block) {
-    __shared__ float s_max[kThreads / 32];
-    float m = 0.0f;
-    for (int r = threadIdx.x; r < rows; r += kThreads) m = fmaxf(m, finite_abs(__ldg(scales + (long long)block * rows + r)));
+// FP16 reaches from 448 * 2^0 down to steps of 2^-24, and e4m3's steps are 2^-9 of a scale: scales down to 2^-15 of the block's
+// largest one fit.  Zero scales stand for zeros and do not count.  (A block of zeros has the scale 1, which counts: its codes
+// are not looked at here.)
+__device__ __forceinline__ void block_top(const float* __restrict__ scales, int rows, float* __restrict__ top,
+                                          uint32_t* __restrict__ wide, unsigned block) {
+    __shared__ float s_max[kThreads / 32], s_min[kThreads / 32];
+    float m = 0.0f, least = __int_as_float(0x7f800000);
+#pragma unroll 8
+    for (int r = threadIdx.x; r < rows; r += kThreads) {
+        const float s = finite_abs(__ldg(scales + (long long)block * rows + r));
+        m = fmaxf(m, s);
+        least = fminf(least, s > 0.0f ? s : __int_as_float(0x7f800000));
+    }
 #pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
+    for (int d = 16; d >= 1; d >>= 1) {
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+        least = fminf(least, __shfl_xor_sync(0xffffffffu, least, d));
+    }
+    if ((threadIdx.x & 31) == 0) {
+        s_max[threadIdx.x >> 5] = m;
+        s_min[threadIdx.x >> 5] = least;
+    }
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) m = fmaxf(m, s_max[w]);
-    if (threadIdx.x == 0) top[block] = m > 0.0f ? m : 1.0f;
+    for (int w = 0; w < kThreads / 32; ++w) {
+        m = fmaxf(m, s_max[w]);
+        least = fminf(least, s_min[w]);
+    }
+    if (threadIdx.x == 0) {
+        top[block] = m > 0.0f ? m : 1.0f;
+        wide[block] = least * 32768.0f < m ? 1u : 0u;
+    }
 }
 
 // What a product needs before it, in one launch: each launch costs the host about 2 us, more than a small one of these takes
@@ -689,6 +711,7 @@ struct PrepareParams {
     const float* scales;
     int scale_rows;
     float* top;
+    uint32_t* wide;
 };
 __global__ void __launch_bounds__(kThreads) prepare_kernel(const __grid_constant__ PrepareParams p) {
     ptx::grid_dependency_wait();
@@ -697,20 +720,25 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const __grid_constant
     if (block < p.pad[0].blocks) return pad_rows(p.pad[0], block);
     block -= p.pad[0].blocks;
     if (block < p.pad[1].blocks) return pad_rows(p.pad[1], block);
-    block_top(p.scales, p.scale_rows, p.top, block - p.pad[1].blocks);
+    block_top(p.scales, p.scale_rows, p.top, p.wide, block - p.pad[1].blocks);
 }
 
-// Eight elements per thread, zeros behind cols up to the next multiple of eight.  The first CTAs add up column sums instead, of
-// the pass before it (a launch less).
+// What dequantize_rows_kernel heeds for FP16.
+struct WideRows {
+    const float* top;           // nullptr for BF16
+    const uint32_t* wide;       // [blocks]
+    int blocks;
+    const __half* split;        // a matrix to split (SplitRequest)
+    long long ld_split, ld_parts;
+    int split_cols;
+    __nv_bfloat16* parts;
+};
+
+// Eight elements per thread, zeros behind cols up to the next multiple of eight; CTA `block` of `blocks`.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kThreads) dequantize_rows_kernel(const uint8_t* __restrict__ q, const float* __restrict__ scales,
-                                                                   const float* __restrict__ top, int rows, int cols,
-                                                                   T* __restrict__ y, long long ld_y,
-                                                                   const __grid_constant__ Bands sums) {
-    ptx::grid_dependency_wait();
-    ptx::grid_launch_dependents();
-    if (blockIdx.x < sums.blocks) return add_bands(sums, blockIdx.x);
-    const unsigned block = blockIdx.x - sums.blocks, blocks = gridDim.x - sums.blocks;
+__device__ __forceinline__ void dequantize_units(const uint8_t* __restrict__ q, const float* __restrict__ scales,
+                                                 const float* __restrict__ top, int rows, int cols, T* __restrict__ y,
+                                                 long long ld_y, unsigned block, unsigned blocks) {
     const int units = (cols + 7) / 8;
     const long long total = (long long)rows * units;
     for (long long i = block * (long long)blockDim.x + threadIdx.x; i < total; i += (long long)blocks * blockDim.x) {
@@ -725,6 +753,42 @@ __global__ void __launch_bounds__(kThreads) dequantize_rows_kernel(const uint8_t
         for (int j = 0; j < 8; ++j) f[j] *= s;
         store8(y + r * ld_y + c0, f);
     }
+}
+
+// The first CTAs add up column sums instead, of the pass before it (a launch less).  One load of codes a thread is under way, so
+// that the pass lives on eight CTAs to an SM.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kThreads, 8) dequantize_rows_kernel(const uint8_t* __restrict__ q, const float* __restrict__ scales,
+                                                                   int rows, int cols, T* __restrict__ y, long long ld_y,
+                                                                   const __grid_constant__ Bands sums,
+                                                                   const __grid_constant__ WideRows w) {
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
+    if (blockIdx.x < sums.blocks) return add_bands(sums, blockIdx.x);
+    const unsigned block = blockIdx.x - sums.blocks, blocks = gridDim.x - sums.blocks;
+    if constexpr (std::is_same<T, __half>::value) {
+        if (any_set(w.wide, w.blocks)) {
+            dequantize_units<__nv_bfloat16, VEC>(q, scales, nullptr, rows, cols, reinterpret_cast<__nv_bfloat16*>(y), ld_y, block,
+                                                 blocks);
+            const int units = (w.split_cols + 7) / 8;
+            const long long total = (long long)rows * units;
+            for (long long i = block * (long long)blockDim.x + threadIdx.x; i < total; i += (long long)blocks * blockDim.x) {
+                const long long r = i / units;
+                const int c0 = int(i - r * units) * 8;
+                Unit8<__half> u;
+                u.template load<true>(w.split + r * w.ld_split, c0, w.split_cols);
+                float v[8], rest[8];
+                u.values(v);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)      // an infinity or NaN goes whole into the first part
+                    rest[j] = fabsf(v[j]) <= 65504.0f ? v[j] - __bfloat162float(__float2bfloat16_rn(v[j])) : 0.0f;
+                store8(w.parts + r * w.ld_parts + c0, v);
+                store8(w.parts + (rows + r) * w.ld_parts + c0, rest);
+            }
+            return;
+        }
+    }
+    dequantize_units<T, VEC>(q, scales, w.top, rows, cols, y, ld_y, block, blocks);
 }
 
 template <typename T>
@@ -862,7 +926,8 @@ PreparedRows prepare_rows(const RowsRequest& a, const RowsRequest& b, const Scal
         p.scales = tops.scales;
         p.scale_rows = tops.rows;
         p.top = tops.top;
-        blocks += (tops.cols + FP8_BLOCK - 1) / FP8_BLOCK;
+        p.wide = tops.wide;
+        blocks += tops.blocks();
     }
     if (blocks == 0) return out;
     launch_dependent(prepare_kernel, dim3(unsigned(blocks)), kThreads, stream, p);
@@ -908,19 +973,22 @@ void finish_sums(const ColumnSums& sums, cudaStream_t stream) {
     CB200_CHECK_LAUNCH();
 }
 
-void dequantize_rows(const uint8_t* q, const float* scales, const float* top, int rows, int cols, void* y, long long ld_y,
-                     int y_type, const ColumnSums& sums, cudaStream_t stream) {
+void dequantize_rows(const uint8_t* q, const float* scales, const ScaleTops& tops, int rows, int cols, void* y, long long ld_y,
+                     int y_type, const ColumnSums& sums, const SplitRequest& split, cudaStream_t stream) {
     const Bands bands = bands_of(sums);
     const bool vec = cols % 8 == 0 && reinterpret_cast<uintptr_t>(q) % 8 == 0;
     const unsigned grid = bands.blocks + pass_grid((long long)rows * ((cols + 7) / 8));
+    WideRows wide{};
     if (y_type == TYPE_F16) {
+        wide = WideRows{tops.top, tops.wide, tops.blocks(), static_cast<const __half*>(split.src), split.ld, split.ld_parts,
+                        split.cols, static_cast<__nv_bfloat16*>(split.parts)};
         __half* out = static_cast<__half*>(y);
-        if (vec) launch_dependent(dequantize_rows_kernel<__half, true>, dim3(grid), kThreads, stream, q, scales, top, rows, cols, out, ld_y, bands);
-        else launch_dependent(dequantize_rows_kernel<__half, false>, dim3(grid), kThreads, stream, q, scales, top, rows, cols, out, ld_y, bands);
+        if (vec) launch_dependent(dequantize_rows_kernel<__half, true>, dim3(grid), kThreads, stream, q, scales, rows, cols, out, ld_y, bands, wide);
+        else launch_dependent(dequantize_rows_kernel<__half, false>, dim3(grid), kThreads, stream, q, scales, rows, cols, out, ld_y, bands, wide);
     } else {
         __nv_bfloat16* out = static_cast<__nv_bfloat16*>(y);
-        if (vec) launch_dependent(dequantize_rows_kernel<__nv_bfloat16, true>, dim3(grid), kThreads, stream, q, scales, top, rows, cols, out, ld_y, bands);
-        else launch_dependent(dequantize_rows_kernel<__nv_bfloat16, false>, dim3(grid), kThreads, stream, q, scales, top, rows, cols, out, ld_y, bands);
+        if (vec) launch_dependent(dequantize_rows_kernel<__nv_bfloat16, true>, dim3(grid), kThreads, stream, q, scales, rows, cols, out, ld_y, bands, wide);
+        else launch_dependent(dequantize_rows_kernel<__nv_bfloat16, false>, dim3(grid), kThreads, stream, q, scales, rows, cols, out, ld_y, bands, wide);
     }
     CB200_CHECK_LAUNCH();
 }

@@ -28,11 +28,14 @@ struct RowsRequest {
     const int32_t* offsets = nullptr;
     int rows_group = 1;
 };
-// top[b] = the largest finite scale of column block b; nothing with top == nullptr.
+// top[b] = the largest finite scale of column block b, and wide[b] = 1 where FP16 does not hold q * (s / top[b]) for all of its
+// scales, 0 where it does; nothing with top == nullptr.
 struct ScaleTops {
     const float* scales = nullptr;      // [block][rows]
     int rows = 0, cols = 0;
     float* top = nullptr;
+    uint32_t* wide = nullptr;
+    int blocks() const { return (cols + FP8_BLOCK - 1) / FP8_BLOCK; }
 };
 struct PreparedRows {
     AlignedRows a, b;
@@ -61,10 +64,19 @@ struct ColumnSums {
 ColumnSums activation_backward_fp8(const void* dy, int type, const uint8_t* z8, const float* z_scales, int act, void* dz,
                                    long long ld_dz, float* db, int rows, int cols, cudaStream_t stream);
 void finish_sums(const ColumnSums& sums, cudaStream_t stream);
-// y = q * (s / top[b]) in a 16-bit type, rows ld_y elements apart, for blocks of 1 x 128; with top == nullptr: y = q * s.
-// Finishes `sums` as well.
-void dequantize_rows(const uint8_t* q, const float* scales, const float* top, int rows, int cols, void* y, long long ld_y,
-                     int y_type, const ColumnSums& sums, cudaStream_t stream);
+// An FP16 matrix as two BF16 matrices whose sum it is, one behind the other in `parts`, rows ld_parts elements apart: 8 of its 11
+// bits and the other 3.  Made only where ScaleTops::wide has an entry set.
+struct SplitRequest {
+    const void* src = nullptr;      // rows as AlignedRows has them
+    long long ld = 0;
+    int cols = 0;
+    void* parts = nullptr;
+    long long ld_parts = 0;
+};
+// y = q * s in a 16-bit type, rows ld_y elements apart, for blocks of 1 x 128.  In FP16, which needs `tops` and `split`,
+// q * (s / top[b]), or, where an entry of tops.wide is set, q * s in BF16, and then `split` is made.  Finishes `sums` as well.
+void dequantize_rows(const uint8_t* q, const float* scales, const ScaleTops& tops, int rows, int cols, void* y, long long ld_y,
+                     int y_type, const ColumnSums& sums, const SplitRequest& split, cudaStream_t stream);
 
 // out[m, n] = sum over `parts` of part[parts][m][ld], in order, rounded to `type`.  ld is a multiple of 4.
 void add_parts(const float* part, int parts, int m, int n, long long ld, void* out, int type, cudaStream_t stream);

@@ -20,6 +20,7 @@
 // 129 us; 86 us this way.)
 #pragma once
 
+#include "device_flags.cuh"
 #include "runtime.h"
 #include "sm100_ptx.cuh"
 #include "umma_gemm.cuh"
@@ -97,6 +98,14 @@ struct RaggedParams {
     uint32_t atom_bytes;
     int chunk_rows;          // TN: rows summed in the tensor core's accumulator before they are added into C
     const float* col_scale;  // TN: nullptr, or a factor for each 128 columns of C
+    // TN of one group, WIDE: if any of these words is set, X is BF16 and Y two BF16 matrices whose sum it is (WideOperands).  The sums
+    // then run over 2 * part_rows rows, part_rows being `rows` rounded up to whole K blocks: those of the first part and those of
+    // the second, each with the rows of X again.  wide_share takes the place of `share`.
+    const uint32_t* wide;
+    int wide_blocks;
+    int part_rows;
+    int wide_share;
+    CUtensorMap map_parts;   // {64, rows, F / 64, 2} box {64, 64, 2, 1}
     uint32_t* status;
     unsigned long long wait_limit_ns;
 };
@@ -264,7 +273,9 @@ __device__ __forceinline__ void load_columns(uint32_t dst, const CUtensorMap* ma
     }
 }
 
-template <RaggedForm FORM, int CTAS, bool BF16, class OutT>
+// WIDE: the operands may come in the form of RaggedParams::wide.  A kernel of its own, as reading the flags and the test in the
+// producer's loop cost 3.5 us of 195 in 8192 x 4096 x 4096.
+template <RaggedForm FORM, int CTAS, bool BF16, class OutT, bool WIDE = false>
 __global__ void __launch_bounds__(RAGGED_THREADS, 1) ragged_gemm_kernel(const __grid_constant__ RaggedParams p) {
 #if defined(__CUDA_ARCH_FEAT_SM100_ALL) || defined(__CUDA_ARCH_FEAT_SM101_ALL) || \
     defined(__CUDA_ARCH_FEAT_SM103_ALL)
@@ -316,12 +327,14 @@ __global__ void __launch_bounds__(RAGGED_THREADS, 1) ragged_gemm_kernel(const __
     const int split = SPLITS ? p.split : 1;
     const int split_rank = SPLITS && split > 1 ? int(ptx::cluster_ctarank()) : 0;
     ptx::grid_dependency_wait();      // the offsets may come from the kernel before
+    bool wide = false;
+    if constexpr (WIDE) wide = any_set(p.wide, p.wide_blocks);
     constexpr bool STEPS = FORM == RaggedForm::NT && CTAS == 1;
     const int step = STEPS ? p.step : 128;
     const int f_tiles = (p.features + step * CTAS - 1) / (step * CTAS);
     const int c_tiles_tn = FORM == RaggedForm::TN ? (p.cols + p.tile_cols - 1) / p.tile_cols : 0;
     if (warp == 0)
-        group_tables(p.offsets, p.groups, p.rows, p.share, f_tiles, FORM == RaggedForm::TN ? c_tiles_tn : -p.tile_cols, group_rows,
+        group_tables(p.offsets, p.groups, WIDE && wide ? 2 * p.part_rows : p.rows, WIDE && wide ? p.wide_share : p.share, f_tiles, FORM == RaggedForm::TN ? c_tiles_tn : -p.tile_cols, group_rows,
                      group_start, p.status);
     ptx::tc_fence_before();
     __syncthreads();
@@ -398,8 +411,16 @@ __global__ void __launch_bounds__(RAGGED_THREADS, 1) ragged_gemm_kernel(const __
                                 }
                             }
                         } else {
-                            load_columns<CTAS>(a_smem, map_a, p.a_chunked, 2, full, feature, t.row0 + k0);
-                            load_columns<CTAS>(b_smem, map_b, p.b_chunked, per / 64, full, col, t.row0 + k0);
+                            int row = t.row0 + k0;
+                            if (WIDE && wide) {
+                                const int part = row >= p.part_rows ? 1 : 0;
+                                row -= part * p.part_rows;
+                                if constexpr (CTAS == 2) ptx::tma_load_4d_pair(a_smem, &p.map_parts, full, 0, row, feature / 64, part);
+                                else ptx::tma_load_4d(a_smem, &p.map_parts, full, 0, row, feature / 64, part);
+                            } else {
+                                load_columns<CTAS>(a_smem, map_a, p.a_chunked, 2, full, feature, row);
+                            }
+                            load_columns<CTAS>(b_smem, map_b, p.b_chunked, per / 64, full, col, row);
                         }
                         if constexpr (FORM != RaggedForm::TN) p.x.template load<CTAS>(b_smem, full, k0, col, per);
                     }
@@ -428,7 +449,7 @@ __global__ void __launch_bounds__(RAGGED_THREADS, 1) ragged_gemm_kernel(const __
             int it = 0;      // accumulators handed over
             for (int u = first_unit; u < num_units; u += unit_stride) {
                 const RaggedTile t = walk.at(u);
-                const uint32_t idesc = ptx::idesc_f16(128 * CTAS, t.umma_n, A_MN ? 1 : 0, B_MN ? 1 : 0, BF16 ? 1 : 0);
+                const uint32_t idesc = ptx::idesc_f16(128 * CTAS, t.umma_n, A_MN ? 1 : 0, B_MN ? 1 : 0, BF16 || (WIDE && wide) ? 1 : 0);
                 int row = t.row0;
                 do {
                     const int blocks = FORM == RaggedForm::TN ? chunk_blocks(t, row) : k_blocks_row;
@@ -524,7 +545,7 @@ __global__ void __launch_bounds__(RAGGED_THREADS, 1) ragged_gemm_kernel(const __
 #pragma unroll
                             for (int j = 0; j < 32; ++j) r[j] = 0u;
                         }
-                        const float scale = p.col_scale != nullptr ? __ldg(p.col_scale + (t.col0 + c) / 128) : 1.0f;
+                        const float scale = p.col_scale != nullptr && !(WIDE && wide) ? __ldg(p.col_scale + (t.col0 + c) / 128) : 1.0f;
                         const int c0 = c / COLS * COLS;
                         if (c == c0) {      // the last store has read the block
                             if (lane == 0) ptx::bulk_wait_group_read<0>();

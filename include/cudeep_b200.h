@@ -193,7 +193,10 @@ int cudeep_b200_linear_backward_data_fp8(const void* dy, const float* dy_scales,
  * type is that of dy, W and dx, F16 or BF16; dw has it or is F32.  dx, dw and db may each be NULL, and
  * then so may what only they need; z8 is not read without an activation.  dz is rounded to `type`
  * before the products, db is not.  x enters dw without rounding if its scales are powers of two
- * (cudeep_b200_quantize_fp8's are), else rounded to `type`. */
+ * (cudeep_b200_quantize_fp8's are), whatever their sizes, else rounded to `type`.  Where the nonzero
+ * scales of 128 columns lie more than 2^15 apart and type is F16, whose exponents do not hold x then,
+ * the product for dw is made in BF16 with dz in two parts (the same values; scales that are no powers
+ * of two round x to BF16) and takes twice as long. */
 int cudeep_b200_linear_backward_saved_fp8(const void* dy, int type, const void* x8, const float* x_scales,
                                           const void* z8, const float* z_scales, int epilogue,
                                           const void* W, void* dx, void* dw, int dw_type, float* db, int M,
