@@ -4,6 +4,8 @@
 #include "ragged_gemm.cuh"
 #include "ragged_plan.h"
 
+#include <type_traits>
+
 namespace cudeep_b200 {
 
 namespace {
@@ -48,9 +50,17 @@ void launch(RaggedParams& p, const RaggedPlan& plan, cudaStream_t stream) {
     p.status = dev.status_word;
     p.wait_limit_ns = 2000000000ull;
     p.split = plan.split;
+    p.chunk_rows = std::is_same<OutT, float>::value ? RAGGED_F32_TERMS : RAGGED_F16_TERMS;
+    p.chunk_blocks = RAGGED_F16_TERMS / RAGGED_BK;
     long long clusters = plan.split > 1 ? plan.units : dev.num_sms / CTAS;
     if (clusters > plan.units) clusters = plan.units;
     const uint32_t smem_bytes = uint32_t(p.stages) * p.stage_bytes + fixed + 1024;
+    const long long terms = FORM != RaggedForm::TN ? (p.k + plan.split - 1) / plan.split : WIDE ? 2ll * p.part_rows : p.rows;
+    Scratch partial;
+    if (sizeof(OutT) == 2 && terms > RAGGED_F16_TERMS) {
+        partial = Scratch(size_t(clusters) * CTAS * plan.split * RAGGED_PARTIAL_FLOATS * sizeof(float), stream);
+        p.partial = static_cast<float*>(partial.ptr);
+    }
     CB200_TRACE("grouped %s %s tcgen05: rows=%d groups=%d features=%d %s=%d tile=%dx%d split=%d stages=%d clusters=%lld",
                 FORM == RaggedForm::NT ? "nt" : FORM == RaggedForm::NN ? "nn" : "tn", BF16 ? "bf16" : "f16", p.rows, p.groups,
                 p.features, FORM == RaggedForm::TN ? "cols" : "k", FORM == RaggedForm::TN ? p.cols : p.k, 128 * CTAS,
@@ -112,7 +122,6 @@ void rows_by_weight(bool nn, const void* a, long long lda, const void* w, long l
     p.share = rows;
     p.features = n;
     p.k = k;
-    p.chunk_rows = RAGGED_BK;
     if (nn) launch_rows<RaggedForm::NN>(p, plan, type, stream);
     else launch_rows<RaggedForm::NT>(p, plan, type, stream);
 }
@@ -182,14 +191,12 @@ void grouped_tn(const void* a, long long lda, const void* b, long long ldb, void
     p.step = 128;
     p.a_chunked = encode_columns(&p.map_a, y, rows, m, 2);
     p.b_chunked = encode_columns(&p.map_b, x, rows, n, plan.tile_cols / plan.ctas / 64);
-    int most_rows = rows;
     if (wide.wide != nullptr) {
         CB200_REQUIRE(type == TYPE_F16 && offsets == nullptr && rows <= (1 << 29), "operands in two parts: FP16, one group of 2^29 rows");
         p.wide = wide.wide;
         p.wide_blocks = wide.blocks;
         p.part_rows = (rows + RAGGED_BK - 1) / RAGGED_BK * RAGGED_BK;
         p.wide_share = parts > 1 ? 2 * p.share : 2 * p.part_rows;
-        most_rows = 2 * p.part_rows;
         const uint64_t row_bytes = uint64_t(wide.ld_parts) * 2;
         const uint64_t dims[4] = {64, uint64_t(rows), uint64_t((m + 63) / 64), 2};
         const uint64_t strides[3] = {row_bytes, 128, row_bytes * uint64_t(rows)};
@@ -219,10 +226,6 @@ void grouped_tn(const void* a, long long lda, const void* b, long long ldb, void
     p.features = m;
     p.cols = n;
     p.col_scale = col_scale;
-    // The tensor core's accumulation loses about 2.4e-9 relative per row summed (it truncates), so a gradient in
-    // single precision is summed over 2048 rows at a time, added up with rounding in the epilogue; a 16-bit one
-    // (2e-3 from its own rounding) in one go.
-    p.chunk_rows = out_type == TYPE_F32 ? 2048 : (most_rows + RAGGED_BK - 1) / RAGGED_BK * RAGGED_BK;
     const bool pairs = plan.ctas == 2;
     if (type == TYPE_BF16) {
         if (pairs) launch_weight<2, true>(p, plan, out_type, stream);

@@ -45,6 +45,12 @@ __host__ __device__ constexpr uint32_t ragged_table_bytes(int groups) { return u
 constexpr uint32_t RAGGED_A_BYTES = 128 * 128;       // one CTA's features of a K block
 constexpr int RAGGED_MAX_STAGES = 12;
 constexpr uint32_t RAGGED_SMEM_BUDGET = 232448 - 1024 - 512;   // minus alignment slack and barriers
+// The tensor core truncates as it adds: sums of positive terms come out about 6e-9 of themselves too low per term (measured: 1.2e-5
+// after 2048 rows, 1.0e-4 after 16384).  So an FP32 result is summed over 2048 terms at a time, a 16-bit one over 16384, a
+// fifth of FP16's half step, and such parts are added up in FP32 with rounding.
+constexpr int RAGGED_F32_TERMS = 2048, RAGGED_F16_TERMS = 16384;
+// The parts of a 16-bit result so far, of one CTA's tile: 128 columns x 32 lanes for each epilogue warp, in global memory.
+constexpr size_t RAGGED_PARTIAL_FLOATS = RAGGED_EPI_WARPS * 128 * 32;
 constexpr uint32_t UMMA_BAD_OFFSETS = 6;             // status word: the offsets decrease or leave [0, rows]
 
 // Rows of a matrix as K blocks of 128 bytes.  One box brings all rows that a CTA stages for a tile, up to 128, rounded up to a
@@ -96,7 +102,9 @@ struct RaggedParams {
     // K blocks per stage, atom_bytes apart.  Two to a barrier instead of one: 8192 x 4096 x 4096 nt 214 -> 187 us.
     int atoms;
     uint32_t atom_bytes;
-    int chunk_rows;          // TN: rows summed in the tensor core's accumulator before they are added into C
+    int chunk_rows;          // TN: rows summed in the tensor core's accumulator before they are added into C or `partial`
+    int chunk_blocks;        // NT, NN: K blocks likewise, a multiple of `atoms`
+    float* partial;          // RAGGED_PARTIAL_FLOATS for each CTA, where a 16-bit result may take more than one chunk
     const float* col_scale;  // TN: nullptr, or a factor for each 128 columns of C
     // TN of one group, WIDE: if any of these words is set, X is BF16 and Y two BF16 matrices whose sum it is (WideOperands).  The sums
     // then run over 2 * part_rows rows, part_rows being `rows` rounded up to whole K blocks: those of the first part and those of
@@ -270,6 +278,19 @@ __device__ __forceinline__ void load_columns(uint32_t dst, const CUtensorMap* ma
     for (int j = 0; j < chunks; ++j) {
         if constexpr (CTAS == 2) ptx::tma_load_2d_pair(dst + j * 8192, map, bar, col + j * 64, row);
         else ptx::tma_load_2d(dst + j * 8192, map, bar, col + j * 64, row);
+    }
+}
+
+// 32 columns of a chunk's sums: with those of the chunks before it (`add`), kept for the next chunk unless this is the last one.
+// `part` is the lane's place in the CTA's partial sums; a lane meets only what it wrote itself.
+__device__ __forceinline__ void join_chunks(float* part, uint32_t (&r)[32], bool add, bool last) {
+    if (add) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + part[32 * j]);
+    }
+    if (!last) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) part[32 * j] = __uint_as_float(r[j]);
     }
 }
 
@@ -450,9 +471,9 @@ __global__ void __launch_bounds__(RAGGED_THREADS, 1) ragged_gemm_kernel(const __
             for (int u = first_unit; u < num_units; u += unit_stride) {
                 const RaggedTile t = walk.at(u);
                 const uint32_t idesc = ptx::idesc_f16(128 * CTAS, t.umma_n, A_MN ? 1 : 0, B_MN ? 1 : 0, BF16 || (WIDE && wide) ? 1 : 0);
-                int row = t.row0;
+                int row = t.row0, k_done = 0;
                 do {
-                    const int blocks = FORM == RaggedForm::TN ? chunk_blocks(t, row) : k_blocks_row;
+                    const int blocks = FORM == RaggedForm::TN ? chunk_blocks(t, row) : min(p.chunk_blocks, k_blocks_row - k_done);
                     if (blocks <= 0) break;
                     const uint32_t acc = it & 1;
                     const uint32_t acc_phase = (it >> 1) & 1;
@@ -501,7 +522,8 @@ __global__ void __launch_bounds__(RAGGED_THREADS, 1) ragged_gemm_kernel(const __
                     }
                     ++it;
                     row += p.chunk_rows;
-                } while (FORM == RaggedForm::TN && row < t.row1);
+                    k_done += p.chunk_blocks;
+                } while (FORM == RaggedForm::TN ? row < t.row1 : k_done < k_blocks_row);
             }
         }
     mma_done:
@@ -510,6 +532,7 @@ __global__ void __launch_bounds__(RAGGED_THREADS, 1) ragged_gemm_kernel(const __
     } else {
         // ------------------------------------------------------------ epilogue
         const uint32_t quarter = warp & 3u;
+        float* partial = p.partial + (size_t(blockIdx.x) * RAGGED_EPI_WARPS + (warp - 2)) * (128 * 32) + lane;
         int it = 0;
         for (int u = first_unit; u < num_units; u += unit_stride) {
             const RaggedTile t = walk.at(u);
@@ -526,7 +549,8 @@ __global__ void __launch_bounds__(RAGGED_THREADS, 1) ragged_gemm_kernel(const __
                 int row = t.row0;
                 do {
                     const bool any = chunk_blocks(t, row) > 0;       // an empty group's gradient is zero
-                    const bool add = row != t.row0;
+                    const bool first = row == t.row0, last = t.row1 - row <= p.chunk_rows;
+                    const bool add = sizeof(OutT) == 4 && !first;      // into C
                     const uint32_t acc = it & 1;
                     if (any) {
                         const bool ok = ptx::mbar_wait(ptx::smem_u32(&bar_acc_full[acc]), (it >> 1) & 1, wctx, UMMA_TIMEOUT_EPILOGUE);
@@ -544,6 +568,10 @@ __global__ void __launch_bounds__(RAGGED_THREADS, 1) ragged_gemm_kernel(const __
                         } else {
 #pragma unroll
                             for (int j = 0; j < 32; ++j) r[j] = 0u;
+                        }
+                        if (sizeof(OutT) == 2 && !(first && last)) {
+                            join_chunks(partial + (c - c_begin) * 32, r, !first, last);
+                            if (!last) continue;
                         }
                         const float scale = p.col_scale != nullptr && !(WIDE && wide) ? __ldg(p.col_scale + (t.col0 + c) / 128) : 1.0f;
                         const int c0 = c / COLS * COLS;
@@ -589,54 +617,55 @@ __global__ void __launch_bounds__(RAGGED_THREADS, 1) ragged_gemm_kernel(const __
                 const int f_end = STEPS ? min(p.features, t.feature0 + step) : p.features;
                 const int c_half = (t.umma_n / 2 + 31) / 32 * 32;      // warps 6..9 take the second half of the columns
                 const int c_begin = (int(warp - 2) >> 2) * c_half, c_end = min(t.col_count, c_begin + c_half);
-                const uint32_t acc = it & 1;
-                if (SPLITS && split > 1) {
-                    // The stage ring is idle once the last MMA is done: it takes this CTA's part, [column][128 features].
-                    const uint32_t part = smem_base + (quarter * 32u + lane) * 4u;
-                    if (k_blocks_row > 0) {
-                        const bool ok = ptx::mbar_wait(ptx::smem_u32(&bar_acc_full[0]), 0, wctx, UMMA_TIMEOUT_EPILOGUE);
+                const bool shared = SPLITS && split > 1;
+                // The stage ring is idle once the last MMA is done: it takes this CTA's part, [column][128 features].
+                const uint32_t part = smem_base + (quarter * 32u + lane) * 4u;
+                OutT* dst = static_cast<OutT*>(p.c) + (long long)t.col0 * p.features + feature;
+                int k_done = 0;
+                do {
+                    const bool any = k_blocks_row > 0;      // a split tile's last CTAs may have nothing to sum
+                    const bool first = k_done == 0, last = k_blocks_row - k_done <= p.chunk_blocks;
+                    const uint32_t acc = it & 1;
+                    if (any) {
+                        const bool ok = ptx::mbar_wait(ptx::smem_u32(&bar_acc_full[acc]), (it >> 1) & 1, wctx, UMMA_TIMEOUT_EPILOGUE);
                         if (!__all_sync(0xffffffffu, ok)) goto epilogue_done;
                         ptx::tc_fence_after();
                     }
+                    const uint32_t t_row = tmem_base + acc * 256u + ((quarter * 32u) << 16);
                     for (int c = c_begin; c < c_end; c += 32) {
                         uint32_t r[32];
-                        if (k_blocks_row > 0) {
-                            ptx::tmem_ld_32x32(tmem_base + ((quarter * 32u) << 16) + c, r);
+                        if (any) {
+                            ptx::tmem_ld_32x32(t_row + c, r);
                             ptx::tmem_ld_wait(r);
                         } else {
 #pragma unroll
                             for (int j = 0; j < 32; ++j) r[j] = 0u;
                         }
+                        if (!(first && last)) {
+                            join_chunks(partial + (c - c_begin) * 32, r, !first, last);
+                            if (!last) continue;
+                        }
+                        if (shared) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (c + j < c_end) ptx::st_shared_f32(part + uint32_t(c + j) * 512u, __uint_as_float(r[j]));
-                    }
-                    continue;
-                }
-                const bool ok = ptx::mbar_wait(ptx::smem_u32(&bar_acc_full[acc]), (it >> 1) & 1, wctx, UMMA_TIMEOUT_EPILOGUE);
-                if (!__all_sync(0xffffffffu, ok)) goto epilogue_done;
-                ptx::tc_fence_after();
-                const uint32_t t_row = tmem_base + acc * 256u + ((quarter * 32u) << 16);
-                OutT* dst = static_cast<OutT*>(p.c) + (long long)t.col0 * p.features + feature;
-                for (int c = c_begin; c < c_end; c += 32) {
-                    uint32_t r[32];
-                    ptx::tmem_ld_32x32(t_row + c, r);
-                    ptx::tmem_ld_wait(r);
-                    if (feature < f_end) {
+                            for (int j = 0; j < 32; ++j)
+                                if (c + j < c_end) ptx::st_shared_f32(part + uint32_t(c + j) * 512u, __uint_as_float(r[j]));
+                        } else if (feature < f_end) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (c + j < c_end)
-                                dst[(long long)(c + j) * p.features] = round_to<OutT>(__uint_as_float(r[j]));
+                            for (int j = 0; j < 32; ++j)
+                                if (c + j < c_end)
+                                    dst[(long long)(c + j) * p.features] = round_to<OutT>(__uint_as_float(r[j]));
+                        }
                     }
-                }
-                ptx::tc_fence_before();
-                __syncwarp();
-                if (lane == 0) {
-                    const uint32_t e = ptx::smem_u32(&bar_acc_empty[acc]);
-                    if (CTAS == 2 && !is_leader) ptx::mbar_arrive_cluster_relaxed(ptx::mapa(e, 0));
-                    else ptx::mbar_arrive(e);
-                }
-                ++it;
+                    ptx::tc_fence_before();
+                    __syncwarp();
+                    if (any && lane == 0) {
+                        const uint32_t e = ptx::smem_u32(&bar_acc_empty[acc]);
+                        if (CTAS == 2 && !is_leader) ptx::mbar_arrive_cluster_relaxed(ptx::mapa(e, 0));
+                        else ptx::mbar_arrive(e);
+                    }
+                    ++it;
+                    k_done += p.chunk_blocks;
+                } while (k_done < k_blocks_row);
             }
         }
     epilogue_done:
