@@ -65,8 +65,13 @@ void launch(RaggedParams& p, const RaggedPlan& plan, cudaStream_t stream) {
                 FORM == RaggedForm::NT ? "nt" : FORM == RaggedForm::NN ? "nn" : "tn", BF16 ? "bf16" : "f16", p.rows, p.groups,
                 p.features, FORM == RaggedForm::TN ? "cols" : "k", FORM == RaggedForm::TN ? p.cols : p.k, 128 * CTAS,
                 plan.tile_cols, plan.split, p.stages, clusters);
-    launch_clusters(ragged_gemm_kernel<FORM, CTAS, BF16, OutT, WIDE>, p, clusters, CTAS * plan.split, RAGGED_THREADS, smem_bytes,
-                    RAGGED_SMEM_BUDGET + 1024, stream);
+    auto run = [&](auto kernel) {
+        launch_clusters(kernel, p, clusters, CTAS * plan.split, RAGGED_THREADS, smem_bytes, RAGGED_SMEM_BUDGET + 1024, stream);
+    };
+    if constexpr (sizeof(OutT) == 2) {
+        if (p.partial != nullptr) return run(ragged_gemm_kernel<FORM, CTAS, BF16, OutT, WIDE, true>);
+    }
+    run(ragged_gemm_kernel<FORM, CTAS, BF16, OutT, WIDE>);
 }
 
 template <RaggedForm FORM>

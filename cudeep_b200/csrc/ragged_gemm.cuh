@@ -295,8 +295,9 @@ __device__ __forceinline__ void join_chunks(float* part, uint32_t (&r)[32], bool
 }
 
 // WIDE: the operands may come in the form of RaggedParams::wide.  A kernel of its own, as reading the flags and the test in the
-// producer's loop cost 3.5 us of 195 in 8192 x 4096 x 4096.
-template <RaggedForm FORM, int CTAS, bool BF16, class OutT, bool WIDE = false>
+// producer's loop cost 3.5 us of 195 in 8192 x 4096 x 4096.  LONG: 16-bit results of more than one chunk, which a kernel that
+// has the code for them pays with 0.2 us even where it is not reached (7.8 us for 300 rows, 1024 -> 640).
+template <RaggedForm FORM, int CTAS, bool BF16, class OutT, bool WIDE = false, bool LONG = false>
 __global__ void __launch_bounds__(RAGGED_THREADS, 1) ragged_gemm_kernel(const __grid_constant__ RaggedParams p) {
 #if defined(__CUDA_ARCH_FEAT_SM100_ALL) || defined(__CUDA_ARCH_FEAT_SM101_ALL) || \
     defined(__CUDA_ARCH_FEAT_SM103_ALL)
@@ -473,7 +474,7 @@ __global__ void __launch_bounds__(RAGGED_THREADS, 1) ragged_gemm_kernel(const __
                 const uint32_t idesc = ptx::idesc_f16(128 * CTAS, t.umma_n, A_MN ? 1 : 0, B_MN ? 1 : 0, BF16 || (WIDE && wide) ? 1 : 0);
                 int row = t.row0, k_done = 0;
                 do {
-                    const int blocks = FORM == RaggedForm::TN ? chunk_blocks(t, row) : min(p.chunk_blocks, k_blocks_row - k_done);
+                    const int blocks = FORM == RaggedForm::TN ? chunk_blocks(t, row) : LONG ? min(p.chunk_blocks, k_blocks_row - k_done) : k_blocks_row;
                     if (blocks <= 0) break;
                     const uint32_t acc = it & 1;
                     const uint32_t acc_phase = (it >> 1) & 1;
@@ -523,7 +524,7 @@ __global__ void __launch_bounds__(RAGGED_THREADS, 1) ragged_gemm_kernel(const __
                     ++it;
                     row += p.chunk_rows;
                     k_done += p.chunk_blocks;
-                } while (FORM == RaggedForm::TN ? row < t.row1 : k_done < k_blocks_row);
+                } while (FORM == RaggedForm::TN ? row < t.row1 : LONG && k_done < k_blocks_row);
             }
         }
     mma_done:
@@ -549,7 +550,7 @@ __global__ void __launch_bounds__(RAGGED_THREADS, 1) ragged_gemm_kernel(const __
                 int row = t.row0;
                 do {
                     const bool any = chunk_blocks(t, row) > 0;       // an empty group's gradient is zero
-                    const bool first = row == t.row0, last = t.row1 - row <= p.chunk_rows;
+                    const bool first = row == t.row0, last = !LONG || t.row1 - row <= p.chunk_rows;
                     const bool add = sizeof(OutT) == 4 && !first;      // into C
                     const uint32_t acc = it & 1;
                     if (any) {
@@ -569,7 +570,7 @@ __global__ void __launch_bounds__(RAGGED_THREADS, 1) ragged_gemm_kernel(const __
 #pragma unroll
                             for (int j = 0; j < 32; ++j) r[j] = 0u;
                         }
-                        if (sizeof(OutT) == 2 && !(first && last)) {
+                        if (LONG && !(first && last)) {
                             join_chunks(partial + (c - c_begin) * 32, r, !first, last);
                             if (!last) continue;
                         }
@@ -624,7 +625,7 @@ __global__ void __launch_bounds__(RAGGED_THREADS, 1) ragged_gemm_kernel(const __
                 int k_done = 0;
                 do {
                     const bool any = k_blocks_row > 0;      // a split tile's last CTAs may have nothing to sum
-                    const bool first = k_done == 0, last = k_blocks_row - k_done <= p.chunk_blocks;
+                    const bool first = k_done == 0, last = !LONG || k_blocks_row - k_done <= p.chunk_blocks;
                     const uint32_t acc = it & 1;
                     if (any) {
                         const bool ok = ptx::mbar_wait(ptx::smem_u32(&bar_acc_full[acc]), (it >> 1) & 1, wctx, UMMA_TIMEOUT_EPILOGUE);
@@ -641,7 +642,7 @@ __global__ void __launch_bounds__(RAGGED_THREADS, 1) ragged_gemm_kernel(const __
 #pragma unroll
                             for (int j = 0; j < 32; ++j) r[j] = 0u;
                         }
-                        if (!(first && last)) {
+                        if (LONG && !(first && last)) {
                             join_chunks(partial + (c - c_begin) * 32, r, !first, last);
                             if (!last) continue;
                         }
@@ -665,7 +666,7 @@ __global__ void __launch_bounds__(RAGGED_THREADS, 1) ragged_gemm_kernel(const __
                     }
                     ++it;
                     k_done += p.chunk_blocks;
-                } while (k_done < k_blocks_row);
+                } while (LONG && k_done < k_blocks_row);
             }
         }
     epilogue_done:
