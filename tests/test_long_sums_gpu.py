@@ -151,3 +151,23 @@ def test_8bit_products_of_more_than_one_accumulator(dev, m, n, k, out):
                                                            CODES[out], m, k, n, None))
     assert dev.sync_status() == 0
     assert ((y.double() / (x @ w) - 1).abs() <= rel).all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("act", [0, 1])
+@pytest.mark.parametrize("m,n", [(5_000_001, 64), (4_194_305, 8), (70_001, 200)])
+def test_every_row_is_in_the_column_sums(dev, m, n, act, dtype):
+    """Row r has a single 1 or 2, in column r % n: all partial sums are whole numbers below 2^24, so the sums are exact in any
+    order, and one row left out or taken twice shows.  65535 bands of 64 rows, the most that a grid's second dimension holds, are
+    4194240 rows."""
+    torch = dev.torch
+    r = torch.arange(m, device=dev.dev)
+    dy = torch.zeros(m, n, dtype=dtype_of(torch, dtype), device=dev.dev)
+    dy[r, r % n] = (1 + (r // 7) % 2).to(dy.dtype)
+    z8, zs = torch.full((m, n), 0x38, dtype=torch.uint8, device=dev.dev), torch.ones(-(-n // 128), m, device=dev.dev)
+    db = torch.full((n,), float("nan"), device=dev.dev)
+    p = dev.ptr
+    dev.check(dev.lib.cudeep_b200_linear_backward_saved_fp8(p(dy), CODES[dtype], None, None, p(z8), p(zs), act, None, None, None,
+                                                            CODES[dtype], p(db), m, n, 8, None))
+    assert dev.sync_status() == 0
+    assert torch.equal(db.double(), dy.double().sum(0))
