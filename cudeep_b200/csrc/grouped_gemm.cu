@@ -197,7 +197,7 @@ void grouped_tn(const void* a, long long lda, const void* b, long long ldb, void
     p.a_chunked = encode_columns(&p.map_a, y, rows, m, 2);
     p.b_chunked = encode_columns(&p.map_b, x, rows, n, plan.tile_cols / plan.ctas / 64);
     if (wide.wide != nullptr) {
-        CB200_REQUIRE(type == TYPE_F16 && offsets == nullptr && rows <= (1 << 29), "operands in two parts: FP16, one group of 2^29 rows");
+        CB200_REQUIRE(type == TYPE_F16 && offsets == nullptr, "operands in two parts: FP16, one group");
         p.wide = wide.wide;
         p.wide_blocks = wide.blocks;
         p.part_rows = (rows + RAGGED_BK - 1) / RAGGED_BK * RAGGED_BK;

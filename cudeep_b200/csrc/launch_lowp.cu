@@ -6,6 +6,8 @@
 #include "grouped_gemm.h"
 #include "lowp_rows.h"
 
+#include <initializer_list>
+
 namespace cudeep {
 namespace kernels {
 
@@ -33,10 +35,16 @@ void check_element_address(const void* p, int bytes, const char* what) {
     CB200_REQUIRE(reinterpret_cast<uintptr_t>(p) % bytes == 0, std::string(what) + " is not aligned to its element type");
 }
 
+// The kernels add up to a tile, or a band of rows, to an extent in 32 bits.
+void check_extents(std::initializer_list<int> extents) {
+    for (int e : extents) CB200_REQUIRE(e <= 2147483647 - 65535, "extents are at most 2^31 - 65536");
+}
+
 void check_grouped(const void* a, const void* b, const void* c, const int32_t* offsets, int groups, int rows, int n, int k) {
     CB200_REQUIRE(a != nullptr && b != nullptr && c != nullptr && offsets != nullptr, "grouped matmul: null pointer");
     CB200_REQUIRE(groups > 0 && groups <= 1024, "grouped matmul: 1 to 1024 groups");
     CB200_REQUIRE(rows >= 0 && n > 0 && k > 0, "grouped matmul: rows must not be negative, the other extents positive");
+    check_extents({rows, n, k});
     check_element_address(a, 2, "A");
     check_element_address(b, 2, "B");
     check_element_address(offsets, 4, "offsets");
@@ -65,6 +73,7 @@ void launch_quantize_fp8(const void* x, ElementType type, long long rows, int co
     const int t = checked_type(type), b = checked_block(block);
     CB200_REQUIRE(x != nullptr && q != nullptr && scales != nullptr, "quantize_fp8: null pointer");
     CB200_REQUIRE(rows >= 0 && cols > 0, "quantize_fp8: rows must not be negative, cols positive");
+    check_extents({cols});
     check_element_address(x, cudeep_b200::elem_bytes(t), "x");
     check_element_address(scales, 4, "scales");
     if (rows == 0) return;
@@ -76,6 +85,7 @@ void launch_dequantize_fp8(const void* q, const float* scales, long long rows, i
     const int t = checked_type(type), b = checked_block(block);
     CB200_REQUIRE(y != nullptr && q != nullptr && scales != nullptr, "dequantize_fp8: null pointer");
     CB200_REQUIRE(rows >= 0 && cols > 0, "dequantize_fp8: rows must not be negative, cols positive");
+    check_extents({cols});
     check_element_address(y, cudeep_b200::elem_bytes(t), "y");
     check_element_address(scales, 4, "scales");
     if (rows == 0) return;
@@ -119,6 +129,7 @@ void launch_linear_forward_fp8(const void* x, const float* x_scales, const void*
     CB200_REQUIRE(x != nullptr && x_scales != nullptr && W != nullptr && w_scales != nullptr && y != nullptr,
                   "linear_fp8: null pointer");
     CB200_REQUIRE(M >= 0 && N > 0 && K > 0, "linear_fp8: M must not be negative, N and K positive");
+    check_extents({M, N, K});
     check_element_address(y, cudeep_b200::elem_bytes(t), "y");
     check_element_address(x_scales, 4, "x_scales");
     check_element_address(w_scales, 4, "w_scales");
@@ -134,6 +145,7 @@ void launch_linear_backward_data_fp8(const void* dy, const float* dy_scales, con
     CB200_REQUIRE(dy != nullptr && dy_scales != nullptr && W != nullptr && w_scales != nullptr && dx != nullptr,
                   "linear_fp8: null pointer");
     CB200_REQUIRE(M >= 0 && N > 0 && K > 0, "linear_fp8: M must not be negative, N and K positive");
+    check_extents({M, N, K});
     check_element_address(dx, cudeep_b200::elem_bytes(t), "dx");
     check_element_address(dy_scales, 4, "dy_scales");
     check_element_address(w_scales, 4, "w_scales");
@@ -154,6 +166,8 @@ void launch_linear_backward_saved_fp8(const void* dy, ElementType type, const vo
     CB200_REQUIRE(act == EPI_NONE || (z8 != nullptr && z_scales != nullptr),
                   "linear_backward_saved: an activation needs z8 and its scales");
     CB200_REQUIRE(M >= 0 && N > 0 && K > 0, "linear_backward_saved: M must not be negative, N and K positive");
+    check_extents({M, N, K});
+    CB200_REQUIRE(dw == nullptr || t != TYPE_F16 || M <= (1 << 29), "linear_backward_saved: at most 2^29 rows for the dw of F16 operands");
     const int wt = dw != nullptr ? checked_type(dw_type) : t;
     CB200_REQUIRE(wt == t || wt == TYPE_F32, "linear_backward_saved: dw is F32 or of dy's type");
     check_element_address(dy, 2, "dy");

@@ -910,6 +910,7 @@ PreparedRows prepare_rows(const RowsRequest& a, const RowsRequest& b, const Scal
             to.ld = m.ld != 0 ? m.ld : m.cols;
             return;
         }
+        CB200_REQUIRE((long long)m.cols * m.elem_size <= 2147483647 - 1023, "a row of this many bytes cannot be copied to a padded one");
         const int units = (m.cols + per_unit - 1) / per_unit;
         to.ld = (long long)units * per_unit;
         to.copy = Scratch(size_t(m.rows) * units * 16, stream);

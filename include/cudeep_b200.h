@@ -150,7 +150,8 @@ int cudeep_b200_gemm_tf32_tuned(const float* A, const float* B, int b_is_nk, flo
 /* No counterpart in the reference: the products of low-precision Linear layers and of layers whose
  * rows are split among experts.  All matrices are row-major and contiguous; any base address that
  * suits its element type and any row length is taken (rows that are not 16-byte multiples are first
- * copied to a padded temporary).  Zero rows are a valid size.  Results must not overlap operands. */
+ * copied to a padded temporary).  Zero rows are a valid size.  Extents are at most 2^31 - 65536, a row
+ * that has to be copied at most 2^31 - 1024 bytes.  Results must not overlap operands. */
 
 /* Element types of the operands passed as void pointers. */
 #define CUDEEP_B200_TYPE_F32 0
@@ -196,7 +197,7 @@ int cudeep_b200_linear_backward_data_fp8(const void* dy, const float* dy_scales,
  * (cudeep_b200_quantize_fp8's are), whatever their sizes, else rounded to `type`.  Where the nonzero
  * scales of 128 columns lie more than 2^15 apart and type is F16, whose exponents do not hold x then,
  * the product for dw is made in BF16 with dz in two parts (the same values; scales that are no powers
- * of two round x to BF16) and takes twice as long. */
+ * of two round x to BF16) and takes twice as long.  With F16 operands dw takes 2^29 rows at most. */
 int cudeep_b200_linear_backward_saved_fp8(const void* dy, int type, const void* x8, const float* x_scales,
                                           const void* z8, const float* z_scales, int epilogue,
                                           const void* W, void* dx, void* dw, int dw_type, float* db, int M,

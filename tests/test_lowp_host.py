@@ -145,3 +145,35 @@ def test_python_refusals(cd):
         cd.grouped_linear(b(4, 9), b(2, 6, 8), T([3], D.int32))
     with pytest.raises(RuntimeError, match="grad"):
         cd.grouped_linear_backward(b(4, 7), b(4, 8), b(2, 6, 8), T([3], D.int32))
+
+
+HUGE = 2147483647
+
+
+@pytest.mark.parametrize("m,n,k", [(HUGE, 8, 8), (8, HUGE, 8), (8, 8, HUGE), (HUGE - 65535 + 1, 8, 8)])
+def test_extents_near_the_end_of_32_bits_are_refused(lib, buf, m, n, k):
+    """Beyond 2^31 - 65536 the kernels' and planners' sums of an extent and a tile would wrap around."""
+    p = ctypes.addressof(buf)
+    p += -p % 16
+    assert "at most" in refused(lib, "cudeep_b200_linear_forward_fp8", p, p, p, p, None, p, 0, m, n, k, 0, None)
+    assert "at most" in refused(lib, "cudeep_b200_linear_backward_data_fp8", p, p, p, p, p, 0, m, n, k, None)
+    assert "at most" in refused(lib, "cudeep_b200_linear_backward_saved_fp8", p, 2, p, p, p, p, 2, p, p, p, 2, p, m, n, k, None)
+    for name in ("cudeep_b200_grouped_matmul_nt", "cudeep_b200_grouped_matmul_nn"):
+        assert "at most" in refused(lib, name, p, p, p, 2, p, 4, m, n, k, None)
+    assert "at most" in refused(lib, "cudeep_b200_grouped_matmul_tn", p, p, p, 2, 0, p, 4, m, n, k, None)
+    if k != 8:
+        assert "at most" in refused(lib, "cudeep_b200_quantize_fp8", p, 2, 1, k, 1, p, p, None)
+        assert "at most" in refused(lib, "cudeep_b200_dequantize_fp8", p, p, 1, k, 1, p, 2, None)
+
+
+def test_rows_of_more_bytes_than_a_copy_counts_are_refused(lib, buf):
+    """Rows that are no 16-byte multiples are copied, counted in bytes by 32 bits.  (Aligned ones of that length are not copied.)"""
+    p = ctypes.addressof(buf)
+    p += -p % 16
+    long = (1 << 30) + 1
+    for name in ("cudeep_b200_grouped_matmul_nt", "cudeep_b200_grouped_matmul_nn"):
+        assert "row" in refused(lib, name, p, p, p, 2, p, 4, 4, 8, long, None)
+    assert "row" in refused(lib, "cudeep_b200_grouped_matmul_tn", p, p, p, 2, 0, p, 4, 4, 8, long, None)
+    assert "row" in refused(lib, "cudeep_b200_linear_backward_saved_fp8", p, 2, p, p, p, p, 2, p, p, p, 2, p, 4, 8, long, None)
+    assert "2^29" in refused(lib, "cudeep_b200_linear_backward_saved_fp8", p, 1, p, p, p, p, 2, p, p, p, 1, p, (1 << 29) + 1, 8, 8,
+                             None)
