@@ -112,20 +112,6 @@ __device__ __forceinline__ __half from_float<__half>(float v) { return __float2h
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// Eight consecutive elements from a 16-byte aligned (32 for float: two loads) address.
-__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
-    const T* t = reinterpret_cast<const T*>(&u);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = to_float(t[j]);
-}
-
 __device__ __forceinline__ float finite_abs(float v) {
     const float a = fabsf(v);
     return a <= 3.402823466e38f ? a : 0.0f;      // NaN compares false
