@@ -45,9 +45,10 @@ __host__ __device__ constexpr uint32_t ragged_table_bytes(int groups) { return u
 constexpr uint32_t RAGGED_A_BYTES = 128 * 128;       // one CTA's features of a K block
 constexpr int RAGGED_MAX_STAGES = 12;
 constexpr uint32_t RAGGED_SMEM_BUDGET = 232448 - 1024 - 512;   // minus alignment slack and barriers
-// The tensor core truncates as it adds: sums of positive terms come out about 6e-9 of themselves too low per term (measured: 1.2e-5
-// after 2048 rows, 1.0e-4 after 16384).  So an FP32 result is summed over 2048 terms at a time, a 16-bit one over 16384, a
-// fifth of FP16's half step, and such parts are added up in FP32 with rounding.
+// The tensor core truncates as it adds: sums of positive FP16 products come out about 6e-9 of themselves too low per term (measured:
+// 1.2e-5 after 2048 rows, 1.0e-4 after 16384; BF16, whose products have fewer bits to lose, 2.5e-6 after 2048).  So an FP32 result
+// is summed over 2048 terms at a time, a 16-bit one over 16384, a fifth of FP16's half step, and such parts are added up in
+// FP32 with rounding.
 constexpr int RAGGED_F32_TERMS = 2048, RAGGED_F16_TERMS = 16384;
 // The parts of a 16-bit result so far, of one CTA's tile: 128 columns x 32 lanes for each epilogue warp, in global memory.
 constexpr size_t RAGGED_PARTIAL_FLOATS = RAGGED_EPI_WARPS * 128 * 32;

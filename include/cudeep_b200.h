@@ -178,8 +178,11 @@ int cudeep_b200_dequantize_fp8(const void* q, const float* scales, long long row
 
 /* y[M,N] = act(x[M,K] * W[N,K]^T + bias[N]) with x and W in 8 bits, x with blocks of 1 x 128 and W
  * with blocks of 128 x 128 as cudeep_b200_quantize_fp8 lays them out (any finite scales are taken,
- * not only powers of two).  Each block of 128 products is summed by the tensor cores, the scaled
- * blocks are added in FP32.  bias (FP32) may be NULL; y_type: any of the three. */
+ * not only powers of two).  Sums are FP32: each block of 128 products is summed by the tensor cores and
+ * the scaled blocks are added with rounding, or, in large products whose scales are all powers of two,
+ * the tensor cores scale and sum 2048 (F32 result) or 16384 elements of K before such an addition.
+ * Sigmoid, alone or in GELU and SiLU, is right relative to itself down to 2^-126.  bias (FP32) may be
+ * NULL; y_type: any of the three. */
 int cudeep_b200_linear_forward_fp8(const void* x, const float* x_scales, const void* W,
                                    const float* w_scales, const float* bias, void* y, int y_type, int M,
                                    int N, int K, int epilogue, cudeep_b200_stream_t stream);
@@ -206,7 +209,9 @@ int cudeep_b200_linear_backward_saved_fp8(const void* dy, int type, const void* 
 /* Products of row groups of any sizes, each group with a matrix of its own.  Group g is the rows
  * [offsets[g], offsets[g + 1]); `offsets` is a DEVICE array of groups + 1 ascending row numbers in
  * [0, rows], read by the kernel, so sizes may come from the kernel before and are never copied to
- * the host.  A group may be empty.  1 to 1024 groups.  type: F16 or BF16; sums are FP32.
+ * the host.  A group may be empty.  1 to 1024 groups.  type: F16 or BF16; sums are FP32, of up to 16384
+ * terms (an F32 result: 2048) in the tensor cores, which truncate as they add (6e-9 of a sum of positive
+ * F16 products per term), and of such parts with rounding.
  *   nt: C[r, N] = A[r, K] * B[g][N, K]^T     (forward of Linear layers)
  *   nn: C[r, N] = A[r, K] * B[g][K, N]       (gradient of the rows)
  *   tn: C[g][M, N] = A_g[., M]^T * B_g[., N] (gradient of the matrices; zeros for an empty group)
