@@ -135,3 +135,47 @@ def test_infinities_stay_in_their_features(dev, kind):
     assert torch.equal(got[~fine].isnan(), want[~fine].isnan())
     inf = want.isinf()
     assert torch.equal(got[inf], want[inf]) and bool(inf.any())
+
+
+@pytest.mark.parametrize("m,n,k,act", [(333, 77, 101, 3), (1, 64, 64, 0), (2500, 64, 136, 0), (1030, 520, 264, 1)])
+def test_captured_calls_follow_the_scales_of_each_replay(dev, m, n, k, act):
+    """Which form x is taken in is decided on the device: a graph replayed on other activations gives what a call of its own
+    gives, and two graphs side by side do not share what they decide by."""
+    torch = dev.torch
+    gen = torch.Generator(device=dev.dev).manual_seed(11)
+    p = dev.ptr
+    z8, zs, _ = kept(dev, torch.randn(m, n, generator=gen, device=dev.dev))
+    dy = torch.randn(m, n, generator=gen, device=dev.dev).half()
+    w = (torch.randn(n, k, generator=gen, device=dev.dev) / n ** 0.5).half()
+    kinds = ["near", "tiny", "columns", "near", "outlier"]
+    inputs = [kept(dev, rows(torch, gen, m, k, kind, dev.dev))[:2] for kind in kinds]
+    want = [gradient(dev, dy, x8, xs, z8, zs, act, w, m, n, k, "f32", ("dx", "dw", "db")) for x8, xs in inputs]
+    slots, graphs = [], []
+    for _ in range(2):
+        x8, xs = (t.clone() for t in inputs[0])
+        dx, dw, db = (torch.full_like(t, float("nan")) for t in (want[0]["dx"], want[0]["dw"], want[0]["db"]))
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g):
+            stream = torch.cuda.current_stream().cuda_stream
+            dev.check(dev.lib.cudeep_b200_linear_backward_saved_fp8(p(dy), 1, p(x8), p(xs), p(z8) if act else None,
+                                                                    p(zs) if act else None, act, p(w), p(dx), p(dw), 0, p(db),
+                                                                    m, n, k, stream))
+        slots.append((x8, xs, dx, dw, db))
+        graphs.append(g)
+    side = [torch.cuda.Stream() for _ in range(2)]
+    for i in range(len(kinds)):
+        pair = (i, (i + 1) % len(kinds))
+        for j, at in enumerate(pair):
+            slots[j][0].copy_(inputs[at][0])
+            slots[j][1].copy_(inputs[at][1])
+            for t in slots[j][2:]:
+                t.fill_(float("nan"))
+        torch.cuda.synchronize()
+        for j in range(2):
+            with torch.cuda.stream(side[j]):
+                graphs[j].replay()
+        assert dev.sync_status() == 0
+        for j, at in enumerate(pair):
+            for t, key in zip(slots[j][2:], ("dx", "dw", "db")):
+                assert torch.equal(t, want[at][key])
